@@ -240,6 +240,28 @@ int mlk_gemm_layout_a_noalloc(const void *a, const void *b, void *c, int m, int 
                               int kernel_id, int p1, int p2, int p3, void *stream);
 size_t mlk_gemm_noalloc_scratch_bytes(void);
 
+/* ------------------------------------------------------------- 4-bit weights
+ * W[n, k] = s[n, k / G] * (q[n, k] - z[n, k / G]): codes q and zero points z of 4 bits (0..15; z = 8 without zero points), one 16-bit
+ * scale (of the activations' kind) and one zero point for G consecutive weights of a row, G = 32, 64 or a multiple of 128 that divides K.
+ * N % 16 == 0, K % 128 == 0, K < 2^23.  No counterpart in the reference. */
+
+/* Codes, row-major [N, K/2] bytes (element 2 i in the low half of byte i) -> tiles of 16 rows x 128 k, [N/16, K/128, 64, 16] bytes: bytes
+ * 4 j .. 4 j + 3 of lane 16 o + r hold k = 128 t + 32 j + 8 o .. + 7 of row r, even ones in the low 16 bits, odd ones in the high 16.
+ * `batch` independent matrices are processed back to back; src and dst on 4 bytes. */
+int mlk_pack_layout_a_w4(const void *src, void *dst, int64_t batch, int n, int k, void *stream);
+int mlk_unpack_layout_a_w4(const void *src, void *dst, int64_t batch, int n, int k, void *stream);
+/* Scales (elem_size 2) or zero points (1), row-major [N, K/G] -> [N/16, K/max(G,128), 16, max(1,128/G)]. */
+int mlk_pack_scales_w4(const void *src, void *dst, int64_t batch, int n, int k, int group, int elem_size, void *stream);
+int mlk_unpack_scales_w4(const void *src, void *dst, int64_t batch, int n, int k, int group, int elem_size, void *stream);
+
+/* C[M, N] = T(alpha * B[M, K] . W^T (+ bias[N])), any M >= 0, fp32 accumulation, no weight rounded; `scale` and `zero` (NULL: none) packed as
+ * above.  A row of B that holds an infinity gives NaN.  a and b on 16 bytes, scale on 8, zero on 4.
+ * workspace: device scratch of at least mlk_gemm_w4_workspace_bytes() bytes under the rules of mlk_gemm_layout_a; may be NULL where
+ * that is 0. */
+int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, const void *b, void *c, int m, int n, int k, int group,
+                         int x_kind, float alpha, const void *bias, void *workspace, size_t workspace_bytes, void *stream);
+size_t mlk_gemm_w4_workspace_bytes(int m, int n, int k);
+
 /* ----------------------------------------------------------------------- MoE */
 
 /* Router: scores (score_fun 0 = softmax, 1 = sigmoid), optional correction

@@ -40,6 +40,13 @@ SIGNATURES = {
     "mlk_gemm_plan_placed": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "mlk_gemm_plan_off16": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "mlk_gemm_counter_bytes": (c_size_t, []),
+    "mlk_pack_layout_a_w4": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
+    "mlk_unpack_layout_a_w4": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
+    "mlk_pack_scales_w4": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "mlk_unpack_scales_w4": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "mlk_gemm_layout_a_w4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                     c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mlk_gemm_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "mlk_fused_routing_gate": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
                                        c_void_p, c_void_p, c_void_p]),
     "mlk_moe_align_tokens": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,

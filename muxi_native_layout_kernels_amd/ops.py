@@ -598,6 +598,149 @@ def _gemm_layoutABC_checked(A, B, alpha=1, beta=0, bias=None):
     return gemm_layoutABC_wapper(A, B, m, n, k, alpha, beta, p1, p2, p3, kid, bias)
 
 
+# ------------------------------------------------------------- 4-bit weights
+class _OnDevice:
+    """The library launches on the current device: makes the tensor's device current for the call where it is another one."""
+
+    def __init__(self, t):
+        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _w4_tensors(named, device):
+    for t, name in named:
+        if t is not None:
+            _check(t.is_cuda, "%s must be a CUDA tensor" % name)
+            _check(t.device == device, "%s must be on the same device as the others" % name)
+            _check(t.is_contiguous(), "%s must be contiguous" % name)
+
+
+def pack_layout_a_w4(codes, scales, zeros=None):
+    """4-bit weights W = s (q - z), row-major, to the layout of `gemm_layoutA_w4` and `fused_experts_w4`.
+
+    codes  uint8 [N, K/2] or [E, N, K/2], two codes 0..15 in a byte, element 2 i in the low half of byte i
+    scales fp16 / bf16 [.., N, K/G], one for G consecutive weights of a row; G = 32, 64 or a multiple of 128
+    zeros  uint8 [.., N, K/G], 0..15, or None: 8 everywhere
+    Returns (A [.., N/16, K/128, 64, 16] uint8, scale and zero [.., N/16, K/max(G,128), 16, max(1,128/G)])."""
+    _check(codes.dtype == torch.uint8 and codes.dim() in (2, 3), "codes must be uint8 [N, K/2] or [E, N, K/2]")
+    _check(scales.dtype in _KIND, "scales must be fp16 or bf16")
+    _check(zeros is None or zeros.dtype == torch.uint8, "zeros must be uint8")
+    n, k = codes.shape[-2], codes.shape[-1] * 2
+    lead = tuple(codes.shape[:-2])
+    _check(n % 16 == 0 and k % 128 == 0 and n > 0 and k > 0, "N % 16 and K % 128 must be 0")
+    _check(scales.dim() == codes.dim() and tuple(scales.shape[:-1]) == lead + (n,), "scales must be [.., N, K/G]")
+    groups = scales.shape[-1]
+    _check(groups > 0 and k % groups == 0, "scales must be [.., N, K/G]")
+    group = k // groups
+    _check(group in (32, 64) or group % 128 == 0, "the group must be 32, 64 or a multiple of 128")
+    _check(zeros is None or zeros.shape == scales.shape, "zeros must have the shape of scales")
+    _w4_tensors(((codes, "codes"), (scales, "scales"), (zeros, "zeros")), codes.device)
+    batch = codes.shape[0] if codes.dim() == 3 else 1
+    per = max(1, 128 // group)
+    lib, shape = _lib.load(), lead + (n // 16, groups // per, 16, per)
+    with _OnDevice(codes):
+        stream = _stream_of(codes)
+        A = torch.empty(lead + (n // 16, k // 128, 64, 16), dtype=torch.uint8, device=codes.device)
+        _lib.check(lib.mlk_pack_layout_a_w4(_ptr(codes), _ptr(A), batch, n, k, stream), "pack_layout_a_w4")
+        out = []
+        for t in (scales, zeros):
+            p = None
+            if t is not None:
+                p = torch.empty(shape, dtype=t.dtype, device=t.device)
+                _lib.check(lib.mlk_pack_scales_w4(_ptr(t), _ptr(p), batch, n, k, group, t.element_size(), stream), "pack_layout_a_w4")
+            out.append(p)
+    return A, out[0], out[1]
+
+
+def unpack_layout_a_w4(A, A_Scale, A_Zero=None):
+    """Inverse of `pack_layout_a_w4`: (codes [.., N, K/2], scales [.., N, K/G], zeros or None)."""
+    n, k, group = _w4_dims(A, A_Scale, A_Zero, A.dim() - 4)
+    _w4_tensors(((A, "A"), (A_Scale, "A_Scale"), (A_Zero, "A_Zero")), A.device)
+    lead = tuple(A.shape[:-4])
+    batch = A.shape[0] if lead else 1
+    lib = _lib.load()
+    with _OnDevice(A):
+        stream = _stream_of(A)
+        codes = torch.empty(lead + (n, k // 2), dtype=torch.uint8, device=A.device)
+        _lib.check(lib.mlk_unpack_layout_a_w4(_ptr(A), _ptr(codes), batch, n, k, stream), "unpack_layout_a_w4")
+        out = []
+        for t in (A_Scale, A_Zero):
+            p = None
+            if t is not None:
+                p = torch.empty(lead + (n, k // group), dtype=t.dtype, device=t.device)
+                _lib.check(lib.mlk_unpack_scales_w4(_ptr(t), _ptr(p), batch, n, k, group, t.element_size(), stream), "unpack_layout_a_w4")
+            out.append(p)
+    return codes, out[0], out[1]
+
+
+def _w4_dims(A, scale, zero, lead, what="A"):
+    """(N, K, group) of packed 4-bit weights with `lead` leading dimensions (0 or 1)."""
+    _check(lead in (0, 1) and A.dim() == 4 + lead and A.dtype == torch.uint8 and tuple(A.shape[-2:]) == (64, 16),
+           "%s must be uint8 [N/16, K/128, 64, 16] (pack_layout_a_w4)" % what)
+    n, k = A.size(-4) * 16, A.size(-3) * 128
+    _check(scale.dim() == A.dim() and scale.size(-2) == 16 and tuple(scale.shape[:-3]) == tuple(A.shape[:-3]) and scale.size(-3) > 0,
+           "the scales of %s must be [N/16, K/max(G,128), 16, max(1,128/G)]" % what)
+    blocks, per = scale.size(-3), scale.size(-1)
+    _check((per in (2, 4) and blocks * 128 == k) or (per == 1 and k % (blocks * 128) == 0 and k > 0),
+           "the scales of %s must be [N/16, K/max(G,128), 16, max(1,128/G)]" % what)
+    _check(scale.dtype in _KIND, "the scales of %s must be fp16 or bf16" % what)
+    _check(zero is None or (zero.dtype == torch.uint8 and zero.shape == scale.shape), "the zero points of %s must be uint8 of the scales' shape" % what)
+    return n, k, 128 // per if per > 1 else k // blocks
+
+
+def _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, what):
+    key = ("w4", A.shape, A_Scale.shape, B.shape, A.dtype, A_Scale.dtype, B.dtype, A.device, A_Scale.device, B.device,
+           None if A_Zero is None else (A_Zero.shape, A_Zero.dtype, A_Zero.device), None if bias is None else (bias.shape, bias.dtype, bias.device))
+    plan = _plans.get(key)
+    if plan is None or beta != 0 or not (A.is_contiguous() and A_Scale.is_contiguous() and B.is_contiguous() and
+                                         (A_Zero is None or A_Zero.is_contiguous()) and (bias is None or bias.is_contiguous())):
+        _check_beta(beta)
+        m, k, group = _w4_dims(A, A_Scale, A_Zero, 0)
+        _check(B.dim() == 2, "B must be a 2D tensor")
+        _check(B.size(1) == k, "A and B must have the same k")
+        _check(B.dtype in _KIND, "Unsupported data type")
+        _check(A_Scale.dtype == B.dtype, "A_Scale must have the activation dtype")
+        _check(bias is None or (bias.dtype == B.dtype and bias.numel() == m), "bias must be [1, m] of the activation dtype")
+        _w4_tensors(((A, "A"), (A_Scale, "A_Scale"), (B, "B"), (A_Zero, "A_Zero"), (bias, "bias")), B.device)
+        lib = _lib.load()
+        plan = _plans[key] = (B.size(0), m, k, group, _KIND[B.dtype], lib.mlk_gemm_w4_workspace_bytes(B.size(0), m, k),
+                              lib.mlk_gemm_counter_bytes(), lib.mlk_gemm_layout_a_w4)
+    n, m, k, group, kind, ws_need, counter_bytes, fn = plan
+    with _OnDevice(B):
+        if B.data_ptr() & 15:
+            B = B.clone()
+        C = torch.empty((n, m), dtype=B.dtype, device=B.device)
+        stream = _stream_of(B)
+        ws_ptr = ws_len = 0
+        if ws_need:
+            ws = _gemm_pool.get(B.device, stream, ws_need, counter_bytes)
+            ws_ptr, ws_len = ws.data_ptr(), ws.numel()
+        rc = fn(A.data_ptr(), A_Scale.data_ptr(), _ptr(A_Zero), B.data_ptr(), C.data_ptr(), n, m, k, group, kind, float(alpha), _ptr(bias), ws_ptr,
+                ws_len, stream)
+        if rc != 0:
+            _lib.check(rc, what)
+    return C
+
+
+def gemm_layoutA_w4(A, A_Scale, B, A_Zero=None, alpha=1, beta=0, bias=None):
+    """C[n, m] = alpha * B[n, k] . W^T (+ bias) with 4-bit weights W = s (q - z) from `pack_layout_a_w4`; any n >= 0, m % 16 == 0,
+    k % 128 == 0.  fp32 sums, one rounding at the end, no weight rounded.  A row of B that holds an infinity gives NaN."""
+    return _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, "gemm_layoutA_w4")
+
+
+def gemv_layoutA_w4(A, A_Scale, B, A_Zero=None, alpha=1, beta=0, bias=None):
+    """The same for one token: B [1, k]."""
+    _check(B.dim() == 2 and B.size(0) == 1, "B must be a vector")
+    return _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, "gemv_layoutA_w4")
+
+
 # ----------------------------------------------------------------------- MoE
 def fused_routing_gate(gating_output, score_fun, batch_size, hidden_size, n_groups, topK_groups, experts_ids,
                        selected_experts_weights, topK, load_balance_bias=None, renormalize=False):
@@ -809,5 +952,5 @@ __all__ = [
     "routing_gate", "experts_compute", "fused_routing_gate",
     "batched_routed_activation_indexed_to_expert_block_indexed", "fused_experts_compute",
     "pack_layout_a", "unpack_layout_a", "experts_compute_raw", "release_workspaces", "workspace_bytes_held",
-    "fused_moe_raw",
+    "fused_moe_raw", "pack_layout_a_w4", "unpack_layout_a_w4", "gemm_layoutA_w4", "gemv_layoutA_w4",
 ]
