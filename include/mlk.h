@@ -41,6 +41,7 @@ extern "C" {
 #define MLK_F16 0
 #define MLK_BF16 1
 #define MLK_FP8_E4M3 2 /* soft-FP8 weights: one e4m3 byte per element */
+#define MLK_F32 3      /* router logits of the balance loss only */
 
 /* output placement of the narrow GeMM */
 #define MLK_C_ROWMAJOR 0 /* C[M, N]                               */
@@ -359,6 +360,42 @@ int mlk_moe_plan(int n_tokens, int n_experts, int topk, int hidden, int inter, i
 /* The same for a workspace of that size (with mlk_moe_workspace_bytes() of scratch: what a call of up to 256 tokens runs). */
 int mlk_moe_pass_plan(int n_tokens, int n_experts, int topk, int hidden, int inter, int w_kind, size_t workspace_bytes,
                       int32_t *out);
+
+/* Expert compute over 4-bit weights from a routing decision: y[t] = T(sum over the token's pairs of weight * W2[e] . (SiLU(gate) * up)),
+ * gate and up from W1[e] . x[t], fp32 sums, the SiLU intermediate rounded to the activations' kind.  w1 [E, 2I, H] and w2 [E, H, I], each
+ * expert packed by mlk_pack_layout_a_w4 / mlk_pack_scales_w4 (batch = E), of one group size G = 32, 64 or a multiple of 128 that divides H
+ * and I; w1_zero and w2_zero both or neither.  topk_ids int32 [T*K], ids outside 0..n_router_experts-1 are dropped; experts_map int32
+ * [n_router_experts] or NULL (n_router_experts == n_experts): -1 drops the pair.  topk_weights [T*K] of x_kind.  y is overwritten, a token
+ * without experts here gets zeros.  H % 128 == 0, I % 128 == 0, E <= 256, K <= 32.  w1, w2, x, y and workspace on 16 bytes, scales on 8, zero
+ * points on 4.  workspace: at least mlk_experts_w4_workspace_bytes(), no initialisation. */
+int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_zero, const void *w2, const void *w2_scale, const void *w2_zero,
+                         const void *x, int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter, int group, int x_kind,
+                         const int32_t *topk_ids, const void *topk_weights, const int32_t *experts_map, void *y, void *workspace,
+                         size_t workspace_bytes, void *stream);
+size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int hidden, int inter);
+
+/* ------------------------------------------------------------- router balance */
+
+/* counts[e] += number of routed pairs (t, k) with topk_ids[t, k] == e and token_mask[t] != 0 (NULL: every token); ids outside
+ * 0..n_experts-1 count nowhere.  counts int32 [n_experts], n_experts <= 256. */
+int mlk_expert_counts(const int32_t *topk_ids, const uint8_t *token_mask, int n_tokens, int topk, int n_experts, int32_t *counts, void *stream);
+
+/* Balance loss of a router, logits [T, E] of x_kind (MLK_F16, MLK_BF16 or MLK_F32):
+ *   loss = coef * mean over the sequences with a valid token of E * sum over e of (c[e] / (K n)) * (P[e] / n)
+ * with n valid tokens of the sequence (token_mask != 0; NULL: all), c[e] of their pairs routed to e, P[e] the sum of their
+ * probabilities: softmax of the logits (score_fun 0) or sigmoids over their sum (1).  A row of logits that are all -inf has no
+ * probability anywhere.  cu_seqlens int32 [n_seq + 1], non-decreasing: tokens cu[s] .. cu[s+1]-1 are sequence s, rows before the first and behind
+ * the last one do not count; NULL with n_seq = 1: all tokens are one sequence.  loss fp32 [1]; counts int32 [E]: all valid tokens' pairs;
+ * share fp32 [n_seq, E]: dloss/dP, which the gradient takes.  Results do not depend on the order in which workgroups run.
+ * workspace: mlk_balance_workspace_bytes(), on 16 bytes, its first mlk_balance_counter_bytes() zero before the first call (left zero). */
+int mlk_balance_loss(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, int topk, const int32_t *topk_ids,
+                     const uint8_t *token_mask, const int32_t *cu_seqlens, int n_seq, float coef, float *loss, int32_t *counts, float *share,
+                     void *workspace, size_t workspace_bytes, void *stream);
+size_t mlk_balance_workspace_bytes(int n_tokens, int n_experts, int n_seq);
+size_t mlk_balance_counter_bytes(void);
+/* dlogits [T, E] of x_kind = grad[0] * dloss/dlogits, zeros where a token does not count; the counts are constants. */
+int mlk_balance_loss_grad(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, const uint8_t *token_mask,
+                          const int32_t *cu_seqlens, int n_seq, const float *share, const float *grad, void *dlogits, void *stream);
 
 #ifdef __cplusplus
 }

@@ -47,6 +47,15 @@ SIGNATURES = {
     "mlk_gemm_layout_a_w4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                      c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mlk_gemm_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "mlk_fused_experts_w4": (c_int, [c_void_p] * 7 + [c_int] * 8 + [c_void_p] * 5 + [c_size_t, c_void_p]),
+    "mlk_experts_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "mlk_expert_counts": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "mlk_balance_loss": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_float,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mlk_balance_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "mlk_balance_counter_bytes": (c_size_t, []),
+    "mlk_balance_loss_grad": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                      c_void_p, c_void_p]),
     "mlk_fused_routing_gate": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
                                        c_void_p, c_void_p, c_void_p]),
     "mlk_moe_align_tokens": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -1,0 +1,491 @@
+// Per-expert counts of a routing decision, and the balance loss of a router with its gradient.
+//
+// For sequences s with valid tokens V_s (not masked), n_s = |V_s| > 0, S' such sequences, K picks a token and E experts:
+//   c[s,e] = pairs of V_s routed to e,   P[s,e] = sum over V_s of p[t,e],   g[s,e] = coef / S' * E / (K n_s^2) * c[s,e],   loss = sum g P
+// with p = softmax(x) or sigmoid(x) / sum sigmoid(x); the counts are constants of the differentiation, so dloss/dp[t,e] = g[s(t),e] and
+//   softmax  dx = p (g - sum p g),      sigmoid  dx = p (1 - sigmoid) (g - sum p g).
+// A row whose probabilities sum to nothing (all logits -inf) has p = 0.
+//
+// Forward: a workgroup takes a chunk of consecutive tokens and walks the sequences that it meets; E / 4 lanes hold a token, four experts each,
+// so that a wave takes 64 / lanes tokens at a time.  Its sums for (chunk c, sequence s) go to slot c + s: going through the tokens either the
+// chunk or the sequence moves on, so no two share a slot.  A second launch adds the slots of a sequence in order, for 64 experts a workgroup; the last
+// workgroup adds their shares of the loss.  No floating-point atomics: the results do not depend on the order in which workgroups run.
+// Backward: the same walk, the logits are read again and their gradient written.
+// Bound by the logits' bytes; below about a thousand tokens by the two launches.
+#include <algorithm>
+
+#include "mlk_common.cuh"
+
+namespace mlk {
+
+constexpr int kBalThreads = 256;
+constexpr int kBalExperts = 256;
+constexpr int kBalCounterBytes = 256;
+
+struct BalanceArgs {
+    const void *logits;
+    const int32_t *ids;
+    const uint8_t *mask;         // null: every token counts
+    const int32_t *cu;           // [S + 1] or null: one sequence
+    int T, E, K, S, score_fun, vec;
+    int chunk, chunks;
+    float coef;
+    float *P;                    // [chunks + S][E]
+    int32_t *cnt;                // [chunks + S][E]
+    int32_t *valid;              // [chunks + S]
+    float *part;                 // [S * expert blocks]
+    int32_t *ticket;             // zero between calls
+    float *loss, *share;         // [1], [S][E]
+    int32_t *counts;             // [E]
+    const float *grad;           // [1]
+    void *dlogits;
+};
+
+struct BalF32 {
+    typedef f32x4 V4;
+    __device__ static __forceinline__ void unpack(const f32x4 &v, float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = v[i];
+    }
+    __device__ static __forceinline__ f32x4 pack(const float (&x)[4]) { return f32x4{x[0], x[1], x[2], x[3]}; }
+    __device__ static __forceinline__ float load(const void *p, size_t i) { return reinterpret_cast<const float *>(p)[i]; }
+    __device__ static __forceinline__ void store(void *p, size_t i, float v) { reinterpret_cast<float *>(p)[i] = v; }
+};
+template <class T>
+struct Bal16 {
+    typedef u32x2 V4;
+    __device__ static __forceinline__ void unpack(const u32x2 &v, float (&x)[4]) {
+        x[0] = T::to_f32(v[0] & 0xffffu);
+        x[1] = T::to_f32(v[0] >> 16);
+        x[2] = T::to_f32(v[1] & 0xffffu);
+        x[3] = T::to_f32(v[1] >> 16);
+    }
+    __device__ static __forceinline__ u32x2 pack(const float (&x)[4]) { return u32x2{T::from_f32x2(x[0], x[1]), T::from_f32x2(x[2], x[3])}; }
+    __device__ static __forceinline__ float load(const void *p, size_t i) { return T::to_f32(reinterpret_cast<const uint16_t *>(p)[i]); }
+    __device__ static __forceinline__ void store(void *p, size_t i, float v) { reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)T::from_f32(v); }
+};
+
+template <class L>
+__device__ __forceinline__ void bal_load(const BalanceArgs &p, int t, int e0, float (&x)[4]) {
+    const size_t at = (size_t)t * p.E + e0;
+    if (p.vec) {
+        if (e0 < p.E) L::unpack(*reinterpret_cast<const typename L::V4 *>(reinterpret_cast<const char *>(p.logits) + at * (sizeof(typename L::V4) / 4)), x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (e0 + i < p.E) x[i] = L::load(p.logits, at + i);
+    }
+}
+
+template <int LPT>
+__device__ __forceinline__ float bal_sum(float v) {
+#pragma unroll
+    for (int m = 1; m < LPT; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+template <int LPT>
+__device__ __forceinline__ float bal_max(float v) {
+#pragma unroll
+    for (int m = 1; m < LPT; m <<= 1) v = fmaxf(v, __shfl_xor(v, m));
+    return v;
+}
+
+// Probabilities of one token, four experts a lane (0 beyond the last expert); `sig`: the sigmoids.
+template <int LPT>
+__device__ __forceinline__ void bal_probs(const BalanceArgs &p, int e0, const float (&x)[4], float (&pr)[4], float (&sig)[4]) {
+    float sum = 0.f;
+    if (p.score_fun == 0) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (e0 + i < p.E) m = fmaxf(m, x[i]);
+        m = bal_max<LPT>(m);
+        if (m == -INFINITY) m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sig[i] = 0.f;
+            pr[i] = e0 + i < p.E ? expf(x[i] - m) : 0.f;
+            sum += pr[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sig[i] = e0 + i < p.E ? 1.f / (1.f + expf(-x[i])) : 0.f;
+            pr[i] = sig[i];
+            sum += pr[i];
+        }
+    }
+    sum = bal_sum<LPT>(sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pr[i] *= inv;
+}
+
+// First sequence that ends behind token t (S if there is none).
+__device__ __forceinline__ int bal_first(const BalanceArgs &p, int t) {
+    if (!p.cu) return 0;
+    int lo = 0, hi = p.S;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (p.cu[mid + 1] > t) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+__device__ __forceinline__ void bal_range(const BalanceArgs &p, int s, int &a, int &b) {
+    a = p.cu ? max(p.cu[s], 0) : 0;
+    b = p.cu ? min(p.cu[s + 1], p.T) : p.T;
+}
+
+template <class L, int LPT>
+__global__ void __launch_bounds__(kBalThreads) balance_partial_kernel(BalanceArgs p) {
+    constexpr int ROWS = kBalThreads / LPT;                 // tokens at a time
+    __shared__ float sums[ROWS * LPT * 4];
+    __shared__ int32_t cnt[kBalExperts];
+    __shared__ int32_t valid;
+    const int tid = threadIdx.x, row = tid / LPT, e0 = (tid % LPT) * 4;
+    const int c0 = blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, p.T);
+    if (blockIdx.x == 0)
+        for (int e = tid; e < p.E; e += kBalThreads) p.counts[e] = 0;        // the second launch adds to them
+    for (int s = bal_first(p, c0); s < p.S; ++s) {
+        int a, b;
+        bal_range(p, s, a, b);
+        if (a >= c1) break;
+        a = max(a, c0);
+        b = min(b, c1);
+        if (a >= b) continue;
+        for (int e = tid; e < p.E; e += kBalThreads) cnt[e] = 0;
+        if (tid == 0) valid = 0;
+        __syncthreads();
+        for (int i = a * p.K + tid; i < b * p.K; i += kBalThreads) {
+            const int e = p.ids[i];
+            if (e >= 0 && e < p.E && (!p.mask || p.mask[i / p.K])) atomicAdd(&cnt[e], 1);
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        int n = 0;
+        for (int t = a + row; t < b; t += ROWS) {
+            if (p.mask && !p.mask[t]) continue;             // the lanes of a token agree
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, pr[4], sig[4];
+            bal_load<L>(p, t, e0, x);
+            bal_probs<LPT>(p, e0, x, pr, sig);
+            ++n;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += pr[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[row * LPT * 4 + e0 + i] = sum[i];
+        if (e0 == 0 && n) atomicAdd(&valid, n);
+        __syncthreads();
+        const size_t slot = (size_t)blockIdx.x + s;
+        for (int e = tid; e < p.E; e += kBalThreads) {
+            float v = 0.f;
+            for (int r = 0; r < ROWS; ++r) v += sums[r * LPT * 4 + e];
+            p.P[slot * p.E + e] = v;
+            p.cnt[slot * p.E + e] = cnt[e];
+        }
+        if (tid == 0) p.valid[slot] = valid;
+        __syncthreads();
+    }
+}
+
+// Slots of sequence s: those of the chunks from c_first to c_last, none where it is empty.
+__device__ __forceinline__ void bal_slots(const BalanceArgs &p, int s, int &first, int &n) {
+    int a, b;
+    bal_range(p, s, a, b);
+    first = s + (a < b ? a / p.chunk : 0);
+    n = a < b ? s + (b - 1) / p.chunk - first + 1 : 0;
+}
+
+// grid (blocks of 64 experts, sequences), 16 waves: wave w adds slots w, w + 16, ... of its 64 experts.
+__global__ void __launch_bounds__(1024) balance_reduce_kernel(BalanceArgs p) {
+    __shared__ float psum[16][64];
+    __shared__ int32_t csum[16][64];
+    __shared__ int32_t nonempty, mine;
+    __shared__ int last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, s = blockIdx.y, e = blockIdx.x * 64 + lane;
+    if (tid == 0) nonempty = mine = 0;
+    __syncthreads();
+    // how many sequences have a valid token: a wave per sequence, or with many a thread
+    if (p.S < 64) {
+        for (int q = wave; q < p.S; q += 16) {
+            int first, n, v = 0;
+            bal_slots(p, q, first, n);
+            for (int i = lane; i < n; i += 64) v += p.valid[first + i];
+            for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+            if (lane == 0 && v) atomicAdd(&nonempty, 1);
+            if (lane == 0 && q == s) mine = v;
+        }
+    } else {
+        for (int q = tid; q < p.S; q += 1024) {
+            int first, n, v = 0;
+            bal_slots(p, q, first, n);
+            for (int i = 0; i < n; ++i) v += p.valid[first + i];
+            if (v) atomicAdd(&nonempty, 1);
+            if (q == s) mine = v;
+        }
+    }
+    int first, n;
+    bal_slots(p, s, first, n);
+    float ps = 0.f;
+    int32_t cs = 0;
+    if (e < p.E) {
+#pragma unroll 4
+        for (int i = wave; i < n; i += 16) {
+            ps += p.P[(size_t)(first + i) * p.E + e];
+            cs += p.cnt[(size_t)(first + i) * p.E + e];
+        }
+    }
+    psum[wave][lane] = ps;
+    csum[wave][lane] = cs;
+    __syncthreads();
+    float share_of_loss = 0.f;
+    if (wave == 0) {
+        for (int w = 1; w < 16; ++w) {
+            ps += psum[w][lane];
+            cs += csum[w][lane];
+        }
+        const float nv = (float)mine;
+        const float g = mine > 0 ? p.coef * ((float)p.E / ((float)p.K * (float)nonempty)) * ((float)cs / nv) / nv : 0.f;
+        if (e < p.E) {
+            p.share[(size_t)s * p.E + e] = g;
+            if (cs) atomicAdd(&p.counts[e], cs);
+            share_of_loss = g * ps;
+        }
+        share_of_loss = bal_sum<64>(share_of_loss);
+        // agent-scope stores: the caches of the XCDs are not coherent for ordinary ones
+        if (lane == 0) {
+            __hip_atomic_store(&p.part[(size_t)s * gridDim.x + blockIdx.x], share_of_loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __builtin_amdgcn_s_waitcnt(0);
+            const int total = gridDim.x * gridDim.y;
+            const int before = __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = before == total - 1;
+            if (last) __hip_atomic_store(p.ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    __syncthreads();
+    if (!last || wave) return;
+    const int total = gridDim.x * gridDim.y;
+    float v = 0.f;
+    for (int i = lane; i < total; i += 64) v += __hip_atomic_load(&p.part[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    v = bal_sum<64>(v);
+    if (lane == 0) *p.loss = v;
+}
+
+template <class L, int LPT>
+__global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(BalanceArgs p) {
+    constexpr int ROWS = kBalThreads / LPT;
+    const int tid = threadIdx.x, row = tid / LPT, e0 = (tid % LPT) * 4;
+    const int c0 = blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, p.T);
+    const float up = *p.grad;
+    int s = bal_first(p, c0);
+    for (int t = c0 + row; t < c1; t += ROWS) {
+        bool counts = true;
+        if (p.cu) {
+            while (s < p.S && p.cu[s + 1] <= t) ++s;
+            counts = s < p.S && p.cu[s] <= t;
+        }
+        if (p.mask && !p.mask[t]) counts = false;
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        if (counts) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, pr[4], sig[4], g[4] = {0.f, 0.f, 0.f, 0.f};
+            bal_load<L>(p, t, e0, x);
+            bal_probs<LPT>(p, e0, x, pr, sig);
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (e0 + i < p.E) g[i] = p.share[(size_t)s * p.E + e0 + i];
+                dot = fmaf(pr[i], g[i], dot);
+            }
+            dot = bal_sum<LPT>(dot);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] = pr[i] * (1.f - sig[i]) * (g[i] - dot) * up;
+        }
+        const size_t at = (size_t)t * p.E + e0;
+        if (p.vec) {
+            if (e0 < p.E) *reinterpret_cast<typename L::V4 *>(reinterpret_cast<char *>(p.dlogits) + at * (sizeof(typename L::V4) / 4)) = L::pack(d);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e0 + i < p.E) L::store(p.dlogits, at + i, d[i]);
+        }
+    }
+}
+
+// counts[e] += pairs routed to e; integer atomics: any order gives the same sums.
+__global__ void __launch_bounds__(256) expert_counts_kernel(const int32_t *__restrict__ ids, const uint8_t *__restrict__ mask, int64_t pairs, int K, int E,
+                                                            int32_t *__restrict__ counts) {
+    __shared__ int32_t cnt[kBalExperts];
+    for (int e = threadIdx.x; e < E; e += 256) cnt[e] = 0;
+    __syncthreads();
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pairs; i += (int64_t)gridDim.x * 256) {
+        const int e = ids[i];
+        if (e >= 0 && e < E && (!mask || mask[i / K])) atomicAdd(&cnt[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += 256)
+        if (cnt[e]) atomicAdd(&counts[e], cnt[e]);
+}
+
+// -------------------------------------------------------------------------------------------------------------------- host
+// Tokens of a chunk: enough for a workgroup of every CU, no fewer than a few passes of a workgroup.
+static int balance_chunk(int T) {
+    const int c = (T + 511) / 512;
+    return c < 32 ? 32 : (c + 31) / 32 * 32;
+}
+
+struct BalanceScratch {
+    int32_t *ticket, *cnt, *valid;
+    float *P, *part;
+};
+static size_t balance_carve(uint8_t *base, int T, int E, int S, BalanceScratch *out) {
+    const int chunk = balance_chunk(T);
+    const size_t slots = (size_t)(T + chunk - 1) / chunk + S;
+    size_t off = kBalCounterBytes;
+    auto take = [&](size_t bytes) {
+        uint8_t *ptr = base ? base + off : nullptr;
+        off = (off + bytes + 255) / 256 * 256;
+        return ptr;
+    };
+    BalanceScratch b;
+    b.ticket = (int32_t *)base;
+    b.P = (float *)take(slots * E * 4);
+    b.cnt = (int32_t *)take(slots * E * 4);
+    b.valid = (int32_t *)take(slots * 4);
+    b.part = (float *)take((size_t)S * ((E + 63) / 64) * 4);
+    if (out) *out = b;
+    return off;
+}
+
+static int balance_check(const void *logits, int x_kind, int score_fun, int T, int E, const int32_t *cu, int n_seq) {
+    MLK_REQUIRE(x_kind == MLK_F16 || x_kind == MLK_BF16 || x_kind == MLK_F32, "balance: logits must be fp16, bf16 or fp32");
+    MLK_REQUIRE(score_fun == 0 || score_fun == 1, "balance: score function must be 0 (softmax) or 1 (sigmoid)");
+    MLK_REQUIRE(T >= 0 && E >= 1 && E <= kBalExperts, "balance: 1..256 experts");
+    MLK_REQUIRE(cu ? n_seq >= 0 && n_seq <= 65535 : n_seq == 1, "balance: 0..65535 sequences, one without cu_seqlens");
+    MLK_REQUIRE(T == 0 || logits, "balance: null pointer");
+    return MLK_OK;
+}
+
+// Rows of four experts can be moved whole.
+static int balance_vec(const void *p, int x_kind, int E) { return E % 4 == 0 && ((uintptr_t)p & (x_kind == MLK_F32 ? 15 : 7)) == 0; }
+
+template <class L>
+static void balance_launch(const BalanceArgs &a, bool grad, hipStream_t s) {
+#define MLK_BAL(LPT)                                                                           \
+    do {                                                                                       \
+        if (grad) balance_grad_kernel<L, LPT><<<a.chunks, kBalThreads, 0, s>>>(a);             \
+        else balance_partial_kernel<L, LPT><<<a.chunks, kBalThreads, 0, s>>>(a);               \
+    } while (0)
+    if (a.E <= 16) MLK_BAL(4);
+    else if (a.E <= 32) MLK_BAL(8);
+    else if (a.E <= 64) MLK_BAL(16);
+    else if (a.E <= 128) MLK_BAL(32);
+    else MLK_BAL(64);
+#undef MLK_BAL
+}
+static void balance_launch_kind(const BalanceArgs &a, int x_kind, bool grad, hipStream_t s) {
+    if (x_kind == MLK_F32) balance_launch<BalF32>(a, grad, s);
+    else if (x_kind == MLK_F16) balance_launch<Bal16<F16>>(a, grad, s);
+    else balance_launch<Bal16<BF16>>(a, grad, s);
+}
+
+__global__ void balance_nothing_kernel(float *loss, int32_t *counts, int E) {
+    if (threadIdx.x == 0) *loss = 0.f;
+    for (int e = threadIdx.x; e < E; e += 256) counts[e] = 0;
+}
+
+}  // namespace mlk
+
+using namespace mlk;
+
+extern "C" {
+
+int mlk_expert_counts(const int32_t *topk_ids, const uint8_t *token_mask, int n_tokens, int topk, int n_experts, int32_t *counts, void *stream) {
+    MLK_REQUIRE(n_tokens >= 0 && topk >= 1, "expert_counts: negative token count, or no picks");
+    MLK_REQUIRE(n_experts >= 1 && n_experts <= kBalExperts, "expert_counts: 1..256 experts");
+    if (n_tokens == 0) return MLK_OK;
+    MLK_REQUIRE(topk_ids && counts, "expert_counts: null pointer");
+    const int64_t pairs = (int64_t)n_tokens * topk;
+    const int64_t wgs = std::min<int64_t>((pairs + 1023) / 1024, 256);
+    expert_counts_kernel<<<(int)wgs, 256, 0, (hipStream_t)stream>>>(topk_ids, token_mask, pairs, topk, n_experts, counts);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
+}
+
+size_t mlk_balance_workspace_bytes(int n_tokens, int n_experts, int n_seq) {
+    if (n_tokens < 0 || n_experts < 1 || n_experts > kBalExperts || n_seq < 0) return 0;
+    return balance_carve(nullptr, n_tokens, n_experts, n_seq, nullptr);
+}
+size_t mlk_balance_counter_bytes(void) { return kBalCounterBytes; }
+
+int mlk_balance_loss(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, int topk, const int32_t *topk_ids,
+                     const uint8_t *token_mask, const int32_t *cu_seqlens, int n_seq, float coef, float *loss, int32_t *counts, float *share,
+                     void *workspace, size_t workspace_bytes, void *stream) {
+    const int rc = balance_check(logits, x_kind, score_fun, n_tokens, n_experts, cu_seqlens, n_seq);
+    if (rc != MLK_OK) return rc;
+    MLK_REQUIRE(topk >= 1 && (int64_t)n_tokens * topk < (1ll << 31), "balance: at least one pick, fewer than 2^31 routed pairs");
+    MLK_REQUIRE(loss && counts && (n_seq == 0 || share), "balance: null pointer");
+    hipStream_t s = (hipStream_t)stream;
+    if (n_tokens == 0 || n_seq == 0) {
+        balance_nothing_kernel<<<1, 256, 0, s>>>(loss, counts, n_experts);
+        MLK_LAUNCH_CHECK();
+        return MLK_OK;
+    }
+    MLK_REQUIRE(topk_ids && workspace && ((uintptr_t)workspace & 15) == 0, "balance: null pointer, or workspace off 16 bytes");
+    if (workspace_bytes < mlk_balance_workspace_bytes(n_tokens, n_experts, n_seq)) return fail(MLK_ERR_WORKSPACE, "balance: workspace too small");
+    BalanceArgs a = {};
+    BalanceScratch w;
+    balance_carve((uint8_t *)workspace, n_tokens, n_experts, n_seq, &w);
+    a.logits = logits;
+    a.ids = topk_ids;
+    a.mask = token_mask;
+    a.cu = cu_seqlens;
+    a.T = n_tokens;
+    a.E = n_experts;
+    a.K = topk;
+    a.S = n_seq;
+    a.score_fun = score_fun;
+    a.vec = balance_vec(logits, x_kind, n_experts);
+    a.chunk = balance_chunk(n_tokens);
+    a.chunks = (n_tokens + a.chunk - 1) / a.chunk;
+    a.coef = coef;
+    a.P = w.P;
+    a.cnt = w.cnt;
+    a.valid = w.valid;
+    a.part = w.part;
+    a.ticket = w.ticket;
+    a.loss = loss;
+    a.share = share;
+    a.counts = counts;
+    balance_launch_kind(a, x_kind, false, s);
+    MLK_LAUNCH_CHECK();
+    balance_reduce_kernel<<<dim3((n_experts + 63) / 64, n_seq), 1024, 0, s>>>(a);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
+}
+
+int mlk_balance_loss_grad(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, const uint8_t *token_mask,
+                          const int32_t *cu_seqlens, int n_seq, const float *share, const float *grad, void *dlogits, void *stream) {
+    const int rc = balance_check(logits, x_kind, score_fun, n_tokens, n_experts, cu_seqlens, n_seq);
+    if (rc != MLK_OK) return rc;
+    if (n_tokens == 0) return MLK_OK;
+    MLK_REQUIRE((n_seq == 0 || share) && grad && dlogits, "balance: null pointer");
+    BalanceArgs a = {};
+    a.logits = logits;
+    a.mask = token_mask;
+    a.cu = cu_seqlens;
+    a.T = n_tokens;
+    a.E = n_experts;
+    a.S = n_seq;
+    a.score_fun = score_fun;
+    a.vec = balance_vec(logits, x_kind, n_experts) && balance_vec(dlogits, x_kind, n_experts);
+    a.chunk = balance_chunk(n_tokens);
+    a.chunks = (n_tokens + a.chunk - 1) / a.chunk;
+    a.share = const_cast<float *>(share);
+    a.grad = grad;
+    a.dlogits = dlogits;
+    balance_launch_kind(a, x_kind, true, (hipStream_t)stream);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
+}
+
+}  // extern "C"

@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(1024) moe_align_kernel(const int32_t *__restri
                                                          int32_t *__restrict__ padded_blocks,
                                                          int32_t *__restrict__ experts_ids, int max_blocks,
                                                          MoeTask *__restrict__ tasks, int32_t *__restrict__ n_tasks,
-                                                         int cb_max, int cb_unit, int32_t *__restrict__ queues) {
+                                                         int cb_max, int cb_unit, int32_t *__restrict__ queues, int id_limit) {
     constexpr int NW = 16;
     __shared__ int cnt[NW][kMaxExperts];   // per-wave counts, then per-wave write cursors
     __shared__ int start[kMaxExperts + 1]; // padded exclusive prefix
@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(1024) moe_align_kernel(const int32_t *__restri
     auto local_expert = [&](int i) -> int {
         if (i >= n_pairs) return -1;
         int e = topk_ids[i];
+        if (e < 0 || e >= id_limit) return -1;
         if (experts_map) e = experts_map[e];
         return (e >= 0 && e < E) ? e : -1;
     };
@@ -417,6 +418,15 @@ __global__ void __launch_bounds__(1024) moe_align_kernel(const int32_t *__restri
         wave_lds_sync();
         if (pos >= 0) sorted_ids[pos] = i;
     });
+}
+
+// The alignment for the expert layers of other files: tasks of up to cb_max blocks; ids outside 0 .. id_limit - 1 are dropped.
+int launch_moe_align(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
+                     int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, hipStream_t s) {
+    moe_align_kernel<<<1, 1024, 0, s>>>(topk_ids, n_pairs, E, experts_map, sorted, cumsum, padded, experts_ids, (n_pairs + E * 15 + 15) / 16, tasks,
+                                        n_tasks, cb_max, 0, nullptr, id_limit);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
 }
 
 // ------------------------------------------------------------ grouped GeMMs
@@ -1673,7 +1683,7 @@ extern "C" int mlk_moe_align_tokens(const int32_t *topk_ids, int n_pairs, int n_
     const int max_blocks = (n_pairs + n_experts * 15 + 15) / 16;
     moe_align_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(topk_ids, n_pairs, n_experts, experts_map, sorted_token_ids,
                                                           cumsum_buffer, padded_num_blocks, experts_ids, max_blocks,
-                                                          nullptr, nullptr, 1, 0, nullptr);
+                                                          nullptr, nullptr, 1, 0, nullptr, INT_MAX);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }
@@ -1841,7 +1851,7 @@ static int experts_compute_impl(const void *w1, const void *w2, const void *x, i
         if (!inline_align) {
             moe_align_kernel<<<1, 1024, 0, s>>>(topk_ids + (size_t)t0 * topk, n_pairs, n_experts, experts_map,
                                                 ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, max_blocks, ws.tasks,
-                                                ws.n_tasks, cb, ps.cb_unit, ps.wide ? ws.queues : nullptr);
+                                                ws.n_tasks, cb, ps.cb_unit, ps.wide ? ws.queues : nullptr, INT_MAX);
             MLK_LAUNCH_CHECK();
         }
         MoeArgs a;

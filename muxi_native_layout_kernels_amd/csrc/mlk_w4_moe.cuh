@@ -1,0 +1,307 @@
+// Expert layers over 4-bit weights: grouped gate/up product with SiLU(gate) * up, grouped down product, weighted sum.
+//
+// Several tokens: the routed pairs are brought into expert order in blocks of 16 (moe_align_kernel); a task is up to TT blocks of one expert, which
+// share one pass over its weights.  The intermediate is kept row-major [slot][I] in the activations' type (slot = place in the order), the
+// weighted products of the down projection in fp32 [pair][H], and a last launch adds a token's pairs in the order of its picks.
+// One token: its picks are the tasks, no alignment; the down projection's waves deal the picks among themselves and write the output at once.
+#pragma once
+
+#include "mlk_moe_args.cuh"
+#include "mlk_w4.cuh"
+
+namespace mlk {
+
+struct W4MoeArgs {
+    W4Matrix w1, w2;             // of expert 0
+    const uint16_t *X;           // [T][H]
+    uint16_t *Y;                 // [T][H]
+    const int32_t *ids;          // [T * K]
+    const uint16_t *wts;         // [T * K]
+    const int32_t *map;          // [id_limit] or null
+    int id_limit, T, K, H, I, E, n_pairs;
+    int blocks1, blocks2;        // blocks of scales of a row group of w1, of w2
+    uint32_t inv;                // w4_inverse() of the tiles of a group
+    const int32_t *sorted;
+    const MoeTask *tasks;
+    const int32_t *n_tasks;
+    uint16_t *hbuf;              // [slot][I]
+    float *obuf;                 // [pair][H]
+};
+
+// Local expert of a pair, -1: dropped.
+__device__ __forceinline__ int w4_expert(const W4MoeArgs &p, int pair) {
+    int e = p.ids[pair];
+    if (e < 0 || e >= p.id_limit) return -1;
+    if (p.map) e = p.map[e];
+    return e >= 0 && e < p.E ? e : -1;
+}
+template <int GS>
+__device__ __forceinline__ W4Matrix w4_of_expert(const W4Matrix &m, int e, int rows, int k, int blocks) {
+    const size_t entries = (size_t)e * rows * blocks * (4 / GS);
+    return W4Matrix{m.codes + (size_t)e * rows * (k >> 1), m.scales + entries, m.zeros + entries};
+}
+
+__host__ __device__ constexpr int w4_moe_ring(int tt, int r) { return tt == 1 ? (r <= 2 ? 4 : 2) : (tt * r <= 8 && tt < 4 ? 2 : 1); }
+__host__ __device__ constexpr int w4_moe1_ring(int r) { return r <= 4 ? 4 : 2; }
+
+// Rows of a gate/up workgroup: R / 2 row groups of gate, then the same of up.
+template <int GS, int R>
+__device__ __forceinline__ void w4_gate_up_rows(W4Rows<R> &rows, const W4MoeArgs &p, int e, int rg0) {
+    const W4Matrix m = w4_of_expert<GS>(p.w1, e, 2 * p.I, p.H, p.blocks1);
+#pragma unroll
+    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r % (R / 2) + (r >= R / 2 ? p.I >> 4 : 0), p.H >> 7, p.blocks1);
+}
+
+template <int CELLS>
+__device__ __forceinline__ void w4_park(f32x4 *red, const f32x4 (&acc)[CELLS], int wave, int lane) {
+#pragma unroll
+    for (int c = 0; c < CELLS; ++c) red[(wave * CELLS + c) * 64 + lane] = acc[c];
+}
+template <int CELLS>
+__device__ __forceinline__ f32x4 w4_fold(const f32x4 *red, int c, int waves, int lane) {
+    f32x4 v = red[c * 64 + lane];
+    for (int w = 1; w < waves; ++w) v += red[(w * CELLS + c) * 64 + lane];
+    return v;
+}
+
+// ---------------------------------------------------------------------------------------------------------- several tokens
+template <class T, int GS, bool ZP, int TT, int R>
+__global__ void __launch_bounds__(512) w4_moe_gate_up_kernel(W4MoeArgs p) {
+    extern __shared__ f32x4 red[];
+    if ((int)blockIdx.y >= *p.n_tasks) return;
+    const MoeTask task = p.tasks[blockIdx.y];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int o = lane >> 4, r16 = lane & 15, rg0 = blockIdx.x * (R / 2);
+    W4Rows<R> rows;
+    w4_gate_up_rows<GS, R>(rows, p, task.expert, rg0);
+    const uint16_t *xrow[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        const int pair = p.sorted[(task.block0 + min(tt, task.nblocks - 1)) * 16 + r16];
+        xrow[tt] = p.X + (size_t)(pair < p.n_pairs ? pair / p.K : 0) * p.H;
+    }
+    f32x4 acc[R][TT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w4_stream<T, GS, ZP, TT, R, w4_moe_ring(TT, R), false>(acc, rows, xrow, nullptr, wave, p.H >> 7, waves, p.inv, lane, false);
+    constexpr int CELLS = R * TT, HALF = CELLS / 2;
+    w4_park<CELLS>(red, reinterpret_cast<const f32x4(&)[CELLS]>(acc), wave, lane);
+    __syncthreads();
+    for (int c = wave; c < HALF; c += waves) {
+        const int r = c / TT, tt = c - r * TT;
+        if (tt >= task.nblocks) continue;
+        const f32x4 g = w4_fold<CELLS>(red, c, waves, lane), u = w4_fold<CELLS>(red, HALF + c, waves, lane);
+        uint16_t *h = p.hbuf + (size_t)((task.block0 + tt) * 16 + o * 4) * p.I + (rg0 + r) * 16 + r16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[(size_t)i * p.I] = (uint16_t)T::from_f32(silu_mul(g[i], u[i]));
+    }
+}
+
+template <class T, int GS, bool ZP, int TT, int R>
+__global__ void __launch_bounds__(512) w4_moe_down_kernel(W4MoeArgs p) {
+    extern __shared__ f32x4 red[];
+    if ((int)blockIdx.y >= *p.n_tasks) return;
+    const MoeTask task = p.tasks[blockIdx.y];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int o = lane >> 4, r16 = lane & 15, rg0 = blockIdx.x * R;
+    const W4Matrix m = w4_of_expert<GS>(p.w2, task.expert, p.H, p.I, p.blocks2);
+    W4Rows<R> rows;
+#pragma unroll
+    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r, p.I >> 7, p.blocks2);
+    const uint16_t *xrow[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) xrow[tt] = p.hbuf + (size_t)((task.block0 + min(tt, task.nblocks - 1)) * 16 + r16) * p.I;
+    f32x4 acc[R][TT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w4_stream<T, GS, ZP, TT, R, w4_moe_ring(TT, R), false>(acc, rows, xrow, nullptr, wave, p.I >> 7, waves, p.inv, lane, false);
+    constexpr int CELLS = R * TT;
+    w4_park<CELLS>(red, reinterpret_cast<const f32x4(&)[CELLS]>(acc), wave, lane);
+    __syncthreads();
+    for (int c = wave; c < CELLS; c += waves) {
+        const int r = c / TT, tt = c - r * TT;
+        if (tt >= task.nblocks) continue;
+        const f32x4 v = w4_fold<CELLS>(red, c, waves, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int pair = p.sorted[(task.block0 + tt) * 16 + o * 4 + i];
+            if (pair < p.n_pairs) p.obuf[(size_t)pair * p.H + (rg0 + r) * 16 + r16] = T::to_f32(p.wts[pair]) * v[i];
+        }
+    }
+}
+
+// y[t] = T(sum over the token's pairs on this card, in pick order)
+template <class T>
+__global__ void __launch_bounds__(256) w4_moe_combine_kernel(W4MoeArgs p) {
+    const int tok = blockIdx.x;
+    for (int n = (blockIdx.y * 256 + threadIdx.x) * 4; n < p.H; n += gridDim.y * 1024) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < p.K; ++k) {
+            const int pair = tok * p.K + k;
+            if (w4_expert(p, pair) >= 0) sum += *reinterpret_cast<const f32x4 *>(p.obuf + (size_t)pair * p.H + n);
+        }
+        u32x2 out;
+        out[0] = T::from_f32x2(sum[0], sum[1]);
+        out[1] = T::from_f32x2(sum[2], sum[3]);
+        *reinterpret_cast<u32x2 *>(p.Y + (size_t)tok * p.H + n) = out;
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------------- one token
+template <class T, int GS, bool ZP, int R>
+__global__ void __launch_bounds__(512) w4_moe1_gate_up_kernel(W4MoeArgs p) {
+    extern __shared__ f32x4 red[];
+    const int e = w4_expert(p, blockIdx.y);
+    if (e < 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int rg0 = blockIdx.x * (R / 2);
+    W4Rows<R> rows;
+    w4_gate_up_rows<GS, R>(rows, p, e, rg0);
+    u32x4 *xl = reinterpret_cast<u32x4 *>(red);
+    for (int i = threadIdx.x; i < p.H >> 3; i += blockDim.x) xl[i] = ld_global_u32x4(p.X + (size_t)i * 8);
+    const uint16_t *xrow[1] = {nullptr};
+    f32x4 acc[R][1];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w4_stream<T, GS, ZP, 1, R, w4_moe1_ring(R), true>(acc, rows, xrow, xl, wave, p.H >> 7, waves, p.inv, lane, true);
+    __syncthreads();
+    // all sixteen tokens of the block are the same one: lanes 0..15 hold the rows
+    float *part = reinterpret_cast<float *>(red);
+    if (lane < 16)
+#pragma unroll
+        for (int r = 0; r < R; ++r) part[(wave * R + r) * 16 + lane] = acc[r][0][0];
+    __syncthreads();
+    const int i = threadIdx.x;
+    if (i < R / 2 * 16) {
+        float g = 0.f, u = 0.f;
+        for (int w = 0; w < waves; ++w) {
+            g += part[w * R * 16 + i];
+            u += part[w * R * 16 + R / 2 * 16 + i];
+        }
+        p.hbuf[(size_t)blockIdx.y * p.I + rg0 * 16 + i] = (uint16_t)T::from_f32(silu_mul(g, u));
+    }
+}
+
+template <class T, int GS, bool ZP, int R>
+__global__ void __launch_bounds__(512) w4_moe1_down_kernel(W4MoeArgs p) {
+    extern __shared__ f32x4 red[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int r16 = lane & 15, rg0 = blockIdx.x * R;
+    // wave w takes picks w % lanes_of, w % lanes_of + lanes_of, ... and of each the tiles of its place among the waves that share it
+    const int side = min(p.K, waves), mine = wave % side, place = wave / side, sharing = (waves - mine + side - 1) / side;
+    float sum[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) sum[r] = 0.f;
+    for (int k = mine; k < p.K; k += side) {
+        const int e = w4_expert(p, k);
+        if (e < 0) continue;
+        const W4Matrix m = w4_of_expert<GS>(p.w2, e, p.H, p.I, p.blocks2);
+        W4Rows<R> rows;
+#pragma unroll
+        for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r, p.I >> 7, p.blocks2);
+        const uint16_t *xrow[1] = {p.hbuf + (size_t)k * p.I};
+        f32x4 acc[R][1];
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+        w4_stream<T, GS, ZP, 1, R, w4_moe_ring(1, R), false>(acc, rows, xrow, nullptr, place, p.I >> 7, sharing, p.inv, lane, false);
+        const float wt = T::to_f32(p.wts[k]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) sum[r] = fmaf(wt, acc[r][0][0], sum[r]);
+    }
+    float *part = reinterpret_cast<float *>(red);
+    if (lane < 16)
+#pragma unroll
+        for (int r = 0; r < R; ++r) part[(wave * R + r) * 16 + r16] = sum[r];
+    __syncthreads();
+    const int i = threadIdx.x;
+    if (i < R * 16) {
+        float v = 0.f;
+        for (int w = 0; w < waves; ++w) v += part[w * R * 16 + i];
+        p.Y[rg0 * 16 + i] = (uint16_t)T::from_f32(v);
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------------------- host
+template <class K>
+static int w4_moe_lds(K kernel, size_t lds, bool (&ready_on)[64]) {
+    if (lds <= 48 * 1024) return MLK_OK;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+    if (!ready_on[dev & 63]) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 150 * 1024);
+        if (e != hipSuccess) return fail(MLK_ERR_LAUNCH, hipGetErrorString(e));
+        ready_on[dev & 63] = true;
+    }
+    return MLK_OK;
+}
+
+struct W4MoePlan {
+    int tt;                  // blocks of 16 tokens per task; 0: one token
+    int r1, r2;              // row groups per workgroup of the gate/up and of the down kernel
+    int max_tasks;
+};
+
+#define MLK_W4_MOE(KERNEL, GRID, WAVES, LDS, ...)                                          \
+    do {                                                                                   \
+        static bool ready_on[64] = {};                                                     \
+        const int rc = w4_moe_lds(&KERNEL<__VA_ARGS__>, LDS, ready_on);                    \
+        if (rc != MLK_OK) return rc;                                                       \
+        KERNEL<__VA_ARGS__><<<GRID, (WAVES) * 64, LDS, s>>>(a);                            \
+        MLK_LAUNCH_CHECK();                                                                \
+    } while (0)
+
+template <class T, int GS, bool ZP, int TT, int R>
+static int w4_moe_gate_up(const W4MoeArgs &a, int max_tasks, hipStream_t s) {
+    MLK_W4_MOE(w4_moe_gate_up_kernel, dim3(a.I / 8 / R, max_tasks), 8, (size_t)8 * R * TT * 1024, T, GS, ZP, TT, R);
+    return MLK_OK;
+}
+template <class T, int GS, bool ZP, int TT, int R>
+static int w4_moe_down(const W4MoeArgs &a, int max_tasks, hipStream_t s) {
+    MLK_W4_MOE(w4_moe_down_kernel, dim3(a.H / 16 / R, max_tasks), 8, (size_t)8 * R * TT * 1024, T, GS, ZP, TT, R);
+    return MLK_OK;
+}
+template <class T, int GS, bool ZP, int R>
+static int w4_moe1_gate_up(const W4MoeArgs &a, hipStream_t s) {
+    const size_t x = (size_t)a.H * 2, part = (size_t)8 * R * 64;
+    MLK_W4_MOE(w4_moe1_gate_up_kernel, dim3(a.I / 8 / R, a.K), 8, (x > part ? x : part), T, GS, ZP, R);
+    return MLK_OK;
+}
+template <class T, int GS, bool ZP, int R>
+static int w4_moe1_down(const W4MoeArgs &a, hipStream_t s) {
+    MLK_W4_MOE(w4_moe1_down_kernel, dim3(a.H / 16 / R), 8, (size_t)8 * R * 64, T, GS, ZP, R);
+    return MLK_OK;
+}
+
+template <class T, int GS, bool ZP>
+int w4_launch_moe(const W4MoeArgs &a, const W4MoePlan &pl, hipStream_t s) {
+    int rc = MLK_ERR_INVALID;
+    if (pl.tt == 0) {
+        if (pl.r1 == 2) rc = w4_moe1_gate_up<T, GS, ZP, 2>(a, s);
+        else if (pl.r1 == 4) rc = w4_moe1_gate_up<T, GS, ZP, 4>(a, s);
+        else rc = w4_moe1_gate_up<T, GS, ZP, 8>(a, s);
+        if (rc != MLK_OK) return rc;
+        if (pl.r2 == 1) return w4_moe1_down<T, GS, ZP, 1>(a, s);
+        if (pl.r2 == 2) return w4_moe1_down<T, GS, ZP, 2>(a, s);
+        return w4_moe1_down<T, GS, ZP, 4>(a, s);
+    }
+    if (pl.tt == 1) {
+        rc = pl.r1 == 8 ? w4_moe_gate_up<T, GS, ZP, 1, 8>(a, pl.max_tasks, s) : w4_moe_gate_up<T, GS, ZP, 1, 4>(a, pl.max_tasks, s);
+        if (rc == MLK_OK) rc = pl.r2 == 8 ? w4_moe_down<T, GS, ZP, 1, 8>(a, pl.max_tasks, s) : w4_moe_down<T, GS, ZP, 1, 4>(a, pl.max_tasks, s);
+    } else if (pl.tt == 2) {
+        rc = w4_moe_gate_up<T, GS, ZP, 2, 4>(a, pl.max_tasks, s);
+        if (rc == MLK_OK) rc = w4_moe_down<T, GS, ZP, 2, 4>(a, pl.max_tasks, s);
+    } else {
+        rc = w4_moe_gate_up<T, GS, ZP, 4, 4>(a, pl.max_tasks, s);
+        if (rc == MLK_OK) rc = w4_moe_down<T, GS, ZP, 4, 4>(a, pl.max_tasks, s);
+    }
+    if (rc != MLK_OK) return rc;
+    w4_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
+}
+
+}  // namespace mlk

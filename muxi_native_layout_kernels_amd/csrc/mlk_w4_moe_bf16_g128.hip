@@ -1,0 +1,6 @@
+// Kernels of the expert layers over 4-bit weights: bf16 activations, groups of 128 weights and more, without zero points.
+#include "mlk_w4_moe.cuh"
+
+namespace mlk {
+template int w4_launch_moe<BF16, 4, false>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);
+}  // namespace mlk

@@ -1,0 +1,6 @@
+// Kernels of the expert layers over 4-bit weights: f16 activations, groups of 32 weights, without zero points.
+#include "mlk_w4_moe.cuh"
+
+namespace mlk {
+template int w4_launch_moe<F16, 1, false>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);
+}  // namespace mlk

@@ -154,3 +154,48 @@ def fused_moe(
     if experts_map is None or experts_map.dtype == torch.int:      # (a converted map is a new tensor every call)
         _plans[key] = (B, H, e1, k2, w_kind, score_fun, num_expert_group, topk_group, w1_scale is not None)
     return y.view(shape)
+
+
+def fused_moe_w4(
+    hidden_states: torch.Tensor,  # [batch_size, hidden_size]
+    w1: torch.Tensor,             # [E, 2I/16, H/128, 64, 16] from `pack_layout_a_w4`
+    w2: torch.Tensor,             # [E, H/16, I/128, 64, 16]
+    gating_output: torch.Tensor,  # [batch_size, num_experts]
+    topk: int,
+    renormalize: bool,
+    w1_scale: torch.Tensor,
+    w2_scale: torch.Tensor,
+    w1_zero: Optional[torch.Tensor] = None,
+    w2_zero: Optional[torch.Tensor] = None,
+    use_grouped_topk: bool = False,
+    num_expert_group: Optional[int] = None,
+    topk_group: Optional[int] = None,
+    gating_bias: Optional[torch.Tensor] = None,
+    score_func: str = "softmax",
+    experts_map: Optional[torch.Tensor] = None,
+    expert_load: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """The MoE layer over 4-bit expert weights: the router of `fused_moe`, then `fused_experts_w4`.  `expert_load` (int32 [num_experts]): the
+    picks of this call are added to it (`expert_counts`), for a server that balances its experts by their load."""
+    if num_expert_group is None:
+        num_expert_group = 1
+    if topk_group is None:
+        topk_group = 1
+    if not use_grouped_topk and num_expert_group != 1:
+        raise ValueError("When use_grouped_topk is False, num_expert_group must be 1.")
+    if score_func not in ("softmax", "sigmoid"):
+        raise ValueError("Unsupported scoring function")
+    ops._check(hidden_states.dim() == 2 and gating_output.dim() == 2 and hidden_states.shape[0] == gating_output.shape[0], "Number of tokens mismatch")
+    ops._check(hidden_states.is_cuda and hidden_states.device == gating_output.device, "hidden_states and gating_output must be on the same CUDA device")
+    ops._check(hidden_states.dtype in ops._KIND and gating_output.dtype == hidden_states.dtype, "gating_output must have the activation dtype")
+    ops._check(gating_output.shape[1] == (w1.shape[0] if experts_map is None else experts_map.numel()),
+               "gating_output must have one column per expert of w1, or per entry of experts_map")
+    with ops._OnDevice(hidden_states):
+        topk_ids, topk_weights = _routing_buffers(hidden_states.shape[0], topk, hidden_states.dtype, hidden_states.device,
+                                                  ops._stream_of(hidden_states))
+        if hidden_states.shape[0] > 0:
+            ops.fused_routing_gate(gating_output, 0 if score_func == "softmax" else 1, hidden_states.shape[0], hidden_states.shape[1], num_expert_group,
+                                   topk_group, topk_ids, topk_weights, topk, gating_bias, renormalize)
+        if expert_load is not None:
+            ops.expert_counts(topk_ids, gating_output.shape[1], out=expert_load)
+    return ops.fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)

@@ -122,11 +122,12 @@ class WorkspacePool:
 
 _gemm_pool = WorkspacePool(1 << 22, zero_prefix=True)
 _moe_pool = WorkspacePool(1 << 20)
+_balance_pool = WorkspacePool(1 << 16, zero_prefix=True)
 
 
 def workspace_bytes_held():
-    """Device bytes the library's scratch pools hold right now (K-split partials, MoE tables and intermediates)."""
-    return _gemm_pool.held_bytes() + _moe_pool.held_bytes()
+    """Device bytes the library's scratch pools hold right now (K-split partials, MoE tables and intermediates, sums of the balance loss)."""
+    return _gemm_pool.held_bytes() + _moe_pool.held_bytes() + _balance_pool.held_bytes()
 
 
 def release_workspaces(retired_only=False):
@@ -135,7 +136,7 @@ def release_workspaces(retired_only=False):
     a HIP graph captured around a call replays with valid pointers; a caller that holds no such graph (or has
     dropped it) calls this after a burst of large batches, or when streams it used are gone.  `retired_only`
     releases just the buffers that a larger one has replaced.  Synchronize the device first."""
-    return _gemm_pool.release(retired_only) + _moe_pool.release(retired_only)
+    return _gemm_pool.release(retired_only) + _moe_pool.release(retired_only) + _balance_pool.release(retired_only)
 
 
 def _workspace(device, nbytes, counter_bytes, stream=None):
@@ -614,7 +615,7 @@ class _OnDevice:
             self.guard.__exit__(*exc)
 
 
-def _w4_tensors(named, device):
+def _check_tensors(named, device):
     for t, name in named:
         if t is not None:
             _check(t.is_cuda, "%s must be a CUDA tensor" % name)
@@ -641,7 +642,7 @@ def pack_layout_a_w4(codes, scales, zeros=None):
     group = k // groups
     _check(group in (32, 64) or group % 128 == 0, "the group must be 32, 64 or a multiple of 128")
     _check(zeros is None or zeros.shape == scales.shape, "zeros must have the shape of scales")
-    _w4_tensors(((codes, "codes"), (scales, "scales"), (zeros, "zeros")), codes.device)
+    _check_tensors(((codes, "codes"), (scales, "scales"), (zeros, "zeros")), codes.device)
     batch = codes.shape[0] if codes.dim() == 3 else 1
     per = max(1, 128 // group)
     lib, shape = _lib.load(), lead + (n // 16, groups // per, 16, per)
@@ -662,7 +663,7 @@ def pack_layout_a_w4(codes, scales, zeros=None):
 def unpack_layout_a_w4(A, A_Scale, A_Zero=None):
     """Inverse of `pack_layout_a_w4`: (codes [.., N, K/2], scales [.., N, K/G], zeros or None)."""
     n, k, group = _w4_dims(A, A_Scale, A_Zero, A.dim() - 4)
-    _w4_tensors(((A, "A"), (A_Scale, "A_Scale"), (A_Zero, "A_Zero")), A.device)
+    _check_tensors(((A, "A"), (A_Scale, "A_Scale"), (A_Zero, "A_Zero")), A.device)
     lead = tuple(A.shape[:-4])
     batch = A.shape[0] if lead else 1
     lib = _lib.load()
@@ -708,7 +709,7 @@ def _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, what):
         _check(B.dtype in _KIND, "Unsupported data type")
         _check(A_Scale.dtype == B.dtype, "A_Scale must have the activation dtype")
         _check(bias is None or (bias.dtype == B.dtype and bias.numel() == m), "bias must be [1, m] of the activation dtype")
-        _w4_tensors(((A, "A"), (A_Scale, "A_Scale"), (B, "B"), (A_Zero, "A_Zero"), (bias, "bias")), B.device)
+        _check_tensors(((A, "A"), (A_Scale, "A_Scale"), (B, "B"), (A_Zero, "A_Zero"), (bias, "bias")), B.device)
         lib = _lib.load()
         plan = _plans[key] = (B.size(0), m, k, group, _KIND[B.dtype], lib.mlk_gemm_w4_workspace_bytes(B.size(0), m, k),
                               lib.mlk_gemm_counter_bytes(), lib.mlk_gemm_layout_a_w4)
@@ -927,6 +928,154 @@ def fused_moe_raw(w1, w2, x, logits, T, E, K, hidden, inter, w_kind, score_fun, 
                "fused_moe")
 
 
+def fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero=None, w2_zero=None, experts_map=None):
+    """The two products of an expert layer over 4-bit weights, from a routing decision (`fused_routing_gate`, or a caller's own).
+
+    hidden_states [T, H] fp16 / bf16; w1 [E, 2I/16, H/128, 64, 16] (gate rows, then up rows), w2 [E, H/16, I/128, 64, 16], their scales and zero
+    points from `pack_layout_a_w4`; topk_ids int32 [T, K], topk_weights [T, K] of the activation dtype; experts_map int32 [experts of
+    the router]: the expert's place in w1 / w2, -1 = on another card.  Ids outside the router's experts are dropped too; a token without an expert here
+    gets zeros.  Returns y [T, H].  fp32 sums; the SiLU intermediate is rounded to the activation dtype, which the second product's matrix
+    instructions take."""
+    x = hidden_states
+    key = ("experts_w4", x.shape, w1.shape, w2.shape, topk_ids.shape, topk_weights.shape, w1_scale.shape, w2_scale.shape, x.dtype, w1.dtype, w2.dtype,
+           topk_ids.dtype, topk_weights.dtype, w1_scale.dtype, w2_scale.dtype, x.device, w1.device, w2.device, topk_ids.device, topk_weights.device,
+           w1_scale.device, w2_scale.device,
+           None if w1_zero is None else (w1_zero.shape, w1_zero.dtype, w1_zero.device),
+           None if w2_zero is None else (w2_zero.shape, w2_zero.dtype, w2_zero.device),
+           None if experts_map is None else (experts_map.shape, experts_map.dtype, experts_map.device))
+    plan = _plans.get(key)
+    if plan is None or not (x.is_contiguous() and w1.is_contiguous() and w2.is_contiguous() and topk_ids.is_contiguous() and topk_weights.is_contiguous() and
+                            w1_scale.is_contiguous() and w2_scale.is_contiguous() and (w1_zero is None or w1_zero.is_contiguous()) and
+                            (w2_zero is None or w2_zero.is_contiguous()) and (experts_map is None or experts_map.is_contiguous())):
+        m1, hidden, group = _w4_dims(w1, w1_scale, w1_zero, 1, "w1")
+        m2, inter, group2 = _w4_dims(w2, w2_scale, w2_zero, 1, "w2")
+        E = w1.size(0)
+        _check(w2.size(0) == E and m1 == 2 * inter and m2 == hidden, "w1 must be [E, 2I, H] and w2 [E, H, I]")
+        _check(group == group2, "w1 and w2 must have the same group size")
+        _check((w1_zero is None) == (w2_zero is None), "zero points for both w1 and w2 or for none")
+        _check(inter % 128 == 0 and hidden % 128 == 0, "hidden and intermediate sizes must be multiples of 128")
+        _check(1 <= E <= 256, "at most 256 experts")
+        _check(x.dim() == 2 and x.size(1) == hidden, "hidden_states must be [T, H]")
+        _check(x.dtype in _KIND, "hidden_states must be fp16 or bf16")
+        _check(w1_scale.dtype == x.dtype and w2_scale.dtype == x.dtype, "scales must have the activation dtype")
+        _check(topk_ids.dim() == 2 and topk_ids.size(0) == x.size(0) and topk_ids.dtype == torch.int32, "topk_ids must be int32 [T, K]")
+        _check(topk_weights.shape == topk_ids.shape and topk_weights.dtype == x.dtype, "topk_weights must be [T, K] of the activation dtype")
+        K = topk_ids.size(1)
+        _check(1 <= K <= 32, "topK must be in 1..32")
+        _check(experts_map is None or (experts_map.dtype == torch.int32 and experts_map.dim() == 1 and experts_map.numel() > 0),
+               "experts_map must be int32 [experts of the router]")
+        _check_tensors(((x, "hidden_states"), (w1, "w1"), (w2, "w2"), (topk_ids, "topk_ids"), (topk_weights, "topk_weights"), (w1_scale, "w1_scale"),
+                     (w2_scale, "w2_scale"), (w1_zero, "w1_zero"), (w2_zero, "w2_zero"), (experts_map, "experts_map")), x.device)
+        lib = _lib.load()
+        plan = _plans[key] = (x.size(0), E, E if experts_map is None else experts_map.numel(), K, hidden, inter, group, _KIND[x.dtype],
+                              lib.mlk_experts_w4_workspace_bytes(x.size(0), E, K, hidden, inter), lib.mlk_fused_experts_w4)
+    T, E, E_router, K, hidden, inter, group, kind, ws_need, fn = plan
+    with _OnDevice(x):
+        if x.data_ptr() & 15:
+            x = x.clone()
+        y = torch.empty((T, hidden), dtype=x.dtype, device=x.device)
+        if T == 0:
+            return y
+        stream = _stream_of(x)
+        ws = _moe_pool.get(x.device, stream, ws_need)
+        rc = fn(w1.data_ptr(), w1_scale.data_ptr(), _ptr(w1_zero), w2.data_ptr(), w2_scale.data_ptr(), _ptr(w2_zero), x.data_ptr(), T, E, E_router, K,
+                hidden, inter, group, kind, topk_ids.data_ptr(), topk_weights.data_ptr(), _ptr(experts_map), y.data_ptr(), ws.data_ptr(), ws.numel(),
+                stream)
+        if rc != 0:
+            _lib.check(rc, "fused_experts_w4")
+    return y
+
+
+# ------------------------------------------------------------- router balance
+def _check_routing(experts_ids, token_mask, device):
+    _check(experts_ids.dtype == torch.int32 and experts_ids.dim() == 2 and experts_ids.size(1) >= 1, "experts_ids must be int32 [T, K]")
+    _check(token_mask is None or (token_mask.dtype in (torch.bool, torch.uint8) and token_mask.dim() == 1 and
+                                  token_mask.size(0) == experts_ids.size(0)), "token_mask must be bool [T]")
+    _check_tensors(((experts_ids, "experts_ids"), (token_mask, "token_mask")), device)
+
+
+def expert_counts(experts_ids, n_experts, token_mask=None, out=None):
+    """How many routed pairs each expert got: int32 [n_experts].  experts_ids int32 [T, K] (`fused_routing_gate`), ids outside 0..n_experts-1
+    count nowhere; token_mask bool [T]: False for padded rows.  With `out` the counts are added to it, for a load that builds up over
+    the steps of a server; the call then is one launch."""
+    _check_routing(experts_ids, token_mask, experts_ids.device)
+    _check(1 <= n_experts <= 256, "1..256 experts")
+    with _OnDevice(experts_ids):
+        if out is None:
+            out = torch.zeros(n_experts, dtype=torch.int32, device=experts_ids.device)
+        else:
+            _check(out.dtype == torch.int32 and tuple(out.shape) == (n_experts,), "out must be int32 [n_experts]")
+            _check_tensors(((out, "out"),), experts_ids.device)
+        rc = _lib.load().mlk_expert_counts(experts_ids.data_ptr(), _ptr(token_mask), experts_ids.size(0), experts_ids.size(1), n_experts,
+                                           out.data_ptr(), _stream_of(experts_ids))
+        if rc != 0:
+            _lib.check(rc, "expert_counts")
+    return out
+
+
+_LOGIT_KIND = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 3}
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, mask, cu, score_fun, coef):
+        T, E = logits.shape
+        n_seq = 1 if cu is None else cu.numel() - 1
+        lib = _lib.load()
+        with _OnDevice(logits):
+            stream = _stream_of(logits)
+            loss = torch.empty((), dtype=torch.float32, device=logits.device)
+            counts = torch.empty(E, dtype=torch.int32, device=logits.device)
+            share = torch.empty((n_seq, E), dtype=torch.float32, device=logits.device)
+            ws = _balance_pool.get(logits.device, stream, lib.mlk_balance_workspace_bytes(T, E, n_seq), lib.mlk_balance_counter_bytes())
+            rc = lib.mlk_balance_loss(logits.data_ptr(), _LOGIT_KIND[logits.dtype], score_fun, T, E, ids.size(1), ids.data_ptr(), _ptr(mask), _ptr(cu),
+                                      n_seq, coef, loss.data_ptr(), counts.data_ptr(), share.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+            if rc != 0:
+                _lib.check(rc, "moe_balance_loss")
+        ctx.save_for_backward(logits, mask, cu, share)
+        ctx.score_fun, ctx.n_seq = score_fun, n_seq
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, _):
+        if dloss is None:
+            return None, None, None, None, None, None
+        logits, mask, cu, share = ctx.saved_tensors
+        with _OnDevice(logits):
+            grad = torch.empty_like(logits)
+            rc = _lib.load().mlk_balance_loss_grad(logits.data_ptr(), _LOGIT_KIND[logits.dtype], ctx.score_fun, logits.size(0), logits.size(1), _ptr(mask),
+                                                   _ptr(cu), ctx.n_seq, share.data_ptr(), dloss.data_ptr(), grad.data_ptr(), _stream_of(logits))
+            if rc != 0:
+                _lib.check(rc, "moe_balance_loss")
+        return grad, None, None, None, None, None
+
+
+def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0, token_mask=None, cu_seqlens=None):
+    """Balance loss of a router and its per-expert counts: (loss fp32 [], counts int32 [E]); differentiable in gating_output.
+
+    loss = coef * mean over the sequences that have a valid token of E * sum_e f_e P_e, f_e = share of their valid tokens' routed pairs that went to e
+    (a constant of the differentiation), P_e = mean over them of the router's probabilities: softmax of the logits, or with "sigmoid" the
+    sigmoids over their sum.  counts: routed pairs of all valid tokens.
+
+    gating_output [T, E] fp16 / bf16 / fp32, E <= 256; experts_ids int32 [T, K] (`fused_routing_gate`); token_mask bool [T], False for padded
+    tokens; cu_seqlens int32 [sequences + 1] on the device, non-decreasing, where each sequence begins and the last one ends (None: all tokens are
+    one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0."""
+    _check(gating_output.dim() == 2 and 1 <= gating_output.size(1) <= 256, "gating_output must be [T, E], at most 256 experts")
+    _check(gating_output.dtype in _LOGIT_KIND, "gating_output must be fp16, bf16 or fp32")
+    _check(gating_output.is_cuda and gating_output.is_contiguous(), "gating_output must be a contiguous CUDA tensor")
+    _check_routing(experts_ids, token_mask, gating_output.device)
+    _check(experts_ids.size(0) == gating_output.size(0), "experts_ids must be int32 [T, K]")
+    if score_func not in ("softmax", "sigmoid"):
+        raise ValueError("Unsupported scoring function")
+    _check(cu_seqlens is None or (cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and 1 <= cu_seqlens.numel() <= 65536),
+           "cu_seqlens must be int32 [sequences + 1], at most 65535 sequences")
+    _check_tensors(((cu_seqlens, "cu_seqlens"),), gating_output.device)
+    return _BalanceLoss.apply(gating_output, experts_ids, token_mask, cu_seqlens, 0 if score_func == "softmax" else 1, float(coef))
+
+
 # ------------------------------------------------- names outside the hot path
 def _out_of_scope(name, why):
     def fn(*args, **kwargs):
@@ -953,4 +1102,5 @@ __all__ = [
     "batched_routed_activation_indexed_to_expert_block_indexed", "fused_experts_compute",
     "pack_layout_a", "unpack_layout_a", "experts_compute_raw", "release_workspaces", "workspace_bytes_held",
     "fused_moe_raw", "pack_layout_a_w4", "unpack_layout_a_w4", "gemm_layoutA_w4", "gemv_layoutA_w4",
+    "fused_experts_w4", "expert_counts", "moe_balance_loss",
 ]
