@@ -261,7 +261,7 @@ int mlk_unpack_scales_w4(const void *src, void *dst, int64_t batch, int n, int k
  * that is 0. */
 int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, const void *b, void *c, int m, int n, int k, int group,
                          int x_kind, float alpha, const void *bias, void *workspace, size_t workspace_bytes, void *stream);
-size_t mlk_gemm_w4_workspace_bytes(int m, int n, int k);
+size_t mlk_gemm_w4_workspace_bytes(int m, int n, int k, int group);
 
 /* ----------------------------------------------------------------------- MoE */
 
@@ -372,7 +372,7 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
                          const void *x, int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter, int group, int x_kind,
                          const int32_t *topk_ids, const void *topk_weights, const int32_t *experts_map, void *y, void *workspace,
                          size_t workspace_bytes, void *stream);
-size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int hidden, int inter);
+size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int hidden, int inter, int group);
 
 /* ------------------------------------------------------------- router balance */
 

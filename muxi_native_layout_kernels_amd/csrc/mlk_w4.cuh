@@ -29,7 +29,10 @@ constexpr int kW4TileK = 128;
 // Group of a tile without a division: `inv` = ceil(2^32 / tiles per group), or 0 where a group is no more than a tile.  Exact for up to 2^16 tiles
 // (the rounding of inv adds less than t * tpg / 2^32 < 1 / tpg).
 __host__ __device__ __forceinline__ uint32_t w4_inverse(int tpg) { return tpg == 1 ? 0u : (uint32_t)((0x100000000ull + tpg - 1) / tpg); }
-__device__ __forceinline__ int w4_block(int t, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)t, inv) : t; }
+__device__ __forceinline__ int w4_block(int t, uint32_t inv) {
+    const uint32_t keep = inv ? 0u : ~0u;                  // no branch in the loops
+    return (int)(__umulhi((uint32_t)t, inv) + ((uint32_t)t & keep));
+}
 
 // Weights of one matrix (or of one expert).
 struct W4Matrix {
@@ -38,16 +41,28 @@ struct W4Matrix {
     const uint8_t *zeros;      // null: 8 everywhere
 };
 
-// MFMA operand: eight codes of one dword, widened to 16 + q in the type T.
+// Mask and bits of 16 for the widening, held in a scalar and a vector register: v_and_or_b32 takes one constant at most, and with both as
+// literals the compiler makes two instructions of it.
 template <class T>
-__device__ __forceinline__ u32x4 w4_widen(uint32_t d) {
-    if constexpr (T::kind == MLK_BF16) {
-        constexpr uint32_t M = 0x00780078u, B = 0x41804180u;
-        return u32x4{((d << 3) & M) | B, ((d >> 1) & M) | B, ((d >> 5) & M) | B, ((d >> 9) & M) | B};
-    } else {
-        constexpr uint32_t M = 0x03c003c0u, B = 0x4c004c00u;
-        return u32x4{((d << 6) & M) | B, ((d << 2) & M) | B, ((d >> 2) & M) | B, ((d >> 6) & M) | B};
+struct W4Const {
+    uint32_t mask, sixteen;
+    __device__ __forceinline__ W4Const() {
+        mask = T::kind == MLK_BF16 ? 0x00780078u : 0x03c003c0u;
+        sixteen = T::kind == MLK_BF16 ? 0x41804180u : 0x4c004c00u;
+        asm volatile("" : "+s"(mask));
+        asm volatile("" : "+v"(sixteen));
     }
+};
+
+// Codes 2 p and 2 p + 1 of a dword, widened to 16 + q in the type T; and all eight: an MFMA operand.
+template <class T>
+__device__ __forceinline__ uint32_t w4_widen1(uint32_t d, int p, const W4Const<T> &c) {
+    constexpr int AT = T::kind == MLK_BF16 ? 3 : 6;        // where the four bits belong
+    return ((4 * p <= AT ? d << (AT - 4 * p) : d >> (4 * p - AT)) & c.mask) | c.sixteen;
+}
+template <class T>
+__device__ __forceinline__ u32x4 w4_widen(uint32_t d, const W4Const<T> &c) {
+    return u32x4{w4_widen1<T>(d, 0, c), w4_widen1<T>(d, 1, c), w4_widen1<T>(d, 2, c), w4_widen1<T>(d, 3, c)};
 }
 
 template <class T>
@@ -96,7 +111,8 @@ __device__ __forceinline__ float w4_offset(const W4Scale<GS> &c, int g) {      /
 
 // One tile (128 k) of R row groups times TT blocks of 16 tokens.
 template <class T, int GS, int TT, int R>
-__device__ __forceinline__ void w4_tile(f32x4 (&acc)[R][TT], const u32x4 (&w)[R], const W4Scale<GS> (&sc)[R], const u32x4 (&x)[TT][4]) {
+__device__ __forceinline__ void w4_tile(f32x4 (&acc)[R][TT], const u32x4 (&w)[R], const W4Scale<GS> (&sc)[R], const u32x4 (&x)[TT][4],
+                                        const W4Const<T> &con) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < 4 / GS; ++g) {
@@ -114,7 +130,7 @@ __device__ __forceinline__ void w4_tile(f32x4 (&acc)[R][TT], const u32x4 (&w)[R]
             for (int tt = 0; tt < TT; ++tt) d[tt] = zero;
 #pragma unroll
             for (int j = g * GS; j < (g + 1) * GS; ++j) {
-                const u32x4 b = w4_widen<T>(w[r][j]);
+                const u32x4 b = w4_widen<T>(w[r][j], con);
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt) d[tt] = T::mfma(x[tt][j], b, d[tt]);
             }
@@ -158,6 +174,7 @@ __device__ __forceinline__ void w4_stream(f32x4 (&acc)[R][TT], const W4Rows<R> &
     u32x4 w[U][R], x[U][XL ? 1 : TT][4];
     W4Scale<GS> sc[U][R];
     const int o = lane >> 4, r16 = lane & 15;
+    const W4Const<T> con;
     auto load = [&](int u, int t) {
         const int at = w4_block(t, inv) * 16 + r16;
 #pragma unroll
@@ -188,9 +205,9 @@ __device__ __forceinline__ void w4_stream(f32x4 (&acc)[R][TT], const W4Rows<R> &
                     u32x4 xv[TT][4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) xv[0][j] = xl[t * 16 + j * 4 + o];
-                    w4_tile<T, GS, TT, R>(acc, w[u], sc[u], xv);
+                    w4_tile<T, GS, TT, R>(acc, w[u], sc[u], xv, con);
                 } else {
-                    w4_tile<T, GS, TT, R>(acc, w[u], sc[u], x[u]);
+                    w4_tile<T, GS, TT, R>(acc, w[u], sc[u], x[u], con);
                 }
                 if (i + u + U < n) load(u, t + U * step);
             }

@@ -1,11 +1,13 @@
 // Linear layers over 4-bit weights: one token (GeMV) to prefill-sized batches.
-#include "mlk_w4_gemm.cuh"
+#include "mlk_w4_panel_gemm.cuh"
 
 namespace mlk {
 
 #define MLK_W4_EXTERN(T, GS)                                                                          \
     extern template int w4_launch_stream<T, GS, false>(const W4GemmArgs &, int, int, int, hipStream_t); \
-    extern template int w4_launch_stream<T, GS, true>(const W4GemmArgs &, int, int, int, hipStream_t);
+    extern template int w4_launch_stream<T, GS, true>(const W4GemmArgs &, int, int, int, hipStream_t);  \
+    extern template int w4_launch_panel<T, GS, false>(const W4PanelArgs &, int, hipStream_t);           \
+    extern template int w4_launch_panel<T, GS, true>(const W4PanelArgs &, int, hipStream_t);
 MLK_W4_EXTERN(F16, 4)
 MLK_W4_EXTERN(F16, 2)
 MLK_W4_EXTERN(F16, 1)
@@ -14,33 +16,101 @@ MLK_W4_EXTERN(BF16, 2)
 MLK_W4_EXTERN(BF16, 1)
 #undef MLK_W4_EXTERN
 
+constexpr size_t kW4CounterBytes = 64 * 1024;      // the front of the workspace that the GeMMs share
+
 struct W4Plan {
-    int r, wgs, waves;
+    int r, wgs, waves;      // streaming kernels
+    int tb;                 // panels: blocks of 32 tokens; 0: streaming kernels
+    int slices;             // of K
 };
 
-// Up to 64 tokens.
-static W4Plan w4_plan_stream(int m, int n) {
-    const int groups = n / 16, cus = device_cus(), most = m <= 16 ? 8 : 4;
-    W4Plan pl;
-    pl.r = 1;
-    while (pl.r < most && groups > pl.r * cus) pl.r *= 2;
-    pl.wgs = groups <= cus ? groups : (groups + pl.r * cus - 1) / (pl.r * cus) * cus;
-    if (pl.wgs > groups) pl.wgs = groups;
-    pl.waves = m == 1 && pl.r <= 2 ? 16 : 8;
+// Up to 64 tokens.  Microseconds on weights from memory, groups of 128, bf16 (r row groups a workgroup, s slices of K):
+//   one to four tokens   one workgroup per CU as far as r <= 4 goes, K whole: 4096 x 4096 r = 1 4.7 (s = 2: 6.3), 4096 x 14336 r = 1 9.8, r = 2 s = 2 10.7; 28672 x 8192 one
+//                        token r = 2 25.7, r = 4 27.5, two tokens r = 4 24.9, r = 2 31.6
+//   more                 the activations weigh more, r = 4 shares them between four row groups; slices bring the workgroups back: 4096 x 14336 at 16 tokens r = 1
+//                        16.7, r = 2 s = 2 13.6, r = 4 s = 4 11.6, at 64 53, 31 and 23; 512 x 7168 at 64 tokens r = 1 27.6, s = 8 8.9.  At least six tiles a slice
+//                        (1280 x 5120 at 16 tokens r = 2 s = 4 6.3, s = 8 9)
+static W4Plan w4_plan_stream(int m, int n, int k) {
+    const int groups = n / 16, tiles = k / 128, cus = device_cus();
+    W4Plan pl = {};
+    pl.tb = 0;
+    pl.slices = pl.r = 1;
+    if (m <= 4) {
+        while (pl.r < 4 && groups > pl.r * cus) pl.r *= 2;
+        if (m == 1 && pl.r == 4 && groups > 4 * cus) pl.r = 2;
+    } else {
+        const int most = tiles / 6 < 1 ? 1 : (tiles / 6 > 8 ? 8 : tiles / 6);
+        pl.r = 4;
+        while (pl.r > 1 && (groups + pl.r - 1) / pl.r * most < 128) pl.r /= 2;
+        const int fill = cus / ((groups + pl.r - 1) / pl.r);
+        pl.slices = fill < 1 ? 1 : (fill > most ? most : fill);
+    }
+    pl.wgs = (groups + pl.r - 1) / pl.r;
+    pl.waves = m == 1 && pl.r == 1 && groups <= cus && tiles >= 16 ? 16 : 8;
     return pl;
 }
 
+// A fitted cost of panels of 32 tb tokens in `slices` slices of K, in microseconds: rounds of one panel per CU; a window of 128 k takes 0.82 (tb = 2) or 1.18 us
+// (tb = 4) with few panels on the chip and 0.2 or 0.5 more with one on every CU; three windows go to the start and the end, one for every 16 groups to the
+// sums of x; launches and sums 6 us, the fold 2 us and its bytes.  Smaller groups cost more vector instructions a window.
+static double w4_panel_cost(int m, int n, int k, int group, int tb, int slices, int cus) {
+    const int panels = (n + 255) / 256 * ((m + 32 * tb - 1) / (32 * tb)), windows = (k / 128 + slices - 1) / slices;
+    const int rounds = (panels * slices + cus - 1) / cus, g = group < 128 ? 128 / group : 1;
+    const double full = rounds > 1 ? 1.0 : (double)panels * slices / cus;
+    const double window = (tb == 2 ? 0.82 + 0.2 * full : 1.18 + 0.5 * full) * (g == 1 ? 1.0 : (g == 2 ? 1.15 : 1.45));
+    return rounds * (windows + (windows * g + 15) / 16 + 3) * window + 6 + (slices > 1 ? 2 + (double)slices * m * n * 8 / 5e6 : 0);
+}
+// And of the streaming kernels from 33 to 64 tokens: the weights' bytes and as many again for every block of 16 tokens and the row groups that share it.
+static double w4_stream_cost(int m, int n, int k) { return 4 + (double)n * k / 2e6 * (0.085 + 0.134 * ((m + 15) / 16)); }
+
+static W4Plan w4_plan(int m, int n, int k, int group) {
+    const W4Plan stream = w4_plan_stream(m < 64 ? m : 64, n, k);
+    if (m <= 32) return stream;
+    W4Plan best = {};
+    double least = m <= 64 ? w4_stream_cost(m, n, k) : 1e30;
+    if (m <= 64) best = stream;
+    const int cus = device_cus();
+    for (int tb = 2; tb <= 4; tb += 2)
+        for (int slices = 1; slices <= 16 && slices * 2 <= k / 128; ++slices) {
+            const double c = w4_panel_cost(m, n, k, group, tb, slices, cus);
+            if (c < least) {
+                least = c;
+                best = W4Plan{0, 0, 0, tb, slices};
+            }
+        }
+    return best.r || best.tb ? best : W4Plan{0, 0, 0, 2, 1};
+}
+static size_t w4_sums_bytes(int m, int k, int group) {
+    return ((size_t)m * w4_sum_pitch(k, group < 128 ? group / 32 : 4) * 16 + 255) / 256 * 256;
+}
+static size_t w4_partial_bytes(const W4Plan &pl, int m, int n, int k, int group) {
+    if (pl.tb) return w4_sums_bytes(m, k, group) + (pl.slices > 1 ? (size_t)pl.slices * m * n * 4 : 0);
+    if (pl.slices <= 1) return 0;
+    return (size_t)pl.slices * pl.wgs * pl.r * ((m + 15) / 16) * 1024;
+}
+
 template <class T, int GS>
-static int w4_stream_of(const W4GemmArgs &a, hipStream_t s) {
-    const W4Plan pl = w4_plan_stream(a.M, a.N);
+static int w4_stream_of(const W4GemmArgs &a, const W4Plan &pl, hipStream_t s) {
     return a.A.zeros ? w4_launch_stream<T, GS, true>(a, pl.r, pl.wgs, pl.waves, s) : w4_launch_stream<T, GS, false>(a, pl.r, pl.wgs, pl.waves, s);
 }
 
-static int w4_stream(const W4GemmArgs &a, int x_kind, int group, hipStream_t s) {
+static int w4_stream(const W4GemmArgs &a, const W4Plan &pl, int x_kind, int group, hipStream_t s) {
     const bool f16 = x_kind == MLK_F16;
-    if (group == 32) return f16 ? w4_stream_of<F16, 1>(a, s) : w4_stream_of<BF16, 1>(a, s);
-    if (group == 64) return f16 ? w4_stream_of<F16, 2>(a, s) : w4_stream_of<BF16, 2>(a, s);
-    return f16 ? w4_stream_of<F16, 4>(a, s) : w4_stream_of<BF16, 4>(a, s);
+    if (group == 32) return f16 ? w4_stream_of<F16, 1>(a, pl, s) : w4_stream_of<BF16, 1>(a, pl, s);
+    if (group == 64) return f16 ? w4_stream_of<F16, 2>(a, pl, s) : w4_stream_of<BF16, 2>(a, pl, s);
+    return f16 ? w4_stream_of<F16, 4>(a, pl, s) : w4_stream_of<BF16, 4>(a, pl, s);
+}
+
+template <class T, int GS>
+static int w4_panel_of(const W4PanelArgs &a, int tb, hipStream_t s) {
+    return a.A.zeros ? w4_launch_panel<T, GS, true>(a, tb, s) : w4_launch_panel<T, GS, false>(a, tb, s);
+}
+
+static int w4_panel(const W4PanelArgs &a, int tb, int x_kind, int group, hipStream_t s) {
+    const bool f16 = x_kind == MLK_F16;
+    if (group == 32) return f16 ? w4_panel_of<F16, 1>(a, tb, s) : w4_panel_of<BF16, 1>(a, tb, s);
+    if (group == 64) return f16 ? w4_panel_of<F16, 2>(a, tb, s) : w4_panel_of<BF16, 2>(a, tb, s);
+    return f16 ? w4_panel_of<F16, 4>(a, tb, s) : w4_panel_of<BF16, 4>(a, tb, s);
 }
 
 // ------------------------------------------------------------------------------------------------------------ relayout
@@ -139,27 +209,50 @@ int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, con
     MLK_REQUIRE(a && scale && b && c, "w4 gemm: null pointer");
     MLK_REQUIRE(aligned16(a) && aligned16(b), "w4 gemm: weights and activations must lie on 16 bytes");
     MLK_REQUIRE(((uintptr_t)scale & 7) == 0 && ((uintptr_t)zero & 3) == 0, "w4 gemm: scales must lie on 8 bytes, zero points on 4");
-    W4GemmArgs p;
-    p.A = W4Matrix{(const uint8_t *)a, (const uint16_t *)scale, (const uint8_t *)zero};
+    const W4Plan pl = w4_plan(m, n, k, group);
+    const size_t part = w4_partial_bytes(pl, m, n, k, group);
+    if (part && (!workspace || workspace_bytes < kW4CounterBytes + part)) return fail(MLK_ERR_WORKSPACE, "w4 gemm: workspace too small");
+    const W4Matrix w = {(const uint8_t *)a, (const uint16_t *)scale, (const uint8_t *)zero};
+    const int blocks = k / (group > 128 ? group : 128);
+    const uint32_t inv = w4_inverse(group > 128 ? group / 128 : 1);
+    if (pl.tb) {
+        W4PanelArgs p = {};
+        p.A = w;
+        p.X = (const uint16_t *)b;
+        p.C = (uint16_t *)c;
+        p.bias = (const uint16_t *)bias;
+        p.alpha = alpha;
+        p.M = m;
+        p.N = n;
+        p.K = k;
+        p.blocks = blocks;
+        p.inv = inv;
+        p.slices = pl.slices;
+        p.sums = (u32x4 *)((uint8_t *)workspace + kW4CounterBytes);
+        p.partial = (float *)((uint8_t *)workspace + kW4CounterBytes + w4_sums_bytes(m, k, group));
+        return w4_panel(p, pl.tb, x_kind, group, (hipStream_t)stream);
+    }
+    W4GemmArgs p = {};
+    p.A = w;
     p.bias = (const uint16_t *)bias;
     p.alpha = alpha;
     p.N = n;
     p.K = k;
-    p.blocks = k / (group > 128 ? group : 128);
-    p.inv = w4_inverse(group > 128 ? group / 128 : 1);
-    p.slices = 1;
-    p.partial = nullptr;
-    p.counters = nullptr;
-    for (int m0 = 0; m0 < m; m0 += 64) {
-        p.M = m - m0 < 64 ? m - m0 : 64;
-        p.X = (const uint16_t *)b + (size_t)m0 * k;
-        p.C = (uint16_t *)c + (size_t)m0 * n;
-        const int rc = w4_stream(p, x_kind, group, (hipStream_t)stream);
-        if (rc != MLK_OK) return rc;
-    }
-    return MLK_OK;
+    p.blocks = blocks;
+    p.inv = inv;
+    p.slices = pl.slices;
+    p.counters = part ? (int *)workspace : nullptr;
+    p.partial = part ? (f32x4 *)((uint8_t *)workspace + kW4CounterBytes) : nullptr;
+    p.M = m;
+    p.X = (const uint16_t *)b;
+    p.C = (uint16_t *)c;
+    return w4_stream(p, pl, x_kind, group, (hipStream_t)stream);
 }
 
-size_t mlk_gemm_w4_workspace_bytes(int m, int n, int k) { return 0; }
+size_t mlk_gemm_w4_workspace_bytes(int m, int n, int k, int group) {
+    if (m <= 0 || n <= 0 || k <= 0 || !w4_group_ok(k, group)) return 0;
+    const size_t part = w4_partial_bytes(w4_plan(m, n, k, group), m, n, k, group);
+    return part ? kW4CounterBytes + part : 0;
+}
 
 }  // extern "C"

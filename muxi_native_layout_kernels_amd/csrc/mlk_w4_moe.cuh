@@ -2,7 +2,7 @@
 //
 // Several tokens: the routed pairs are brought into expert order in blocks of 16 (moe_align_kernel); a task is up to TT blocks of one expert, which
 // share one pass over its weights.  The intermediate is kept row-major [slot][I] in the activations' type (slot = place in the order), the
-// weighted products of the down projection in fp32 [pair][H], and a last launch adds a token's pairs in the order of its picks.
+// weighted products of the down projection in fp32 [pair][slice][H], and a last launch adds a token's pairs in the order of its picks.
 // One token: its picks are the tasks, no alignment; the down projection's waves deal the picks among themselves and write the output at once.
 #pragma once
 
@@ -25,7 +25,9 @@ struct W4MoeArgs {
     const MoeTask *tasks;
     const int32_t *n_tasks;
     uint16_t *hbuf;              // [slot][I]
-    float *obuf;                 // [pair][H]
+    float *obuf;                 // [pair][slice][H]
+    int slices;                  // of the down projection's k
+    u32x4 *sums1, *sums2;        // panels: sums of x, of the intermediate (w4_sums_kernel)
 };
 
 // Local expert of a pair, -1: dropped.
@@ -142,7 +144,10 @@ __global__ void __launch_bounds__(256) w4_moe_combine_kernel(W4MoeArgs p) {
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < p.K; ++k) {
             const int pair = tok * p.K + k;
-            if (w4_expert(p, pair) >= 0) sum += *reinterpret_cast<const f32x4 *>(p.obuf + (size_t)pair * p.H + n);
+            if (w4_expert(p, pair) < 0) continue;
+            f32x4 v = *reinterpret_cast<const f32x4 *>(p.obuf + (size_t)pair * p.slices * p.H + n);
+            for (int sl = 1; sl < p.slices; ++sl) v += *reinterpret_cast<const f32x4 *>(p.obuf + ((size_t)pair * p.slices + sl) * p.H + n);
+            sum += v;
         }
         u32x2 out;
         out[0] = T::from_f32x2(sum[0], sum[1]);
@@ -243,6 +248,8 @@ struct W4MoePlan {
     int tt;                  // blocks of 16 tokens per task; 0: one token
     int r1, r2;              // row groups per workgroup of the gate/up and of the down kernel
     int max_tasks;
+    bool panels;             // tasks of 4 or 8 blocks run panels
+    int slices;              // of their down projection
 };
 
 #define MLK_W4_MOE(KERNEL, GRID, WAVES, LDS, ...)                                          \
@@ -288,16 +295,8 @@ int w4_launch_moe(const W4MoeArgs &a, const W4MoePlan &pl, hipStream_t s) {
         if (pl.r2 == 2) return w4_moe1_down<T, GS, ZP, 2>(a, s);
         return w4_moe1_down<T, GS, ZP, 4>(a, s);
     }
-    if (pl.tt == 1) {
-        rc = pl.r1 == 8 ? w4_moe_gate_up<T, GS, ZP, 1, 8>(a, pl.max_tasks, s) : w4_moe_gate_up<T, GS, ZP, 1, 4>(a, pl.max_tasks, s);
-        if (rc == MLK_OK) rc = pl.r2 == 8 ? w4_moe_down<T, GS, ZP, 1, 8>(a, pl.max_tasks, s) : w4_moe_down<T, GS, ZP, 1, 4>(a, pl.max_tasks, s);
-    } else if (pl.tt == 2) {
-        rc = w4_moe_gate_up<T, GS, ZP, 2, 4>(a, pl.max_tasks, s);
-        if (rc == MLK_OK) rc = w4_moe_down<T, GS, ZP, 2, 4>(a, pl.max_tasks, s);
-    } else {
-        rc = w4_moe_gate_up<T, GS, ZP, 4, 4>(a, pl.max_tasks, s);
-        if (rc == MLK_OK) rc = w4_moe_down<T, GS, ZP, 4, 4>(a, pl.max_tasks, s);
-    }
+    rc = w4_moe_gate_up<T, GS, ZP, 1, 8>(a, pl.max_tasks, s);
+    if (rc == MLK_OK) rc = w4_moe_down<T, GS, ZP, 1, 8>(a, pl.max_tasks, s);
     if (rc != MLK_OK) return rc;
     w4_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
     MLK_LAUNCH_CHECK();

@@ -1,11 +1,15 @@
 // Expert layers over 4-bit weights: arguments, workspace, passes.
-#include "mlk_w4_moe.cuh"
+#include <initializer_list>
+
+#include "mlk_w4_moe_panel.cuh"
 
 namespace mlk {
 
 #define MLK_W4_EXTERN(T, GS)                                                                              \
     extern template int w4_launch_moe<T, GS, false>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);   \
-    extern template int w4_launch_moe<T, GS, true>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);
+    extern template int w4_launch_moe<T, GS, true>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);    \
+    extern template int w4_launch_moe_panel<T, GS, false>(const W4MoeArgs &, const W4MoePlan &, const int32_t *, int, hipStream_t);   \
+    extern template int w4_launch_moe_panel<T, GS, true>(const W4MoeArgs &, const W4MoePlan &, const int32_t *, int, hipStream_t);
 MLK_W4_EXTERN(F16, 4)
 MLK_W4_EXTERN(F16, 2)
 MLK_W4_EXTERN(F16, 1)
@@ -22,7 +26,8 @@ constexpr int kW4MoePairs = 16384;      // routed pairs of a pass: bounds the sc
 static int w4_moe_pass_tokens(int n_tokens, int topk) { return n_tokens < kW4MoePairs / topk ? n_tokens : kW4MoePairs / topk; }
 
 static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter) {
-    W4MoePlan pl;
+    W4MoePlan pl = {};
+    pl.slices = 1;
     const int cus = device_cus(), pairs = tokens * topk;
     if (tokens == 1) {
         pl.tt = 0;
@@ -33,12 +38,24 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
         pl.max_tasks = topk;
         return pl;
     }
+    // Routed pairs of an expert that is reached.  Up to 16 on average the streaming kernels, one block of 16 tokens a task; above, panels: 8 experts of
+    // 4096 x 14336, top-2, at 48 tokens (12) 196 us against 224 with panels of 64 tokens, at 100 (25) 285 against 240; 64 experts of 2048 x 1408, top-6, at 100
+    // tokens (9) 111 against 120, at 200 (19) 150 against 127.  Panels of 128 tokens from 110 on: 8 experts at 500 tokens (125) 550 us both, at 1000 (250)
+    // 871 against 911; 64 experts at 1000 (94) 271 against 253, at 2000 (188) 404 against 424.
     const int reached = pairs < E ? pairs : E, load = (pairs + reached - 1) / reached;
-    pl.tt = load <= 16 ? 1 : (load <= 32 ? 2 : 4);
-    pl.r1 = pl.r2 = pl.tt == 1 ? 8 : 4;
+    pl.panels = load > 16 && (int64_t)tokens * hidden < (1ll << 31);
+    pl.tt = pl.panels ? (load <= 110 ? 4 : 8) : 1;
     // an expert's last task may be short: at most one more than its blocks fill
     const int64_t most = (int64_t)E + pairs / (16 * pl.tt);
     pl.max_tasks = (int)(most < pairs ? most : pairs);
+    if (!pl.panels) {
+        pl.r1 = pl.r2 = 8;
+        return pl;
+    }
+    // Two K slices of a long down projection that would leave CUs without a panel in its last round: 8 experts of 4096 x 14336 at 100 tokens 276 -> 240 us, at
+    // 1000 871 -> 830; with 16 windows (2048) or panels for two rounds the second sum costs more (64 experts at 300 tokens 144 -> 161).
+    const int wgs = (hidden + 255) / 256 * reached * ((load + 16 * pl.tt - 1) / (16 * pl.tt));
+    if (wgs < 2 * cus && inter / 128 >= 64) pl.slices = 2;
     return pl;
 }
 
@@ -47,9 +64,10 @@ struct W4MoeWorkspace {
     int32_t *n_tasks, *sorted, *cumsum, *padded, *experts_ids;
     uint16_t *hbuf;
     float *obuf;
+    u32x4 *sums1, *sums2;
 };
 
-static size_t w4_moe_carve(uint8_t *base, int tokens, int E, int topk, int hidden, int inter, W4MoeWorkspace *ws) {
+static size_t w4_moe_carve(uint8_t *base, const W4MoePlan &pl, int tokens, int E, int topk, int hidden, int inter, int group, W4MoeWorkspace *ws) {
     const int64_t pairs = (int64_t)tokens * topk, padded = pairs + E * 15, blocks = (padded + 15) / 16;
     size_t off = 0;
     auto take = [&](size_t bytes) {
@@ -65,7 +83,10 @@ static size_t w4_moe_carve(uint8_t *base, int tokens, int E, int topk, int hidde
     w.padded = (int32_t *)take(sizeof(int32_t));
     w.experts_ids = (int32_t *)take(sizeof(int32_t) * (size_t)blocks);
     w.hbuf = (uint16_t *)take((size_t)blocks * 16 * inter * 2);
-    w.obuf = (float *)take((size_t)pairs * hidden * 4);
+    w.obuf = (float *)take((size_t)pairs * pl.slices * hidden * 4);
+    const int gs = group < 128 ? group / 32 : 4;
+    w.sums1 = (u32x4 *)take(pl.panels ? (size_t)tokens * w4_sum_pitch(hidden, gs) * 16 : 0);
+    w.sums2 = (u32x4 *)take(pl.panels ? (size_t)blocks * 16 * w4_sum_pitch(inter, gs) * 16 : 0);
     if (ws) *ws = w;
     return off;
 }
@@ -76,9 +97,17 @@ using namespace mlk;
 
 extern "C" {
 
-size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int hidden, int inter) {
-    if (n_tokens <= 0 || n_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0) return 0;
-    return w4_moe_carve(nullptr, w4_moe_pass_tokens(n_tokens, topk), n_experts, topk, hidden, inter, nullptr);
+// What a call needs: a long one goes in passes of one size and a shorter last one, whose plan may differ.
+size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int hidden, int inter, int group) {
+    if (n_tokens <= 0 || n_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0 || group < 32) return 0;
+    const int step = w4_moe_pass_tokens(n_tokens, topk), rest = n_tokens % step;
+    size_t most = 0;
+    for (int t : {step, rest}) {
+        if (t == 0) continue;
+        const size_t need = w4_moe_carve(nullptr, w4_moe_plan(t, n_experts, topk, hidden, inter), t, n_experts, topk, hidden, inter, group, nullptr);
+        if (need > most) most = need;
+    }
+    return most;
 }
 
 int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_zero, const void *w2, const void *w2_scale, const void *w2_zero,
@@ -101,7 +130,7 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
                 "experts w4: weights, activations, outputs and workspace must lie on 16 bytes");
     MLK_REQUIRE((((uintptr_t)w1_scale | (uintptr_t)w2_scale) & 7) == 0 && (((uintptr_t)w1_zero | (uintptr_t)w2_zero) & 3) == 0,
                 "experts w4: scales must lie on 8 bytes, zero points on 4");
-    if (workspace_bytes < mlk_experts_w4_workspace_bytes(n_tokens, n_experts, topk, hidden, inter))
+    if (workspace_bytes < mlk_experts_w4_workspace_bytes(n_tokens, n_experts, topk, hidden, inter, group))
         return fail(MLK_ERR_WORKSPACE, "experts w4: workspace too small");
     hipStream_t s = (hipStream_t)stream;
     W4MoeArgs a;
@@ -125,14 +154,18 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
         a.Y = (uint16_t *)y + (size_t)t0 * hidden;
         a.ids = topk_ids + (size_t)t0 * topk;
         a.wts = (const uint16_t *)topk_weights + (size_t)t0 * topk;
+        const W4MoePlan pl = w4_moe_plan(a.T, n_experts, topk, hidden, inter);
         W4MoeWorkspace ws;
-        w4_moe_carve((uint8_t *)workspace, a.T, n_experts, topk, hidden, inter, &ws);
+        w4_moe_carve((uint8_t *)workspace, pl, a.T, n_experts, topk, hidden, inter, group, &ws);
         a.sorted = ws.sorted;
         a.tasks = ws.tasks;
         a.n_tasks = ws.n_tasks;
         a.hbuf = ws.hbuf;
         a.obuf = ws.obuf;
-        const W4MoePlan pl = w4_moe_plan(a.T, n_experts, topk, hidden, inter);
+        a.slices = pl.slices;
+        a.sums1 = ws.sums1;
+        a.sums2 = ws.sums2;
+        const int max_slots = (int)(((int64_t)a.n_pairs + n_experts * 15 + 15) / 16 * 16);
         int rc = MLK_OK;
         if (pl.tt) {
             rc = launch_moe_align(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks,
@@ -140,7 +173,13 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
             if (rc != MLK_OK) return rc;
         }
         const bool zp = w1_zero != nullptr, f16 = x_kind == MLK_F16;
-#define MLK_W4_GO(T, GS) rc = zp ? w4_launch_moe<T, GS, true>(a, pl, s) : w4_launch_moe<T, GS, false>(a, pl, s)
+#define MLK_W4_GO(T, GS)                                                                                                                     \
+    do {                                                                                                                                         \
+        if (pl.panels)                                                                                                                           \
+            rc = zp ? w4_launch_moe_panel<T, GS, true>(a, pl, ws.padded, max_slots, s) : w4_launch_moe_panel<T, GS, false>(a, pl, ws.padded, max_slots, s); \
+        else                                                                                                                                     \
+            rc = zp ? w4_launch_moe<T, GS, true>(a, pl, s) : w4_launch_moe<T, GS, false>(a, pl, s);                                              \
+    } while (0)
         if (group == 32) {
             if (f16) MLK_W4_GO(F16, 1);
             else MLK_W4_GO(BF16, 1);

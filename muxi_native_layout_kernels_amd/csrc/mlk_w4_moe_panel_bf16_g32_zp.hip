@@ -1,0 +1,6 @@
+// Panels of the expert layers over 4-bit weights: bf16 activations, groups of 32 weights, with zero points.
+#include "mlk_w4_moe_panel.cuh"
+
+namespace mlk {
+template int w4_launch_moe_panel<BF16, 1, true>(const W4MoeArgs &, const W4MoePlan &, const int32_t *, int, hipStream_t);
+}  // namespace mlk

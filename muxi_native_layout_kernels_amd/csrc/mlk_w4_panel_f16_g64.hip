@@ -1,0 +1,6 @@
+// Panels of the 4-bit linear layers: f16 activations, groups of 64 weights, without zero points.
+#include "mlk_w4_panel_gemm.cuh"
+
+namespace mlk {
+template int w4_launch_panel<F16, 2, false>(const W4PanelArgs &, int, hipStream_t);
+}  // namespace mlk

@@ -711,7 +711,7 @@ def _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, what):
         _check(bias is None or (bias.dtype == B.dtype and bias.numel() == m), "bias must be [1, m] of the activation dtype")
         _check_tensors(((A, "A"), (A_Scale, "A_Scale"), (B, "B"), (A_Zero, "A_Zero"), (bias, "bias")), B.device)
         lib = _lib.load()
-        plan = _plans[key] = (B.size(0), m, k, group, _KIND[B.dtype], lib.mlk_gemm_w4_workspace_bytes(B.size(0), m, k),
+        plan = _plans[key] = (B.size(0), m, k, group, _KIND[B.dtype], lib.mlk_gemm_w4_workspace_bytes(B.size(0), m, k, group),
                               lib.mlk_gemm_counter_bytes(), lib.mlk_gemm_layout_a_w4)
     n, m, k, group, kind, ws_need, counter_bytes, fn = plan
     with _OnDevice(B):
@@ -968,7 +968,7 @@ def fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2
                      (w2_scale, "w2_scale"), (w1_zero, "w1_zero"), (w2_zero, "w2_zero"), (experts_map, "experts_map")), x.device)
         lib = _lib.load()
         plan = _plans[key] = (x.size(0), E, E if experts_map is None else experts_map.numel(), K, hidden, inter, group, _KIND[x.dtype],
-                              lib.mlk_experts_w4_workspace_bytes(x.size(0), E, K, hidden, inter), lib.mlk_fused_experts_w4)
+                              lib.mlk_experts_w4_workspace_bytes(x.size(0), E, K, hidden, inter, group), lib.mlk_fused_experts_w4)
     T, E, E_router, K, hidden, inter, group, kind, ws_need, fn = plan
     with _OnDevice(x):
         if x.data_ptr() & 15:
