@@ -6,8 +6,9 @@
 //   softmax  dx = p (g - sum p g),      sigmoid  dx = p (1 - sigmoid) (g - sum p g).
 // A row whose probabilities sum to nothing (all logits -inf) has p = 0.
 //
-// Forward: a workgroup takes a chunk of consecutive tokens and walks the sequences that it meets; E / 4 lanes hold a token, four experts each,
-// so that a wave takes 64 / lanes tokens at a time.  Its sums for (chunk c, sequence s) go to slot c + s: going through the tokens either the
+// Forward: a workgroup takes a chunk of consecutive tokens and walks the sequences that it meets; 4 to 16 lanes hold a token, 4 to 16 experts each, so that
+// a wave takes at least four tokens at a time and a sum over the experts is at most four exchanges within 16 lanes (32749 tokens x 256 experts in
+// fp32: with 64 lanes of four experts a token and six exchanges through LDS 22 us forward and 33 backward).  Its sums for (chunk c, sequence s) go to slot c + s: going through the tokens either the
 // chunk or the sequence moves on, so no two share a slot.  A second launch adds the slots of a sequence in order, for 64 experts a workgroup; the last
 // workgroup adds their shares of the loss.  No floating-point atomics: the results do not depend on the order in which workgroups run.
 // Backward: the same walk, the logits are read again and their gradient written.
@@ -65,60 +66,83 @@ struct Bal16 {
     __device__ static __forceinline__ void store(void *p, size_t i, float v) { reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)T::from_f32(v); }
 };
 
-template <class L>
-__device__ __forceinline__ void bal_load(const BalanceArgs &p, int t, int e0, float (&x)[4]) {
-    const size_t at = (size_t)t * p.E + e0;
-    if (p.vec) {
-        if (e0 < p.E) L::unpack(*reinterpret_cast<const typename L::V4 *>(reinterpret_cast<const char *>(p.logits) + at * (sizeof(typename L::V4) / 4)), x);
-    } else {
+// Experts of a lane: vector v holds 4 (v LPT + lane) .. + 3.
+template <int LPT>
+__device__ __forceinline__ int bal_expert(int v, int l) { return (v * LPT + l) * 4; }
+
+template <class L, int LPT, int NV>
+__device__ __forceinline__ void bal_load(const BalanceArgs &p, int t, int l, float (&x)[NV][4]) {
+    const size_t row = (size_t)t * p.E;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (e0 + i < p.E) x[i] = L::load(p.logits, at + i);
+    for (int v = 0; v < NV; ++v) {
+        const int e0 = bal_expert<LPT>(v, l);
+        if (p.vec) {
+            if (e0 < p.E)
+                L::unpack(*reinterpret_cast<const typename L::V4 *>(reinterpret_cast<const char *>(p.logits) + (row + e0) * (sizeof(typename L::V4) / 4)), x[v]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e0 + i < p.E) x[v][i] = L::load(p.logits, row + e0 + i);
+        }
     }
 }
 
-template <int LPT>
-__device__ __forceinline__ float bal_sum(float v) {
-#pragma unroll
-    for (int m = 1; m < LPT; m <<= 1) v += __shfl_xor(v, m);
+// A value of another lane of the same 16, without LDS: lane ^ 1, lane ^ 2 (quad_perm), the other quad of 8 and the other 8 (mirrors).
+template <int STEP>
+__device__ __forceinline__ float bal_other(float v) {
+    constexpr int ctrl = STEP == 1 ? 0xb1 : (STEP == 2 ? 0x4e : (STEP == 4 ? 0x141 : 0x140));
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), ctrl, 0xf, 0xf, true));
+}
+template <int LPT, class F>
+__device__ __forceinline__ float bal_fold(float v, F f) {
+    v = f(v, bal_other<1>(v));
+    v = f(v, bal_other<2>(v));
+    if constexpr (LPT >= 8) v = f(v, bal_other<4>(v));
+    if constexpr (LPT >= 16) v = f(v, bal_other<8>(v));
     return v;
 }
 template <int LPT>
-__device__ __forceinline__ float bal_max(float v) {
-#pragma unroll
-    for (int m = 1; m < LPT; m <<= 1) v = fmaxf(v, __shfl_xor(v, m));
+__device__ __forceinline__ float bal_sum(float v) { return bal_fold<LPT>(v, [](float a, float b) { return a + b; }); }
+template <int LPT>
+__device__ __forceinline__ float bal_max(float v) { return bal_fold<LPT>(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float bal_wave_sum(float v) {
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
     return v;
 }
 
-// Probabilities of one token, four experts a lane (0 beyond the last expert); `sig`: the sigmoids.
-template <int LPT>
-__device__ __forceinline__ void bal_probs(const BalanceArgs &p, int e0, const float (&x)[4], float (&pr)[4], float (&sig)[4]) {
-    float sum = 0.f;
+// Probabilities of one token (0 beyond the last expert); `sig`: the sigmoids.
+template <int LPT, int NV>
+__device__ __forceinline__ void bal_probs(const BalanceArgs &p, int l, const float (&x)[NV][4], float (&pr)[NV][4], float (&sig)[NV][4]) {
+    float sum = 0.f, m = -INFINITY;
     if (p.score_fun == 0) {
-        float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (e0 + i < p.E) m = fmaxf(m, x[i]);
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (bal_expert<LPT>(v, l) + i < p.E) m = fmaxf(m, x[v][i]);
         m = bal_max<LPT>(m);
         if (m == -INFINITY) m = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sig[i] = 0.f;
-            pr[i] = e0 + i < p.E ? expf(x[i] - m) : 0.f;
-            sum += pr[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sig[i] = e0 + i < p.E ? 1.f / (1.f + expf(-x[i])) : 0.f;
-            pr[i] = sig[i];
-            sum += pr[i];
-        }
     }
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool is = bal_expert<LPT>(v, l) + i < p.E;
+            sig[v][i] = 0.f;
+            if (p.score_fun == 0) {
+                pr[v][i] = is ? expf(x[v][i] - m) : 0.f;
+            } else {
+                sig[v][i] = is ? 1.f / (1.f + expf(-x[v][i])) : 0.f;
+                pr[v][i] = sig[v][i];
+            }
+            sum += pr[v][i];
+        }
     sum = bal_sum<LPT>(sum);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pr[i] *= inv;
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pr[v][i] *= inv;
 }
 
 // First sequence that ends behind token t (S if there is none).
@@ -137,13 +161,13 @@ __device__ __forceinline__ void bal_range(const BalanceArgs &p, int s, int &a, i
     b = p.cu ? min(p.cu[s + 1], p.T) : p.T;
 }
 
-template <class L, int LPT>
+template <class L, int LPT, int NV>
 __global__ void __launch_bounds__(kBalThreads) balance_partial_kernel(BalanceArgs p) {
-    constexpr int ROWS = kBalThreads / LPT;                 // tokens at a time
-    __shared__ float sums[ROWS * LPT * 4];
+    constexpr int ROWS = kBalThreads / LPT, COLS = LPT * NV * 4;         // tokens at a time, experts with room for
+    __shared__ float sums[ROWS * COLS];
     __shared__ int32_t cnt[kBalExperts];
     __shared__ int32_t valid;
-    const int tid = threadIdx.x, row = tid / LPT, e0 = (tid % LPT) * 4;
+    const int tid = threadIdx.x, row = tid / LPT, l = tid % LPT;
     const int c0 = blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, p.T);
     if (blockIdx.x == 0)
         for (int e = tid; e < p.E; e += kBalThreads) p.counts[e] = 0;        // the second launch adds to them
@@ -161,25 +185,28 @@ __global__ void __launch_bounds__(kBalThreads) balance_partial_kernel(BalanceArg
             const int e = p.ids[i];
             if (e >= 0 && e < p.E && (!p.mask || p.mask[i / p.K])) atomicAdd(&cnt[e], 1);
         }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float sum[NV][4] = {};
         int n = 0;
         for (int t = a + row; t < b; t += ROWS) {
             if (p.mask && !p.mask[t]) continue;             // the lanes of a token agree
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, pr[4], sig[4];
-            bal_load<L>(p, t, e0, x);
-            bal_probs<LPT>(p, e0, x, pr, sig);
+            float x[NV][4] = {}, pr[NV][4], sig[NV][4];
+            bal_load<L, LPT, NV>(p, t, l, x);
+            bal_probs<LPT, NV>(p, l, x, pr, sig);
             ++n;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += pr[i];
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[v][i] += pr[v][i];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[row * LPT * 4 + e0 + i] = sum[i];
-        if (e0 == 0 && n) atomicAdd(&valid, n);
+        for (int v = 0; v < NV; ++v)
+            *reinterpret_cast<f32x4 *>(&sums[row * COLS + bal_expert<LPT>(v, l)]) = f32x4{sum[v][0], sum[v][1], sum[v][2], sum[v][3]};
+        if (l == 0 && n) atomicAdd(&valid, n);
         __syncthreads();
         const size_t slot = (size_t)blockIdx.x + s;
         for (int e = tid; e < p.E; e += kBalThreads) {
             float v = 0.f;
-            for (int r = 0; r < ROWS; ++r) v += sums[r * LPT * 4 + e];
+            for (int r = 0; r < ROWS; ++r) v += sums[r * COLS + e];
             p.P[slot * p.E + e] = v;
             p.cnt[slot * p.E + e] = cnt[e];
         }
@@ -251,7 +278,7 @@ __global__ void __launch_bounds__(1024) balance_reduce_kernel(BalanceArgs p) {
             if (cs) atomicAdd(&p.counts[e], cs);
             share_of_loss = g * ps;
         }
-        share_of_loss = bal_sum<64>(share_of_loss);
+        share_of_loss = bal_wave_sum(share_of_loss);
         // agent-scope stores: the caches of the XCDs are not coherent for ordinary ones
         if (lane == 0) {
             __hip_atomic_store(&p.part[(size_t)s * gridDim.x + blockIdx.x], share_of_loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -267,14 +294,14 @@ __global__ void __launch_bounds__(1024) balance_reduce_kernel(BalanceArgs p) {
     const int total = gridDim.x * gridDim.y;
     float v = 0.f;
     for (int i = lane; i < total; i += 64) v += __hip_atomic_load(&p.part[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    v = bal_sum<64>(v);
+    v = bal_wave_sum(v);
     if (lane == 0) *p.loss = v;
 }
 
-template <class L, int LPT>
+template <class L, int LPT, int NV>
 __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(BalanceArgs p) {
     constexpr int ROWS = kBalThreads / LPT;
-    const int tid = threadIdx.x, row = tid / LPT, e0 = (tid % LPT) * 4;
+    const int tid = threadIdx.x, row = tid / LPT, l = tid % LPT;
     const int c0 = blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, p.T);
     const float up = *p.grad;
     int s = bal_first(p, c0);
@@ -285,35 +312,46 @@ __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(BalanceArgs p
             counts = s < p.S && p.cu[s] <= t;
         }
         if (p.mask && !p.mask[t]) counts = false;
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        float d[NV][4] = {};
         if (counts) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, pr[4], sig[4], g[4] = {0.f, 0.f, 0.f, 0.f};
-            bal_load<L>(p, t, e0, x);
-            bal_probs<LPT>(p, e0, x, pr, sig);
+            float x[NV][4] = {}, pr[NV][4], sig[NV][4], g[NV][4] = {};
+            bal_load<L, LPT, NV>(p, t, l, x);
+            const float *share = p.share + (size_t)s * p.E;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (bal_expert<LPT>(v, l) + i < p.E) g[v][i] = share[bal_expert<LPT>(v, l) + i];
+            bal_probs<LPT, NV>(p, l, x, pr, sig);
             float dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (e0 + i < p.E) g[i] = p.share[(size_t)s * p.E + e0 + i];
-                dot = fmaf(pr[i], g[i], dot);
-            }
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dot = fmaf(pr[v][i], g[v][i], dot);
             dot = bal_sum<LPT>(dot);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] = pr[i] * (1.f - sig[i]) * (g[i] - dot) * up;
-        }
-        const size_t at = (size_t)t * p.E + e0;
-        if (p.vec) {
-            if (e0 < p.E) *reinterpret_cast<typename L::V4 *>(reinterpret_cast<char *>(p.dlogits) + at * (sizeof(typename L::V4) / 4)) = L::pack(d);
-        } else {
+            for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (e0 + i < p.E) L::store(p.dlogits, at + i, d[i]);
+                for (int i = 0; i < 4; ++i) d[v][i] = pr[v][i] * (1.f - sig[v][i]) * (g[v][i] - dot) * up;
+        }
+        const size_t at = (size_t)t * p.E;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int e0 = bal_expert<LPT>(v, l);
+            if (p.vec) {
+                if (e0 < p.E) *reinterpret_cast<typename L::V4 *>(reinterpret_cast<char *>(p.dlogits) + (at + e0) * (sizeof(typename L::V4) / 4)) = L::pack(d[v]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (e0 + i < p.E) L::store(p.dlogits, at + e0 + i, d[v][i]);
+            }
         }
     }
 }
 
-// counts[e] += pairs routed to e; integer atomics: any order gives the same sums.
+// counts[e] += pairs routed to e (integer atomics: any order gives the same sums), or, in one workgroup and not to be added to, counts[e] = that.
 __global__ void __launch_bounds__(256) expert_counts_kernel(const int32_t *__restrict__ ids, const uint8_t *__restrict__ mask, int64_t pairs, int K, int E,
-                                                            int32_t *__restrict__ counts) {
+                                                            int32_t *__restrict__ counts, bool store) {
     __shared__ int32_t cnt[kBalExperts];
     for (int e = threadIdx.x; e < E; e += 256) cnt[e] = 0;
     __syncthreads();
@@ -322,8 +360,13 @@ __global__ void __launch_bounds__(256) expert_counts_kernel(const int32_t *__res
         if (e >= 0 && e < E && (!mask || mask[i / K])) atomicAdd(&cnt[e], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += 256)
-        if (cnt[e]) atomicAdd(&counts[e], cnt[e]);
+    for (int e = threadIdx.x; e < E; e += 256) {
+        if (store) counts[e] = cnt[e];
+        else if (cnt[e]) atomicAdd(&counts[e], cnt[e]);
+    }
+}
+__global__ void __launch_bounds__(256) expert_counts_zero_kernel(int32_t *counts, int E) {
+    if ((int)threadIdx.x < E) counts[threadIdx.x] = 0;
 }
 
 // -------------------------------------------------------------------------------------------------------------------- host
@@ -370,16 +413,16 @@ static int balance_vec(const void *p, int x_kind, int E) { return E % 4 == 0 && 
 
 template <class L>
 static void balance_launch(const BalanceArgs &a, bool grad, hipStream_t s) {
-#define MLK_BAL(LPT)                                                                           \
+#define MLK_BAL(LPT, NV)                                                                       \
     do {                                                                                       \
-        if (grad) balance_grad_kernel<L, LPT><<<a.chunks, kBalThreads, 0, s>>>(a);             \
-        else balance_partial_kernel<L, LPT><<<a.chunks, kBalThreads, 0, s>>>(a);               \
+        if (grad) balance_grad_kernel<L, LPT, NV><<<a.chunks, kBalThreads, 0, s>>>(a);         \
+        else balance_partial_kernel<L, LPT, NV><<<a.chunks, kBalThreads, 0, s>>>(a);           \
     } while (0)
-    if (a.E <= 16) MLK_BAL(4);
-    else if (a.E <= 32) MLK_BAL(8);
-    else if (a.E <= 64) MLK_BAL(16);
-    else if (a.E <= 128) MLK_BAL(32);
-    else MLK_BAL(64);
+    if (a.E <= 16) MLK_BAL(4, 1);
+    else if (a.E <= 32) MLK_BAL(8, 1);
+    else if (a.E <= 64) MLK_BAL(16, 1);
+    else if (a.E <= 128) MLK_BAL(16, 2);
+    else MLK_BAL(16, 4);
 #undef MLK_BAL
 }
 static void balance_launch_kind(const BalanceArgs &a, int x_kind, bool grad, hipStream_t s) {
@@ -399,14 +442,21 @@ using namespace mlk;
 
 extern "C" {
 
-int mlk_expert_counts(const int32_t *topk_ids, const uint8_t *token_mask, int n_tokens, int topk, int n_experts, int32_t *counts, void *stream) {
+int mlk_expert_counts(const int32_t *topk_ids, const uint8_t *token_mask, int n_tokens, int topk, int n_experts, int accumulate, int32_t *counts,
+                      void *stream) {
     MLK_REQUIRE(n_tokens >= 0 && topk >= 1, "expert_counts: negative token count, or no picks");
     MLK_REQUIRE(n_experts >= 1 && n_experts <= kBalExperts, "expert_counts: 1..256 experts");
-    if (n_tokens == 0) return MLK_OK;
-    MLK_REQUIRE(topk_ids && counts, "expert_counts: null pointer");
+    MLK_REQUIRE(counts && (n_tokens == 0 || topk_ids), "expert_counts: null pointer");
+    hipStream_t s = (hipStream_t)stream;
+    // one workgroup up to 4096 pairs: it needs no zeros to add to, and takes 3 us for them
     const int64_t pairs = (int64_t)n_tokens * topk;
-    const int64_t wgs = std::min<int64_t>((pairs + 1023) / 1024, 256);
-    expert_counts_kernel<<<(int)wgs, 256, 0, (hipStream_t)stream>>>(topk_ids, token_mask, pairs, topk, n_experts, counts);
+    const int64_t wgs = pairs <= 4096 ? 1 : std::min<int64_t>((pairs + 1023) / 1024, 256);
+    if (!accumulate && wgs > 1) {
+        expert_counts_zero_kernel<<<1, 256, 0, s>>>(counts, n_experts);
+        MLK_LAUNCH_CHECK();
+    }
+    if (pairs == 0 && accumulate) return MLK_OK;
+    expert_counts_kernel<<<(int)wgs, 256, 0, s>>>(topk_ids, token_mask, pairs, topk, n_experts, counts, !accumulate && wgs == 1);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }

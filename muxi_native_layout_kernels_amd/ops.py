@@ -997,16 +997,17 @@ def _check_routing(experts_ids, token_mask, device):
 def expert_counts(experts_ids, n_experts, token_mask=None, out=None):
     """How many routed pairs each expert got: int32 [n_experts].  experts_ids int32 [T, K] (`fused_routing_gate`), ids outside 0..n_experts-1
     count nowhere; token_mask bool [T]: False for padded rows.  With `out` the counts are added to it, for a load that builds up over
-    the steps of a server; the call then is one launch."""
+    the steps of a server."""
     _check_routing(experts_ids, token_mask, experts_ids.device)
     _check(1 <= n_experts <= 256, "1..256 experts")
     with _OnDevice(experts_ids):
-        if out is None:
-            out = torch.zeros(n_experts, dtype=torch.int32, device=experts_ids.device)
-        else:
+        add = out is not None
+        if add:
             _check(out.dtype == torch.int32 and tuple(out.shape) == (n_experts,), "out must be int32 [n_experts]")
             _check_tensors(((out, "out"),), experts_ids.device)
-        rc = _lib.load().mlk_expert_counts(experts_ids.data_ptr(), _ptr(token_mask), experts_ids.size(0), experts_ids.size(1), n_experts,
+        else:
+            out = torch.empty(n_experts, dtype=torch.int32, device=experts_ids.device)
+        rc = _lib.load().mlk_expert_counts(experts_ids.data_ptr(), _ptr(token_mask), experts_ids.size(0), experts_ids.size(1), n_experts, add,
                                            out.data_ptr(), _stream_of(experts_ids))
         if rc != 0:
             _lib.check(rc, "expert_counts")
@@ -1016,24 +1017,27 @@ def expert_counts(experts_ids, n_experts, token_mask=None, out=None):
 _LOGIT_KIND = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 3}
 
 
+def _balance_forward(logits, ids, mask, cu, score_fun, coef, plan):
+    T, E, K, kind, n_seq, ws_need, counter_bytes, fn, _ = plan
+    with _OnDevice(logits):
+        device, stream = logits.device, _stream_of(logits)
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        counts = torch.empty(E, dtype=torch.int32, device=device)
+        share = torch.empty(n_seq * E, dtype=torch.float32, device=device)
+        ws = _balance_pool.get(device, stream, ws_need, counter_bytes)
+        rc = fn(logits.data_ptr(), kind, score_fun, T, E, K, ids.data_ptr(), _ptr(mask), _ptr(cu), n_seq, coef, loss.data_ptr(), counts.data_ptr(),
+                share.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        if rc != 0:
+            _lib.check(rc, "moe_balance_loss")
+    return loss, counts, share
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, ids, mask, cu, score_fun, coef):
-        T, E = logits.shape
-        n_seq = 1 if cu is None else cu.numel() - 1
-        lib = _lib.load()
-        with _OnDevice(logits):
-            stream = _stream_of(logits)
-            loss = torch.empty((), dtype=torch.float32, device=logits.device)
-            counts = torch.empty(E, dtype=torch.int32, device=logits.device)
-            share = torch.empty((n_seq, E), dtype=torch.float32, device=logits.device)
-            ws = _balance_pool.get(logits.device, stream, lib.mlk_balance_workspace_bytes(T, E, n_seq), lib.mlk_balance_counter_bytes())
-            rc = lib.mlk_balance_loss(logits.data_ptr(), _LOGIT_KIND[logits.dtype], score_fun, T, E, ids.size(1), ids.data_ptr(), _ptr(mask), _ptr(cu),
-                                      n_seq, coef, loss.data_ptr(), counts.data_ptr(), share.data_ptr(), ws.data_ptr(), ws.numel(), stream)
-            if rc != 0:
-                _lib.check(rc, "moe_balance_loss")
+    def forward(ctx, logits, ids, mask, cu, score_fun, coef, plan):
+        loss, counts, share = _balance_forward(logits, ids, mask, cu, score_fun, coef, plan)
         ctx.save_for_backward(logits, mask, cu, share)
-        ctx.score_fun, ctx.n_seq = score_fun, n_seq
+        ctx.score_fun, ctx.plan = score_fun, plan
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts
@@ -1042,15 +1046,16 @@ class _BalanceLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss, _):
         if dloss is None:
-            return None, None, None, None, None, None
+            return None, None, None, None, None, None, None
         logits, mask, cu, share = ctx.saved_tensors
+        T, E, _, kind, n_seq, _, _, _, fn = ctx.plan
         with _OnDevice(logits):
             grad = torch.empty_like(logits)
-            rc = _lib.load().mlk_balance_loss_grad(logits.data_ptr(), _LOGIT_KIND[logits.dtype], ctx.score_fun, logits.size(0), logits.size(1), _ptr(mask),
-                                                   _ptr(cu), ctx.n_seq, share.data_ptr(), dloss.data_ptr(), grad.data_ptr(), _stream_of(logits))
+            rc = fn(logits.data_ptr(), kind, ctx.score_fun, T, E, _ptr(mask), _ptr(cu), n_seq, share.data_ptr(), dloss.data_ptr(), grad.data_ptr(),
+                    _stream_of(logits))
             if rc != 0:
                 _lib.check(rc, "moe_balance_loss")
-        return grad, None, None, None, None, None
+        return grad, None, None, None, None, None, None
 
 
 def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0, token_mask=None, cu_seqlens=None):
@@ -1063,17 +1068,30 @@ def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0,
     gating_output [T, E] fp16 / bf16 / fp32, E <= 256; experts_ids int32 [T, K] (`fused_routing_gate`); token_mask bool [T], False for padded
     tokens; cu_seqlens int32 [sequences + 1] on the device, non-decreasing, where each sequence begins and the last one ends (None: all tokens are
     one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0."""
-    _check(gating_output.dim() == 2 and 1 <= gating_output.size(1) <= 256, "gating_output must be [T, E], at most 256 experts")
-    _check(gating_output.dtype in _LOGIT_KIND, "gating_output must be fp16, bf16 or fp32")
-    _check(gating_output.is_cuda and gating_output.is_contiguous(), "gating_output must be a contiguous CUDA tensor")
-    _check_routing(experts_ids, token_mask, gating_output.device)
-    _check(experts_ids.size(0) == gating_output.size(0), "experts_ids must be int32 [T, K]")
+    logits = gating_output
+    key = ("balance", logits.shape, logits.dtype, logits.device, experts_ids.shape, experts_ids.dtype, experts_ids.device,
+           None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.device),
+           None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.dtype, cu_seqlens.device))
+    plan = _plans.get(key)
+    if plan is None or not (logits.is_contiguous() and experts_ids.is_contiguous() and (token_mask is None or token_mask.is_contiguous()) and
+                            (cu_seqlens is None or cu_seqlens.is_contiguous())):
+        _check(logits.dim() == 2 and 1 <= logits.size(1) <= 256, "gating_output must be [T, E], at most 256 experts")
+        _check(logits.dtype in _LOGIT_KIND, "gating_output must be fp16, bf16 or fp32")
+        _check(logits.is_cuda and logits.is_contiguous(), "gating_output must be a contiguous CUDA tensor")
+        _check_routing(experts_ids, token_mask, logits.device)
+        _check(experts_ids.size(0) == logits.size(0), "experts_ids must be int32 [T, K]")
+        _check(cu_seqlens is None or (cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and 1 <= cu_seqlens.numel() <= 65536),
+               "cu_seqlens must be int32 [sequences + 1], at most 65535 sequences")
+        _check_tensors(((cu_seqlens, "cu_seqlens"),), logits.device)
+        lib, (T, E), n_seq = _lib.load(), logits.shape, 1 if cu_seqlens is None else cu_seqlens.numel() - 1
+        plan = _plans[key] = (T, E, experts_ids.size(1), _LOGIT_KIND[logits.dtype], n_seq, lib.mlk_balance_workspace_bytes(T, E, n_seq),
+                              lib.mlk_balance_counter_bytes(), lib.mlk_balance_loss, lib.mlk_balance_loss_grad)
     if score_func not in ("softmax", "sigmoid"):
         raise ValueError("Unsupported scoring function")
-    _check(cu_seqlens is None or (cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and 1 <= cu_seqlens.numel() <= 65536),
-           "cu_seqlens must be int32 [sequences + 1], at most 65535 sequences")
-    _check_tensors(((cu_seqlens, "cu_seqlens"),), gating_output.device)
-    return _BalanceLoss.apply(gating_output, experts_ids, token_mask, cu_seqlens, 0 if score_func == "softmax" else 1, float(coef))
+    score_fun = 0 if score_func == "softmax" else 1
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _BalanceLoss.apply(logits, experts_ids, token_mask, cu_seqlens, score_fun, float(coef), plan)
+    return _balance_forward(logits, experts_ids, token_mask, cu_seqlens, score_fun, float(coef), plan)[:2]
 
 
 # ------------------------------------------------- names outside the hot path
