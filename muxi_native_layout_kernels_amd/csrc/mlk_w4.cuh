@@ -11,7 +11,7 @@
 // No weight is rounded: 16 + q is exact in both 16-bit types (the code is the top four bits of the mantissa of a number in 16..31), so the
 // matrix cores sum (16 + q) x over a group in fp32, and
 //   sum over the group of W x = s * (sum (16 + q) x - (16 + z) * sum x)
-// goes to the running sums with two fp32 operations per output, group and lane.  sum x comes from the matrix cores too (an operand of ones), in the
+// goes to the running sums with one or two fp32 operations per output, group and lane.  sum x comes from the matrix cores too (an operand of ones), in the
 // lanes and registers where the products end.  Widening to q - z instead would need a subtraction per pair of weights, which bf16 has no packed
 // instruction for; the 16 costs some two bits of the 24 that the fp32 sums hold.
 //
@@ -41,28 +41,33 @@ struct W4Matrix {
     const uint8_t *zeros;      // null: 8 everywhere
 };
 
-// Mask and bits of 16 for the widening, held in a scalar and a vector register: v_and_or_b32 takes one constant at most, and with both as
-// literals the compiler makes two instructions of it.
-template <class T>
+// Widening of the codes: to 16 + q, or (ADD) to 32 + 15 - z + q, where the bits to add hold 32 + 15 - z of the row's group.  AT: where the four bits belong.
+// Mask and bits of 16 live in a scalar and a vector register: v_and_or_b32 takes one constant at most, and with both as literals the compiler makes
+// two instructions of it.
+template <class T, bool ADD = false>
 struct W4Const {
-    uint32_t mask, sixteen;
+    static constexpr int AT = (T::kind == MLK_BF16 ? 3 : 6) - (ADD ? 1 : 0);
+    uint32_t mask, bits;
     __device__ __forceinline__ W4Const() {
-        mask = T::kind == MLK_BF16 ? 0x00780078u : 0x03c003c0u;
-        sixteen = T::kind == MLK_BF16 ? 0x41804180u : 0x4c004c00u;
+        mask = 0x000f000fu << AT;
+        bits = T::kind == MLK_BF16 ? (ADD ? 0x42004200u : 0x41804180u) : (ADD ? 0x50005000u : 0x4c004c00u);
         asm volatile("" : "+s"(mask));
-        asm volatile("" : "+v"(sixteen));
+        asm volatile("" : "+v"(bits));
     }
+    // of a group with zero point z, in both halves
+    __device__ __forceinline__ uint32_t added(uint32_t z) const { return bits + (15u - z) * (0x00010001u << AT); }
 };
 
-// Codes 2 p and 2 p + 1 of a dword, widened to 16 + q in the type T; and all eight: an MFMA operand.
-template <class T>
-__device__ __forceinline__ uint32_t w4_widen1(uint32_t d, int p, const W4Const<T> &c) {
-    constexpr int AT = T::kind == MLK_BF16 ? 3 : 6;        // where the four bits belong
-    return ((4 * p <= AT ? d << (AT - 4 * p) : d >> (4 * p - AT)) & c.mask) | c.sixteen;
+// Codes 2 p and 2 p + 1 of a dword; and all eight: an MFMA operand.
+template <class T, bool ADD>
+__device__ __forceinline__ uint32_t w4_widen1(uint32_t d, int p, const W4Const<T, ADD> &c, uint32_t bits) {
+    constexpr int AT = W4Const<T, ADD>::AT;
+    const uint32_t q = (4 * p <= AT ? d << (AT - 4 * p) : d >> (4 * p - AT)) & c.mask;
+    return ADD ? q + bits : q | bits;
 }
-template <class T>
-__device__ __forceinline__ u32x4 w4_widen(uint32_t d, const W4Const<T> &c) {
-    return u32x4{w4_widen1<T>(d, 0, c), w4_widen1<T>(d, 1, c), w4_widen1<T>(d, 2, c), w4_widen1<T>(d, 3, c)};
+template <class T, bool ADD>
+__device__ __forceinline__ u32x4 w4_widen(uint32_t d, const W4Const<T, ADD> &c, uint32_t bits) {
+    return u32x4{w4_widen1<T, ADD>(d, 0, c, bits), w4_widen1<T, ADD>(d, 1, c, bits), w4_widen1<T, ADD>(d, 2, c, bits), w4_widen1<T, ADD>(d, 3, c, bits)};
 }
 
 template <class T>
@@ -109,11 +114,30 @@ __device__ __forceinline__ float w4_offset(const W4Scale<GS> &c, int g) {      /
     return 16.f + (float)((c.z >> (8 * g)) & 0xffu);
 }
 
+// How a tile takes the offset of the widened codes out again, sum (q - z) x = sum (offset + q) x - (offset + z) sum x with sum x by an operand of ones:
+// where the offset is the same for all rows, as the initial value of the products' sums, whose operand of ones then holds minus the offset.  Without zero points it
+// is 24; with them 47, if 15 - z is added to every pair of codes (16 instructions a row group and tile instead of four for every block of tokens and
+// group: ADD from five of these on).
+template <int GS, bool ZP, int TT>
+__host__ __device__ constexpr bool w4_add() { return ZP && TT * (4 / GS) > 4; }
+template <class T>
+__device__ __forceinline__ u32x4 w4_minus24() {
+    constexpr uint32_t v = T::kind == MLK_BF16 ? 0xc1c0c1c0u : 0xce00ce00u;
+    return u32x4{v, v, v, v};
+}
+template <class T>
+__device__ __forceinline__ u32x4 w4_minus47() {
+    constexpr uint32_t v = T::kind == MLK_BF16 ? 0xc23cc23cu : 0xd1e0d1e0u;
+    return u32x4{v, v, v, v};
+}
+
 // One tile (128 k) of R row groups times TT blocks of 16 tokens.
-template <class T, int GS, int TT, int R>
+template <class T, int GS, bool ZP, int TT, int R>
 __device__ __forceinline__ void w4_tile(f32x4 (&acc)[R][TT], const u32x4 (&w)[R], const W4Scale<GS> (&sc)[R], const u32x4 (&x)[TT][4],
-                                        const W4Const<T> &con) {
+                                        const W4Const<T, w4_add<GS, ZP, TT>()> &con) {
+    constexpr bool ADD = w4_add<GS, ZP, TT>(), START = !ZP || ADD;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const u32x4 ones = !ZP ? w4_minus24<T>() : (ADD ? w4_minus47<T>() : w4_ones<T>());
 #pragma unroll
     for (int g = 0; g < 4 / GS; ++g) {
         f32x4 xs[TT];
@@ -121,24 +145,23 @@ __device__ __forceinline__ void w4_tile(f32x4 (&acc)[R][TT], const u32x4 (&w)[R]
         for (int tt = 0; tt < TT; ++tt) {
             xs[tt] = zero;
 #pragma unroll
-            for (int j = g * GS; j < (g + 1) * GS; ++j) xs[tt] = T::mfma(x[tt][j], w4_ones<T>(), xs[tt]);
+            for (int j = g * GS; j < (g + 1) * GS; ++j) xs[tt] = T::mfma(x[tt][j], ones, xs[tt]);
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
+            const uint32_t bits = ADD ? con.added((sc[r].z >> (8 * g)) & 0xffu) : con.bits;
             f32x4 d[TT];
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt) d[tt] = zero;
-#pragma unroll
             for (int j = g * GS; j < (g + 1) * GS; ++j) {
-                const u32x4 b = w4_widen<T>(w[r][j], con);
+                const u32x4 b = w4_widen<T, ADD>(w[r][j], con, bits);
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) d[tt] = T::mfma(x[tt][j], b, d[tt]);
+                for (int tt = 0; tt < TT; ++tt) d[tt] = T::mfma(x[tt][j], b, j > g * GS ? d[tt] : (START ? xs[tt] : zero));
             }
             const float s = w4_scale<T, GS>(sc[r], g), o = w4_offset<GS>(sc[r], g);
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) acc[r][tt][v] = fmaf(s, fmaf(-o, xs[tt][v], d[tt][v]), acc[r][tt][v]);
+                for (int v = 0; v < 4; ++v) acc[r][tt][v] = fmaf(s, START ? d[tt][v] : fmaf(-o, xs[tt][v], d[tt][v]), acc[r][tt][v]);
         }
         // The sums are taken here: left alone the compiler sinks them behind the last group and holds the products of every group until then
         // (R = 4, TT = 1, groups of 32: 204 registers, and 134 with this).
@@ -174,7 +197,7 @@ __device__ __forceinline__ void w4_stream(f32x4 (&acc)[R][TT], const W4Rows<R> &
     u32x4 w[U][R], x[U][XL ? 1 : TT][4];
     W4Scale<GS> sc[U][R];
     const int o = lane >> 4, r16 = lane & 15;
-    const W4Const<T> con;
+    const W4Const<T, w4_add<GS, ZP, TT>()> con;
     auto load = [&](int u, int t) {
         const int at = w4_block(t, inv) * 16 + r16;
 #pragma unroll
@@ -205,9 +228,9 @@ __device__ __forceinline__ void w4_stream(f32x4 (&acc)[R][TT], const W4Rows<R> &
                     u32x4 xv[TT][4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) xv[0][j] = xl[t * 16 + j * 4 + o];
-                    w4_tile<T, GS, TT, R>(acc, w[u], sc[u], xv, con);
+                    w4_tile<T, GS, ZP, TT, R>(acc, w[u], sc[u], xv, con);
                 } else {
-                    w4_tile<T, GS, TT, R>(acc, w[u], sc[u], x[u], con);
+                    w4_tile<T, GS, ZP, TT, R>(acc, w[u], sc[u], x[u], con);
                 }
                 if (i + u + U < n) load(u, t + U * step);
             }

@@ -151,7 +151,7 @@ struct W4Panel {
         };
         // operand register q of a window's 32: step q / 4, register q % 4
         u32x4 w[2][8];
-        auto widen = [&](u32x4 (&dst)[8], int q) { dst[q >> 2][q & 3] = w4_widen1<T>(raw[(q >> 2) & 1][q >> 3], q & 3, con); };
+        auto widen = [&](u32x4 (&dst)[8], int q) { dst[q >> 2][q & 3] = w4_widen1<T, false>(raw[(q >> 2) & 1][q >> 3], q & 3, con, con.bits); };
         const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         f32x16 d[2];
         u32x4 x[RING];
