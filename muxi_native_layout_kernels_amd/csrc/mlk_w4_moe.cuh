@@ -27,6 +27,7 @@ struct W4MoeArgs {
     uint16_t *hbuf;              // [slot][I]
     float *obuf;                 // [pair][slice][H]
     int slices;                  // of the down projection's k
+    int wk1, wk2;                // streaming kernels: waves that share a row group's k; the 8 / wk sets of them take different row groups
     u32x4 *sums1, *sums2;        // panels: sums of x, of the intermediate (w4_sums_kernel)
 };
 
@@ -43,15 +44,15 @@ __device__ __forceinline__ W4Matrix w4_of_expert(const W4Matrix &m, int e, int r
     return W4Matrix{m.codes + (size_t)e * rows * (k >> 1), m.scales + entries, m.zeros + entries};
 }
 
-__host__ __device__ constexpr int w4_moe_ring(int tt, int r) { return tt == 1 ? (r <= 2 ? 4 : 2) : (tt * r <= 8 && tt < 4 ? 2 : 1); }
-__host__ __device__ constexpr int w4_moe1_ring(int r) { return r <= 4 ? 4 : 2; }
+__host__ __device__ constexpr int w4_moe_ring(int r) { return r <= 2 ? 4 : 2; }
 
-// Rows of a gate/up workgroup: R / 2 row groups of gate, then the same of up.
+// Rows of a gate/up wave: R / 2 row groups of gate, then the same of up; past the last one it again.
 template <int GS, int R>
 __device__ __forceinline__ void w4_gate_up_rows(W4Rows<R> &rows, const W4MoeArgs &p, int e, int rg0) {
     const W4Matrix m = w4_of_expert<GS>(p.w1, e, 2 * p.I, p.H, p.blocks1);
+    const int groups = p.I >> 4;
 #pragma unroll
-    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r % (R / 2) + (r >= R / 2 ? p.I >> 4 : 0), p.H >> 7, p.blocks1);
+    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, min(rg0 + r % (R / 2), groups - 1) + (r >= R / 2 ? groups : 0), p.H >> 7, p.blocks1);
 }
 
 template <int CELLS>
@@ -67,71 +68,62 @@ __device__ __forceinline__ f32x4 w4_fold(const f32x4 *red, int c, int waves, int
 }
 
 // ---------------------------------------------------------------------------------------------------------- several tokens
-template <class T, int GS, bool ZP, int TT, int R>
+// One block of 16 tokens a task.  Eight waves: wk of them share the k of R row groups, tile by tile, and add their sums through LDS in wave order.  With all
+// eight on one set of row groups the 16 tiles of K = 2048 are two a wave, and a workgroup is mostly its start and end.
+template <class T, int GS, bool ZP, int R>
 __global__ void __launch_bounds__(512) w4_moe_gate_up_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     if ((int)blockIdx.y >= *p.n_tasks) return;
     const MoeTask task = p.tasks[blockIdx.y];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int o = lane >> 4, r16 = lane & 15, rg0 = blockIdx.x * (R / 2);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = p.wk1;
+    const int o = lane >> 4, r16 = lane & 15, set = wave / wk, place = wave - set * wk, rg0 = (blockIdx.x * (8 / wk) + set) * (R / 2);
     W4Rows<R> rows;
     w4_gate_up_rows<GS, R>(rows, p, task.expert, rg0);
-    const uint16_t *xrow[TT];
+    const int pair = p.sorted[task.block0 * 16 + r16];
+    const uint16_t *xrow[1] = {p.X + (size_t)(pair < p.n_pairs ? pair / p.K : 0) * p.H};
+    f32x4 acc[R][1];
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-        const int pair = p.sorted[(task.block0 + min(tt, task.nblocks - 1)) * 16 + r16];
-        xrow[tt] = p.X + (size_t)(pair < p.n_pairs ? pair / p.K : 0) * p.H;
-    }
-    f32x4 acc[R][TT];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    w4_stream<T, GS, ZP, TT, R, w4_moe_ring(TT, R), false>(acc, rows, xrow, nullptr, wave, p.H >> 7, waves, p.inv, lane, false);
-    constexpr int CELLS = R * TT, HALF = CELLS / 2;
-    w4_park<CELLS>(red, reinterpret_cast<const f32x4(&)[CELLS]>(acc), wave, lane);
+    for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w4_stream<T, GS, ZP, 1, R, w4_moe_ring(R), false>(acc, rows, xrow, nullptr, place, p.H >> 7, wk, p.inv, lane, false);
+    constexpr int HALF = R / 2;
+    w4_park<R>(red, reinterpret_cast<const f32x4(&)[R]>(acc), wave, lane);
     __syncthreads();
-    for (int c = wave; c < HALF; c += waves) {
-        const int r = c / TT, tt = c - r * TT;
-        if (tt >= task.nblocks) continue;
-        const f32x4 g = w4_fold<CELLS>(red, c, waves, lane), u = w4_fold<CELLS>(red, HALF + c, waves, lane);
-        uint16_t *h = p.hbuf + (size_t)((task.block0 + tt) * 16 + o * 4) * p.I + (rg0 + r) * 16 + r16;
+    const f32x4 *mine = red + (size_t)set * wk * R * 64;
+    for (int c = place; c < HALF; c += wk) {
+        if (rg0 + c >= p.I >> 4) continue;
+        const f32x4 g = w4_fold<R>(mine, c, wk, lane), u = w4_fold<R>(mine, HALF + c, wk, lane);
+        uint16_t *h = p.hbuf + (size_t)(task.block0 * 16 + o * 4) * p.I + (rg0 + c) * 16 + r16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[(size_t)i * p.I] = (uint16_t)T::from_f32(silu_mul(g[i], u[i]));
     }
 }
 
-template <class T, int GS, bool ZP, int TT, int R>
+template <class T, int GS, bool ZP, int R>
 __global__ void __launch_bounds__(512) w4_moe_down_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     if ((int)blockIdx.y >= *p.n_tasks) return;
     const MoeTask task = p.tasks[blockIdx.y];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int o = lane >> 4, r16 = lane & 15, rg0 = blockIdx.x * R;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = p.wk2;
+    const int o = lane >> 4, r16 = lane & 15, set = wave / wk, place = wave - set * wk, rg0 = (blockIdx.x * (8 / wk) + set) * R, groups = p.H >> 4;
     const W4Matrix m = w4_of_expert<GS>(p.w2, task.expert, p.H, p.I, p.blocks2);
     W4Rows<R> rows;
 #pragma unroll
-    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r, p.I >> 7, p.blocks2);
-    const uint16_t *xrow[TT];
+    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, min(rg0 + r, groups - 1), p.I >> 7, p.blocks2);
+    const uint16_t *xrow[1] = {p.hbuf + (size_t)(task.block0 * 16 + r16) * p.I};
+    f32x4 acc[R][1];
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) xrow[tt] = p.hbuf + (size_t)((task.block0 + min(tt, task.nblocks - 1)) * 16 + r16) * p.I;
-    f32x4 acc[R][TT];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    w4_stream<T, GS, ZP, TT, R, w4_moe_ring(TT, R), false>(acc, rows, xrow, nullptr, wave, p.I >> 7, waves, p.inv, lane, false);
-    constexpr int CELLS = R * TT;
-    w4_park<CELLS>(red, reinterpret_cast<const f32x4(&)[CELLS]>(acc), wave, lane);
+    for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w4_stream<T, GS, ZP, 1, R, w4_moe_ring(R), false>(acc, rows, xrow, nullptr, place, p.I >> 7, wk, p.inv, lane, false);
+    w4_park<R>(red, reinterpret_cast<const f32x4(&)[R]>(acc), wave, lane);
     __syncthreads();
-    for (int c = wave; c < CELLS; c += waves) {
-        const int r = c / TT, tt = c - r * TT;
-        if (tt >= task.nblocks) continue;
-        const f32x4 v = w4_fold<CELLS>(red, c, waves, lane);
+    const f32x4 *mine = red + (size_t)set * wk * R * 64;
+    for (int c = place; c < R; c += wk) {
+        if (rg0 + c >= groups) continue;
+        const f32x4 v = w4_fold<R>(mine, c, wk, lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int pair = p.sorted[(task.block0 + tt) * 16 + o * 4 + i];
-            if (pair < p.n_pairs) p.obuf[(size_t)pair * p.H + (rg0 + r) * 16 + r16] = T::to_f32(p.wts[pair]) * v[i];
+            const int pair = p.sorted[task.block0 * 16 + o * 4 + i];
+            if (pair < p.n_pairs) p.obuf[(size_t)pair * p.H + (rg0 + c) * 16 + r16] = T::to_f32(p.wts[pair]) * v[i];
         }
     }
 }
@@ -172,7 +164,7 @@ __global__ void __launch_bounds__(512) w4_moe1_gate_up_kernel(W4MoeArgs p) {
     f32x4 acc[R][1];
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-    w4_stream<T, GS, ZP, 1, R, w4_moe1_ring(R), true>(acc, rows, xrow, xl, wave, p.H >> 7, waves, p.inv, lane, true);
+    w4_stream<T, GS, ZP, 1, R, 4, true>(acc, rows, xrow, xl, wave, p.H >> 7, waves, p.inv, lane, true);
     __syncthreads();
     // all sixteen tokens of the block are the same one: lanes 0..15 hold the rows
     float *part = reinterpret_cast<float *>(red);
@@ -212,7 +204,7 @@ __global__ void __launch_bounds__(512) w4_moe1_down_kernel(W4MoeArgs p) {
         f32x4 acc[R][1];
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-        w4_stream<T, GS, ZP, 1, R, w4_moe_ring(1, R), false>(acc, rows, xrow, nullptr, place, p.I >> 7, sharing, p.inv, lane, false);
+        w4_stream<T, GS, ZP, 1, R, w4_moe_ring(R), false>(acc, rows, xrow, nullptr, place, p.I >> 7, sharing, p.inv, lane, false);
         const float wt = T::to_f32(p.wts[k]);
 #pragma unroll
         for (int r = 0; r < R; ++r) sum[r] = fmaf(wt, acc[r][0][0], sum[r]);
@@ -246,8 +238,8 @@ static int w4_moe_lds(K kernel, size_t lds, bool (&ready_on)[64]) {
 
 struct W4MoePlan {
     int tt;                  // blocks of 16 tokens per task; 0: one token
-    int r1, r2;              // row groups per workgroup of the gate/up and of the down kernel
     int max_tasks;
+    int wk1, wk2;
     bool panels;             // tasks of 4 or 8 blocks run panels
     int slices;              // of their down projection
 };
@@ -261,14 +253,16 @@ struct W4MoePlan {
         MLK_LAUNCH_CHECK();                                                                \
     } while (0)
 
-template <class T, int GS, bool ZP, int TT, int R>
+template <class T, int GS, bool ZP, int R>
 static int w4_moe_gate_up(const W4MoeArgs &a, int max_tasks, hipStream_t s) {
-    MLK_W4_MOE(w4_moe_gate_up_kernel, dim3(a.I / 8 / R, max_tasks), 8, (size_t)8 * R * TT * 1024, T, GS, ZP, TT, R);
+    const int each = 8 / a.wk1 * (R / 2);
+    MLK_W4_MOE(w4_moe_gate_up_kernel, dim3((a.I / 16 + each - 1) / each, max_tasks), 8, (size_t)8 * R * 1024, T, GS, ZP, R);
     return MLK_OK;
 }
-template <class T, int GS, bool ZP, int TT, int R>
+template <class T, int GS, bool ZP, int R>
 static int w4_moe_down(const W4MoeArgs &a, int max_tasks, hipStream_t s) {
-    MLK_W4_MOE(w4_moe_down_kernel, dim3(a.H / 16 / R, max_tasks), 8, (size_t)8 * R * TT * 1024, T, GS, ZP, TT, R);
+    const int each = 8 / a.wk2 * R;
+    MLK_W4_MOE(w4_moe_down_kernel, dim3((a.H / 16 + each - 1) / each, max_tasks), 8, (size_t)8 * R * 1024, T, GS, ZP, R);
     return MLK_OK;
 }
 template <class T, int GS, bool ZP, int R>
@@ -287,16 +281,13 @@ template <class T, int GS, bool ZP>
 int w4_launch_moe(const W4MoeArgs &a, const W4MoePlan &pl, hipStream_t s) {
     int rc = MLK_ERR_INVALID;
     if (pl.tt == 0) {
-        if (pl.r1 == 2) rc = w4_moe1_gate_up<T, GS, ZP, 2>(a, s);
-        else if (pl.r1 == 4) rc = w4_moe1_gate_up<T, GS, ZP, 4>(a, s);
-        else rc = w4_moe1_gate_up<T, GS, ZP, 8>(a, s);
-        if (rc != MLK_OK) return rc;
-        if (pl.r2 == 1) return w4_moe1_down<T, GS, ZP, 1>(a, s);
-        if (pl.r2 == 2) return w4_moe1_down<T, GS, ZP, 2>(a, s);
-        return w4_moe1_down<T, GS, ZP, 4>(a, s);
+        // one row group of gate and of up (8 experts of 4096 x 14336: the layer 43.8 us, with two 52.5), one of the down projection (52.4 and 56.6)
+        rc = w4_moe1_gate_up<T, GS, ZP, 2>(a, s);
+        return rc == MLK_OK ? w4_moe1_down<T, GS, ZP, 1>(a, s) : rc;
     }
-    rc = w4_moe_gate_up<T, GS, ZP, 1, 8>(a, pl.max_tasks, s);
-    if (rc == MLK_OK) rc = w4_moe_down<T, GS, ZP, 1, 8>(a, pl.max_tasks, s);
+    // four row groups a wave: 128 registers, two workgroups on a CU (8 experts at 16 tokens: 120 us, with eight 139, with two 129)
+    rc = w4_moe_gate_up<T, GS, ZP, 4>(a, pl.max_tasks, s);
+    if (rc == MLK_OK) rc = w4_moe_down<T, GS, ZP, 4>(a, pl.max_tasks, s);
     if (rc != MLK_OK) return rc;
     w4_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
     MLK_LAUNCH_CHECK();
