@@ -7,12 +7,14 @@
 // A row whose probabilities sum to nothing (all logits -inf) has p = 0.
 //
 // Forward: a workgroup takes a chunk of consecutive tokens and walks the sequences that it meets; 4 to 16 lanes hold a token, 4 to 16 experts each, so that
-// a wave takes at least four tokens at a time and a sum over the experts is at most four exchanges within 16 lanes (32749 tokens x 256 experts in
-// fp32: with 64 lanes of four experts a token and six exchanges through LDS 22 us forward and 33 backward).  Its sums for (chunk c, sequence s) go to slot c + s: going through the tokens either the
-// chunk or the sequence moves on, so no two share a slot.  A second launch adds the slots of a sequence in order, for 64 experts a workgroup; the last
-// workgroup adds their shares of the loss.  No floating-point atomics: the results do not depend on the order in which workgroups run.
-// Backward: the same walk, the logits are read again and their gradient written.
-// Bound by the logits' bytes; below about a thousand tokens by the two launches.
+// a wave takes at least four tokens at a time and a sum over the experts is at most four exchanges within 16 lanes.  Its sums for (chunk c, sequence s)
+// go to slot c + s: going through the tokens either the chunk or the sequence moves on, so no two share a slot.  A second launch adds the slots of a
+// sequence in order, for 64 experts a workgroup; the last workgroup adds their shares of the loss.  No floating-point atomics: the results do not depend on
+// the order in which workgroups run.
+// Backward: the same walk, the logits are read again and their gradient written; a lane keeps the shares of its experts until the sequence changes.
+// 32749 tokens x 256 experts in fp32, 9 sequences (33.5 MB: 4.9 us forward, 9.7 backward): 19.4 + 5.8 us forward, 18.4 backward; with 64 lanes of four
+// experts a token and exchanges through LDS 22 and 33, without the next token's logits in flight 23 and 25.  Below about 16384 x 64 bf16 (4.4 + 7.5 and
+// 4.3 us) it is the launches and the dependent loads at a chunk's start.
 #include <algorithm>
 
 #include "mlk_common.cuh"
@@ -28,7 +30,7 @@ struct BalanceArgs {
     const int32_t *ids;
     const uint8_t *mask;         // null: every token counts
     const int32_t *cu;           // [S + 1] or null: one sequence
-    int T, E, K, S, score_fun, vec;
+    int T, E, K, S, score_fun;
     int chunk, chunks;
     float coef;
     float *P;                    // [chunks + S][E]
@@ -44,17 +46,19 @@ struct BalanceArgs {
 
 struct BalF32 {
     typedef f32x4 V4;
+    typedef float V1;
     __device__ static __forceinline__ void unpack(const f32x4 &v, float (&x)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = v[i];
     }
     __device__ static __forceinline__ f32x4 pack(const float (&x)[4]) { return f32x4{x[0], x[1], x[2], x[3]}; }
-    __device__ static __forceinline__ float load(const void *p, size_t i) { return reinterpret_cast<const float *>(p)[i]; }
-    __device__ static __forceinline__ void store(void *p, size_t i, float v) { reinterpret_cast<float *>(p)[i] = v; }
+    __device__ static __forceinline__ float to_f32(float v) { return v; }
+    __device__ static __forceinline__ float from_f32(float v) { return v; }
 };
 template <class T>
 struct Bal16 {
     typedef u32x2 V4;
+    typedef uint16_t V1;
     __device__ static __forceinline__ void unpack(const u32x2 &v, float (&x)[4]) {
         x[0] = T::to_f32(v[0] & 0xffffu);
         x[1] = T::to_f32(v[0] >> 16);
@@ -62,27 +66,44 @@ struct Bal16 {
         x[3] = T::to_f32(v[1] >> 16);
     }
     __device__ static __forceinline__ u32x2 pack(const float (&x)[4]) { return u32x2{T::from_f32x2(x[0], x[1]), T::from_f32x2(x[2], x[3])}; }
-    __device__ static __forceinline__ float load(const void *p, size_t i) { return T::to_f32(reinterpret_cast<const uint16_t *>(p)[i]); }
-    __device__ static __forceinline__ void store(void *p, size_t i, float v) { reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)T::from_f32(v); }
+    __device__ static __forceinline__ float to_f32(uint16_t v) { return T::to_f32(v); }
+    __device__ static __forceinline__ uint16_t from_f32(float v) { return (uint16_t)T::from_f32(v); }
 };
 
 // Experts of a lane: vector v holds 4 (v LPT + lane) .. + 3.
 template <int LPT>
 __device__ __forceinline__ int bal_expert(int v, int l) { return (v * LPT + l) * 4; }
 
-template <class L, int LPT, int NV>
-__device__ __forceinline__ void bal_load(const BalanceArgs &p, int t, int l, float (&x)[NV][4]) {
-    const size_t row = (size_t)t * p.E;
+// The logits of a token as they lie in memory; experts past the last one read the last again.  No branch: the next token's are in flight while one
+// is computed.
+template <class L, int NV, bool VEC>
+struct BalRaw {
+    typename L::V4 v[VEC ? NV : 1];
+    typename L::V1 e[VEC ? 1 : NV][4];
+};
+template <class L, int LPT, int NV, bool VEC>
+__device__ __forceinline__ void bal_load(const BalanceArgs &p, int t, int l, BalRaw<L, NV, VEC> &raw) {
+    const typename L::V1 *row = reinterpret_cast<const typename L::V1 *>(p.logits) + (size_t)t * p.E;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int e0 = bal_expert<LPT>(v, l);
-        if (p.vec) {
-            if (e0 < p.E)
-                L::unpack(*reinterpret_cast<const typename L::V4 *>(reinterpret_cast<const char *>(p.logits) + (row + e0) * (sizeof(typename L::V4) / 4)), x[v]);
+        if constexpr (VEC) {
+            raw.v[v] = *reinterpret_cast<const typename L::V4 *>(row + min(e0, p.E - 4));
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (e0 + i < p.E) x[v][i] = L::load(p.logits, row + e0 + i);
+            for (int i = 0; i < 4; ++i) raw.e[v][i] = row[min(e0 + i, p.E - 1)];
+        }
+    }
+}
+template <class L, int NV, bool VEC>
+__device__ __forceinline__ void bal_unpack(const BalRaw<L, NV, VEC> &raw, float (&x)[NV][4]) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        if constexpr (VEC) {
+            L::unpack(raw.v[v], x[v]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[v][i] = L::to_f32(raw.e[v][i]);
         }
     }
 }
@@ -145,14 +166,15 @@ __device__ __forceinline__ void bal_probs(const BalanceArgs &p, int l, const flo
         for (int i = 0; i < 4; ++i) pr[v][i] *= inv;
 }
 
-// First sequence that ends behind token t (S if there is none).
+// First sequence that ends behind token t (S if there is none), for the whole wave: 64 ends at a time, one load for up to 64 sequences.
 __device__ __forceinline__ int bal_first(const BalanceArgs &p, int t) {
     if (!p.cu) return 0;
-    int lo = 0, hi = p.S;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (p.cu[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
+    int lo = 0, n = p.S;                                  // lo ends are known to be no later than t, the next n may be
+    while (n > 0) {
+        const int step = (n + 63) / 64, at = lo + ((int)(threadIdx.x & 63) + 1) * step;
+        const int ahead = __popcll(__ballot(at <= lo + n && p.cu[min(at, p.S)] <= t));
+        lo += ahead * step;
+        n = min(step - 1, p.S - lo);
     }
     return lo;
 }
@@ -161,7 +183,9 @@ __device__ __forceinline__ void bal_range(const BalanceArgs &p, int s, int &a, i
     b = p.cu ? min(p.cu[s + 1], p.T) : p.T;
 }
 
-template <class L, int LPT, int NV>
+__device__ __forceinline__ bool bal_counts(const BalanceArgs &p, int t) { return !p.mask || p.mask[t]; }
+
+template <class L, int LPT, int NV, bool VEC>
 __global__ void __launch_bounds__(kBalThreads) balance_partial_kernel(BalanceArgs p) {
     constexpr int ROWS = kBalThreads / LPT, COLS = LPT * NV * 4;         // tokens at a time, experts with room for
     __shared__ float sums[ROWS * COLS];
@@ -178,6 +202,9 @@ __global__ void __launch_bounds__(kBalThreads) balance_partial_kernel(BalanceArg
         a = max(a, c0);
         b = min(b, c1);
         if (a >= b) continue;
+        BalRaw<L, NV, VEC> next;
+        bal_load<L, LPT, NV, VEC>(p, min(a + row, b - 1), l, next);
+        bool next_is = bal_counts(p, min(a + row, b - 1));
         for (int e = tid; e < p.E; e += kBalThreads) cnt[e] = 0;
         if (tid == 0) valid = 0;
         __syncthreads();
@@ -188,9 +215,12 @@ __global__ void __launch_bounds__(kBalThreads) balance_partial_kernel(BalanceArg
         float sum[NV][4] = {};
         int n = 0;
         for (int t = a + row; t < b; t += ROWS) {
-            if (p.mask && !p.mask[t]) continue;             // the lanes of a token agree
-            float x[NV][4] = {}, pr[NV][4], sig[NV][4];
-            bal_load<L, LPT, NV>(p, t, l, x);
+            float x[NV][4], pr[NV][4], sig[NV][4];
+            bal_unpack<L, NV, VEC>(next, x);
+            const bool is = next_is;
+            bal_load<L, LPT, NV, VEC>(p, min(t + ROWS, b - 1), l, next);
+            next_is = bal_counts(p, min(t + ROWS, b - 1));
+            if (!is) continue;                              // the lanes of a token agree
             bal_probs<LPT, NV>(p, l, x, pr, sig);
             ++n;
 #pragma unroll
@@ -298,30 +328,50 @@ __global__ void __launch_bounds__(1024) balance_reduce_kernel(BalanceArgs p) {
     if (lane == 0) *p.loss = v;
 }
 
-template <class L, int LPT, int NV>
+template <class L, int LPT, int NV, bool VEC>
 __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(BalanceArgs p) {
     constexpr int ROWS = kBalThreads / LPT;
     const int tid = threadIdx.x, row = tid / LPT, l = tid % LPT;
     const int c0 = blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, p.T);
+    BalRaw<L, NV, VEC> next;
+    bal_load<L, LPT, NV, VEC>(p, min(c0 + row, c1 - 1), l, next);
+    bool next_is = bal_counts(p, min(c0 + row, c1 - 1));
     const float up = *p.grad;
-    int s = bal_first(p, c0);
-    for (int t = c0 + row; t < c1; t += ROWS) {
-        bool counts = true;
-        if (p.cu) {
-            while (s < p.S && p.cu[s + 1] <= t) ++s;
-            counts = s < p.S && p.cu[s] <= t;
+    // the sequence that this token lies in or ahead of, tokens a .. b - 1, and its shares
+    int s = bal_first(p, c0), a = 0, b = 0;
+    float g[NV][4] = {};
+    auto enter = [&]() {
+        if (s >= p.S) {
+            a = b = p.T;
+            return;
         }
-        if (p.mask && !p.mask[t]) counts = false;
-        float d[NV][4] = {};
-        if (counts) {
-            float x[NV][4] = {}, pr[NV][4], sig[NV][4], g[NV][4] = {};
-            bal_load<L, LPT, NV>(p, t, l, x);
-            const float *share = p.share + (size_t)s * p.E;
+        bal_range(p, s, a, b);
+        const float *share = p.share + (size_t)s * p.E;
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            const int e0 = bal_expert<LPT>(v, l);
+            if constexpr (VEC) {
+                BalF32::unpack(*reinterpret_cast<const f32x4 *>(share + min(e0, p.E - 4)), g[v]);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (bal_expert<LPT>(v, l) + i < p.E) g[v][i] = share[bal_expert<LPT>(v, l) + i];
+                for (int i = 0; i < 4; ++i) g[v][i] = share[min(e0 + i, p.E - 1)];
+            }
+        }
+    };
+    enter();
+    for (int t = c0 + row; t < c1; t += ROWS) {
+        float x[NV][4], d[NV][4] = {};
+        bal_unpack<L, NV, VEC>(next, x);
+        bool is = next_is;
+        bal_load<L, LPT, NV, VEC>(p, min(t + ROWS, c1 - 1), l, next);
+        next_is = bal_counts(p, min(t + ROWS, c1 - 1));
+        if (t >= b && s < p.S) {
+            do ++s;
+            while (s < p.S && p.cu[s + 1] <= t);
+            enter();
+        }
+        if (is && a <= t && t < b) {
+            float pr[NV][4], sig[NV][4];
             bal_probs<LPT, NV>(p, l, x, pr, sig);
             float dot = 0.f;
 #pragma unroll
@@ -334,16 +384,16 @@ __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(BalanceArgs p
 #pragma unroll
                 for (int i = 0; i < 4; ++i) d[v][i] = pr[v][i] * (1.f - sig[v][i]) * (g[v][i] - dot) * up;
         }
-        const size_t at = (size_t)t * p.E;
+        typename L::V1 *out = reinterpret_cast<typename L::V1 *>(p.dlogits) + (size_t)t * p.E;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int e0 = bal_expert<LPT>(v, l);
-            if (p.vec) {
-                if (e0 < p.E) *reinterpret_cast<typename L::V4 *>(reinterpret_cast<char *>(p.dlogits) + (at + e0) * (sizeof(typename L::V4) / 4)) = L::pack(d[v]);
+            if constexpr (VEC) {
+                if (e0 < p.E) *reinterpret_cast<typename L::V4 *>(out + e0) = L::pack(d[v]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (e0 + i < p.E) L::store(p.dlogits, at + e0 + i, d[v][i]);
+                    if (e0 + i < p.E) out[e0 + i] = L::from_f32(d[v][i]);
             }
         }
     }
@@ -409,14 +459,14 @@ static int balance_check(const void *logits, int x_kind, int score_fun, int T, i
 }
 
 // Rows of four experts can be moved whole.
-static int balance_vec(const void *p, int x_kind, int E) { return E % 4 == 0 && ((uintptr_t)p & (x_kind == MLK_F32 ? 15 : 7)) == 0; }
+static bool balance_vec(const void *p, int x_kind, int E) { return E % 4 == 0 && ((uintptr_t)p & (x_kind == MLK_F32 ? 15 : 7)) == 0; }
 
-template <class L>
+template <class L, bool VEC>
 static void balance_launch(const BalanceArgs &a, bool grad, hipStream_t s) {
 #define MLK_BAL(LPT, NV)                                                                       \
     do {                                                                                       \
-        if (grad) balance_grad_kernel<L, LPT, NV><<<a.chunks, kBalThreads, 0, s>>>(a);         \
-        else balance_partial_kernel<L, LPT, NV><<<a.chunks, kBalThreads, 0, s>>>(a);           \
+        if (grad) balance_grad_kernel<L, LPT, NV, VEC><<<a.chunks, kBalThreads, 0, s>>>(a);    \
+        else balance_partial_kernel<L, LPT, NV, VEC><<<a.chunks, kBalThreads, 0, s>>>(a);      \
     } while (0)
     if (a.E <= 16) MLK_BAL(4, 1);
     else if (a.E <= 32) MLK_BAL(8, 1);
@@ -425,10 +475,15 @@ static void balance_launch(const BalanceArgs &a, bool grad, hipStream_t s) {
     else MLK_BAL(16, 4);
 #undef MLK_BAL
 }
-static void balance_launch_kind(const BalanceArgs &a, int x_kind, bool grad, hipStream_t s) {
-    if (x_kind == MLK_F32) balance_launch<BalF32>(a, grad, s);
-    else if (x_kind == MLK_F16) balance_launch<Bal16<F16>>(a, grad, s);
-    else balance_launch<Bal16<BF16>>(a, grad, s);
+template <class L>
+static void balance_launch_vec(const BalanceArgs &a, bool vec, bool grad, hipStream_t s) {
+    if (vec) balance_launch<L, true>(a, grad, s);
+    else balance_launch<L, false>(a, grad, s);
+}
+static void balance_launch_kind(const BalanceArgs &a, int x_kind, bool vec, bool grad, hipStream_t s) {
+    if (x_kind == MLK_F32) balance_launch_vec<BalF32>(a, vec, grad, s);
+    else if (x_kind == MLK_F16) balance_launch_vec<Bal16<F16>>(a, vec, grad, s);
+    else balance_launch_vec<Bal16<BF16>>(a, vec, grad, s);
 }
 
 __global__ void balance_nothing_kernel(float *loss, int32_t *counts, int E) {
@@ -494,7 +549,6 @@ int mlk_balance_loss(const void *logits, int x_kind, int score_fun, int n_tokens
     a.K = topk;
     a.S = n_seq;
     a.score_fun = score_fun;
-    a.vec = balance_vec(logits, x_kind, n_experts);
     a.chunk = balance_chunk(n_tokens);
     a.chunks = (n_tokens + a.chunk - 1) / a.chunk;
     a.coef = coef;
@@ -506,7 +560,7 @@ int mlk_balance_loss(const void *logits, int x_kind, int score_fun, int n_tokens
     a.loss = loss;
     a.share = share;
     a.counts = counts;
-    balance_launch_kind(a, x_kind, false, s);
+    balance_launch_kind(a, x_kind, balance_vec(logits, x_kind, n_experts), false, s);
     MLK_LAUNCH_CHECK();
     balance_reduce_kernel<<<dim3((n_experts + 63) / 64, n_seq), 1024, 0, s>>>(a);
     MLK_LAUNCH_CHECK();
@@ -527,13 +581,13 @@ int mlk_balance_loss_grad(const void *logits, int x_kind, int score_fun, int n_t
     a.E = n_experts;
     a.S = n_seq;
     a.score_fun = score_fun;
-    a.vec = balance_vec(logits, x_kind, n_experts) && balance_vec(dlogits, x_kind, n_experts);
+    const bool vec = balance_vec(logits, x_kind, n_experts) && balance_vec(dlogits, x_kind, n_experts) && ((uintptr_t)share & 15) == 0;
     a.chunk = balance_chunk(n_tokens);
     a.chunks = (n_tokens + a.chunk - 1) / a.chunk;
     a.share = const_cast<float *>(share);
     a.grad = grad;
     a.dlogits = dlogits;
-    balance_launch_kind(a, x_kind, true, (hipStream_t)stream);
+    balance_launch_kind(a, x_kind, vec, true, (hipStream_t)stream);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }
