@@ -34,13 +34,12 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
         pl.max_tasks = topk;
         return pl;
     }
-    // Routed pairs of an expert that is reached.  Up to 16 on average the streaming kernels, one block of 16 tokens a task; above, panels: 8 experts of
-    // 4096 x 14336, top-2, at 48 tokens (12) 196 us against 224 with panels of 64 tokens, at 100 (25) 285 against 240; 64 experts of 2048 x 1408, top-6, at 100
-    // tokens (9) 111 against 120, at 200 (19) 150 against 127.  Panels of 128 tokens from 110 on: 8 experts at 500 tokens (125) 550 us both, at 1000 (250)
-    // 871 against 911; 64 experts at 1000 (94) 271 against 253, at 2000 (188) 404 against 424.
+    // Routed pairs of an expert that is reached.  Up to 20 on average the streaming kernels, one block of 16 tokens a task; above, panels: 8 experts of
+    // 4096 x 14336, top-2, at 48 tokens (12) 189 us against 237 with panels, at 80 (20) 262 against 238, at 130 (32) 336 against 234; 128 experts of 2048 x 768,
+    // top-8, at 200 (12) 137 against 189, at 300 (18) 172 against 196, at 400 (25) 207 against 209.
     const int reached = pairs < E ? pairs : E, load = (pairs + reached - 1) / reached;
-    pl.panels = load > 16 && (int64_t)tokens * hidden < (1ll << 31);
-    pl.tt = pl.panels ? (load <= 110 ? 4 : 8) : 1;
+    pl.panels = load > 20 && (int64_t)tokens * hidden < (1ll << 31);
+    pl.tt = pl.panels ? 8 : 1;
     // an expert's last task may be short: at most one more than its blocks fill
     const int64_t most = (int64_t)E + pairs / (16 * pl.tt);
     pl.max_tasks = (int)(most < pairs ? most : pairs);
@@ -52,7 +51,7 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
         return pl;
     }
     // Two K slices of a long down projection that would leave CUs without a panel in its last round: 8 experts of 4096 x 14336 at 100 tokens 276 -> 240 us, at
-    // 1000 871 -> 830; with 16 windows (2048) or panels for two rounds the second sum costs more (64 experts at 300 tokens 144 -> 161).
+    // 320 389 -> 343, at 1000 853 -> 811; with 16 windows (2048) or panels for two rounds the second sum costs more (64 experts at 300 tokens 144 -> 161).
     const int wgs = (hidden + 255) / 256 * reached * ((load + 16 * pl.tt - 1) / (16 * pl.tt));
     if (wgs < 2 * cus && inter / 128 >= 64) pl.slices = 2;
     return pl;

@@ -12,11 +12,8 @@
 namespace mlk {
 
 template <class T, int GS, bool ZP, int TB>
-__global__ void __launch_bounds__(512, 2) w4_moe_gate_up_panel_kernel(W4MoeArgs p) {
+__device__ __forceinline__ void w4_gate_up_panel(const W4MoeArgs &p, const MoeTask &task, u32x4 *win) {
     using P = W4Panel<T, GS, ZP, TB>;
-    extern __shared__ u32x4 win[];
-    if ((int)blockIdx.y >= *p.n_tasks) return;
-    const MoeTask task = p.tasks[blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, i32 = lane & 31, tiles = p.H >> 7, rg = blockIdx.x * 8 + wave;
     const int slot0 = task.block0 * 16, slots = task.nblocks * 16;
@@ -55,11 +52,8 @@ __global__ void __launch_bounds__(512, 2) w4_moe_gate_up_panel_kernel(W4MoeArgs 
 }
 
 template <class T, int GS, bool ZP, int TB>
-__global__ void __launch_bounds__(512, 2) w4_moe_down_panel_kernel(W4MoeArgs p) {
+__device__ __forceinline__ void w4_down_panel(const W4MoeArgs &p, const MoeTask &task, u32x4 *win) {
     using P = W4Panel<T, GS, ZP, TB>;
-    extern __shared__ u32x4 win[];
-    if ((int)blockIdx.y >= *p.n_tasks) return;
-    const MoeTask task = p.tasks[blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, i32 = lane & 31, tiles = p.I >> 7, groups = p.H >> 4, rg = blockIdx.x * 16 + wave * 2, sl = blockIdx.z;
     const int slot0 = task.block0 * 16, slots = task.nblocks * 16;
@@ -90,29 +84,43 @@ __global__ void __launch_bounds__(512, 2) w4_moe_down_panel_kernel(W4MoeArgs p) 
         }
 }
 
-template <class T, int GS, bool ZP, int TB>
-static int w4_moe_panels(const W4MoeArgs &a, const W4MoePlan &pl, const int32_t *blocks, int max_slots, hipStream_t s) {
-    using P = W4Panel<T, GS, ZP, TB>;
-    int rc = w4_launch_sums<T, GS>(a.X, a.sums1, a.T, a.H, nullptr, s);
-    if (rc != MLK_OK) return rc;
-    static bool ready1[64] = {}, ready2[64] = {};
-    rc = panel_lds_attribute(&w4_moe_gate_up_panel_kernel<T, GS, ZP, TB>, P::lds_bytes, ready1);
-    if (rc == MLK_OK) rc = panel_lds_attribute(&w4_moe_down_panel_kernel<T, GS, ZP, TB>, P::lds_bytes, ready2);
-    if (rc != MLK_OK) return rc;
-    w4_moe_gate_up_panel_kernel<T, GS, ZP, TB><<<dim3(a.I / 128, pl.max_tasks), 512, P::lds_bytes, s>>>(a);
-    MLK_LAUNCH_CHECK();
-    rc = w4_launch_sums<T, GS>(a.hbuf, a.sums2, max_slots, a.I, blocks, s);
-    if (rc != MLK_OK) return rc;
-    w4_moe_down_panel_kernel<T, GS, ZP, TB><<<dim3((a.H + 255) / 256, pl.max_tasks, a.slices), 512, P::lds_bytes, s>>>(a);
-    MLK_LAUNCH_CHECK();
-    w4_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
-    MLK_LAUNCH_CHECK();
-    return MLK_OK;
+// Panels of 128 tokens; an expert's last one is a panel of 64 where its tokens fit in that (8 experts of 4096 x 14336, top-2, at 1000 tokens 890 -> 815 us).
+// Panels of 64 for all lose from 50 tokens an expert on, up to 25 %, and gain at most 5 % below.
+template <class T, int GS, bool ZP>
+__global__ void __launch_bounds__(512, 2) w4_moe_gate_up_panel_kernel(W4MoeArgs p) {
+    extern __shared__ u32x4 win[];
+    if ((int)blockIdx.y >= *p.n_tasks) return;
+    const MoeTask task = p.tasks[blockIdx.y];
+    if (task.nblocks <= 4) w4_gate_up_panel<T, GS, ZP, 2>(p, task, win);
+    else w4_gate_up_panel<T, GS, ZP, 4>(p, task, win);
+}
+template <class T, int GS, bool ZP>
+__global__ void __launch_bounds__(512, 2) w4_moe_down_panel_kernel(W4MoeArgs p) {
+    extern __shared__ u32x4 win[];
+    if ((int)blockIdx.y >= *p.n_tasks) return;
+    const MoeTask task = p.tasks[blockIdx.y];
+    if (task.nblocks <= 4) w4_down_panel<T, GS, ZP, 2>(p, task, win);
+    else w4_down_panel<T, GS, ZP, 4>(p, task, win);
 }
 
 template <class T, int GS, bool ZP>
 int w4_launch_moe_panel(const W4MoeArgs &a, const W4MoePlan &pl, const int32_t *blocks, int max_slots, hipStream_t s) {
-    return pl.tt == 4 ? w4_moe_panels<T, GS, ZP, 2>(a, pl, blocks, max_slots, s) : w4_moe_panels<T, GS, ZP, 4>(a, pl, blocks, max_slots, s);
+    constexpr size_t lds = W4Panel<T, GS, ZP, 4>::lds_bytes;
+    int rc = w4_launch_sums<T, GS>(a.X, a.sums1, a.T, a.H, nullptr, s);
+    if (rc != MLK_OK) return rc;
+    static bool ready1[64] = {}, ready2[64] = {};
+    rc = panel_lds_attribute(&w4_moe_gate_up_panel_kernel<T, GS, ZP>, lds, ready1);
+    if (rc == MLK_OK) rc = panel_lds_attribute(&w4_moe_down_panel_kernel<T, GS, ZP>, lds, ready2);
+    if (rc != MLK_OK) return rc;
+    w4_moe_gate_up_panel_kernel<T, GS, ZP><<<dim3(a.I / 128, pl.max_tasks), 512, lds, s>>>(a);
+    MLK_LAUNCH_CHECK();
+    rc = w4_launch_sums<T, GS>(a.hbuf, a.sums2, max_slots, a.I, blocks, s);
+    if (rc != MLK_OK) return rc;
+    w4_moe_down_panel_kernel<T, GS, ZP><<<dim3((a.H + 255) / 256, pl.max_tasks, a.slices), 512, lds, s>>>(a);
+    MLK_LAUNCH_CHECK();
+    w4_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
 }
 
 }  // namespace mlk
