@@ -256,8 +256,8 @@ int mlk_pack_scales_w4(const void *src, void *dst, int64_t batch, int n, int k, 
 int mlk_unpack_scales_w4(const void *src, void *dst, int64_t batch, int n, int k, int group, int elem_size, void *stream);
 
 /* C[M, N] = T(alpha * B[M, K] . W^T (+ bias[N])), any M >= 0, fp32 accumulation, no weight rounded; `scale` and `zero` (NULL: none) packed as
- * above.  A row of B that holds an infinity gives NaN.  a and b on 16 bytes, scale on 8, zero on 4.
- * workspace: device scratch of at least mlk_gemm_w4_workspace_bytes() bytes under the rules of mlk_gemm_layout_a; may be NULL where
+ * above.  A row of B that holds an infinity, or bf16 numbers so large that 64 times the sum of their magnitudes passes the fp32 range, gives NaN.
+ * a, b, c and workspace on 16 bytes, scale on 8, zero on 4.  workspace: device scratch of at least mlk_gemm_w4_workspace_bytes() bytes under the rules of mlk_gemm_layout_a; may be NULL where
  * that is 0. */
 int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, const void *b, void *c, int m, int n, int k, int group,
                          int x_kind, float alpha, const void *bias, void *workspace, size_t workspace_bytes, void *stream);
@@ -387,7 +387,8 @@ int mlk_expert_counts(const int32_t *topk_ids, const uint8_t *token_mask, int n_
  * probabilities: softmax of the logits (score_fun 0) or sigmoids over their sum (1).  A row of logits that are all -inf has no
  * probability anywhere.  cu_seqlens int32 [n_seq + 1], non-decreasing: tokens cu[s] .. cu[s+1]-1 are sequence s, rows before the first and behind
  * the last one do not count; NULL with n_seq = 1: all tokens are one sequence.  loss fp32 [1]; counts int32 [E]: all valid tokens' pairs;
- * share fp32 [n_seq, E]: dloss/dP, which the gradient takes.  Results do not depend on the order in which workgroups run.
+ * share fp32 [n_seq, E]: dloss/dP, which the gradient takes.  n_tokens and
+ * n_tokens * topk at most 2^30, n_seq at most 65535, E at most 256.  Results do not depend on the order in which workgroups run.
  * workspace: mlk_balance_workspace_bytes(), on 16 bytes, its first mlk_balance_counter_bytes() zero before the first call (left zero). */
 int mlk_balance_loss(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, int topk, const int32_t *topk_ids,
                      const uint8_t *token_mask, const int32_t *cu_seqlens, int n_seq, float coef, float *loss, int32_t *counts, float *share,

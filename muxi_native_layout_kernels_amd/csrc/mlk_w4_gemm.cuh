@@ -26,6 +26,8 @@ struct W4GemmArgs {
     int *counters;         // [workgroup], zero between calls
 };
 
+constexpr int kW4TokenLds = 128 * 1024;      // bytes of LDS that one token may take
+
 // Waves a workgroup may have, so that the ring fits the registers.
 __host__ __device__ constexpr int w4_stream_waves(int tt, int r, bool xl) { return xl ? 16 : 8; }
 __host__ __device__ constexpr int w4_ring(int tt, int r, bool xl) {
@@ -135,7 +137,7 @@ int w4_launch_stream(const W4GemmArgs &a, int r, int wgs, int waves, hipStream_t
         if (r == 2) return w4_launch_stream_one<T, GS, ZP, TT, 2, XL>(a, wgs, waves, s);       \
         if (r == 4) return w4_launch_stream_one<T, GS, ZP, TT, 4, XL>(a, wgs, waves, s);       \
     } while (0)
-    if (a.M == 1 && (a.K / kW4TileK + a.slices - 1) / a.slices * 256 <= 128 * 1024) {
+    if (a.M == 1 && (a.K / kW4TileK + a.slices - 1) / a.slices * 256 <= kW4TokenLds) {
         if (r == 1) return w4_launch_stream_one<T, GS, ZP, 1, 1, true>(a, wgs, waves, s);
         if (r == 2) return w4_launch_stream_one<T, GS, ZP, 1, 2, true>(a, wgs, waves, s);
     }

@@ -46,7 +46,7 @@ static W4Plan w4_plan_stream(int m, int n, int k) {
         pl.slices = fill < 1 ? 1 : (fill > most ? most : fill);
     }
     pl.wgs = (groups + pl.r - 1) / pl.r;
-    pl.waves = m == 1 && pl.r == 1 && groups <= cus && tiles >= 16 ? 16 : 8;
+    pl.waves = m == 1 && pl.r == 1 && groups <= cus && tiles >= 16 && tiles * 256 <= kW4TokenLds ? 16 : 8;      // 16: only with the token in LDS
     return pl;
 }
 
@@ -54,8 +54,8 @@ static W4Plan w4_plan_stream(int m, int n, int k) {
 // (tb = 4) with few panels on the chip and 0.2 or 0.5 more with one on every CU; three windows go to the start and the end, one for every 16 groups to the
 // sums of x; launches and sums 6 us, the fold 2 us and its bytes.  Smaller groups cost more vector instructions a window.
 static double w4_panel_cost(int m, int n, int k, int group, int tb, int slices, int cus) {
-    const int panels = (n + 255) / 256 * ((m + 32 * tb - 1) / (32 * tb)), windows = (k / 128 + slices - 1) / slices;
-    const int rounds = (panels * slices + cus - 1) / cus, g = group < 128 ? 128 / group : 1;
+    const int64_t panels = ((int64_t)n + 255) / 256 * (((int64_t)m + 32 * tb - 1) / (32 * tb)), rounds = (panels * slices + cus - 1) / cus;
+    const int windows = (k / 128 + slices - 1) / slices, g = group < 128 ? 128 / group : 1;
     const double full = rounds > 1 ? 1.0 : (double)panels * slices / cus;
     const double window = (tb == 2 ? 0.82 + 0.2 * full : 1.18 + 0.5 * full) * (g == 1 ? 1.0 : (g == 2 ? 1.15 : 1.45));
     return rounds * (windows + (windows * g + 15) / 16 + 3) * window + 6 + (slices > 1 ? 2 + (double)slices * m * n * 8 / 5e6 : 0);
@@ -207,7 +207,7 @@ int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, con
     MLK_REQUIRE(x_kind == MLK_F16 || x_kind == MLK_BF16, "w4 gemm: activations must be fp16 or bf16");
     if (m == 0 || n == 0) return MLK_OK;
     MLK_REQUIRE(a && scale && b && c, "w4 gemm: null pointer");
-    MLK_REQUIRE(aligned16(a) && aligned16(b), "w4 gemm: weights and activations must lie on 16 bytes");
+    MLK_REQUIRE(aligned16(a) && aligned16(b) && aligned16(c) && aligned16(workspace), "w4 gemm: weights, activations, outputs and workspace must lie on 16 bytes");
     MLK_REQUIRE(((uintptr_t)scale & 7) == 0 && ((uintptr_t)zero & 3) == 0, "w4 gemm: scales must lie on 8 bytes, zero points on 4");
     const W4Plan pl = w4_plan(m, n, k, group);
     const size_t part = w4_partial_bytes(pl, m, n, k, group);

@@ -732,7 +732,8 @@ def _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, what):
 
 def gemm_layoutA_w4(A, A_Scale, B, A_Zero=None, alpha=1, beta=0, bias=None):
     """C[n, m] = alpha * B[n, k] . W^T (+ bias) with 4-bit weights W = s (q - z) from `pack_layout_a_w4`; any n >= 0, m % 16 == 0,
-    k % 128 == 0.  fp32 sums, one rounding at the end, no weight rounded.  A row of B that holds an infinity gives NaN."""
+    k % 128 == 0.  fp32 sums, one rounding at the end, no weight rounded.  A row of B that holds an infinity, or bf16 numbers so large that 64
+    times the sum of their magnitudes passes the fp32 range, gives NaN."""
     return _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, "gemm_layoutA_w4")
 
 
