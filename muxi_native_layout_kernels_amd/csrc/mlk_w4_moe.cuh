@@ -1,7 +1,7 @@
 // Expert layers over 4-bit weights: grouped gate/up product with SiLU(gate) * up, grouped down product, weighted sum.
 //
-// Several tokens: the routed pairs are brought into expert order in blocks of 16 (moe_align_kernel); a task is up to TT blocks of one expert, which
-// share one pass over its weights.  The intermediate is kept row-major [slot][I] in the activations' type (slot = place in the order), the
+// Several tokens: the routed pairs are brought into expert order in blocks of 16 (moe_align_kernel); a task is a block (panels: up to eight) of one
+// expert, which share one pass over its weights.  The intermediate is kept row-major [slot][I] in the activations' type (slot = place in the order), the
 // weighted products of the down projection in fp32 [pair][slice][H], and a last launch adds a token's pairs in the order of its picks.
 // One token: its picks are the tasks, no alignment; the down projection's waves deal the picks among themselves and write the output at once.
 #pragma once
@@ -240,7 +240,7 @@ struct W4MoePlan {
     int tt;                  // blocks of 16 tokens per task; 0: one token
     int max_tasks;
     int wk1, wk2;
-    bool panels;             // tasks of 4 or 8 blocks run panels
+    bool panels;             // tasks of up to 8 blocks run panels
     int slices;              // of their down projection
 };
 

@@ -29,7 +29,7 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
     W4MoePlan pl = {};
     pl.slices = 1;
     const int cus = device_cus(), pairs = tokens * topk;
-    if (tokens == 1) {
+    if (tokens == 1 && hidden <= 64 * 1024) {                // the token is staged in LDS
         pl.tt = 0;
         pl.max_tasks = topk;
         return pl;
@@ -97,7 +97,7 @@ extern "C" {
 
 // What a call needs: a long one goes in passes of one size and a shorter last one, whose plan may differ.
 size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int hidden, int inter, int group) {
-    if (n_tokens <= 0 || n_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0 || group < 32) return 0;
+    if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0 || group < 32) return 0;
     const int step = w4_moe_pass_tokens(n_tokens, topk), rest = n_tokens % step;
     size_t most = 0;
     for (int t : {step, rest}) {

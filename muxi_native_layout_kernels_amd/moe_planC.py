@@ -196,6 +196,7 @@ def fused_moe_w4(
         if hidden_states.shape[0] > 0:
             ops.fused_routing_gate(gating_output, 0 if score_func == "softmax" else 1, hidden_states.shape[0], hidden_states.shape[1], num_expert_group,
                                    topk_group, topk_ids, topk_weights, topk, gating_bias, renormalize)
-        if expert_load is not None:
+        y = ops.fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
+        if expert_load is not None:                                    # last: a call that is refused counts nothing
             ops.expert_counts(topk_ids, gating_output.shape[1], out=expert_load)
-    return ops.fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
+    return y
