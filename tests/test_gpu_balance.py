@@ -172,3 +172,14 @@ def test_counts(mlk, T, E, K):
         assert got.dtype == torch.int32 and torch.equal(got.cpu(), want)
         again = mlk.expert_counts(ids.cuda(), E, token_mask=None if m is None else m.cuda(), out=got)
         assert again is got and torch.equal(got.cpu(), 2 * want)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_many_short_sequences(mlk, sigmoid):
+    g = torch.Generator().manual_seed(8)
+    T, E, K = 5000, 20, 2
+    logits, ids = case(T, E, K, torch.float32, 3)
+    cuts = torch.randint(0, T + 1, (1500,), generator=g).sort()[0].int()                     # some of them empty
+    mask = torch.rand(T, generator=g) < 0.6
+    check(mlk, logits, ids, sigmoid, 1.0, None, cuts)
+    check(mlk, logits, ids, sigmoid, 1.0, mask, cuts)
