@@ -1,0 +1,307 @@
+"""GPU: how the 4-bit products, their expert layers, the balance loss and the expert counts are called: every launch plan, captured graphs, streams, alignment,
+long offsets, rows behind the last one."""
+import pytest
+import torch
+
+from helpers import randn
+from test_gpu_w4 import assert_within, on_gpu, term_size, w4_weights
+from test_gpu_w4_experts import check as check_experts
+from test_gpu_w4_experts import expected as expected_experts
+from test_gpu_w4_experts import layer, routing
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("tokens,n,k,group,zeros,dtype", [
+    (1, 8208, 256, 64, True, BF), (3, 8208, 256, 64, False, HF), (1, 16400, 128, 32, False, BF), (1, 32, 70016, 128, True, HF), (2, 32, 70016, 128, False, BF),
+    (5, 2064, 7168, 128, False, HF), (20, 2064, 7168, 32, True, BF), (37, 2064, 2560, 64, True, HF), (60, 2064, 7168, 3584, False, BF), (40, 8208, 256, 32, True, HF),
+    (1, 16, 1280, 640, False, HF), (2050, 272, 7168, 128, True, BF), (1025, 4112, 384, 128, False, HF), (1025, 4112, 512, 32, True, BF),
+    (2050, 2064, 2048, 64, False, BF), (300, 528, 2048, 64, True, HF), (129, 16, 256, 32, False, HF)])
+def test_every_plan_against_64_bits(mlk, tokens, n, k, group, zeros, dtype):
+    codes, s, z, w = w4_weights(n, k, group, dtype, zeros, tokens + n)
+    x = randn((tokens, k), dtype, 1.0, 3)
+    A, S, Z = mlk.pack_layout_a_w4(*on_gpu(codes, s, z))
+    got = mlk.gemm_layoutA_w4(A, S, x.cuda(), Z)
+    assert_within(got, x.double() @ w.t(), term_size(x, s, group), dtype, k, "product")
+    again = mlk.gemm_layoutA_w4(A, S, x.cuda(), Z)
+    assert torch.equal(got, again)                       # no sum's order depends on which workgroup comes first
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 40, 100, 600])
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_extreme_weights_and_activations(mlk, tokens, dtype):
+    """Codes and zero points at their ends, scales of zero, subnormal and large, activations of one sign (the offset of the codes cancels most)."""
+    n, k, group = 272, 1024, 64
+    codes, s, z, _ = w4_weights(n, k, group, dtype, True, 5)
+    q = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2)
+    q[:64], z[:32], z[32:64] = 15, 0, 15
+    q[64:128], z[64:96], z[96:128] = 0, 0, 15
+    s[::7], s[1::7], s[2::7] = 0.0, torch.finfo(dtype).smallest_normal / 4, 3.0
+    w = ((q.double().unflatten(-1, (k // group, group)) - z.double().unsqueeze(-1)) * s.double().unsqueeze(-1)).flatten(-2)
+    x = randn((tokens, k), dtype, 1.0, 3).abs()
+    x[0, 1::2] = 0.0
+    A, S, Z = mlk.pack_layout_a_w4(*on_gpu((q[..., 0::2] | (q[..., 1::2] << 4)).contiguous(), s, z))
+    got, want = mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, alpha=0.125), 0.125 * (x.double() @ w.t())
+    assert want.abs().max() < torch.finfo(dtype).max / 2
+    assert_within(got, want, term_size(x, s, group) * 0.125, dtype, k, "product")
+
+
+@pytest.mark.parametrize("tokens", [2, 40, 300])
+def test_a_row_with_nan_or_infinity_keeps_to_itself(mlk, tokens):
+    codes, s, z, _ = w4_weights(528, 1024, 128, BF, True, 1)
+    A, S, Z = mlk.pack_layout_a_w4(*on_gpu(codes, s, z))
+    x = randn((tokens, 1024), BF, 1.0, 2).cuda()
+    clean = mlk.gemm_layoutA_w4(A, S, x, Z)
+    x[0, 5], x[tokens - 1, 1023] = float("nan"), float("inf")
+    got = mlk.gemm_layoutA_w4(A, S, x, Z)
+    assert got[0].isnan().all() and got[-1].isnan().all() and torch.equal(got[1:-1], clean[1:-1])
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 50, 130])
+def test_activations_off_16_bytes_and_empty_batches(mlk, tokens):
+    codes, s, z, _ = w4_weights(272, 640, 128, HF, False, 1)
+    A, S, Z = mlk.pack_layout_a_w4(*on_gpu(codes, s, z))
+    flat = randn((tokens * 640 + 1,), HF, 1.0, 2).cuda()
+    off = flat[1:].view(tokens, 640)
+    assert off.data_ptr() % 16 != 0
+    assert torch.equal(mlk.gemm_layoutA_w4(A, S, off, Z), mlk.gemm_layoutA_w4(A, S, off.clone(), Z))
+    assert mlk.gemm_layoutA_w4(A, S, off[:0], Z).shape == (0, 272)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        mlk.gemm_layoutA_w4(A, S, randn((tokens, 1280), HF, 1.0, 2).cuda()[:, ::2])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mlk.gemm_layoutA_w4(A, S, off, bias=torch.zeros(1, 272, dtype=HF))
+    p1, p2, _, _ = layer(4, 128, 128, 128, HF, False, 3)
+    (a1, s1, _), (a2, s2, _) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    x = flat[1:1 + tokens * 128].view(tokens, 128)
+    ids, wts = on_gpu(*routing(tokens, 4, 2, HF, 1))
+    assert torch.equal(mlk.fused_experts_w4(x, a1, a2, ids, wts, s1, s2), mlk.fused_experts_w4(x.clone(), a1, a2, ids, wts, s1, s2))
+    assert mlk.fused_experts_w4(x[:0], a1, a2, ids[:0], wts[:0], s1, s2).shape == (0, 128)
+
+
+@pytest.mark.parametrize("tokens,n,k", [(1, 512, 2048), (17, 512, 7168), (50, 272, 640), (65, 272, 1152), (1030, 1040, 384)])
+def test_rows_behind_the_last_one_are_left(mlk, tokens, n, k):
+    from muxi_native_layout_kernels_amd import _lib
+    lib = _lib.load()
+    codes, s, _, _ = w4_weights(n, k, 128, BF, False, 1)
+    A, S, _ = mlk.pack_layout_a_w4(*on_gpu(codes, s, None))
+    x = randn((tokens, k), BF, 1.0, 2).cuda()
+    c = torch.full((tokens + 8, n), 7.0, dtype=BF, device="cuda")
+    need = lib.mlk_gemm_w4_workspace_bytes(tokens, n, k, 128)
+    ws = torch.zeros(need + 4096, dtype=torch.uint8, device="cuda")
+    ws[need:] = 91
+    rc = lib.mlk_gemm_layout_a_w4(A.data_ptr(), S.data_ptr(), None, x.data_ptr(), c.data_ptr(), tokens, n, k, 128, 1, 1.0, None, ws.data_ptr(), need,
+                                  torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.mlk_last_error()
+    assert torch.equal(c[:tokens], mlk.gemm_layoutA_w4(A, S, x)) and (c[tokens:] == 7.0).all() and (ws[need:] == 91).all()
+    if need:
+        assert (ws[:lib.mlk_gemm_counter_bytes()] == 0).all()
+
+
+@pytest.mark.parametrize("T,E,K", [(1, 8, 2), (7, 8, 2), (90, 8, 2), (1100, 8, 2), (2100, 16, 8)])
+def test_experts_keep_to_their_rows_and_workspace(mlk, T, E, K):
+    from muxi_native_layout_kernels_amd import _lib
+    lib = _lib.load()
+    H, I = 256, 128
+    p1, p2, w1, w2 = layer(E, H, I, 64, HF, True, T)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    x = randn((T, H), HF, 1.0, T)
+    ids, wts = routing(T, E, K, HF, T)
+    xd, idsd, wtsd = on_gpu(x, ids, wts)
+    y = torch.full((T + 8, H), 7.0, dtype=HF, device="cuda")
+    need = lib.mlk_experts_w4_workspace_bytes(T, E, K, H, I, 64)
+    ws = torch.randint(0, 256, (need + 4096,), dtype=torch.uint8, device="cuda")          # anything
+    ws[need:] = 91
+    rc = lib.mlk_fused_experts_w4(a1.data_ptr(), s1.data_ptr(), z1.data_ptr(), a2.data_ptr(), s2.data_ptr(), z2.data_ptr(), xd.data_ptr(), T, E, E, K, H, I, 64, 0,
+                                  idsd.data_ptr(), wtsd.data_ptr(), None, y.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.mlk_last_error()
+    assert (y[T:] == 7.0).all() and (ws[need:] == 91).all()
+    assert torch.equal(y[:T], mlk.fused_experts_w4(xd, a1, a2, idsd, wtsd, s1, s2, z1, z2))
+    check_experts(y[:T], expected_experts(x, w1, w2, p1[1], p2[1], ids, wts), HF, "experts")
+
+
+@pytest.mark.parametrize("T,E,K,H,I,group,zeros,dtype", [
+    (1, 2, 2, 3328, 128, 128, True, BF), (9, 2, 1, 3328, 128, 32, False, HF), (9, 2, 2, 128, 3328, 64, True, BF), (60, 2, 1, 256, 8192, 128, False, BF),
+    (150, 2, 2, 128, 8192, 64, True, HF), (1, 2, 2, 65664, 128, 128, False, BF), (3, 2, 1, 128, 65664, 128, True, BF), (33, 200, 32, 128, 128, 128, False, HF)])
+def test_experts_of_every_plan(mlk, T, E, K, H, I, group, zeros, dtype):
+    p1, p2, w1, w2 = layer(E, H, I, group, dtype, zeros, T)
+    x = randn((T, H), dtype, 1.0, T)
+    ids, wts = routing(T, E, K, dtype, T)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    call = lambda: mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2)
+    got = call()
+    check_experts(got, expected_experts(x, w1, w2, p1[1], p2[1], ids, wts), dtype, "experts")
+    assert torch.equal(got, call())
+
+
+def test_offsets_past_32_bits(mlk):
+    """Weights of more than 4 GiB, and an output of more than 2^32 elements: any bytes are valid codes, the last rows are unpacked for the reference."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, k = 1 << 20, 8448
+    A = torch.randint(0, 256, (n // 16, k // 128, 64, 16), dtype=torch.uint8, device="cuda", generator=g)
+    S = torch.full((n // 16, k // 128, 16, 1), 2.0 ** -9, dtype=BF, device="cuda")
+    last = mlk.unpack_layout_a_w4(A[-4:].contiguous(), S[-4:].contiguous())[0].cpu()
+    w = (torch.stack((last & 15, last >> 4), dim=-1).flatten(-2).double() - 8) * 2.0 ** -9
+    s = torch.full((64, k // 128), 2.0 ** -9, dtype=BF)
+    for tokens in (1, 20, 80):
+        x = randn((tokens, k), BF, 1.0, tokens)
+        got = mlk.gemm_layoutA_w4(A, S, x.cuda())[:, -64:]
+        assert_within(got, x.double() @ w.t(), term_size(x, s, 128), BF, k, "last rows")
+    # experts: the last of many against it alone
+    E, H, I = 256, 4096, 4224
+    del A, S
+    a1 = torch.randint(0, 256, (E, 2 * I // 16, H // 128, 64, 16), dtype=torch.uint8, device="cuda", generator=g)
+    a2 = torch.randint(0, 256, (E, H // 16, I // 128, 64, 16), dtype=torch.uint8, device="cuda", generator=g)
+    assert a1.numel() > 1 << 32
+    s1 = torch.full((E, 2 * I // 16, H // 128, 16, 1), 2.0 ** -9, dtype=BF, device="cuda")
+    s2 = torch.full((E, H // 16, I // 128, 16, 1), 2.0 ** -9, dtype=BF, device="cuda")
+    for T in (1, 12):
+        x, wts = randn((T, H), BF, 1.0, T).cuda(), torch.ones((T, 1), dtype=BF, device="cuda")
+        many = mlk.fused_experts_w4(x, a1, a2, torch.full((T, 1), E - 1, dtype=torch.int32, device="cuda"), wts, s1, s2)
+        one = mlk.fused_experts_w4(x, a1[-1:], a2[-1:], torch.zeros((T, 1), dtype=torch.int32, device="cuda"), wts, s1[-1:], s2[-1:])
+        assert torch.equal(many, one) and many.abs().sum() > 0
+    del a1, a2, s1, s2
+    codes, s, _, w = w4_weights(1 << 20, 128, 128, BF, False, 2)
+    A, S, _ = mlk.pack_layout_a_w4(*on_gpu(codes, s, None))
+    x = randn((4200, 128), BF, 1.0, 3)
+    got = mlk.gemm_layoutA_w4(A, S, x.cuda())
+    assert got.numel() > 1 << 32
+    for rows in (slice(0, 8), slice(4192, 4200)):
+        for cols in (slice(0, 64), slice((1 << 20) - 64, 1 << 20)):
+            assert_within(got[rows, cols], x[rows].double() @ w[cols].t(), term_size(x[rows], s[cols], 128), BF, 128, "corner")
+
+
+def test_two_streams_at_once(mlk):
+    """Calls that share K between workgroups, experts and balance losses on two streams side by side give what they give alone."""
+    codes, s, z, _ = w4_weights(1024, 7168, 128, BF, True, 1)
+    A, S, Z = mlk.pack_layout_a_w4(*on_gpu(codes, s, z))
+    p1, p2, _, _ = layer(8, 256, 256, 128, BF, True, 2)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    jobs = []
+    for T in (16, 200):
+        x, x2 = randn((T, 7168), BF, 1.0, T).cuda(), randn((T, 256), BF, 1.0, T).cuda()
+        ids, wts = on_gpu(*routing(T, 8, 2, BF, T))
+        logits = randn((T, 8), BF, 1.0, T).cuda()
+        jobs.append(lambda x=x, x2=x2, ids=ids, wts=wts, logits=logits: (
+            mlk.gemm_layoutA_w4(A, S, x, Z), mlk.fused_experts_w4(x2, a1, a2, ids, wts, s1, s2, z1, z2), mlk.moe_balance_loss(logits, ids)[0], mlk.expert_counts(ids, 8)))
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for _ in range(20):
+        for st, job, out in zip(streams, jobs, got):
+            with torch.cuda.stream(st):
+                out.append(job())
+    torch.cuda.synchronize()
+    for out, ref in zip(got, want):
+        for one in out:
+            assert all(torch.equal(a, b) for a, b in zip(one, ref))
+
+
+def replays(run, inputs, fresh):
+    """Captures run() on a stream of its own, replays it on three further inputs with eager calls in between, checks every replay against the eager result."""
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        run()                                            # every shape once: the capture allocates no workspace
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        out = run()
+    for i in range(4):
+        for t, v in zip(inputs, fresh(i)):
+            t.data.copy_(v)
+        want = [t.clone() for t in run()]                # eager, on the default stream
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+        run()
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("tokens", [1, 16, 50, 100, 2050])
+def test_products_in_a_graph(mlk, tokens):
+    codes, s, z, _ = w4_weights(272, 7168, 128, HF, True, 1)
+    A, S, Z = mlk.pack_layout_a_w4(*on_gpu(codes, s, z))
+    x = randn((tokens, 7168), HF, 1.0, 0).cuda()
+    replays(lambda: [mlk.gemm_layoutA_w4(A, S, x, Z)], [x], lambda i: [randn((tokens, 7168), HF, 1.0, i + 1)])
+
+
+@pytest.mark.parametrize("T", [1, 20, 300, 2100])
+def test_router_experts_and_counts_in_a_graph(mlk, T):
+    from muxi_layout_kernels.muxi_moe_planC import fused_moe_w4
+    E, K, H, I = 16, 8, 256, 256
+    p1, p2, _, _ = layer(E, H, I, 128, BF, True, 2)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    x, logits = randn((T, H), BF, 1.0, 0).cuda(), randn((T, E), BF, 1.0, 1).cuda()
+    load = torch.zeros(E, dtype=torch.int32, device="cuda")
+
+    def run():
+        before = load.clone()
+        y = fused_moe_w4(x, a1, a2, logits, K, True, s1, s2, z1, z2, expert_load=load)
+        return [y, load - before]
+    replays(run, [x, logits], lambda i: [randn((T, H), BF, 1.0, i + 2), randn((T, E), BF, 1.0, i + 9)])
+
+
+@pytest.mark.parametrize("sequences", [None, 5, 100])
+def test_balance_loss_and_gradient_in_a_graph(mlk, sequences):
+    """Forward and backward; the leaf's eager losses are dropped before the capture, and while it runs."""
+    T, E, K = 3000, 64, 6
+    logits = randn((T, E), BF, 1.0, 0).cuda().requires_grad_(True)
+    ids = torch.randint(0, E, (T, K), dtype=torch.int32, device="cuda")
+    cu = None if sequences is None else torch.linspace(0, T, sequences + 1).int().cuda()
+    up = torch.tensor(3.0, device="cuda")
+
+    def run():
+        loss, counts = mlk.moe_balance_loss(logits, ids, cu_seqlens=cu)
+        grad, = torch.autograd.grad(loss, logits, grad_outputs=up)
+        return [loss.detach(), counts, grad]
+    g = torch.Generator().manual_seed(3)
+    replays(run, [logits, ids], lambda i: [randn((T, E), BF, 1.0, i + 1), torch.randint(0, E, (T, K), dtype=torch.int32, generator=g)])
+
+
+def test_counts_in_a_graph(mlk):
+    for T, E in ((64, 256), (30000, 64)):
+        ids = torch.randint(0, E, (T, 6), dtype=torch.int32, device="cuda")
+        replays(lambda: [mlk.expert_counts(ids, E)], [ids], lambda i: [torch.randint(0, E, (T, 6), dtype=torch.int32)])
+
+
+@pytest.mark.parametrize("dtype", [HF, BF, torch.float32])
+@pytest.mark.parametrize("E", [8, 64, 256])
+def test_logits_off_their_vectors(mlk, dtype, E):
+    """A view that begins one element on: the loss, the counts and the gradient are those of its copy."""
+    T, K = 333, 4
+    flat = randn((T * E + 1,), dtype, 1.0, E).cuda()
+    ids = torch.randint(0, E, (T, K), dtype=torch.int32, device="cuda")
+    out = []
+    for view in (flat[1:].view(T, E), flat[1:].clone().view(T, E)):
+        leaf = view.detach().requires_grad_(True)
+        loss, counts = mlk.moe_balance_loss(leaf, ids, "sigmoid")
+        out.append((loss.detach(), counts, torch.autograd.grad(loss, leaf)[0]))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+def test_workspaces_are_counted_and_released(mlk):
+    logits, ids = torch.randn(5000, 64, device="cuda"), torch.zeros((5000, 2), dtype=torch.int32, device="cuda")
+    before = mlk.moe_balance_loss(logits, ids)[0]
+    torch.cuda.synchronize()
+    assert mlk.ops.workspace_bytes_held() > 0
+    assert mlk.ops.release_workspaces() > 0 and mlk.ops.workspace_bytes_held() == 0
+    assert torch.equal(mlk.moe_balance_loss(logits, ids)[0], before)
+
+
+def test_a_refused_layer_counts_nothing(mlk):
+    from muxi_layout_kernels.muxi_moe_planC import fused_moe_w4
+    p1, p2, _, _ = layer(4, 128, 128, 128, BF, True, 1)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    load = torch.zeros(4, dtype=torch.int32, device="cuda")
+    x, logits = randn((3, 128), BF, 1.0, 1).cuda(), randn((3, 4), BF, 1.0, 2).cuda()
+    with pytest.raises(RuntimeError, match="both w1 and w2"):
+        fused_moe_w4(x, a1, a2, logits, 2, True, s1, s2, z1, None, expert_load=load)
+    with pytest.raises(RuntimeError, match="n_experts"):
+        fused_moe_w4(x, a1, a2, logits, 2, True, s1, s2, z1, z2, expert_load=load[:3])
+    assert (load == 0).all()
+    fused_moe_w4(x, a1, a2, logits, 2, True, s1, s2, z1, z2, expert_load=load)
+    assert load.sum() == 6
