@@ -68,10 +68,15 @@ __device__ __forceinline__ f32x4 w4_fold(const f32x4 *red, int c, int waves, int
 }
 
 // ---------------------------------------------------------------------------------------------------------- several tokens
+// Registers: 128 for two workgroups on a CU (without the bound 132 with zero points and 58.8 -> 60.1 us for 128 experts of 2048 x 768 at 50 tokens); groups of 32 with
+// zero points would spill.
+template <int GS, bool ZP>
+__host__ __device__ constexpr int w4_moe_waves() { return GS == 1 && ZP ? 2 : 4; }
+
 // One block of 16 tokens a task.  Eight waves: wk of them share the k of R row groups, tile by tile, and add their sums through LDS in wave order.  With all
 // eight on one set of row groups the 16 tiles of K = 2048 are two a wave, and a workgroup is mostly its start and end.
 template <class T, int GS, bool ZP, int R>
-__global__ void __launch_bounds__(512) w4_moe_gate_up_kernel(W4MoeArgs p) {
+__global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     if ((int)blockIdx.y >= *p.n_tasks) return;
     const MoeTask task = p.tasks[blockIdx.y];
@@ -99,7 +104,7 @@ __global__ void __launch_bounds__(512) w4_moe_gate_up_kernel(W4MoeArgs p) {
 }
 
 template <class T, int GS, bool ZP, int R>
-__global__ void __launch_bounds__(512) w4_moe_down_kernel(W4MoeArgs p) {
+__global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_down_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     if ((int)blockIdx.y >= *p.n_tasks) return;
     const MoeTask task = p.tasks[blockIdx.y];
@@ -183,32 +188,36 @@ __global__ void __launch_bounds__(512) w4_moe1_gate_up_kernel(W4MoeArgs p) {
     }
 }
 
-template <class T, int GS, bool ZP, int R>
+// XL: the intermediates of all picks are staged in LDS, which leaves registers for eight tiles in flight (8 experts of 4096 x 14336: the layer 43.0 -> 41.7 us).
+template <class T, int GS, bool ZP, int R, bool XL>
 __global__ void __launch_bounds__(512) w4_moe1_down_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int r16 = lane & 15, rg0 = blockIdx.x * R;
-    // wave w takes picks w % lanes_of, w % lanes_of + lanes_of, ... and of each the tiles of its place among the waves that share it
+    u32x4 *xl = reinterpret_cast<u32x4 *>(red);
+    if constexpr (XL)
+        for (int i = threadIdx.x; i < p.K * (p.I >> 3); i += blockDim.x) xl[i] = ld_global_u32x4(p.hbuf + (size_t)i * 8);
+    // wave w takes picks w % side, w % side + side, ... and of each the tiles of its place among the waves that share it
     const int side = min(p.K, waves), mine = wave % side, place = wave / side, sharing = (waves - mine + side - 1) / side;
     float sum[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) sum[r] = 0.f;
     for (int k = mine; k < p.K; k += side) {
-        const int e = w4_expert(p, k);
-        if (e < 0) continue;
-        const W4Matrix m = w4_of_expert<GS>(p.w2, e, p.H, p.I, p.blocks2);
+        const int e = w4_expert(p, k), tiles = p.I >> 7;                  // a dropped pick has no tiles
+        const W4Matrix m = w4_of_expert<GS>(p.w2, max(e, 0), p.H, p.I, p.blocks2);
         W4Rows<R> rows;
 #pragma unroll
-        for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r, p.I >> 7, p.blocks2);
+        for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r, tiles, p.blocks2);
         const uint16_t *xrow[1] = {p.hbuf + (size_t)k * p.I};
         f32x4 acc[R][1];
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-        w4_stream<T, GS, ZP, 1, R, w4_moe_ring(R), false>(acc, rows, xrow, nullptr, place, p.I >> 7, sharing, p.inv, lane, false);
-        const float wt = T::to_f32(p.wts[k]);
+        w4_stream<T, GS, ZP, 1, R, XL ? 8 : w4_moe_ring(R), XL>(acc, rows, xrow, xl + k * (p.I >> 3), place, e < 0 ? 0 : tiles, sharing, p.inv, lane, k == mine);
+        const float wt = e < 0 ? 0.f : T::to_f32(p.wts[k]);
 #pragma unroll
         for (int r = 0; r < R; ++r) sum[r] = fmaf(wt, acc[r][0][0], sum[r]);
     }
+    if constexpr (XL) __syncthreads();                    // the other waves still read the intermediates
     float *part = reinterpret_cast<float *>(red);
     if (lane < 16)
 #pragma unroll
@@ -273,7 +282,10 @@ static int w4_moe1_gate_up(const W4MoeArgs &a, hipStream_t s) {
 }
 template <class T, int GS, bool ZP, int R>
 static int w4_moe1_down(const W4MoeArgs &a, hipStream_t s) {
-    MLK_W4_MOE(w4_moe1_down_kernel, dim3(a.H / 16 / R), 8, (size_t)8 * R * 64, T, GS, ZP, R);
+    const size_t h = (size_t)a.K * a.I * 2;
+    const size_t part = (size_t)8 * R * 64;
+    if (h <= 128 * 1024) MLK_W4_MOE(w4_moe1_down_kernel, dim3(a.H / 16 / R), 8, (h > part ? h : part), T, GS, ZP, R, true);
+    else MLK_W4_MOE(w4_moe1_down_kernel, dim3(a.H / 16 / R), 8, part, T, GS, ZP, R, false);
     return MLK_OK;
 }
 
