@@ -8,8 +8,8 @@ namespace mlk {
 #define MLK_W4_EXTERN(T, GS)                                                                              \
     extern template int w4_launch_moe<T, GS, false>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);   \
     extern template int w4_launch_moe<T, GS, true>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);    \
-    extern template int w4_launch_moe_panel<T, GS, false>(const W4MoeArgs &, const W4MoePlan &, const int32_t *, int, hipStream_t);   \
-    extern template int w4_launch_moe_panel<T, GS, true>(const W4MoeArgs &, const W4MoePlan &, const int32_t *, int, hipStream_t);
+    extern template int w4_launch_moe_panel<T, GS, false>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);   \
+    extern template int w4_launch_moe_panel<T, GS, true>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);
 MLK_W4_EXTERN(F16, 4)
 MLK_W4_EXTERN(F16, 2)
 MLK_W4_EXTERN(F16, 1)
@@ -165,7 +165,6 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
         a.wk2 = pl.wk2;
         a.sums1 = ws.sums1;
         a.sums2 = ws.sums2;
-        const int max_slots = (int)(((int64_t)a.n_pairs + n_experts * 15 + 15) / 16 * 16);
         int rc = MLK_OK;
         if (pl.tt) {
             rc = launch_moe_align(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks,
@@ -176,7 +175,7 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
 #define MLK_W4_GO(T, GS)                                                                                                                     \
     do {                                                                                                                                         \
         if (pl.panels)                                                                                                                           \
-            rc = zp ? w4_launch_moe_panel<T, GS, true>(a, pl, ws.padded, max_slots, s) : w4_launch_moe_panel<T, GS, false>(a, pl, ws.padded, max_slots, s); \
+            rc = zp ? w4_launch_moe_panel<T, GS, true>(a, pl, s) : w4_launch_moe_panel<T, GS, false>(a, pl, s);                                  \
         else                                                                                                                                     \
             rc = zp ? w4_launch_moe<T, GS, true>(a, pl, s) : w4_launch_moe<T, GS, false>(a, pl, s);                                              \
     } while (0)

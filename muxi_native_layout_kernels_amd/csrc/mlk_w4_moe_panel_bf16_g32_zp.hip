@@ -2,5 +2,5 @@
 #include "mlk_w4_moe_panel.cuh"
 
 namespace mlk {
-template int w4_launch_moe_panel<BF16, 1, true>(const W4MoeArgs &, const W4MoePlan &, const int32_t *, int, hipStream_t);
+template int w4_launch_moe_panel<BF16, 1, true>(const W4MoeArgs &, const W4MoePlan &, hipStream_t);
 }  // namespace mlk

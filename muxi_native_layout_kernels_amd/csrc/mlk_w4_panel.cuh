@@ -33,36 +33,42 @@ namespace mlk {
 // Octets of sum x of a token: one for each group of a window (128 k), and one of zeros behind the last.
 __host__ __device__ constexpr int w4_sum_pitch(int k, int gs) { return k / 128 * (4 / gs) + 1; }
 
-// c[token][window * G + g] = parts of the sum of the group's 32 GS activations; 4 GS lanes read a group.  `blocks`: null, or how many blocks of 16
-// tokens there are, known on the device only.
+// Sum of eight activations in a lane and those of 32 GS: of 4 GS lanes; and its parts.
 template <class T, int GS>
-__global__ void __launch_bounds__(256) w4_sums_kernel(const uint16_t *__restrict__ x, u32x4 *__restrict__ c, int tokens, int k,
-                                                      const int32_t *__restrict__ blocks) {
+__device__ __forceinline__ float w4_group_sum(const u32x4 &v) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += T::to_f32(v[j] & 0xffffu) + T::to_f32(v[j] >> 16);
+#pragma unroll
+    for (int m = 1; m < 4 * GS; m <<= 1) s += __shfl_xor(s, m);
+    return s;
+}
+__device__ __forceinline__ u32x4 w4_sum_parts(float s) {
+    const uint32_t c1 = f32_to_bf16_bits(s);
+    const float r1 = s - bf16_bits_to_f32(c1);
+    const uint32_t c2 = f32_to_bf16_bits(r1), c3 = f32_to_bf16_bits(r1 - bf16_bits_to_f32(c2));
+    return u32x4{c1 | c2 << 16, c3 | c1 << 16, c2, 0u};
+}
+
+// c[token][window * G + g] = parts of the sum of the group's 32 GS activations.
+template <class T, int GS>
+__global__ void __launch_bounds__(256) w4_sums_kernel(const uint16_t *__restrict__ x, u32x4 *__restrict__ c, int tokens, int k) {
     constexpr int LANES = 4 * GS;
-    if (blocks) tokens = min(tokens, 16 * *blocks);
     const int per_token = k / 8, pitch = w4_sum_pitch(k, GS);
     const int64_t total = (int64_t)tokens * per_token;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {        // total is a multiple of 16
         const int64_t token = i / per_token;
         const int at = (int)(i - token * per_token);
-        const u32x4 v = ld_global_u32x4(x + i * 8);
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s += T::to_f32(v[j] & 0xffffu) + T::to_f32(v[j] >> 16);
-#pragma unroll
-        for (int m = 1; m < LANES; m <<= 1) s += __shfl_xor(s, m);
-        const uint32_t c1 = f32_to_bf16_bits(s);
-        const float r1 = s - bf16_bits_to_f32(c1);
-        const uint32_t c2 = f32_to_bf16_bits(r1), c3 = f32_to_bf16_bits(r1 - bf16_bits_to_f32(c2));
-        if (at % LANES == 0) c[token * pitch + at / LANES] = u32x4{c1 | c2 << 16, c3 | c1 << 16, c2, 0u};
+        const float s = w4_group_sum<T, GS>(ld_global_u32x4(x + i * 8));
+        if (at % LANES == 0) c[token * pitch + at / LANES] = w4_sum_parts(s);
         if (at == 0) c[token * pitch + pitch - 1] = u32x4{0u, 0u, 0u, 0u};
     }
 }
 
 template <class T, int GS>
-static int w4_launch_sums(const uint16_t *x, u32x4 *c, int tokens, int k, const int32_t *blocks, hipStream_t s) {
+static int w4_launch_sums(const uint16_t *x, u32x4 *c, int tokens, int k, hipStream_t s) {
     const int64_t wgs = ((int64_t)tokens * (k / 8) + 255) / 256;
-    w4_sums_kernel<T, GS><<<(int)(wgs < 2048 ? wgs : 2048), 256, 0, s>>>(x, c, tokens, k, blocks);
+    w4_sums_kernel<T, GS><<<(int)(wgs < 2048 ? wgs : 2048), 256, 0, s>>>(x, c, tokens, k);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }

@@ -104,7 +104,7 @@ static int w4_launch_panel_one(W4PanelArgs a, hipStream_t s) {
     static bool ready_on[64] = {};
     const int rc = panel_lds_attribute(&w4_panel_kernel<T, GS, ZP, TB>, P::lds_bytes, ready_on);
     if (rc != MLK_OK) return rc;
-    const int rc2 = w4_launch_sums<T, GS>(a.X, a.sums, a.M, a.K, nullptr, s);
+    const int rc2 = w4_launch_sums<T, GS>(a.X, a.sums, a.M, a.K, s);
     if (rc2 != MLK_OK) return rc2;
     w4_panel_kernel<T, GS, ZP, TB><<<a.row_tiles * a.token_tiles * a.slices, 512, P::lds_bytes, s>>>(a);
     MLK_LAUNCH_CHECK();
