@@ -34,6 +34,9 @@ __host__ __device__ constexpr int w4_ring(int tt, int r, bool xl) {
     return xl ? (r == 1 ? 8 : 4) : (tt == 1 ? (r <= 2 ? 4 : 2) : (tt * r <= 8 && tt < 4 ? 2 : 1));
 }
 
+// Cells that the waves add at a time: eight waves of 16 take 128 KiB of LDS.
+__host__ __device__ constexpr int w4_fold_cells(int cells) { return cells > 16 ? cells / 2 : cells; }
+
 template <class T, int GS, bool ZP, int TT, int R, bool XL>
 __global__ void __launch_bounds__(w4_stream_waves(TT, R, XL) * 64) w4_stream_kernel(W4GemmArgs p) {
     extern __shared__ u32x4 lds[];
@@ -73,17 +76,19 @@ __global__ void __launch_bounds__(w4_stream_waves(TT, R, XL) * 64) w4_stream_ker
     };
     auto part = [&](int s, int c) { return p.partial + (((size_t)blockIdx.x * p.slices + s) * CELLS + c) * 64; };
     f32x4 *red = reinterpret_cast<f32x4 *>(lds);
-    if constexpr (XL) __syncthreads();                    // the other waves still read the token
+    constexpr int FOLD = w4_fold_cells(CELLS);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int c0 = 0; c0 < CELLS; c0 += FOLD) {
+        if (XL || c0 > 0) __syncthreads();                // the other waves still read the token, or the cells before
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) red[(wave * CELLS + r * TT + tt) * 64 + lane] = acc[r][tt];
-    __syncthreads();
-    for (int c = wave; c < CELLS; c += waves) {
-        f32x4 v = red[c * 64 + lane];
-        for (int w = 1; w < waves; ++w) v += red[(w * CELLS + c) * 64 + lane];
-        if (p.slices == 1) store(c, v);
-        else st_agent_planar(part(blockIdx.y, c), 64, lane, v);
+        for (int c = c0; c < c0 + FOLD; ++c) red[(wave * FOLD + c - c0) * 64 + lane] = acc[c / TT][c % TT];
+        __syncthreads();
+        for (int c = c0 + wave; c < c0 + FOLD; c += waves) {
+            f32x4 v = red[(c - c0) * 64 + lane];
+            for (int w = 1; w < waves; ++w) v += red[(w * FOLD + c - c0) * 64 + lane];
+            if (p.slices == 1) store(c, v);
+            else st_agent_planar(part(blockIdx.y, c), 64, lane, v);
+        }
     }
     if (p.slices == 1) return;
     // every wave waits for its own stores before the barrier and the arrival is counted behind it: whoever sees all the others can read their sums
@@ -107,7 +112,7 @@ static int w4_launch_stream_one(W4GemmArgs a, int wgs, int waves, hipStream_t s)
     a.rg_more = groups % wgs;
     a.t_each = t / a.slices;
     a.t_more = t % a.slices;
-    size_t lds = (size_t)waves * R * TT * 1024;
+    size_t lds = (size_t)waves * w4_fold_cells(R * TT) * 1024;
     if (XL && (size_t)per_slice * 256 > lds) lds = (size_t)per_slice * 256;
     if (waves > w4_stream_waves(TT, R, XL) || lds > 150 * 1024) return fail(MLK_ERR_INVALID, "w4 gemm: launch parameters");
     if (lds > 48 * 1024) {
@@ -126,7 +131,7 @@ static int w4_launch_stream_one(W4GemmArgs a, int wgs, int waves, hipStream_t s)
     return MLK_OK;
 }
 
-// r = row groups per workgroup the kernel is built for: 1, 2 or 4; wgs * r >= N / 16.  One token is staged in LDS (r = 1, 2; a slice of 64 K at most): 4096 x 4096
+// r = row groups per workgroup the kernel is built for: 1, 2 or 4, from five tokens to 48 also 8; wgs * r >= N / 16.  One token is staged in LDS (r = 1, 2; a slice of 64 K at most): 4096 x 4096
 // 4.7 us against 5.1.
 template <class T, int GS, bool ZP>
 int w4_launch_stream(const W4GemmArgs &a, int r, int wgs, int waves, hipStream_t s) {
@@ -136,6 +141,7 @@ int w4_launch_stream(const W4GemmArgs &a, int r, int wgs, int waves, hipStream_t
         if (r == 1) return w4_launch_stream_one<T, GS, ZP, TT, 1, XL>(a, wgs, waves, s);       \
         if (r == 2) return w4_launch_stream_one<T, GS, ZP, TT, 2, XL>(a, wgs, waves, s);       \
         if (r == 4) return w4_launch_stream_one<T, GS, ZP, TT, 4, XL>(a, wgs, waves, s);       \
+        if (TT < 4 && r == 8) return w4_launch_stream_one<T, GS, ZP, (TT < 4 ? TT : 1), 8, XL>(a, wgs, waves, s); \
     } while (0)
     if (a.M == 1 && (a.K / kW4TileK + a.slices - 1) / a.slices * 256 <= kW4TokenLds) {
         if (r == 1) return w4_launch_stream_one<T, GS, ZP, 1, 1, true>(a, wgs, waves, s);

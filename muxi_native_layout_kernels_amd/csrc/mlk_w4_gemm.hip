@@ -1,4 +1,6 @@
 // Linear layers over 4-bit weights: one token (GeMV) to prefill-sized batches.
+#include <algorithm>
+
 #include "mlk_w4_panel_gemm.cuh"
 
 namespace mlk {
@@ -27,9 +29,13 @@ struct W4Plan {
 // Up to 64 tokens.  Microseconds on weights from memory, groups of 128, bf16 (r row groups a workgroup, s slices of K):
 //   one to four tokens   one workgroup per CU as far as r <= 4 goes, K whole: 4096 x 4096 r = 1 4.7 (s = 2: 6.3), 4096 x 14336 r = 1 9.8, r = 2 s = 2 10.7; 28672 x 8192 one
 //                        token r = 2 25.7, r = 4 27.5, two tokens r = 4 24.9, r = 2 31.6
-//   more                 the activations weigh more, r = 4 shares them between four row groups; slices bring the workgroups back: 4096 x 14336 at 16 tokens r = 1
+//   more                 the activations weigh more (every workgroup reads all of them): r = 8 where that many row groups each, in slices of 48 tiles at least, leave
+//                        three quarters of the CUs a workgroup (up to 48 tokens: its sums fit the registers): 28672 x 8192 at 32 tokens r = 4 45.7, r = 8 32.6,
+//                        at 16 31.2 and 28.8; 27648 x 5120 at 48 39.0 and 29.1; 28672 x 4096 at 16 16.6 and 17.3; not 13824 x 5120 at 32, r = 4 18.8, r = 8 s = 2 19.1.
+//                        Else r = 4, and slices bring the workgroups back: 4096 x 14336 at 16 tokens r = 1
 //                        16.7, r = 2 s = 2 13.6, r = 4 s = 4 11.6, at 64 53, 31 and 23; 512 x 7168 at 64 tokens r = 1 27.6, s = 8 8.9.  At least six tiles a slice
-//                        (1280 x 5120 at 16 tokens r = 2 s = 4 6.3, s = 8 9)
+//                        (1280 x 5120 at 16 tokens r = 2 s = 4 6.3, s = 8 9).  More workgroups than CUs have four waves (57344 x 2048 at 32 tokens r = 8 25.0, with four
+//                        22.2; fewer eight: 28672 x 8192 32.9, with four 37.8)
 static W4Plan w4_plan_stream(int m, int n, int k) {
     const int groups = n / 16, tiles = k / 128, cus = device_cus();
     W4Plan pl = {};
@@ -38,15 +44,23 @@ static W4Plan w4_plan_stream(int m, int n, int k) {
     if (m <= 4) {
         while (pl.r < 4 && groups > pl.r * cus) pl.r *= 2;
         if (m == 1 && pl.r == 4 && groups > 4 * cus) pl.r = 2;
+        pl.wgs = (groups + pl.r - 1) / pl.r;
+        pl.waves = m == 1 && pl.r == 1 && groups <= cus && tiles >= 16 && tiles * 256 <= kW4TokenLds ? 16 : 8;      // 16: only with the token in LDS
+        return pl;
+    }
+    auto slices_of = [&](int wgs, int most) { return std::max(1, std::min(cus / wgs, most)); };
+    const int wide = (groups + 7) / 8;
+    if (m <= 48 && 4 * wide * slices_of(wide, tiles / 48) >= 3 * cus) {
+        pl.r = 8;
+        pl.slices = slices_of(wide, tiles / 48);
     } else {
-        const int most = tiles / 6 < 1 ? 1 : (tiles / 6 > 8 ? 8 : tiles / 6);
+        const int most = std::max(1, std::min(tiles / 6, 8));
         pl.r = 4;
         while (pl.r > 1 && (groups + pl.r - 1) / pl.r * most < 128) pl.r /= 2;
-        const int fill = cus / ((groups + pl.r - 1) / pl.r);
-        pl.slices = fill < 1 ? 1 : (fill > most ? most : fill);
+        pl.slices = slices_of((groups + pl.r - 1) / pl.r, most);
     }
     pl.wgs = (groups + pl.r - 1) / pl.r;
-    pl.waves = m == 1 && pl.r == 1 && groups <= cus && tiles >= 16 && tiles * 256 <= kW4TokenLds ? 16 : 8;      // 16: only with the token in LDS
+    pl.waves = pl.wgs > cus ? 4 : 8;
     return pl;
 }
 
@@ -60,14 +74,14 @@ static double w4_panel_cost(int m, int n, int k, int group, int tb, int slices, 
     const double window = (tb == 2 ? 0.82 + 0.2 * full : 1.18 + 0.5 * full) * (g == 1 ? 1.0 : (g == 2 ? 1.15 : 1.45));
     return rounds * (windows + (windows * g + 15) / 16 + 3) * window + 6 + (slices > 1 ? 2 + (double)slices * m * n * 8 / 5e6 : 0);
 }
-// And of the streaming kernels from 33 to 64 tokens: the weights' bytes and as many again for every block of 16 tokens and the row groups that share it.
-static double w4_stream_cost(int m, int n, int k) { return 4 + (double)n * k / 2e6 * (0.085 + 0.134 * ((m + 15) / 16)); }
+// And of the streaming kernels from 33 to 64 tokens: the weights' bytes, and the activations' for every block of 16 tokens and the row groups that share them.
+static double w4_stream_cost(int m, int n, int k, int r) { return 4 + (double)n * k / 2e6 * (0.085 + (r == 8 ? 0.082 : 0.134) * ((m + 15) / 16)); }
 
 static W4Plan w4_plan(int m, int n, int k, int group) {
     const W4Plan stream = w4_plan_stream(m < 64 ? m : 64, n, k);
     if (m <= 32) return stream;
     W4Plan best = {};
-    double least = m <= 64 ? w4_stream_cost(m, n, k) : 1e30;
+    double least = m <= 64 ? w4_stream_cost(m, n, k, stream.r) : 1e30;
     if (m <= 64) best = stream;
     const int cus = device_cus();
     for (int tb = 2; tb <= 4; tb += 2)

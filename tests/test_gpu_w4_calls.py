@@ -305,3 +305,27 @@ def test_a_refused_layer_counts_nothing(mlk):
     assert (load == 0).all()
     fused_moe_w4(x, a1, a2, logits, 2, True, s1, s2, z1, z2, expert_load=load)
     assert load.sum() == 6
+
+
+@pytest.mark.parametrize("n,k,group,zeros,dtype", [(24592, 384, 128, False, BF), (24592, 256, 32, True, HF), (57360, 128, 64, True, BF), (8192, 18432, 128, True, HF),
+                                                   (4112, 36864, 32, False, BF)])
+@pytest.mark.parametrize("tokens", [5, 16, 20, 33, 48, 49])
+def test_eight_row_groups_a_workgroup(mlk, tokens, n, k, group, zeros, dtype):
+    """Tall and long weights: any bytes are valid codes, some of the rows are unpacked for the reference."""
+    g = torch.Generator(device="cuda").manual_seed(n + tokens)
+    per = max(1, 128 // group)
+    shape = (n // 16, k // max(128, group), 16, per)
+    A = torch.randint(0, 256, (n // 16, k // 128, 64, 16), dtype=torch.uint8, device="cuda", generator=g)
+    S = ((torch.rand(shape, device="cuda", generator=g) + 0.5) * (k ** -0.5 / 4.6)).to(dtype)
+    Z = torch.randint(0, 16, shape, dtype=torch.uint8, device="cuda", generator=g) if zeros else None
+    x, bias = randn((tokens, k), dtype, 1.0, 3), randn((1, n), dtype, 1.0, 4)
+    got = mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, bias=bias.cuda())
+    assert torch.equal(got, mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, bias=bias.cuda()))
+    for first in (0, n // 32 - 3, n // 16 - 9):                      # nine row groups from here
+        rows = slice(first, first + 9)
+        codes, s, z = mlk.unpack_layout_a_w4(A[rows].contiguous(), S[rows].contiguous(), None if Z is None else Z[rows].contiguous())
+        q = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).cpu().double()
+        off = torch.full(s.shape, 8.0, dtype=torch.float64) if z is None else z.cpu().double()
+        w = (q - off.repeat_interleave(group, dim=1)) * s.cpu().double().repeat_interleave(group, dim=1)
+        cols = slice(first * 16, (first + 9) * 16)
+        assert_within(got[:, cols], x.double() @ w.t() + bias[:, cols].double(), term_size(x, s.cpu(), group) + bias[:, cols].double().abs(), dtype, k, "rows %d" % first)
