@@ -27,6 +27,7 @@ struct W4MoeArgs {
     uint16_t *hbuf;              // [slot][I]
     float *obuf;                 // [pair][slice][H]
     int slices;                  // of the down projection's k
+    bool few;                    // streaming kernels: at most 64 pairs, every wave finds its task by itself (sorted, tasks and n_tasks are not read)
     int wk1, wk2;                // streaming kernels: waves that share a row group's k; the 8 / wk sets of them take different row groups
     u32x4 *sums1, *sums2;        // panels: sums of x, of the intermediate (w4_sums_kernel)
 };
@@ -73,19 +74,57 @@ __device__ __forceinline__ f32x4 w4_fold(const f32x4 *red, int c, int waves, int
 template <int GS, bool ZP>
 __host__ __device__ constexpr int w4_moe_waves() { return GS == 1 && ZP ? 2 : 4; }
 
+// The 16 slots of a task: expert, place of the first in the order, and the pair in slot lane % 16 (n_pairs: none).  False: no such task.
+// With few pairs a wave takes them one per lane, goes through the experts in the order of their first pair and counts their blocks: no alignment
+// launch (64 experts of 2048 x 1408, top-6, 4 tokens: 39.6 -> 36.4 us).
+struct W4MoeBlock {
+    int expert, slot0, pair;
+};
+__device__ __forceinline__ bool w4_moe_block(const W4MoeArgs &p, int task, int lane, W4MoeBlock &b) {
+    if (!p.few) {
+        if (task >= *p.n_tasks) return false;
+        const MoeTask t = p.tasks[task];
+        b.expert = t.expert;
+        b.slot0 = t.block0 * 16;
+        b.pair = p.sorted[b.slot0 + (lane & 15)];
+        return true;
+    }
+    const int e = lane < p.n_pairs ? w4_expert(p, lane) : -1;
+    unsigned long long todo = __ballot(e >= 0);
+    int before = 0;
+    while (todo) {
+        const int first = __builtin_amdgcn_readfirstlane(__ffsll((long long)todo) - 1), expert = __builtin_amdgcn_readlane(e, first);
+        const unsigned long long same = __ballot(e == expert);
+        const int pairs = __popcll(same), blocks = (pairs + 15) >> 4;
+        if (task < before + blocks) {
+            const int block = task - before, rank = __popcll(same & ((1ull << lane) - 1ull));
+            const bool here = e == expert && rank >> 4 == block;
+            // every pair of this block sends its number to the lane of its slot, the others to the last lane
+            const int sent = __builtin_amdgcn_ds_permute((here ? rank & 15 : 63) * 4, lane);
+            const int got = __shfl(sent, lane & 15);
+            b.expert = expert;
+            b.slot0 = task * 16;
+            b.pair = block * 16 + (lane & 15) < pairs ? got : p.n_pairs;
+            return true;
+        }
+        before += blocks;
+        todo &= ~same;
+    }
+    return false;
+}
+
 // One block of 16 tokens a task.  Eight waves: wk of them share the k of R row groups, tile by tile, and add their sums through LDS in wave order.  With all
 // eight on one set of row groups the 16 tiles of K = 2048 are two a wave, and a workgroup is mostly its start and end.
 template <class T, int GS, bool ZP, int R>
 __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
-    if ((int)blockIdx.y >= *p.n_tasks) return;
-    const MoeTask task = p.tasks[blockIdx.y];
+    W4MoeBlock task;
+    if (!w4_moe_block(p, blockIdx.y, threadIdx.x & 63, task)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = p.wk1;
     const int o = lane >> 4, r16 = lane & 15, set = wave / wk, place = wave - set * wk, rg0 = (blockIdx.x * (8 / wk) + set) * (R / 2);
     W4Rows<R> rows;
     w4_gate_up_rows<GS, R>(rows, p, task.expert, rg0);
-    const int pair = p.sorted[task.block0 * 16 + r16];
-    const uint16_t *xrow[1] = {p.X + (size_t)(pair < p.n_pairs ? pair / p.K : 0) * p.H};
+    const uint16_t *xrow[1] = {p.X + (size_t)(task.pair < p.n_pairs ? task.pair / p.K : 0) * p.H};
     f32x4 acc[R][1];
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -97,7 +136,7 @@ __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_
     for (int c = place; c < HALF; c += wk) {
         if (rg0 + c >= p.I >> 4) continue;
         const f32x4 g = w4_fold<R>(mine, c, wk, lane), u = w4_fold<R>(mine, HALF + c, wk, lane);
-        uint16_t *h = p.hbuf + (size_t)(task.block0 * 16 + o * 4) * p.I + (rg0 + c) * 16 + r16;
+        uint16_t *h = p.hbuf + (size_t)(task.slot0 + o * 4) * p.I + (rg0 + c) * 16 + r16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[(size_t)i * p.I] = (uint16_t)T::from_f32(silu_mul(g[i], u[i]));
     }
@@ -106,15 +145,17 @@ __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_
 template <class T, int GS, bool ZP, int R>
 __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_down_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
-    if ((int)blockIdx.y >= *p.n_tasks) return;
-    const MoeTask task = p.tasks[blockIdx.y];
+    W4MoeBlock task;
+    if (!w4_moe_block(p, blockIdx.y, threadIdx.x & 63, task)) return;
+    __shared__ int pairs[16];
+    if (threadIdx.x < 16) pairs[threadIdx.x] = task.pair;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = p.wk2;
     const int o = lane >> 4, r16 = lane & 15, set = wave / wk, place = wave - set * wk, rg0 = (blockIdx.x * (8 / wk) + set) * R, groups = p.H >> 4;
     const W4Matrix m = w4_of_expert<GS>(p.w2, task.expert, p.H, p.I, p.blocks2);
     W4Rows<R> rows;
 #pragma unroll
     for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, min(rg0 + r, groups - 1), p.I >> 7, p.blocks2);
-    const uint16_t *xrow[1] = {p.hbuf + (size_t)(task.block0 * 16 + r16) * p.I};
+    const uint16_t *xrow[1] = {p.hbuf + (size_t)(task.slot0 + r16) * p.I};
     f32x4 acc[R][1];
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -127,7 +168,7 @@ __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_down_ker
         const f32x4 v = w4_fold<R>(mine, c, wk, lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int pair = p.sorted[task.block0 * 16 + o * 4 + i];
+            const int pair = pairs[o * 4 + i];
             if (pair < p.n_pairs) p.obuf[(size_t)pair * p.H + (rg0 + c) * 16 + r16] = T::to_f32(p.wts[pair]) * v[i];
         }
     }
@@ -249,6 +290,7 @@ struct W4MoePlan {
     int tt;                  // blocks of 16 tokens per task; 0: one token
     int max_tasks;
     int wk1, wk2;
+    bool few;
     bool panels;             // tasks of up to 8 blocks run panels
     int slices;              // of their down projection
 };

@@ -48,6 +48,7 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
         // 64 of 2048 x 1408, down at 32 tokens 73.5 and 70.4); with many, eight (8 of 4096 x 14336 at 16 tokens 119.5, with two 123 each).
         pl.wk1 = hidden / 128 >= 24 ? 8 : 2;
         pl.wk2 = inter / 128 >= 24 ? 8 : 2;
+        pl.few = pairs <= 64;
         return pl;
     }
     // Two K slices of a long down projection that would leave CUs without a panel in its last round: 8 experts of 4096 x 14336 at 100 tokens 276 -> 240 us, at
@@ -161,12 +162,13 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
         a.hbuf = ws.hbuf;
         a.obuf = ws.obuf;
         a.slices = pl.slices;
+        a.few = pl.few;
         a.wk1 = pl.wk1;
         a.wk2 = pl.wk2;
         a.sums1 = ws.sums1;
         a.sums2 = ws.sums2;
         int rc = MLK_OK;
-        if (pl.tt) {
+        if (pl.tt && !pl.few) {
             rc = launch_moe_align(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks,
                                   ws.n_tasks, pl.tt, s);
             if (rc != MLK_OK) return rc;

@@ -329,3 +329,19 @@ def test_eight_row_groups_a_workgroup(mlk, tokens, n, k, group, zeros, dtype):
         w = (q - off.repeat_interleave(group, dim=1)) * s.cpu().double().repeat_interleave(group, dim=1)
         cols = slice(first * 16, (first + 9) * 16)
         assert_within(got[:, cols], x.double() @ w.t() + bias[:, cols].double(), term_size(x, s.cpu(), group) + bias[:, cols].double().abs(), dtype, k, "rows %d" % first)
+
+
+@pytest.mark.parametrize("T,E,K,same", [(2, 3, 1, True), (3, 40, 20, False), (32, 4, 2, False), (33, 4, 2, False), (64, 2, 1, True), (64, 5, 1, False), (7, 200, 9, False)])
+def test_few_pairs_and_one_more(mlk, T, E, K, same):
+    """Up to 64 pairs the kernels find their tasks by themselves, above an alignment launch does: experts with none, one, 16, 17 and all of the pairs, some dropped."""
+    p1, p2, w1, w2 = layer(E, 128, 256, 64, BF, True, T)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    x = randn((T, 128), BF, 1.0, T)
+    ids, wts = routing(T, E, K, BF, T)
+    if same:
+        ids[:] = E - 1
+    ids[T // 2, 0] = -1
+    got = mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2)
+    check_experts(got, expected_experts(x, w1, w2, p1[1], p2[1], ids, wts), BF, "experts")
+    gone = torch.full_like(ids, E)
+    assert (mlk.fused_experts_w4(x.cuda(), a1, a2, gone.cuda(), wts.cuda(), s1, s2, z1, z2) == 0).all()
