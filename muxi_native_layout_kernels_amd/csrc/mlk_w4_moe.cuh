@@ -27,7 +27,6 @@ struct W4MoeArgs {
     uint16_t *hbuf;              // [slot][I]
     float *obuf;                 // [pair][slice][H]
     int slices;                  // of the down projection's k
-    bool few;                    // streaming kernels: at most 64 pairs, every wave finds its task by itself (sorted, tasks and n_tasks are not read)
     int wk1, wk2;                // streaming kernels: waves that share a row group's k; the 8 / wk sets of them take different row groups
     u32x4 *sums1, *sums2;        // panels: sums of x, of the intermediate (w4_sums_kernel)
 };
@@ -75,13 +74,14 @@ template <int GS, bool ZP>
 __host__ __device__ constexpr int w4_moe_waves() { return GS == 1 && ZP ? 2 : 4; }
 
 // The 16 slots of a task: expert, place of the first in the order, and the pair in slot lane % 16 (n_pairs: none).  False: no such task.
-// With few pairs a wave takes them one per lane, goes through the experts in the order of their first pair and counts their blocks: no alignment
+// FEW, at most 64 pairs: a wave takes them one per lane, goes through the experts in the order of their first pair and counts their blocks: no alignment
 // launch (64 experts of 2048 x 1408, top-6, 4 tokens: 39.6 -> 36.4 us).
 struct W4MoeBlock {
     int expert, slot0, pair;
 };
+template <bool FEW>
 __device__ __forceinline__ bool w4_moe_block(const W4MoeArgs &p, int task, int lane, W4MoeBlock &b) {
-    if (!p.few) {
+    if constexpr (!FEW) {
         if (task >= *p.n_tasks) return false;
         const MoeTask t = p.tasks[task];
         b.expert = t.expert;
@@ -115,11 +115,11 @@ __device__ __forceinline__ bool w4_moe_block(const W4MoeArgs &p, int task, int l
 
 // One block of 16 tokens a task.  Eight waves: wk of them share the k of R row groups, tile by tile, and add their sums through LDS in wave order.  With all
 // eight on one set of row groups the 16 tiles of K = 2048 are two a wave, and a workgroup is mostly its start and end.
-template <class T, int GS, bool ZP, int R>
+template <class T, int GS, bool ZP, int R, bool FEW>
 __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     W4MoeBlock task;
-    if (!w4_moe_block(p, blockIdx.y, threadIdx.x & 63, task)) return;
+    if (!w4_moe_block<FEW>(p, blockIdx.y, threadIdx.x & 63, task)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = p.wk1;
     const int o = lane >> 4, r16 = lane & 15, set = wave / wk, place = wave - set * wk, rg0 = (blockIdx.x * (8 / wk) + set) * (R / 2);
     W4Rows<R> rows;
@@ -142,11 +142,11 @@ __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_
     }
 }
 
-template <class T, int GS, bool ZP, int R>
+template <class T, int GS, bool ZP, int R, bool FEW>
 __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_down_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     W4MoeBlock task;
-    if (!w4_moe_block(p, blockIdx.y, threadIdx.x & 63, task)) return;
+    if (!w4_moe_block<FEW>(p, blockIdx.y, threadIdx.x & 63, task)) return;
     __shared__ int pairs[16];
     if (threadIdx.x < 16) pairs[threadIdx.x] = task.pair;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = p.wk2;
@@ -290,7 +290,7 @@ struct W4MoePlan {
     int tt;                  // blocks of 16 tokens per task; 0: one token
     int max_tasks;
     int wk1, wk2;
-    bool few;
+    bool few;                // at most 64 pairs, no alignment
     bool panels;             // tasks of up to 8 blocks run panels
     int slices;              // of their down projection
 };
@@ -304,16 +304,16 @@ struct W4MoePlan {
         MLK_LAUNCH_CHECK();                                                                \
     } while (0)
 
-template <class T, int GS, bool ZP, int R>
+template <class T, int GS, bool ZP, int R, bool FEW>
 static int w4_moe_gate_up(const W4MoeArgs &a, int max_tasks, hipStream_t s) {
     const int each = 8 / a.wk1 * (R / 2);
-    MLK_W4_MOE(w4_moe_gate_up_kernel, dim3((a.I / 16 + each - 1) / each, max_tasks), 8, (size_t)8 * R * 1024, T, GS, ZP, R);
+    MLK_W4_MOE(w4_moe_gate_up_kernel, dim3((a.I / 16 + each - 1) / each, max_tasks), 8, (size_t)8 * R * 1024, T, GS, ZP, R, FEW);
     return MLK_OK;
 }
-template <class T, int GS, bool ZP, int R>
+template <class T, int GS, bool ZP, int R, bool FEW>
 static int w4_moe_down(const W4MoeArgs &a, int max_tasks, hipStream_t s) {
     const int each = 8 / a.wk2 * R;
-    MLK_W4_MOE(w4_moe_down_kernel, dim3((a.H / 16 + each - 1) / each, max_tasks), 8, (size_t)8 * R * 1024, T, GS, ZP, R);
+    MLK_W4_MOE(w4_moe_down_kernel, dim3((a.H / 16 + each - 1) / each, max_tasks), 8, (size_t)8 * R * 1024, T, GS, ZP, R, FEW);
     return MLK_OK;
 }
 template <class T, int GS, bool ZP, int R>
@@ -340,8 +340,8 @@ int w4_launch_moe(const W4MoeArgs &a, const W4MoePlan &pl, hipStream_t s) {
         return rc == MLK_OK ? w4_moe1_down<T, GS, ZP, 1>(a, s) : rc;
     }
     // four row groups a wave: 128 registers, two workgroups on a CU (8 experts at 16 tokens: 120 us, with eight 139, with two 129)
-    rc = w4_moe_gate_up<T, GS, ZP, 4>(a, pl.max_tasks, s);
-    if (rc == MLK_OK) rc = w4_moe_down<T, GS, ZP, 4>(a, pl.max_tasks, s);
+    rc = pl.few ? w4_moe_gate_up<T, GS, ZP, 4, true>(a, pl.max_tasks, s) : w4_moe_gate_up<T, GS, ZP, 4, false>(a, pl.max_tasks, s);
+    if (rc == MLK_OK) rc = pl.few ? w4_moe_down<T, GS, ZP, 4, true>(a, pl.max_tasks, s) : w4_moe_down<T, GS, ZP, 4, false>(a, pl.max_tasks, s);
     if (rc != MLK_OK) return rc;
     w4_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
     MLK_LAUNCH_CHECK();

@@ -162,7 +162,6 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
         a.hbuf = ws.hbuf;
         a.obuf = ws.obuf;
         a.slices = pl.slices;
-        a.few = pl.few;
         a.wk1 = pl.wk1;
         a.wk2 = pl.wk2;
         a.sums1 = ws.sums1;
