@@ -697,8 +697,9 @@ def _w4_dims(A, scale, zero, lead, what="A"):
 
 
 def _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, what):
-    key = ("w4", A.shape, A_Scale.shape, B.shape, A.dtype, A_Scale.dtype, B.dtype, A.device, A_Scale.device, B.device,
-           None if A_Zero is None else (A_Zero.shape, A_Zero.dtype, A_Zero.device), None if bias is None else (bias.shape, bias.dtype, bias.device))
+    device = B.get_device()
+    key = ("w4", A.shape, A_Scale.shape, B.shape, A.dtype, A_Scale.dtype, B.dtype, A.get_device(), A_Scale.get_device(), device,
+           None if A_Zero is None else (A_Zero.shape, A_Zero.dtype, A_Zero.get_device()), None if bias is None else (bias.shape, bias.dtype, bias.get_device()))
     plan = _plans.get(key)
     if plan is None or beta != 0 or not (A.is_contiguous() and A_Scale.is_contiguous() and B.is_contiguous() and
                                          (A_Zero is None or A_Zero.is_contiguous()) and (bias is None or bias.is_contiguous())):
@@ -713,20 +714,27 @@ def _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, what):
         lib = _lib.load()
         plan = _plans[key] = (B.size(0), m, k, group, _KIND[B.dtype], lib.mlk_gemm_w4_workspace_bytes(B.size(0), m, k, group),
                               lib.mlk_gemm_counter_bytes(), lib.mlk_gemm_layout_a_w4)
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _w4_launch(plan, A, A_Scale, B, A_Zero, alpha, bias, what)
+    return _w4_launch(plan, A, A_Scale, B, A_Zero, alpha, bias, what)
+
+
+def _w4_launch(plan, A, A_Scale, B, A_Zero, alpha, bias, what):
     n, m, k, group, kind, ws_need, counter_bytes, fn = plan
-    with _OnDevice(B):
-        if B.data_ptr() & 15:
-            B = B.clone()
-        C = torch.empty((n, m), dtype=B.dtype, device=B.device)
-        stream = _stream_of(B)
-        ws_ptr = ws_len = 0
-        if ws_need:
-            ws = _gemm_pool.get(B.device, stream, ws_need, counter_bytes)
-            ws_ptr, ws_len = ws.data_ptr(), ws.numel()
-        rc = fn(A.data_ptr(), A_Scale.data_ptr(), _ptr(A_Zero), B.data_ptr(), C.data_ptr(), n, m, k, group, kind, float(alpha), _ptr(bias), ws_ptr,
-                ws_len, stream)
-        if rc != 0:
-            _lib.check(rc, what)
+    b_ptr = B.data_ptr()
+    if b_ptr & 15:
+        B = B.clone()
+        b_ptr = B.data_ptr()
+    C = B.new_empty((n, m))
+    stream = _stream_of(B)
+    ws_ptr = ws_len = 0
+    if ws_need:
+        ws = _gemm_pool.get(B.device, stream, ws_need, counter_bytes)
+        ws_ptr, ws_len = ws.data_ptr(), ws.numel()
+    rc = fn(A.data_ptr(), A_Scale.data_ptr(), _ptr(A_Zero), b_ptr, C.data_ptr(), n, m, k, group, kind, float(alpha), _ptr(bias), ws_ptr, ws_len, stream)
+    if rc != 0:
+        _lib.check(rc, what)
     return C
 
 
@@ -999,19 +1007,32 @@ def expert_counts(experts_ids, n_experts, token_mask=None, out=None):
     """How many routed pairs each expert got: int32 [n_experts].  experts_ids int32 [T, K] (`fused_routing_gate`), ids outside 0..n_experts-1
     count nowhere; token_mask bool [T]: False for padded rows.  With `out` the counts are added to it, for a load that builds up over
     the steps of a server."""
-    _check_routing(experts_ids, token_mask, experts_ids.device)
-    _check(1 <= n_experts <= 256, "1..256 experts")
-    with _OnDevice(experts_ids):
-        add = out is not None
-        if add:
+    device = experts_ids.get_device()
+    key = ("counts", n_experts, experts_ids.shape, experts_ids.dtype, device,
+           None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.get_device()),
+           None if out is None else (out.shape, out.dtype, out.get_device()))
+    plan = _plans.get(key)
+    if plan is None or not (experts_ids.is_contiguous() and (token_mask is None or token_mask.is_contiguous()) and (out is None or out.is_contiguous())):
+        _check_routing(experts_ids, token_mask, experts_ids.device)
+        _check(1 <= n_experts <= 256, "1..256 experts")
+        if out is not None:
             _check(out.dtype == torch.int32 and tuple(out.shape) == (n_experts,), "out must be int32 [n_experts]")
             _check_tensors(((out, "out"),), experts_ids.device)
-        else:
-            out = torch.empty(n_experts, dtype=torch.int32, device=experts_ids.device)
-        rc = _lib.load().mlk_expert_counts(experts_ids.data_ptr(), _ptr(token_mask), experts_ids.size(0), experts_ids.size(1), n_experts, add,
-                                           out.data_ptr(), _stream_of(experts_ids))
-        if rc != 0:
-            _lib.check(rc, "expert_counts")
+        plan = _plans[key] = (experts_ids.size(0), experts_ids.size(1), _lib.load().mlk_expert_counts)
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _counts_launch(plan, experts_ids, n_experts, token_mask, out)
+    return _counts_launch(plan, experts_ids, n_experts, token_mask, out)
+
+
+def _counts_launch(plan, experts_ids, n_experts, token_mask, out):
+    n_tokens, topk, fn = plan
+    add = out is not None
+    if not add:
+        out = experts_ids.new_empty(n_experts)
+    rc = fn(experts_ids.data_ptr(), _ptr(token_mask), n_tokens, topk, n_experts, add, out.data_ptr(), _stream_of(experts_ids))
+    if rc != 0:
+        _lib.check(rc, "expert_counts")
     return out
 
 
@@ -1019,17 +1040,23 @@ _LOGIT_KIND = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 3}
 
 
 def _balance_forward(logits, ids, mask, cu, score_fun, coef, plan):
+    if logits.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return _balance_launch(logits, ids, mask, cu, score_fun, coef, plan)
+    return _balance_launch(logits, ids, mask, cu, score_fun, coef, plan)
+
+
+def _balance_launch(logits, ids, mask, cu, score_fun, coef, plan):
     T, E, K, kind, n_seq, ws_need, counter_bytes, fn, _ = plan
-    with _OnDevice(logits):
-        device, stream = logits.device, _stream_of(logits)
-        loss = torch.empty((), dtype=torch.float32, device=device)
-        counts = torch.empty(E, dtype=torch.int32, device=device)
-        share = torch.empty(n_seq * E, dtype=torch.float32, device=device)
-        ws = _balance_pool.get(device, stream, ws_need, counter_bytes)
-        rc = fn(logits.data_ptr(), kind, score_fun, T, E, K, ids.data_ptr(), _ptr(mask), _ptr(cu), n_seq, coef, loss.data_ptr(), counts.data_ptr(),
-                share.data_ptr(), ws.data_ptr(), ws.numel(), stream)
-        if rc != 0:
-            _lib.check(rc, "moe_balance_loss")
+    stream = _stream_of(logits)
+    loss = logits.new_empty((), dtype=torch.float32)
+    counts = ids.new_empty(E)
+    share = logits.new_empty(n_seq * E, dtype=torch.float32)
+    ws = _balance_pool.get(logits.device, stream, ws_need, counter_bytes)
+    rc = fn(logits.data_ptr(), kind, score_fun, T, E, K, ids.data_ptr(), _ptr(mask), _ptr(cu), n_seq, coef, loss.data_ptr(), counts.data_ptr(),
+            share.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    if rc != 0:
+        _lib.check(rc, "moe_balance_loss")
     return loss, counts, share
 
 
@@ -1070,9 +1097,9 @@ def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0,
     tokens; cu_seqlens int32 [sequences + 1] on the device, non-decreasing, where each sequence begins and the last one ends (None: all tokens are
     one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0."""
     logits = gating_output
-    key = ("balance", logits.shape, logits.dtype, logits.device, experts_ids.shape, experts_ids.dtype, experts_ids.device,
-           None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.device),
-           None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.dtype, cu_seqlens.device))
+    key = ("balance", logits.shape, logits.dtype, logits.get_device(), experts_ids.shape, experts_ids.dtype, experts_ids.get_device(),
+           None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.get_device()),
+           None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.dtype, cu_seqlens.get_device()))
     plan = _plans.get(key)
     if plan is None or not (logits.is_contiguous() and experts_ids.is_contiguous() and (token_mask is None or token_mask.is_contiguous()) and
                             (cu_seqlens is None or cu_seqlens.is_contiguous())):
