@@ -377,9 +377,10 @@ size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int
 /* ------------------------------------------------------------- router balance */
 
 /* counts[e] = (accumulate != 0: +=) number of routed pairs (t, k) with topk_ids[t, k] == e and token_mask[t] != 0 (NULL: every token); ids
- * outside 0..n_experts-1 count nowhere.  counts int32 [n_experts], n_experts <= 256. */
+ * outside 0..n_experts-1 count nowhere.  counts int32 [n_experts], n_experts <= 256.  workspace: mlk_balance_counter_bytes() bytes on 16, zero before the
+ * first call (left zero; the front of mlk_balance_loss's serves); may be NULL with accumulate and up to 4096 pairs. */
 int mlk_expert_counts(const int32_t *topk_ids, const uint8_t *token_mask, int n_tokens, int topk, int n_experts, int accumulate, int32_t *counts,
-                      void *stream);
+                      void *workspace, void *stream);
 
 /* Balance loss of a router, logits [T, E] of x_kind (MLK_F16, MLK_BF16 or MLK_F32):
  *   loss = coef * mean over the sequences with a valid token of E * sum over e of (c[e] / (K n)) * (P[e] / n)

@@ -23,7 +23,7 @@ namespace mlk {
 
 constexpr int kBalThreads = 256;
 constexpr int kBalExperts = 256;
-constexpr int kBalCounterBytes = 256;
+constexpr int kBalCounterBytes = 2048;      // in front: the loss's ticket, at 256 that of the counts, at 512 their totals
 constexpr int kBalMost = 1 << 30;    // tokens and routed pairs: a step past the last one still is an int
 constexpr int kBalManySeq = 64;      // sequences from which on a launch of its own counts their tokens
 
@@ -413,24 +413,42 @@ __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(BalanceArgs p
     }
 }
 
-// counts[e] += pairs routed to e (integer atomics: any order gives the same sums), or, in one workgroup and not to be added to, counts[e] = that.
+// How the sums of the workgroups get to counts: added to it (integer atomics: any order gives the same), stored by the only workgroup, or added to `total`, which is
+// zero between calls, until the last workgroup stores that and clears it (30000 tokens, 6 picks: with a launch that clears counts ahead 10.9 us a call, so 7.0).
+enum class CountsTo { kAdd, kStore, kTotal };
+template <CountsTo TO>
 __global__ void __launch_bounds__(256) expert_counts_kernel(const int32_t *__restrict__ ids, const uint8_t *__restrict__ mask, int64_t pairs, int K, int E,
-                                                            int32_t *__restrict__ counts, bool store) {
+                                                            int32_t *__restrict__ counts, int32_t *__restrict__ total, int32_t *__restrict__ ticket) {
     __shared__ int32_t cnt[kBalExperts];
-    for (int e = threadIdx.x; e < E; e += 256) cnt[e] = 0;
+    __shared__ int last;
+    const int tid = threadIdx.x;
+    for (int e = tid; e < E; e += 256) cnt[e] = 0;
     __syncthreads();
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pairs; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < pairs; i += (int64_t)gridDim.x * 256) {
         const int e = ids[i];
         if (e >= 0 && e < E && (!mask || mask[i / K])) atomicAdd(&cnt[e], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += 256) {
-        if (store) counts[e] = cnt[e];
-        else if (cnt[e]) atomicAdd(&counts[e], cnt[e]);
+    int32_t *to = TO == CountsTo::kTotal ? total : counts;
+    for (int e = tid; e < E; e += 256) {
+        if constexpr (TO == CountsTo::kStore) to[e] = cnt[e];
+        else if (cnt[e]) atomicAdd(&to[e], cnt[e]);
     }
-}
-__global__ void __launch_bounds__(256) expert_counts_zero_kernel(int32_t *counts, int E) {
-    if ((int)threadIdx.x < E) counts[threadIdx.x] = 0;
+    if constexpr (TO == CountsTo::kTotal) {
+        // every wave waits for its own additions before the barrier and the arrival is counted behind it
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (tid == 0) {
+            last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+            if (last) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last) return;
+        for (int e = tid; e < E; e += 256) {
+            counts[e] = __hip_atomic_load(&total[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&total[e], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
 }
 
 // -------------------------------------------------------------------------------------------------------------------- host
@@ -514,20 +532,24 @@ using namespace mlk;
 extern "C" {
 
 int mlk_expert_counts(const int32_t *topk_ids, const uint8_t *token_mask, int n_tokens, int topk, int n_experts, int accumulate, int32_t *counts,
-                      void *stream) {
+                      void *workspace, void *stream) {
     MLK_REQUIRE(n_tokens >= 0 && topk >= 1, "expert_counts: negative token count, or no picks");
     MLK_REQUIRE(n_experts >= 1 && n_experts <= kBalExperts, "expert_counts: 1..256 experts");
     MLK_REQUIRE(counts && (n_tokens == 0 || topk_ids), "expert_counts: null pointer");
     hipStream_t s = (hipStream_t)stream;
-    // one workgroup up to 4096 pairs: it needs no zeros to add to, and takes 3 us for them
+    // one workgroup up to 4096 pairs: it has no others to wait for, and takes 3 us for them
     const int64_t pairs = (int64_t)n_tokens * topk;
-    const int64_t wgs = pairs <= 4096 ? 1 : std::min<int64_t>((pairs + 1023) / 1024, 256);
-    if (!accumulate && wgs > 1) {
-        expert_counts_zero_kernel<<<1, 256, 0, s>>>(counts, n_experts);
-        MLK_LAUNCH_CHECK();
-    }
+    const int wgs = pairs <= 4096 ? 1 : (int)std::min<int64_t>((pairs + 1023) / 1024, 256);
     if (pairs == 0 && accumulate) return MLK_OK;
-    expert_counts_kernel<<<(int)wgs, 256, 0, s>>>(topk_ids, token_mask, pairs, topk, n_experts, counts, !accumulate && wgs == 1);
+    if (accumulate) {
+        expert_counts_kernel<CountsTo::kAdd><<<wgs, 256, 0, s>>>(topk_ids, token_mask, pairs, topk, n_experts, counts, nullptr, nullptr);
+    } else if (wgs == 1) {
+        expert_counts_kernel<CountsTo::kStore><<<1, 256, 0, s>>>(topk_ids, token_mask, pairs, topk, n_experts, counts, nullptr, nullptr);
+    } else {
+        MLK_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0, "expert_counts: more than 4096 pairs need a workspace, on 16 bytes");
+        int32_t *w = (int32_t *)workspace;
+        expert_counts_kernel<CountsTo::kTotal><<<wgs, 256, 0, s>>>(topk_ids, token_mask, pairs, topk, n_experts, counts, w + 128, w + 64);
+    }
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }

@@ -1018,7 +1018,9 @@ def expert_counts(experts_ids, n_experts, token_mask=None, out=None):
         if out is not None:
             _check(out.dtype == torch.int32 and tuple(out.shape) == (n_experts,), "out must be int32 [n_experts]")
             _check_tensors(((out, "out"),), experts_ids.device)
-        plan = _plans[key] = (experts_ids.size(0), experts_ids.size(1), _lib.load().mlk_expert_counts)
+        lib = _lib.load()
+        ws_need = lib.mlk_balance_counter_bytes() if out is None and experts_ids.numel() > 4096 else 0
+        plan = _plans[key] = (experts_ids.size(0), experts_ids.size(1), ws_need, lib.mlk_expert_counts)
     if device != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _counts_launch(plan, experts_ids, n_experts, token_mask, out)
@@ -1026,11 +1028,12 @@ def expert_counts(experts_ids, n_experts, token_mask=None, out=None):
 
 
 def _counts_launch(plan, experts_ids, n_experts, token_mask, out):
-    n_tokens, topk, fn = plan
-    add = out is not None
+    n_tokens, topk, ws_need, fn = plan
+    add, stream = out is not None, _stream_of(experts_ids)
     if not add:
         out = experts_ids.new_empty(n_experts)
-    rc = fn(experts_ids.data_ptr(), _ptr(token_mask), n_tokens, topk, n_experts, add, out.data_ptr(), _stream_of(experts_ids))
+    ws = _balance_pool.get(experts_ids.device, stream, ws_need, ws_need).data_ptr() if ws_need else 0
+    rc = fn(experts_ids.data_ptr(), _ptr(token_mask), n_tokens, topk, n_experts, add, out.data_ptr(), ws, stream)
     if rc != 0:
         _lib.check(rc, "expert_counts")
     return out

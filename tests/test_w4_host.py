@@ -191,7 +191,8 @@ def test_c_interface_of_the_balance_loss_refuses():
                      (dict(g=None), b"null"), (dict(d=None), b"null")):
         said(lib, grad(**kw), word)
     assert grad(t=0) == 0
-    for kw, word in ((dict(n_tokens=-1), b"negative"), (dict(topk=0), b"picks"), (dict(n_experts=300), b"256"), (dict(counts=None), b"null"), (dict(topk_ids=None), b"null")):
-        a = dict(topk_ids=FAKE, token_mask=None, n_tokens=4, topk=2, n_experts=8, accumulate=0, counts=FAKE, stream=None)
+    for kw, word in ((dict(n_tokens=-1), b"negative"), (dict(topk=0), b"picks"), (dict(n_experts=300), b"256"), (dict(counts=None), b"null"), (dict(topk_ids=None), b"null"),
+                     (dict(n_tokens=2049), b"workspace"), (dict(n_tokens=2049, workspace=FAKE + 8), b"16 bytes")):
+        a = dict(topk_ids=FAKE, token_mask=None, n_tokens=4, topk=2, n_experts=8, accumulate=0, counts=FAKE, workspace=None, stream=None)
         a.update(kw)
         said(lib, lib.mlk_expert_counts(*a.values()), word)
