@@ -27,7 +27,6 @@ struct W4MoeArgs {
     uint16_t *hbuf;              // [slot][I]
     float *obuf;                 // [pair][slice][H]
     int slices;                  // of the down projection's k
-    int wk1, wk2;                // streaming kernels: waves that share a row group's k; the 8 / wk sets of them take different row groups
     u32x4 *sums1, *sums2;        // panels: sums of x, of the intermediate (w4_sums_kernel)
 };
 
@@ -46,13 +45,12 @@ __device__ __forceinline__ W4Matrix w4_of_expert(const W4Matrix &m, int e, int r
 
 __host__ __device__ constexpr int w4_moe_ring(int r) { return r <= 2 ? 4 : 2; }
 
-// Rows of a gate/up wave: R / 2 row groups of gate, then the same of up; past the last one it again.
+// Rows of a gate/up workgroup: R / 2 row groups of gate, then the same of up.
 template <int GS, int R>
 __device__ __forceinline__ void w4_gate_up_rows(W4Rows<R> &rows, const W4MoeArgs &p, int e, int rg0) {
     const W4Matrix m = w4_of_expert<GS>(p.w1, e, 2 * p.I, p.H, p.blocks1);
-    const int groups = p.I >> 4;
 #pragma unroll
-    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, min(rg0 + r % (R / 2), groups - 1) + (r >= R / 2 ? groups : 0), p.H >> 7, p.blocks1);
+    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r % (R / 2) + (r >= R / 2 ? p.I >> 4 : 0), p.H >> 7, p.blocks1);
 }
 
 template <int CELLS>
@@ -68,7 +66,7 @@ __device__ __forceinline__ f32x4 w4_fold(const f32x4 *red, int c, int waves, int
 }
 
 // ---------------------------------------------------------------------------------------------------------- several tokens
-// Registers: 128 for two workgroups on a CU (without the bound 132 with zero points and 58.8 -> 60.1 us for 128 experts of 2048 x 768 at 50 tokens); groups of 32 with
+// Registers: 128 for four workgroups on a CU (128 experts of 2048 x 768 at 50 tokens, zero points: 58.8 us, without the bound 60.1 with 132); groups of 32 with
 // zero points would spill.
 template <int GS, bool ZP>
 __host__ __device__ constexpr int w4_moe_waves() { return GS == 1 && ZP ? 2 : 4; }
@@ -113,29 +111,30 @@ __device__ __forceinline__ bool w4_moe_block(const W4MoeArgs &p, int task, int l
     return false;
 }
 
-// One block of 16 tokens a task.  Eight waves: wk of them share the k of R row groups, tile by tile, and add their sums through LDS in wave order.  With all
-// eight on one set of row groups the 16 tiles of K = 2048 are two a wave, and a workgroup is mostly its start and end.
+// One block of 16 tokens a task.  Four waves share the k of R row groups, tile by tile, and add their sums through LDS in wave order.  Small workgroups even out
+// over the CUs: with eight waves 128 experts of 2048 x 768 at 50 tokens 87 us, with four 81; 64 of 2048 x 1408 at 4 tokens 35 and 31; 8 of 4096 x 14336 at 16 132
+// and 127; two sets of two waves, each on row groups of its own, are between.
+constexpr int kW4MoeWaves = 4;
+
 template <class T, int GS, bool ZP, int R, bool FEW>
-__global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_kernel(W4MoeArgs p) {
+__global__ void __launch_bounds__(kW4MoeWaves * 64, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     W4MoeBlock task;
     if (!w4_moe_block<FEW>(p, blockIdx.y, threadIdx.x & 63, task)) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = p.wk1;
-    const int o = lane >> 4, r16 = lane & 15, set = wave / wk, place = wave - set * wk, rg0 = (blockIdx.x * (8 / wk) + set) * (R / 2);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int o = lane >> 4, r16 = lane & 15, rg0 = blockIdx.x * (R / 2);
     W4Rows<R> rows;
     w4_gate_up_rows<GS, R>(rows, p, task.expert, rg0);
     const uint16_t *xrow[1] = {p.X + (size_t)(task.pair < p.n_pairs ? task.pair / p.K : 0) * p.H};
     f32x4 acc[R][1];
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-    w4_stream<T, GS, ZP, 1, R, w4_moe_ring(R), false>(acc, rows, xrow, nullptr, place, p.H >> 7, wk, p.inv, lane, false);
+    w4_stream<T, GS, ZP, 1, R, w4_moe_ring(R), false>(acc, rows, xrow, nullptr, wave, p.H >> 7, kW4MoeWaves, p.inv, lane, false);
     constexpr int HALF = R / 2;
     w4_park<R>(red, reinterpret_cast<const f32x4(&)[R]>(acc), wave, lane);
     __syncthreads();
-    const f32x4 *mine = red + (size_t)set * wk * R * 64;
-    for (int c = place; c < HALF; c += wk) {
-        if (rg0 + c >= p.I >> 4) continue;
-        const f32x4 g = w4_fold<R>(mine, c, wk, lane), u = w4_fold<R>(mine, HALF + c, wk, lane);
+    for (int c = wave; c < HALF; c += kW4MoeWaves) {
+        const f32x4 g = w4_fold<R>(red, c, kW4MoeWaves, lane), u = w4_fold<R>(red, HALF + c, kW4MoeWaves, lane);
         uint16_t *h = p.hbuf + (size_t)(task.slot0 + o * 4) * p.I + (rg0 + c) * 16 + r16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[(size_t)i * p.I] = (uint16_t)T::from_f32(silu_mul(g[i], u[i]));
@@ -143,29 +142,27 @@ __global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_gate_up_
 }
 
 template <class T, int GS, bool ZP, int R, bool FEW>
-__global__ void __launch_bounds__(512, (w4_moe_waves<GS, ZP>())) w4_moe_down_kernel(W4MoeArgs p) {
+__global__ void __launch_bounds__(kW4MoeWaves * 64, (w4_moe_waves<GS, ZP>())) w4_moe_down_kernel(W4MoeArgs p) {
     extern __shared__ f32x4 red[];
     W4MoeBlock task;
     if (!w4_moe_block<FEW>(p, blockIdx.y, threadIdx.x & 63, task)) return;
     __shared__ int pairs[16];
     if (threadIdx.x < 16) pairs[threadIdx.x] = task.pair;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = p.wk2;
-    const int o = lane >> 4, r16 = lane & 15, set = wave / wk, place = wave - set * wk, rg0 = (blockIdx.x * (8 / wk) + set) * R, groups = p.H >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int o = lane >> 4, r16 = lane & 15, rg0 = blockIdx.x * R;
     const W4Matrix m = w4_of_expert<GS>(p.w2, task.expert, p.H, p.I, p.blocks2);
     W4Rows<R> rows;
 #pragma unroll
-    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, min(rg0 + r, groups - 1), p.I >> 7, p.blocks2);
+    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r, p.I >> 7, p.blocks2);
     const uint16_t *xrow[1] = {p.hbuf + (size_t)(task.slot0 + r16) * p.I};
     f32x4 acc[R][1];
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-    w4_stream<T, GS, ZP, 1, R, w4_moe_ring(R), false>(acc, rows, xrow, nullptr, place, p.I >> 7, wk, p.inv, lane, false);
+    w4_stream<T, GS, ZP, 1, R, w4_moe_ring(R), false>(acc, rows, xrow, nullptr, wave, p.I >> 7, kW4MoeWaves, p.inv, lane, false);
     w4_park<R>(red, reinterpret_cast<const f32x4(&)[R]>(acc), wave, lane);
     __syncthreads();
-    const f32x4 *mine = red + (size_t)set * wk * R * 64;
-    for (int c = place; c < R; c += wk) {
-        if (rg0 + c >= groups) continue;
-        const f32x4 v = w4_fold<R>(mine, c, wk, lane);
+    for (int c = wave; c < R; c += kW4MoeWaves) {
+        const f32x4 v = w4_fold<R>(red, c, kW4MoeWaves, lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int pair = pairs[o * 4 + i];
@@ -289,7 +286,6 @@ static int w4_moe_lds(K kernel, size_t lds, bool (&ready_on)[64]) {
 struct W4MoePlan {
     int tt;                  // blocks of 16 tokens per task; 0: one token
     int max_tasks;
-    int wk1, wk2;
     bool few;                // at most 64 pairs, no alignment
     bool panels;             // tasks of up to 8 blocks run panels
     int slices;              // of their down projection
@@ -306,14 +302,12 @@ struct W4MoePlan {
 
 template <class T, int GS, bool ZP, int R, bool FEW>
 static int w4_moe_gate_up(const W4MoeArgs &a, int max_tasks, hipStream_t s) {
-    const int each = 8 / a.wk1 * (R / 2);
-    MLK_W4_MOE(w4_moe_gate_up_kernel, dim3((a.I / 16 + each - 1) / each, max_tasks), 8, (size_t)8 * R * 1024, T, GS, ZP, R, FEW);
+    MLK_W4_MOE(w4_moe_gate_up_kernel, dim3(a.I / 8 / R, max_tasks), kW4MoeWaves, (size_t)kW4MoeWaves * R * 1024, T, GS, ZP, R, FEW);
     return MLK_OK;
 }
 template <class T, int GS, bool ZP, int R, bool FEW>
 static int w4_moe_down(const W4MoeArgs &a, int max_tasks, hipStream_t s) {
-    const int each = 8 / a.wk2 * R;
-    MLK_W4_MOE(w4_moe_down_kernel, dim3((a.H / 16 + each - 1) / each, max_tasks), 8, (size_t)8 * R * 1024, T, GS, ZP, R, FEW);
+    MLK_W4_MOE(w4_moe_down_kernel, dim3(a.H / 16 / R, max_tasks), kW4MoeWaves, (size_t)kW4MoeWaves * R * 1024, T, GS, ZP, R, FEW);
     return MLK_OK;
 }
 template <class T, int GS, bool ZP, int R>
@@ -339,7 +333,7 @@ int w4_launch_moe(const W4MoeArgs &a, const W4MoePlan &pl, hipStream_t s) {
         rc = w4_moe1_gate_up<T, GS, ZP, 2>(a, s);
         return rc == MLK_OK ? w4_moe1_down<T, GS, ZP, 1>(a, s) : rc;
     }
-    // four row groups a wave: 128 registers, two workgroups on a CU (8 experts at 16 tokens: 120 us, with eight 139, with two 129)
+    // four row groups a wave: 128 registers (8 experts at 16 tokens: 120 us, with eight 139, with two 129)
     rc = pl.few ? w4_moe_gate_up<T, GS, ZP, 4, true>(a, pl.max_tasks, s) : w4_moe_gate_up<T, GS, ZP, 4, false>(a, pl.max_tasks, s);
     if (rc == MLK_OK) rc = pl.few ? w4_moe_down<T, GS, ZP, 4, true>(a, pl.max_tasks, s) : w4_moe_down<T, GS, ZP, 4, false>(a, pl.max_tasks, s);
     if (rc != MLK_OK) return rc;

@@ -44,10 +44,6 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
     const int64_t most = (int64_t)E + pairs / (16 * pl.tt);
     pl.max_tasks = (int)(most < pairs ? most : pairs);
     if (!pl.panels) {
-        // Waves that share a row group's k: with few tiles of 128 in all, two (gate/up of 128 experts of 2048 x 768 at 100 tokens 122 us with eight, 112 with two;
-        // 64 of 2048 x 1408, down at 32 tokens 73.5 and 70.4); with many, eight (8 of 4096 x 14336 at 16 tokens 119.5, with two 123 each).
-        pl.wk1 = hidden / 128 >= 24 ? 8 : 2;
-        pl.wk2 = inter / 128 >= 24 ? 8 : 2;
         pl.few = pairs <= 64;
         return pl;
     }
@@ -162,8 +158,6 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
         a.hbuf = ws.hbuf;
         a.obuf = ws.obuf;
         a.slices = pl.slices;
-        a.wk1 = pl.wk1;
-        a.wk2 = pl.wk2;
         a.sums1 = ws.sums1;
         a.sums2 = ws.sums2;
         int rc = MLK_OK;
