@@ -34,11 +34,12 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
         pl.max_tasks = topk;
         return pl;
     }
-    // Routed pairs of an expert that is reached.  Up to 20 on average the streaming kernels, one block of 16 tokens a task; above, panels: 8 experts of
-    // 4096 x 14336, top-2, at 48 tokens (12) 189 us against 237 with panels, at 80 (20) 262 against 238, at 130 (32) 336 against 234; 128 experts of 2048 x 768,
-    // top-8, at 200 (12) 137 against 189, at 300 (18) 172 against 196, at 400 (25) 207 against 209.
+    // Routed pairs of an expert that is reached.  Up to 30 on average the streaming kernels, one block of 16 tokens a task, and above panels: 128 experts of
+    // 2048 x 768, top-8, at 400 tokens (25) 163 us against 208 with panels, at 500 (31) 189 and 209, at 800 (50) 259 and 266; 64 of 2048 x 1408, top-6, at 300 (28) 145
+    // and 147, at 400 (37) 175 and 160; 16 of 4096 x 2048, top-4, at 120 (30) 119 and 125, at 160 (40) 143 and 130.  Larger experts, which the second task of one
+    // finds in no cache, to 22: 8 of 4096 x 14336, top-2, at 64 tokens (16) 207 and 232, at 80 (20) 246 and 244, at 130 (32) 377 and 246.
     const int reached = pairs < E ? pairs : E, load = (pairs + reached - 1) / reached;
-    pl.panels = load > 20 && (int64_t)tokens * hidden < (1ll << 31);
+    pl.panels = load > ((int64_t)hidden * inter <= (1 << 24) ? 30 : 22) && (int64_t)tokens * hidden < (1ll << 31);
     pl.tt = pl.panels ? 8 : 1;
     // an expert's last task may be short: at most one more than its blocks fill
     const int64_t most = (int64_t)E + pairs / (16 * pl.tt);
