@@ -131,8 +131,8 @@ def workspace_bytes_held():
 
 
 def release_workspaces(retired_only=False):
-    """Give the scratch memory of the K-split GeMMs and of the fused MoE back to torch's allocator and return the
-    number of bytes released.  The pools keep one buffer per (device, stream) and never free by themselves, so that
+    """Give the scratch memory of the K-split GeMMs, of the fused MoE and of the balance loss back to torch's allocator and
+    return the number of bytes released.  The pools keep one buffer per (device, stream) and never free by themselves, so that
     a HIP graph captured around a call replays with valid pointers; a caller that holds no such graph (or has
     dropped it) calls this after a burst of large batches, or when streams it used are gone.  `retired_only`
     releases just the buffers that a larger one has replaced.  Synchronize the device first."""

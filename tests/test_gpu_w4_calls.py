@@ -345,3 +345,30 @@ def test_few_pairs_and_one_more(mlk, T, E, K, same):
     check_experts(got, expected_experts(x, w1, w2, p1[1], p2[1], ids, wts), BF, "experts")
     gone = torch.full_like(ids, E)
     assert (mlk.fused_experts_w4(x.cuda(), a1, a2, gone.cuda(), wts.cuda(), s1, s2, z1, z2) == 0).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 100])
+def test_subnormal_activations_count(mlk, tokens):
+    """fp16 activations below 2^-14 all of them: the results are some hundred times the least number, and off by its half at most."""
+    n, k, group = 272, 1024, 128
+    codes, s, z, _ = w4_weights(n, k, group, HF, True, 5)
+    s = torch.ones_like(s)
+    q = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).double()
+    w = q - z.double().repeat_interleave(group, dim=1)
+    x = (randn((tokens, k), torch.float32, 1.0, 3) * 1e-6).to(HF)
+    assert (x.abs() < 2.0 ** -14).all() and (x != 0).any()
+    A, S, Z = mlk.pack_layout_a_w4(*on_gpu(codes, s, z))
+    assert_within(mlk.gemm_layoutA_w4(A, S, x.cuda(), Z), x.double() @ w.t(), term_size(x, s, group), HF, k, "product")
+
+
+def test_one_workspace_for_counts_and_losses(mlk):
+    """Counts of a long prompt and balance losses in turn on one stream, of different sizes: what one leaves is what the other expects."""
+    g = torch.Generator().manual_seed(4)
+    for T, E in ((3000, 64), (9000, 256), (1500, 8), (20000, 100)):
+        ids = torch.randint(-1, E + 1, (T, 6), generator=g, dtype=torch.int32)
+        kept = ids[(ids >= 0) & (ids < E)].long()
+        want = torch.bincount(kept, minlength=E).int()
+        logits = torch.randn((T, E), generator=g).cuda()
+        for _ in range(3):
+            assert torch.equal(mlk.expert_counts(ids.cuda(), E).cpu(), want)
+            assert torch.equal(mlk.moe_balance_loss(logits, ids.cuda())[1].cpu(), want)
