@@ -1,9 +1,10 @@
-// Streaming kernel of the 4-bit linear layers: up to 64 tokens, bound by the weights' bytes.
+// Streaming kernel of the 4-bit linear layers, for few tokens or little weight: bound by the weights' bytes, with more tokens by what the workgroups read of
+// the activations.
 //
 // A workgroup owns up to R consecutive row groups (of 16 rows); its waves deal the tiles of 128 k among themselves (tile t to wave t mod waves, so
 // that together they read each row group front to back) and add their sums through LDS in wave order.  The row groups are dealt out evenly over the
 // grid; `slices` workgroups may share a set of row groups, each on its own range of k: the last one to arrive adds their fp32 sums in the
-// order of k.
+// order of k.  Workgroups take up to 64 tokens (blockIdx.z).
 #pragma once
 
 #include "mlk_w4.cuh"
@@ -23,7 +24,7 @@ struct W4GemmArgs {
     int rg_each, rg_more;  // row groups of a workgroup; the first rg_more workgroups have one more
     int t_each, t_more;    // tiles of a slice, likewise
     f32x4 *partial;        // [workgroup][slice][cell][two planes of 64 x 8 bytes]
-    int *counters;         // [workgroup], zero between calls
+    int *counters;         // [workgroup (x, z)], zero between calls
 };
 
 constexpr int kW4TokenLds = 128 * 1024;      // bytes of LDS that one token may take
@@ -51,9 +52,10 @@ __global__ void __launch_bounds__(w4_stream_waves(TT, R, XL) * 64) w4_stream_ker
     W4Rows<R> rows;
 #pragma unroll
     for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, p.A, rg0 + min(r, nr - 1), tiles, p.blocks);
+    const int m0 = blockIdx.z * (TT * 16);
     const uint16_t *xrow[TT];
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) xrow[tt] = p.X + (size_t)min(tt * 16 + r16, p.M - 1) * p.K;
+    for (int tt = 0; tt < TT; ++tt) xrow[tt] = p.X + (size_t)min(m0 + tt * 16 + r16, p.M - 1) * p.K;
     f32x4 acc[R][TT];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -70,11 +72,12 @@ __global__ void __launch_bounds__(w4_stream_waves(TT, R, XL) * 64) w4_stream_ker
         const float b = p.bias ? T::to_f32(p.bias[row]) : 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int token = tt * 16 + o * 4 + i;
+            const int token = m0 + tt * 16 + o * 4 + i;
             if (token < p.M) p.C[(size_t)token * p.N + row] = (uint16_t)T::from_f32(p.alpha * v[i] + b);
         }
     };
-    auto part = [&](int s, int c) { return p.partial + (((size_t)blockIdx.x * p.slices + s) * CELLS + c) * 64; };
+    const int set = blockIdx.z * gridDim.x + blockIdx.x;
+    auto part = [&](int s, int c) { return p.partial + (((size_t)set * p.slices + s) * CELLS + c) * 64; };
     f32x4 *red = reinterpret_cast<f32x4 *>(lds);
     constexpr int FOLD = w4_fold_cells(CELLS);
 #pragma unroll
@@ -95,9 +98,9 @@ __global__ void __launch_bounds__(w4_stream_waves(TT, R, XL) * 64) w4_stream_ker
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0) {
-        const int before = __hip_atomic_fetch_add(&p.counters[blockIdx.x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int before = __hip_atomic_fetch_add(&p.counters[set], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         s_last = before == p.slices - 1;
-        if (s_last) __hip_atomic_store(&p.counters[blockIdx.x], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (s_last) __hip_atomic_store(&p.counters[set], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (!s_last) return;
@@ -126,15 +129,15 @@ static int w4_launch_stream_one(W4GemmArgs a, int wgs, int waves, hipStream_t s)
             ready_on[dev & 63] = true;
         }
     }
-    w4_stream_kernel<T, GS, ZP, TT, R, XL><<<dim3(wgs, a.slices), waves * 64, lds, s>>>(a);
+    w4_stream_kernel<T, GS, ZP, TT, R, XL><<<dim3(wgs, a.slices, XL ? 1 : (a.M + TT * 16 - 1) / (TT * 16)), waves * 64, lds, s>>>(a);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }
 
-// r = row groups per workgroup the kernel is built for: 1, 2 or 4, from five tokens to 48 also 8; wgs * r >= N / 16.  One token is staged in LDS (r = 1, 2; a slice of 64 K at most): 4096 x 4096
+// r = row groups per workgroup the kernel is built for: 1, 2 or 4, with tt up to 3 also 8; tt = blocks of 16 tokens per workgroup; wgs * r >= N / 16.  One token is staged in LDS (r = 1, 2; a slice of 64 K at most): 4096 x 4096
 // 4.7 us against 5.1.
 template <class T, int GS, bool ZP>
-int w4_launch_stream(const W4GemmArgs &a, int r, int wgs, int waves, hipStream_t s) {
+int w4_launch_stream(const W4GemmArgs &a, int r, int tt, int wgs, int waves, hipStream_t s) {
     if ((int64_t)r * wgs < a.N / 16 || wgs > a.N / 16) return fail(MLK_ERR_INVALID, "w4 gemm: launch parameters");
 #define MLK_W4_R(TT, XL)                                                                  \
     do {                                                                                  \
@@ -147,11 +150,11 @@ int w4_launch_stream(const W4GemmArgs &a, int r, int wgs, int waves, hipStream_t
         if (r == 1) return w4_launch_stream_one<T, GS, ZP, 1, 1, true>(a, wgs, waves, s);
         if (r == 2) return w4_launch_stream_one<T, GS, ZP, 1, 2, true>(a, wgs, waves, s);
     }
-    if (a.M <= 16) {
+    if (tt == 1) {
         MLK_W4_R(1, false);
-    } else if (a.M <= 32) {
+    } else if (tt == 2) {
         MLK_W4_R(2, false);
-    } else if (a.M <= 48) {
+    } else if (tt == 3) {
         MLK_W4_R(3, false);
     } else {
         MLK_W4_R(4, false);

@@ -6,8 +6,8 @@
 namespace mlk {
 
 #define MLK_W4_EXTERN(T, GS)                                                                          \
-    extern template int w4_launch_stream<T, GS, false>(const W4GemmArgs &, int, int, int, hipStream_t); \
-    extern template int w4_launch_stream<T, GS, true>(const W4GemmArgs &, int, int, int, hipStream_t);  \
+    extern template int w4_launch_stream<T, GS, false>(const W4GemmArgs &, int, int, int, int, hipStream_t); \
+    extern template int w4_launch_stream<T, GS, true>(const W4GemmArgs &, int, int, int, int, hipStream_t);  \
     extern template int w4_launch_panel<T, GS, false>(const W4PanelArgs &, int, hipStream_t);           \
     extern template int w4_launch_panel<T, GS, true>(const W4PanelArgs &, int, hipStream_t);
 MLK_W4_EXTERN(F16, 4)
@@ -21,19 +21,19 @@ MLK_W4_EXTERN(BF16, 1)
 constexpr size_t kW4CounterBytes = 64 * 1024;      // the front of the workspace that the GeMMs share
 
 struct W4Plan {
-    int r, wgs, waves;      // streaming kernels
+    int r, tt, wgs, waves;  // streaming kernels: row groups and blocks of 16 tokens of a workgroup
     int tb;                 // panels: blocks of 32 tokens; 0: streaming kernels
     int slices;             // of K
 };
 
-// Up to 64 tokens.  Microseconds on weights from memory, groups of 128, bf16 (r row groups a workgroup, s slices of K):
+// Up to 32 tokens.  Microseconds on weights from memory, groups of 128, bf16 (r row groups a workgroup, s slices of K):
 //   one to four tokens   one workgroup per CU as far as r <= 4 goes, K whole: 4096 x 4096 r = 1 4.7 (s = 2: 6.3), 4096 x 14336 r = 1 9.8, r = 2 s = 2 10.7; 28672 x 8192 one
 //                        token r = 2 25.7, r = 4 27.5, two tokens r = 4 24.9, r = 2 31.6
 //   more                 the activations weigh more (every workgroup reads all of them): r = 8 where that many row groups each, in slices of 48 tiles at least, leave
-//                        three quarters of the CUs a workgroup (up to 48 tokens: its sums fit the registers): 28672 x 8192 at 32 tokens r = 4 45.7, r = 8 32.6,
-//                        at 16 31.2 and 28.8; 27648 x 5120 at 48 39.0 and 29.1; 28672 x 4096 at 16 16.6 and 17.3; not 13824 x 5120 at 32, r = 4 18.8, r = 8 s = 2 19.1.
+//                        three quarters of the CUs a workgroup: 28672 x 8192 at 32 tokens r = 4 45.7, r = 8 32.6,
+//                        at 16 31.2 and 28.8; 27648 x 5120 at 32 30.0 and 22.8; 28672 x 4096 at 16 16.6 and 17.3; not 13824 x 5120 at 32, r = 4 18.8, r = 8 s = 2 19.1.
 //                        Else r = 4, and slices bring the workgroups back: 4096 x 14336 at 16 tokens r = 1
-//                        16.7, r = 2 s = 2 13.6, r = 4 s = 4 11.6, at 64 53, 31 and 23; 512 x 7168 at 64 tokens r = 1 27.6, s = 8 8.9.  At least six tiles a slice
+//                        16.7, r = 2 s = 2 13.6, r = 4 s = 4 11.6.  At least six tiles a slice
 //                        (1280 x 5120 at 16 tokens r = 2 s = 4 6.3, s = 8 9).  More workgroups than CUs have four waves (57344 x 2048 at 32 tokens r = 8 25.0, with four
 //                        22.2; fewer eight: 28672 x 8192 32.9, with four 37.8)
 static W4Plan w4_plan_stream(int m, int n, int k) {
@@ -41,6 +41,7 @@ static W4Plan w4_plan_stream(int m, int n, int k) {
     W4Plan pl = {};
     pl.tb = 0;
     pl.slices = pl.r = 1;
+    pl.tt = (m + 15) / 16;
     if (m <= 4) {
         while (pl.r < 4 && groups > pl.r * cus) pl.r *= 2;
         if (m == 1 && pl.r == 4 && groups > 4 * cus) pl.r = 2;
@@ -50,7 +51,7 @@ static W4Plan w4_plan_stream(int m, int n, int k) {
     }
     auto slices_of = [&](int wgs, int most) { return std::max(1, std::min(cus / wgs, most)); };
     const int wide = (groups + 7) / 8;
-    if (m <= 48 && 4 * wide * slices_of(wide, tiles / 48) >= 3 * cus) {
+    if (4 * wide * slices_of(wide, tiles / 48) >= 3 * cus) {
         pl.r = 8;
         pl.slices = slices_of(wide, tiles / 48);
     } else {
@@ -74,25 +75,47 @@ static double w4_panel_cost(int m, int n, int k, int group, int tb, int slices, 
     const double window = (tb == 2 ? 0.82 + 0.2 * full : 1.18 + 0.5 * full) * (g == 1 ? 1.0 : (g == 2 ? 1.15 : 1.45));
     return rounds * (windows + (windows * g + 15) / 16 + 3) * window + 6 + (slices > 1 ? 2 + (double)slices * m * n * 8 / 5e6 : 0);
 }
-// And of the streaming kernels from 33 to 64 tokens: the weights' bytes, and the activations' for every block of 16 tokens and the row groups that share them.
-static double w4_stream_cost(int m, int n, int k, int r) { return 4 + (double)n * k / 2e6 * (0.085 + (r == 8 ? 0.082 : 0.134) * ((m + 15) / 16)); }
+// And of the streaming kernels with tt blocks of 16 tokens and r row groups a workgroup: a tile of 128 k takes 0.05 us and 0.027 for every block and row group (r = 8
+// 0.0235), or what the workgroups on the chip read of the activations for it at 9.2 TB/s, which L2 gives, or what one reads at 48 GB/s; a round of workgroups 1.4,
+// slices 2.5 (r = 8 3.5) and their bytes.
+// 256 workgroups each: 4096 x 4096 at 100 tokens tt = 2 r = 4 12.8 us, at 160 tt = 3 16.2, at 256 tt = 4 20.8; 1280 x 5120 at 100 tt = 3 r = 1 16.6, tt = 3 r = 4 in four slices 10.8.
+static double w4_stream_cost(int m, int n, int k, int group, int tt, int r, int slices, int cus) {
+    const int64_t wgs = ((int64_t)n / 16 + r - 1) / r * (((int64_t)m + 16 * tt - 1) / (16 * tt)) * slices, rounds = (wgs + cus - 1) / cus;
+    const double work = (r == 8 ? 0.06 + 0.0235 * tt * r : 0.05 + 0.0268 * tt * r) * (group == 32 ? 1.2 : (group == 64 ? 1.05 : 1.0));
+    const double tile = std::max({work, 4096.0 * tt * std::min<int64_t>(wgs, cus) / 9.2e6, (4096.0 * tt + 1024.0 * r) / 48e3});
+    return 2.6 + rounds * (1.4 + (k / 128 + slices - 1) / slices * tile) + (slices > 1 ? (r == 8 ? 3.5 : 2.5) + (double)slices * n * ((m + 15) / 16 * 16) * 8 / 5e6 : 0);
+}
 
+// Above 32 tokens the cheaper of panels and streaming kernels by those costs (512 x 7168 at 100 tokens panels 17.9, streaming 8.7; 1024 x 1024 at 256 14.8 and 5.1;
+// 4096 x 4096 at 160 23.8 and 16.2, at 500 32.0 and 39.8; 11008 x 4096 at 100 26.9 and 34.4).
 static W4Plan w4_plan(int m, int n, int k, int group) {
-    const W4Plan stream = w4_plan_stream(m < 64 ? m : 64, n, k);
-    if (m <= 32) return stream;
+    if (m <= 32) return w4_plan_stream(m, n, k);
+    const int cus = device_cus(), groups = n / 16, tiles = k / 128;
     W4Plan best = {};
-    double least = m <= 64 ? w4_stream_cost(m, n, k, stream.r) : 1e30;
-    if (m <= 64) best = stream;
-    const int cus = device_cus();
-    for (int tb = 2; tb <= 4; tb += 2)
-        for (int slices = 1; slices <= 16 && slices * 2 <= k / 128; ++slices) {
-            const double c = w4_panel_cost(m, n, k, group, tb, slices, cus);
-            if (c < least) {
-                least = c;
-                best = W4Plan{0, 0, 0, tb, slices};
+    double least = 1e300;
+    auto panels = [&](int tb, int slices) {
+        const double c = w4_panel_cost(m, n, k, group, tb, slices, cus);
+        if (c < least) {
+            least = c;
+            best = W4Plan{0, 0, 0, 0, tb, slices};
+        }
+    };
+    for (int tb = 2; tb <= 4; tb += 2) {
+        panels(tb, 1);
+        for (int slices = 2; slices <= 16 && slices * 2 <= tiles; ++slices) panels(tb, slices);
+    }
+    for (int tt = 2; tt <= 4; ++tt)
+        for (int r = 1; r <= (tt < 4 ? 8 : 4); r *= 2) {
+            const int64_t blocks = ((int64_t)m + 16 * tt - 1) / (16 * tt), wgs = (groups + r - 1) / r;
+            for (int slices = 1; slices == 1 || (slices <= 8 && slices * 6 <= tiles && wgs * blocks * slices <= 2 * cus); ++slices) {
+                const double c = w4_stream_cost(m, n, k, group, tt, r, slices, cus);
+                if (c < least && blocks <= 65535) {
+                    least = c;
+                    best = W4Plan{r, tt, (int)wgs, wgs * blocks * slices > cus ? 4 : 8, 0, slices};
+                }
             }
         }
-    return best.r || best.tb ? best : W4Plan{0, 0, 0, 2, 1};
+    return best;
 }
 static size_t w4_sums_bytes(int m, int k, int group) {
     return ((size_t)m * w4_sum_pitch(k, group < 128 ? group / 32 : 4) * 16 + 255) / 256 * 256;
@@ -100,12 +123,12 @@ static size_t w4_sums_bytes(int m, int k, int group) {
 static size_t w4_partial_bytes(const W4Plan &pl, int m, int n, int k, int group) {
     if (pl.tb) return w4_sums_bytes(m, k, group) + (pl.slices > 1 ? (size_t)pl.slices * m * n * 4 : 0);
     if (pl.slices <= 1) return 0;
-    return (size_t)pl.slices * pl.wgs * pl.r * ((m + 15) / 16) * 1024;
+    return (size_t)pl.slices * pl.wgs * pl.r * ((m + 16 * pl.tt - 1) / (16 * pl.tt) * pl.tt) * 1024;
 }
 
 template <class T, int GS>
 static int w4_stream_of(const W4GemmArgs &a, const W4Plan &pl, hipStream_t s) {
-    return a.A.zeros ? w4_launch_stream<T, GS, true>(a, pl.r, pl.wgs, pl.waves, s) : w4_launch_stream<T, GS, false>(a, pl.r, pl.wgs, pl.waves, s);
+    return a.A.zeros ? w4_launch_stream<T, GS, true>(a, pl.r, pl.tt, pl.wgs, pl.waves, s) : w4_launch_stream<T, GS, false>(a, pl.r, pl.tt, pl.wgs, pl.waves, s);
 }
 
 static int w4_stream(const W4GemmArgs &a, const W4Plan &pl, int x_kind, int group, hipStream_t s) {

@@ -2,5 +2,5 @@
 #include "mlk_w4_gemm.cuh"
 
 namespace mlk {
-template int w4_launch_stream<BF16, 2, false>(const W4GemmArgs &, int, int, int, hipStream_t);
+template int w4_launch_stream<BF16, 2, false>(const W4GemmArgs &, int, int, int, int, hipStream_t);
 }  // namespace mlk

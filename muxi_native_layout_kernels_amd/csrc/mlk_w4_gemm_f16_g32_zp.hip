@@ -2,5 +2,5 @@
 #include "mlk_w4_gemm.cuh"
 
 namespace mlk {
-template int w4_launch_stream<F16, 1, true>(const W4GemmArgs &, int, int, int, hipStream_t);
+template int w4_launch_stream<F16, 1, true>(const W4GemmArgs &, int, int, int, int, hipStream_t);
 }  // namespace mlk
