@@ -1,4 +1,4 @@
-// Panels of the 4-bit products for more tokens than the streaming kernels take: 256 weight rows x 32 TB tokens a workgroup, eight waves of two row
+// Panels of the 4-bit products for many tokens: 256 weight rows x 32 TB tokens a workgroup, eight waves of two row
 // groups (32 rows) each, all on the same tokens.
 //
 // What a panel costs, in cycles of a CU and a window of 128 k (TB = 4; two waves on each SIMD):

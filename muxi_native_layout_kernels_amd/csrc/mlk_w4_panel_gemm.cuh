@@ -1,4 +1,4 @@
-// The 4-bit linear layers above 64 tokens: panels (mlk_w4_panel.cuh), whole or in K slices that a second launch adds.
+// The 4-bit linear layers with many tokens: panels (mlk_w4_panel.cuh), whole or in K slices that a second launch adds.
 #pragma once
 
 #include "mlk_w4_gemm.cuh"

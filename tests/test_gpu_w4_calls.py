@@ -307,28 +307,67 @@ def test_a_refused_layer_counts_nothing(mlk):
     assert load.sum() == 6
 
 
-@pytest.mark.parametrize("n,k,group,zeros,dtype", [(24592, 384, 128, False, BF), (24592, 256, 32, True, HF), (57360, 128, 64, True, BF), (8192, 18432, 128, True, HF),
-                                                   (4112, 36864, 32, False, BF)])
-@pytest.mark.parametrize("tokens", [5, 16, 20, 33, 48, 49])
-def test_eight_row_groups_a_workgroup(mlk, tokens, n, k, group, zeros, dtype):
-    """Tall and long weights: any bytes are valid codes, some of the rows are unpacked for the reference."""
-    g = torch.Generator(device="cuda").manual_seed(n + tokens)
-    per = max(1, 128 // group)
-    shape = (n // 16, k // max(128, group), 16, per)
+def packed_at_random(n, k, group, zeros, dtype, seed):
+    """Weights in the layout on the GPU: any bytes are valid codes."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    shape = (n // 16, k // max(128, group), 16, max(1, 128 // group))
     A = torch.randint(0, 256, (n // 16, k // 128, 64, 16), dtype=torch.uint8, device="cuda", generator=g)
     S = ((torch.rand(shape, device="cuda", generator=g) + 0.5) * (k ** -0.5 / 4.6)).to(dtype)
     Z = torch.randint(0, 16, shape, dtype=torch.uint8, device="cuda", generator=g) if zeros else None
-    x, bias = randn((tokens, k), dtype, 1.0, 3), randn((1, n), dtype, 1.0, 4)
-    got = mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, bias=bias.cuda())
-    assert torch.equal(got, mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, bias=bias.cuda()))
-    for first in (0, n // 32 - 3, n // 16 - 9):                      # nine row groups from here
-        rows = slice(first, first + 9)
+    return A, S, Z
+
+
+def check_some_rows(mlk, A, S, Z, group, x, bias, got):
+    """Nine row groups at the start, in the middle and at the end against 64 bits."""
+    k, groups = x.shape[1], A.shape[0]
+    for first in (0, groups // 2 - 3, groups - 9):
+        rows, cols = slice(first, first + 9), slice(first * 16, (first + 9) * 16)
         codes, s, z = mlk.unpack_layout_a_w4(A[rows].contiguous(), S[rows].contiguous(), None if Z is None else Z[rows].contiguous())
         q = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).cpu().double()
         off = torch.full(s.shape, 8.0, dtype=torch.float64) if z is None else z.cpu().double()
         w = (q - off.repeat_interleave(group, dim=1)) * s.cpu().double().repeat_interleave(group, dim=1)
-        cols = slice(first * 16, (first + 9) * 16)
-        assert_within(got[:, cols], x.double() @ w.t() + bias[:, cols].double(), term_size(x, s.cpu(), group) + bias[:, cols].double().abs(), dtype, k, "rows %d" % first)
+        b = bias[:, cols].double()
+        assert_within(got[:, cols], x.double() @ w.t() + b, term_size(x, s.cpu(), group) + b.abs(), x.dtype, k, "rows %d" % first)
+
+
+@pytest.mark.parametrize("n,k,group,zeros,dtype", [(24592, 384, 128, False, BF), (24592, 256, 32, True, HF), (57360, 128, 64, True, BF), (8192, 18432, 128, True, HF),
+                                                   (4112, 36864, 32, False, BF)])
+@pytest.mark.parametrize("tokens", [5, 16, 20, 33, 48, 49])
+def test_eight_row_groups_a_workgroup(mlk, tokens, n, k, group, zeros, dtype):
+    A, S, Z = packed_at_random(n, k, group, zeros, dtype, n + tokens)
+    x, bias = randn((tokens, k), dtype, 1.0, 3), randn((1, n), dtype, 1.0, 4)
+    got = mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, bias=bias.cuda())
+    assert torch.equal(got, mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, bias=bias.cuda()))
+    check_some_rows(mlk, A, S, Z, group, x, bias, got)
+
+
+@pytest.mark.parametrize("tokens,n,k,group,zeros,dtype", [
+    (257, 11024, 1024, 32, True, HF), (257, 11024, 1024, 64, False, BF), (257, 11024, 1152, 128, True, BF), (515, 11024, 1024, 64, True, HF), (2050, 11024, 1024, 32, False, BF),
+    (515, 11024, 1152, 128, False, HF), (130, 4112, 14336, 128, True, BF), (257, 4112, 8192, 64, False, HF), (70, 8208, 14336, 64, True, BF), (70, 11024, 8192, 128, False, BF),
+    (257, 8208, 14336, 32, True, BF), (515, 4112, 14336, 32, False, HF), (515, 11024, 1024, 512, True, BF)])
+def test_panels(mlk, tokens, n, k, group, zeros, dtype):
+    """Panels of 64 and of 128 tokens, whole and in slices of k; the last one holds a single row group."""
+    from muxi_native_layout_kernels_amd import _lib
+    per = 128 // group if group < 128 else 1
+    sums = (tokens * (k // 128 * per + 1) * 16 + 255) // 256 * 256
+    need = _lib.load().mlk_gemm_w4_workspace_bytes(tokens, n, k, group) - 65536 - sums
+    assert need >= 0 and need % (tokens * n * 4) == 0, "the plan has no panels here: take another size"
+    A, S, Z = packed_at_random(n, k, group, zeros, dtype, n + tokens)
+    x, bias = randn((tokens, k), dtype, 1.0, 3), randn((1, n), dtype, 1.0, 4)
+    got = mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, bias=bias.cuda())
+    check_some_rows(mlk, A, S, Z, group, x, bias, got)
+    x[3, 7] = float("nan")                               # keeps to its row
+    other = mlk.gemm_layoutA_w4(A, S, x.cuda(), Z, bias=bias.cuda())
+    assert other[3].isnan().all() and torch.equal(other[4:], got[4:]) and torch.equal(other[:3], got[:3])
+
+
+@pytest.mark.parametrize("tokens", [300, 1030])
+def test_panels_in_a_graph_and_off_16_bytes(mlk, tokens):
+    A, S, Z = packed_at_random(11024, 1024, 64, True, BF, 1)
+    x = randn((tokens, 1024), BF, 1.0, 0).cuda()
+    replays(lambda: [mlk.gemm_layoutA_w4(A, S, x, Z)], [x], lambda i: [randn((tokens, 1024), BF, 1.0, i + 1)])
+    off = torch.empty(tokens * 1024 + 1, dtype=BF, device="cuda")[1:].view(tokens, 1024).copy_(x)
+    assert off.data_ptr() % 16 and torch.equal(mlk.gemm_layoutA_w4(A, S, off, Z), mlk.gemm_layoutA_w4(A, S, x, Z))
 
 
 @pytest.mark.parametrize("T,E,K,same", [(2, 3, 1, True), (3, 40, 20, False), (32, 4, 2, False), (33, 4, 2, False), (64, 2, 1, True), (64, 5, 1, False), (7, 200, 9, False)])
