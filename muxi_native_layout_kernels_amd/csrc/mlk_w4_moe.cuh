@@ -1,7 +1,7 @@
 // Expert layers over 4-bit weights: grouped gate/up product with SiLU(gate) * up, grouped down product, weighted sum.
 //
-// Several tokens: the routed pairs are brought into expert order in blocks of 16 (moe_align_kernel); a task is a block (panels: up to eight) of one
-// expert, which share one pass over its weights.  The intermediate is kept row-major [slot][I] in the activations' type (slot = place in the order), the
+// Several tokens: the routed pairs are brought into expert order in blocks of 16 (moe_align_kernel); a task is a block, or up to two (panels: up to
+// eight) of one expert, which share one pass over its weights.  The intermediate is kept row-major [slot][I] in the activations' type (slot = place in the order), the
 // weighted products of the down projection in fp32 [pair][slice][H], and a last launch adds a token's pairs in the order of its picks.
 // One token: its picks are the tasks, no alignment; the down projection's waves deal the picks among themselves and write the output at once.
 #pragma once
@@ -171,6 +171,84 @@ __global__ void __launch_bounds__(kW4MoeWaves * 64, (w4_moe_waves<GS, ZP>())) w4
     }
 }
 
+// More pairs an expert: a task is one or two blocks, and a wave takes eight row groups, so that a workgroup's activations, which it reads whole, come to twice as many
+// rows and the weights to twice as many tokens (8 experts of 4096 x 14336, top-2, 64 tokens: 238 -> 159 us).
+template <class T, int GS, bool ZP, int TT, int R>
+__device__ __forceinline__ void w4_moe_gate_up_blocks(const W4MoeArgs &p, const MoeTask &task, f32x4 *red) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int o = lane >> 4, r16 = lane & 15, rg0 = blockIdx.x * (R / 2);
+    W4Rows<R> rows;
+    w4_gate_up_rows<GS, R>(rows, p, task.expert, rg0);
+    const uint16_t *xrow[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        const int pair = p.sorted[(task.block0 + tt) * 16 + r16];
+        xrow[tt] = p.X + (size_t)(pair < p.n_pairs ? pair / p.K : 0) * p.H;
+    }
+    f32x4 acc[R][TT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w4_stream<T, GS, ZP, TT, R, TT == 1 ? 2 : 1, false>(acc, rows, xrow, nullptr, wave, p.H >> 7, kW4MoeWaves, p.inv, lane, false);
+    constexpr int CELLS = R * TT, HALF = CELLS / 2;
+    w4_park<CELLS>(red, reinterpret_cast<const f32x4(&)[CELLS]>(acc), wave, lane);
+    __syncthreads();
+    for (int c = wave; c < HALF; c += kW4MoeWaves) {
+        const int r = c / TT, tt = c - r * TT;
+        const f32x4 g = w4_fold<CELLS>(red, c, kW4MoeWaves, lane), u = w4_fold<CELLS>(red, HALF + c, kW4MoeWaves, lane);
+        uint16_t *h = p.hbuf + (size_t)((task.block0 + tt) * 16 + o * 4) * p.I + (rg0 + r) * 16 + r16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[(size_t)i * p.I] = (uint16_t)T::from_f32(silu_mul(g[i], u[i]));
+    }
+}
+template <class T, int GS, bool ZP, int TT, int R>
+__device__ __forceinline__ void w4_moe_down_blocks(const W4MoeArgs &p, const MoeTask &task, f32x4 *red) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int o = lane >> 4, r16 = lane & 15, rg0 = blockIdx.x * R;
+    const W4Matrix m = w4_of_expert<GS>(p.w2, task.expert, p.H, p.I, p.blocks2);
+    W4Rows<R> rows;
+#pragma unroll
+    for (int r = 0; r < R; ++r) w4_row<GS, R>(rows, r, m, rg0 + r, p.I >> 7, p.blocks2);
+    const uint16_t *xrow[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) xrow[tt] = p.hbuf + (size_t)((task.block0 + tt) * 16 + r16) * p.I;
+    f32x4 acc[R][TT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w4_stream<T, GS, ZP, TT, R, TT == 1 ? 2 : 1, false>(acc, rows, xrow, nullptr, wave, p.I >> 7, kW4MoeWaves, p.inv, lane, false);
+    constexpr int CELLS = R * TT;
+    w4_park<CELLS>(red, reinterpret_cast<const f32x4(&)[CELLS]>(acc), wave, lane);
+    __syncthreads();
+    for (int c = wave; c < CELLS; c += kW4MoeWaves) {
+        const int r = c / TT, tt = c - r * TT;
+        const f32x4 v = w4_fold<CELLS>(red, c, kW4MoeWaves, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int pair = p.sorted[(task.block0 + tt) * 16 + o * 4 + i];
+            if (pair < p.n_pairs) p.obuf[(size_t)pair * p.H + (rg0 + r) * 16 + r16] = T::to_f32(p.wts[pair]) * v[i];
+        }
+    }
+}
+template <class T, int GS, bool ZP>
+__global__ void __launch_bounds__(kW4MoeWaves * 64, 2) w4_moe_gate_up2_kernel(W4MoeArgs p) {
+    extern __shared__ f32x4 red[];
+    if ((int)blockIdx.y >= *p.n_tasks) return;
+    const MoeTask task = p.tasks[blockIdx.y];
+    if (task.nblocks == 1) w4_moe_gate_up_blocks<T, GS, ZP, 1, 8>(p, task, red);
+    else w4_moe_gate_up_blocks<T, GS, ZP, 2, 8>(p, task, red);
+}
+template <class T, int GS, bool ZP>
+__global__ void __launch_bounds__(kW4MoeWaves * 64, 2) w4_moe_down2_kernel(W4MoeArgs p) {
+    extern __shared__ f32x4 red[];
+    if ((int)blockIdx.y >= *p.n_tasks) return;
+    const MoeTask task = p.tasks[blockIdx.y];
+    if (task.nblocks == 1) w4_moe_down_blocks<T, GS, ZP, 1, 8>(p, task, red);
+    else w4_moe_down_blocks<T, GS, ZP, 2, 8>(p, task, red);
+}
+
 // y[t] = T(sum over the token's pairs on this card, in pick order)
 template <class T>
 __global__ void __launch_bounds__(256) w4_moe_combine_kernel(W4MoeArgs p) {
@@ -332,6 +410,13 @@ int w4_launch_moe(const W4MoeArgs &a, const W4MoePlan &pl, hipStream_t s) {
         // one row group of gate and of up (8 experts of 4096 x 14336: the layer 43.8 us, with two 52.5), one of the down projection (52.4 and 56.6)
         rc = w4_moe1_gate_up<T, GS, ZP, 2>(a, s);
         return rc == MLK_OK ? w4_moe1_down<T, GS, ZP, 1>(a, s) : rc;
+    }
+    if (pl.tt == 2) {
+        MLK_W4_MOE(w4_moe_gate_up2_kernel, dim3(a.I / 64, pl.max_tasks), kW4MoeWaves, (size_t)kW4MoeWaves * 16 * 1024, T, GS, ZP);
+        MLK_W4_MOE(w4_moe_down2_kernel, dim3(a.H / 128, pl.max_tasks), kW4MoeWaves, (size_t)kW4MoeWaves * 16 * 1024, T, GS, ZP);
+        w4_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
+        MLK_LAUNCH_CHECK();
+        return MLK_OK;
     }
     // four row groups a wave: 128 registers (8 experts at 16 tokens: 120 us, with eight 139, with two 129)
     rc = pl.few ? w4_moe_gate_up<T, GS, ZP, 4, true>(a, pl.max_tasks, s) : w4_moe_gate_up<T, GS, ZP, 4, false>(a, pl.max_tasks, s);

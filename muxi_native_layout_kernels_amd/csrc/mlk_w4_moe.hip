@@ -34,18 +34,19 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
         pl.max_tasks = topk;
         return pl;
     }
-    // Routed pairs of an expert that is reached.  Up to 30 on average the streaming kernels, one block of 16 tokens a task, and above panels: 128 experts of
-    // 2048 x 768, top-8, at 400 tokens (25) 163 us against 208 with panels, at 500 (31) 189 and 209, at 800 (50) 259 and 266; 64 of 2048 x 1408, top-6, at 300 (28) 145
-    // and 147, at 400 (37) 175 and 160; 16 of 4096 x 2048, top-4, at 120 (30) 119 and 125, at 160 (40) 143 and 130.  Larger experts, which the second task of one
-    // finds in no cache, to 22: 8 of 4096 x 14336, top-2, at 64 tokens (16) 207 and 232, at 80 (20) 246 and 244, at 130 (32) 377 and 246.
+    // Routed pairs of an expert that is reached.  Up to 8 on average a block of 16 tokens is a task, above up to two blocks, and with many panels (us with one, two, panels):
+    //   8 experts of 4096 x 14336, top-2      at 32 tokens (8) 141, 143, 234; at 36 (9) 178, 154, 240; at 100 (25) 309, 220, 245; at 160 (40) 442, 265, 252; at 300 (75) two 440, 328
+    //   256 of 7168 x 2048, top-8             at 400 (12) 1453, 1164, 1753; at 1000 (31) 2689, 1880, 2098; at 2000 (62) two 3177, 2817
+    //   128 of 2048 x 768, top-8              at 130 (8) 97, 100, 164; at 160 (10) 109, 107, 181; at 800 (50) 257, 224, 268; at 1300 (81) two 325, 330; at 2000 (125) 468, 437
+    //   64 of 2048 x 1408, top-6              at 100 (9) 84, 82, 126; at 500 (46) 205, 157, 176; at 1000 (93) two 263, 257
     const int reached = pairs < E ? pairs : E, load = (pairs + reached - 1) / reached;
-    pl.panels = load > ((int64_t)hidden * inter <= (1 << 24) ? 30 : 22) && (int64_t)tokens * hidden < (1ll << 31);
-    pl.tt = pl.panels ? 8 : 1;
+    pl.panels = load > ((int64_t)hidden * inter <= (1 << 23) ? 80 : 40) && (int64_t)tokens * hidden < (1ll << 31);
+    pl.tt = pl.panels ? 8 : (load > 8 ? 2 : 1);
     // an expert's last task may be short: at most one more than its blocks fill
     const int64_t most = (int64_t)E + pairs / (16 * pl.tt);
     pl.max_tasks = (int)(most < pairs ? most : pairs);
     if (!pl.panels) {
-        pl.few = pairs <= 64;
+        pl.few = pl.tt == 1 && pairs <= 64;
         return pl;
     }
     // Two K slices of a long down projection that would leave CUs without a panel in its last round: 8 experts of 4096 x 14336 at 100 tokens 276 -> 240 us, at

@@ -411,3 +411,21 @@ def test_one_workspace_for_counts_and_losses(mlk):
         for _ in range(3):
             assert torch.equal(mlk.expert_counts(ids.cuda(), E).cpu(), want)
             assert torch.equal(mlk.moe_balance_loss(logits, ids.cuda())[1].cpu(), want)
+
+
+@pytest.mark.parametrize("T,E,K,H,I,group,zeros,dtype", [
+    (20, 4, 2, 256, 128, 32, True, BF), (33, 3, 1, 128, 384, 64, False, HF), (77, 6, 3, 640, 128, 128, True, HF), (60, 2, 2, 256, 8192, 64, True, BF), (140, 4, 1, 384, 256, 32, False, HF),
+    (150, 8, 4, 128, 128, 128, False, BF)])
+def test_experts_of_two_blocks_a_task(mlk, T, E, K, H, I, group, zeros, dtype):
+    """9 to 80 pairs an expert: full and half tasks, an expert with none, one with all, dropped pairs."""
+    p1, p2, w1, w2 = layer(E, H, I, group, dtype, zeros, T)
+    x = randn((T, H), dtype, 1.0, T)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    for case in range(3):
+        ids, wts = routing(T, E, K, dtype, T + case)
+        if case == 1:
+            ids[ids == 0] = -1                           # nobody's
+        if case == 2:
+            ids[:, 0] = E - 1
+        y = mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2)
+        check_experts(y, expected_experts(x, w1, w2, p1[1], p2[1], ids, wts), dtype, "experts, routing %d" % case)
