@@ -28,7 +28,9 @@ struct W4Plan {
 
 // Up to 32 tokens.  Microseconds on weights from memory, groups of 128, bf16 (r row groups a workgroup, s slices of K):
 //   one to four tokens   one workgroup per CU as far as r <= 4 goes, K whole: 4096 x 4096 r = 1 4.7 (s = 2: 6.3), 4096 x 14336 r = 1 9.8, r = 2 s = 2 10.7; 28672 x 8192 one
-//                        token r = 2 25.7, r = 4 27.5, two tokens r = 4 24.9, r = 2 31.6
+//                        token r = 2 25.7, r = 4 27.5, two tokens r = 4 24.9, r = 2 31.6.  So, with m * tiles up to 600, where that gives between half of the CUs and all
+//                        a workgroup: 4096 x 4096 at 8 tokens 7.1 in slices, 5.7 whole, at 16 7.2 and 7.0, at 24 8.2 and 8.6; 8192 x 8192 at 8 11.3 and 10.8, at 16 12.1 and
+//                        12.8; 7168 x 2304 at 32 8.5 and 7.7
 //   more                 the activations weigh more (every workgroup reads all of them): r = 8 where that many row groups each, in slices of 48 tiles at least, leave
 //                        three quarters of the CUs a workgroup: 28672 x 8192 at 32 tokens r = 4 45.7, r = 8 32.6,
 //                        at 16 31.2 and 28.8; 27648 x 5120 at 32 30.0 and 22.8; 28672 x 4096 at 16 16.6 and 17.3; not 13824 x 5120 at 32, r = 4 18.8, r = 8 s = 2 19.1.
@@ -42,7 +44,7 @@ static W4Plan w4_plan_stream(int m, int n, int k) {
     pl.tb = 0;
     pl.slices = pl.r = 1;
     pl.tt = (m + 15) / 16;
-    if (m <= 4) {
+    if (m <= 4 || (m * tiles <= 600 && 2 * groups > cus && groups <= 4 * cus)) {
         while (pl.r < 4 && groups > pl.r * cus) pl.r *= 2;
         if (m == 1 && pl.r == 4 && groups > 4 * cus) pl.r = 2;
         pl.wgs = (groups + pl.r - 1) / pl.r;
