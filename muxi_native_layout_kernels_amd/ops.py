@@ -1074,19 +1074,46 @@ class _BalanceLoss(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dloss, _):
-        if dloss is None:
-            return None, None, None, None, None, None, None
-        logits, mask, cu, share = ctx.saved_tensors
-        T, E, _, kind, n_seq, _, _, _, fn = ctx.plan
-        with _OnDevice(logits):
-            grad = torch.empty_like(logits)
-            rc = fn(logits.data_ptr(), kind, ctx.score_fun, T, E, _ptr(mask), _ptr(cu), n_seq, share.data_ptr(), dloss.data_ptr(), grad.data_ptr(),
-                    _stream_of(logits))
-            if rc != 0:
-                _lib.check(rc, "moe_balance_loss")
-        return grad, None, None, None, None, None, None
+        if torch.is_grad_enabled() and dloss is not None:                       # create_graph
+            with torch.no_grad():
+                grad = _balance_backward(ctx, dloss)[0]
+            return _FirstDerivative.apply(grad.requires_grad_(True)), None, None, None, None, None, None
+        return _balance_backward(ctx, dloss)
+
+
+class _FirstDerivative(torch.autograd.Function):
+    """The gradient as it is; its own derivative is refused, not taken for zero."""
+
+    @staticmethod
+    def forward(ctx, grad):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("moe_balance_loss: the gradient cannot be differentiated again")
+
+
+def _balance_backward(ctx, dloss):
+    if dloss is None:
+        return None, None, None, None, None, None, None
+    logits, mask, cu, share = ctx.saved_tensors
+    if logits.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            grad = _balance_grad_launch(ctx, dloss, logits, mask, cu, share)
+    else:
+        grad = _balance_grad_launch(ctx, dloss, logits, mask, cu, share)
+    return grad, None, None, None, None, None, None
+
+
+def _balance_grad_launch(ctx, dloss, logits, mask, cu, share):
+    T, E, _, kind, n_seq, _, _, _, fn = ctx.plan
+    grad = torch.empty_like(logits)
+    rc = fn(logits.data_ptr(), kind, ctx.score_fun, T, E, _ptr(mask), _ptr(cu), n_seq, share.data_ptr(), dloss.data_ptr(), grad.data_ptr(),
+            _stream_of(logits))
+    if rc != 0:
+        _lib.check(rc, "moe_balance_loss")
+    return grad
 
 
 def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0, token_mask=None, cu_seqlens=None):
@@ -1098,7 +1125,7 @@ def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0,
 
     gating_output [T, E] fp16 / bf16 / fp32, E <= 256; experts_ids int32 [T, K] (`fused_routing_gate`); token_mask bool [T], False for padded
     tokens; cu_seqlens int32 [sequences + 1] on the device, non-decreasing, where each sequence begins and the last one ends (None: all tokens are
-    one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0."""
+    one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0.  A second derivative is refused."""
     logits = gating_output
     key = ("balance", logits.shape, logits.dtype, logits.get_device(), experts_ids.shape, experts_ids.dtype, experts_ids.get_device(),
            None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.get_device()),

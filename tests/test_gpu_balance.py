@@ -183,3 +183,18 @@ def test_many_short_sequences(mlk, sigmoid):
     mask = torch.rand(T, generator=g) < 0.6
     check(mlk, logits, ids, sigmoid, 1.0, None, cuts)
     check(mlk, logits, ids, sigmoid, 1.0, mask, cuts)
+
+
+def test_a_second_derivative_is_refused(mlk):
+    logits, ids = case(50, 16, 2, torch.float32, 6)
+    leaf = logits.cuda().requires_grad_(True)
+    loss, counts = mlk.moe_balance_loss(leaf, ids.cuda())
+    assert not counts.requires_grad
+    plain, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    grad, = torch.autograd.grad(loss, leaf, create_graph=True)
+    assert torch.equal(grad.detach(), plain)
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        (grad.sum() + (leaf * leaf).sum()).backward()
+    with torch.no_grad():
+        quiet, _ = mlk.moe_balance_loss(leaf, ids.cuda())
+    assert not quiet.requires_grad and torch.equal(quiet, loss.detach())
