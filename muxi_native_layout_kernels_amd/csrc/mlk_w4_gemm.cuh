@@ -134,31 +134,28 @@ static int w4_launch_stream_one(W4GemmArgs a, int wgs, int waves, hipStream_t s)
     return MLK_OK;
 }
 
-// r = row groups per workgroup the kernel is built for: 1, 2 or 4, with tt up to 3 also 8; tt = blocks of 16 tokens per workgroup; wgs * r >= N / 16.  One token is staged in LDS (r = 1, 2; a slice of 64 K at most): 4096 x 4096
+// r = row groups per workgroup, tt = blocks of 16 tokens: what w4_plan() picks of them; wgs * r >= N / 16.  One token is staged in LDS (r = 1, 2; a slice of 64 K at most): 4096 x 4096
 // 4.7 us against 5.1.
 template <class T, int GS, bool ZP>
 int w4_launch_stream(const W4GemmArgs &a, int r, int tt, int wgs, int waves, hipStream_t s) {
     if ((int64_t)r * wgs < a.N / 16 || wgs > a.N / 16) return fail(MLK_ERR_INVALID, "w4 gemm: launch parameters");
-#define MLK_W4_R(TT, XL)                                                                  \
-    do {                                                                                  \
-        if (r == 1) return w4_launch_stream_one<T, GS, ZP, TT, 1, XL>(a, wgs, waves, s);       \
-        if (r == 2) return w4_launch_stream_one<T, GS, ZP, TT, 2, XL>(a, wgs, waves, s);       \
-        if (r == 4) return w4_launch_stream_one<T, GS, ZP, TT, 4, XL>(a, wgs, waves, s);       \
-        if (TT < 4 && r == 8) return w4_launch_stream_one<T, GS, ZP, (TT < 4 ? TT : 1), 8, XL>(a, wgs, waves, s); \
-    } while (0)
+#define MLK_W4_R(TT, R) if (tt == TT && r == R) return w4_launch_stream_one<T, GS, ZP, TT, R, false>(a, wgs, waves, s)
     if (a.M == 1 && (a.K / kW4TileK + a.slices - 1) / a.slices * 256 <= kW4TokenLds) {
         if (r == 1) return w4_launch_stream_one<T, GS, ZP, 1, 1, true>(a, wgs, waves, s);
         if (r == 2) return w4_launch_stream_one<T, GS, ZP, 1, 2, true>(a, wgs, waves, s);
     }
-    if (tt == 1) {
-        MLK_W4_R(1, false);
-    } else if (tt == 2) {
-        MLK_W4_R(2, false);
-    } else if (tt == 3) {
-        MLK_W4_R(3, false);
-    } else {
-        MLK_W4_R(4, false);
-    }
+    MLK_W4_R(1, 1);
+    MLK_W4_R(1, 2);
+    MLK_W4_R(1, 4);
+    MLK_W4_R(1, 8);
+    MLK_W4_R(2, 1);
+    MLK_W4_R(2, 2);
+    MLK_W4_R(2, 4);
+    MLK_W4_R(2, 8);
+    MLK_W4_R(3, 2);
+    MLK_W4_R(3, 4);
+    MLK_W4_R(3, 8);
+    MLK_W4_R(4, 4);
 #undef MLK_W4_R
     return fail(MLK_ERR_INVALID, "w4 gemm: launch parameters");
 }

@@ -107,7 +107,7 @@ static W4Plan w4_plan(int m, int n, int k, int group) {
         for (int slices = 2; slices <= 16 && slices * 2 <= tiles; ++slices) panels(tb, slices);
     }
     for (int tt = 2; tt <= 4; ++tt)
-        for (int r = 1; r <= (tt < 4 ? 8 : 4); r *= 2) {
+        for (int r = tt == 2 ? 1 : (tt == 3 ? 2 : 4); r <= (tt < 4 ? 8 : 4); r *= 2) {            // others are the cheapest for one shape in thousands
             const int64_t blocks = ((int64_t)m + 16 * tt - 1) / (16 * tt), wgs = (groups + r - 1) / r;
             for (int slices = 1; slices == 1 || (slices <= 8 && slices * 6 <= tiles && wgs * blocks * slices <= 2 * cus); ++slices) {
                 const double c = w4_stream_cost(m, n, k, group, tt, r, slices, cus);

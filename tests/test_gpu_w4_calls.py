@@ -79,7 +79,8 @@ def test_activations_off_16_bytes_and_empty_batches(mlk, tokens):
     assert mlk.fused_experts_w4(x[:0], a1, a2, ids[:0], wts[:0], s1, s2).shape == (0, 128)
 
 
-@pytest.mark.parametrize("tokens,n,k", [(1, 512, 2048), (17, 512, 7168), (50, 272, 640), (65, 272, 1152), (1030, 1040, 384)])
+@pytest.mark.parametrize("tokens,n,k", [(1, 512, 2048), (17, 512, 7168), (50, 272, 640), (65, 272, 1152), (100, 512, 7168), (250, 528, 5120), (1030, 1040, 384), (257, 4112, 8192),
+                                        (515, 11024, 1024)])
 def test_rows_behind_the_last_one_are_left(mlk, tokens, n, k):
     from muxi_native_layout_kernels_amd import _lib
     lib = _lib.load()
