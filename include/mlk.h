@@ -372,7 +372,7 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
                          const void *x, int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter, int group, int x_kind,
                          const int32_t *topk_ids, const void *topk_weights, const int32_t *experts_map, void *y, void *workspace,
                          size_t workspace_bytes, void *stream);
-size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int hidden, int inter, int group);
+size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter, int group);
 
 /* ------------------------------------------------------------- router balance */
 

@@ -48,7 +48,7 @@ SIGNATURES = {
                                      c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mlk_gemm_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "mlk_fused_experts_w4": (c_int, [c_void_p] * 7 + [c_int] * 8 + [c_void_p] * 5 + [c_size_t, c_void_p]),
-    "mlk_experts_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "mlk_experts_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "mlk_expert_counts": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "mlk_balance_loss": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_float,
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),

@@ -1,4 +1,5 @@
 // Expert layers over 4-bit weights: arguments, workspace, passes.
+#include <algorithm>
 #include <initializer_list>
 
 #include "mlk_w4_moe_panel.cuh"
@@ -25,7 +26,7 @@ constexpr int kW4MoePairs = 16384;      // routed pairs of a pass: bounds the sc
 
 static int w4_moe_pass_tokens(int n_tokens, int topk) { return n_tokens < kW4MoePairs / topk ? n_tokens : kW4MoePairs / topk; }
 
-static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter) {
+static W4MoePlan w4_moe_plan(int tokens, int E, int n_router, int topk, int hidden, int inter) {
     W4MoePlan pl = {};
     pl.slices = 1;
     const int cus = device_cus(), pairs = tokens * topk;
@@ -39,7 +40,9 @@ static W4MoePlan w4_moe_plan(int tokens, int E, int topk, int hidden, int inter)
     //   256 of 7168 x 2048, top-8             at 400 (12) 1453, 1164, 1753; at 1000 (31) 2689, 1880, 2098; at 2000 (62) two 3177, 2817
     //   128 of 2048 x 768, top-8              at 130 (8) 97, 100, 164; at 160 (10) 109, 107, 181; at 800 (50) 257, 224, 268; at 1300 (81) two 325, 330; at 2000 (125) 468, 437
     //   64 of 2048 x 1408, top-6              at 100 (9) 84, 82, 126; at 500 (46) 205, 157, 176; at 1000 (93) two 263, 257
-    const int reached = pairs < E ? pairs : E, load = (pairs + reached - 1) / reached;
+    // With E of the router's experts here that share of the pairs is expected here.
+    const int here = (int)std::max<int64_t>(1, std::min<int64_t>(pairs, (int64_t)pairs * E / n_router));
+    const int reached = std::min(here, E), load = (here + reached - 1) / reached;
     pl.panels = load > ((int64_t)hidden * inter <= (1 << 23) ? 80 : 40) && (int64_t)tokens * hidden < (1ll << 31);
     pl.tt = pl.panels ? 8 : (load > 8 ? 2 : 1);
     // an expert's last task may be short: at most one more than its blocks fill
@@ -95,13 +98,13 @@ using namespace mlk;
 extern "C" {
 
 // What a call needs: a long one goes in passes of one size and a shorter last one, whose plan may differ.
-size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int topk, int hidden, int inter, int group) {
-    if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0 || group < 32) return 0;
+size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter, int group) {
+    if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || n_router_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0 || group < 32) return 0;
     const int step = w4_moe_pass_tokens(n_tokens, topk), rest = n_tokens % step;
     size_t most = 0;
     for (int t : {step, rest}) {
         if (t == 0) continue;
-        const size_t need = w4_moe_carve(nullptr, w4_moe_plan(t, n_experts, topk, hidden, inter), t, n_experts, topk, hidden, inter, group, nullptr);
+        const size_t need = w4_moe_carve(nullptr, w4_moe_plan(t, n_experts, n_router_experts, topk, hidden, inter), t, n_experts, topk, hidden, inter, group, nullptr);
         if (need > most) most = need;
     }
     return most;
@@ -127,7 +130,7 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
                 "experts w4: weights, activations, outputs and workspace must lie on 16 bytes");
     MLK_REQUIRE((((uintptr_t)w1_scale | (uintptr_t)w2_scale) & 7) == 0 && (((uintptr_t)w1_zero | (uintptr_t)w2_zero) & 3) == 0,
                 "experts w4: scales must lie on 8 bytes, zero points on 4");
-    if (workspace_bytes < mlk_experts_w4_workspace_bytes(n_tokens, n_experts, topk, hidden, inter, group))
+    if (workspace_bytes < mlk_experts_w4_workspace_bytes(n_tokens, n_experts, n_router_experts, topk, hidden, inter, group))
         return fail(MLK_ERR_WORKSPACE, "experts w4: workspace too small");
     hipStream_t s = (hipStream_t)stream;
     W4MoeArgs a;
@@ -151,7 +154,7 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
         a.Y = (uint16_t *)y + (size_t)t0 * hidden;
         a.ids = topk_ids + (size_t)t0 * topk;
         a.wts = (const uint16_t *)topk_weights + (size_t)t0 * topk;
-        const W4MoePlan pl = w4_moe_plan(a.T, n_experts, topk, hidden, inter);
+        const W4MoePlan pl = w4_moe_plan(a.T, n_experts, n_router_experts, topk, hidden, inter);
         W4MoeWorkspace ws;
         w4_moe_carve((uint8_t *)workspace, pl, a.T, n_experts, topk, hidden, inter, group, &ws);
         a.sorted = ws.sorted;

@@ -976,8 +976,9 @@ def fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2
         _check_tensors(((x, "hidden_states"), (w1, "w1"), (w2, "w2"), (topk_ids, "topk_ids"), (topk_weights, "topk_weights"), (w1_scale, "w1_scale"),
                      (w2_scale, "w2_scale"), (w1_zero, "w1_zero"), (w2_zero, "w2_zero"), (experts_map, "experts_map")), x.device)
         lib = _lib.load()
-        plan = _plans[key] = (x.size(0), E, E if experts_map is None else experts_map.numel(), K, hidden, inter, group, _KIND[x.dtype],
-                              lib.mlk_experts_w4_workspace_bytes(x.size(0), E, K, hidden, inter, group), lib.mlk_fused_experts_w4)
+        E_router = E if experts_map is None else experts_map.numel()
+        plan = _plans[key] = (x.size(0), E, E_router, K, hidden, inter, group, _KIND[x.dtype],
+                              lib.mlk_experts_w4_workspace_bytes(x.size(0), E, E_router, K, hidden, inter, group), lib.mlk_fused_experts_w4)
     T, E, E_router, K, hidden, inter, group, kind, ws_need, fn = plan
     with _OnDevice(x):
         if x.data_ptr() & 15:

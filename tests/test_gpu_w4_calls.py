@@ -110,7 +110,7 @@ def test_experts_keep_to_their_rows_and_workspace(mlk, T, E, K):
     ids, wts = routing(T, E, K, HF, T)
     xd, idsd, wtsd = on_gpu(x, ids, wts)
     y = torch.full((T + 8, H), 7.0, dtype=HF, device="cuda")
-    need = lib.mlk_experts_w4_workspace_bytes(T, E, K, H, I, 64)
+    need = lib.mlk_experts_w4_workspace_bytes(T, E, E, K, H, I, 64)
     ws = torch.randint(0, 256, (need + 4096,), dtype=torch.uint8, device="cuda")          # anything
     ws[need:] = 91
     rc = lib.mlk_fused_experts_w4(a1.data_ptr(), s1.data_ptr(), z1.data_ptr(), a2.data_ptr(), s2.data_ptr(), z2.data_ptr(), xd.data_ptr(), T, E, E, K, H, I, 64, 0,
@@ -430,3 +430,22 @@ def test_experts_of_two_blocks_a_task(mlk, T, E, K, H, I, group, zeros, dtype):
             ids[:, 0] = E - 1
         y = mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2)
         check_experts(y, expected_experts(x, w1, w2, p1[1], p2[1], ids, wts), dtype, "experts, routing %d" % case)
+
+
+@pytest.mark.parametrize("T,E,held,K", [(160, 64, 4, 4), (200, 16, 4, 2), (700, 16, 4, 2), (60, 12, 3, 8)])
+@pytest.mark.parametrize("here", ["its share", "all", "none"])
+def test_a_share_of_the_experts_whatever_comes(mlk, T, E, held, K, here):
+    """Plans expect the held experts' share of the pairs; all of them or none may come."""
+    p1, p2, w1, w2 = layer(held, 128, 256, 128, BF, True, T)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    x = randn((T, 128), BF, 1.0, T)
+    ids, wts = routing(T, E, K, BF, T)
+    emap = torch.full((E,), -1, dtype=torch.int32)
+    emap[:held] = torch.arange(held, dtype=torch.int32)
+    if here == "all":
+        ids = ids % held
+    if here == "none":
+        ids = ids % (E - held) + held
+    ids = ids.int().contiguous()
+    y = mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2, experts_map=emap.cuda())
+    check_experts(y, expected_experts(x, w1, w2, p1[1], p2[1], ids, wts, emap), BF, "experts here")

@@ -128,11 +128,16 @@ def test_c_interface_of_the_products_refuses():
     said(lib, gemm(s=FAKE + 4), b"8 bytes")
     said(lib, gemm(z=FAKE + 2), b"on 4")
     assert gemm(m=0) == 0 and gemm(n=0) == 0
-    for m, n, k, group in ((16, 4096, 14336, 128), (100, 512, 1024, 32), (2000, 1024, 1024, 64)):
+    scratch = 0
+    for m, n, k, group in ((16, 4096, 14336, 128), (100, 512, 1024, 32), (2000, 1024, 1024, 64), (100, 512, 7168, 128), (500, 11008, 4096, 64), (4000, 4096, 4096, 32)):
         need = lib.mlk_gemm_w4_workspace_bytes(m, n, k, group)
+        if need == 0:                                    # runs whole
+            continue
         assert need > 64 * 1024
+        scratch += 1
         said(lib, gemm(m=m, n=n, k=k, group=group, ws=FAKE, ws_bytes=need - 1), b"workspace", -3)
         said(lib, gemm(m=m, n=n, k=k, group=group), b"workspace", -3)
+    assert scratch >= 4
     assert lib.mlk_gemm_w4_workspace_bytes(1, 4096, 4096, 128) == 0
     for bad in ((0, 16, 128, 128), (1, 0, 128, 128), (1, 16, 0, 128), (1, 16, 128, 48), (1, 16, 128, 256), (-5, 16, 128, 128)):
         assert lib.mlk_gemm_w4_workspace_bytes(*bad) == 0
@@ -159,13 +164,13 @@ def test_c_interface_of_the_experts_refuses():
         said(lib, experts(**kw), word)
     assert experts(t=0) == 0
     for t in (1, 4, 500, 20000):
-        need = lib.mlk_experts_w4_workspace_bytes(t, 8, 2, 256, 128, 128)
+        need = lib.mlk_experts_w4_workspace_bytes(t, 8, 8, 2, 256, 128, 128)
         assert need > 0
         said(lib, experts(t=t, ws_bytes=need - 1), b"workspace", -3)
     # passes of 16384 pairs: a long prompt needs no more than its longest pass
-    assert lib.mlk_experts_w4_workspace_bytes(1 << 20, 8, 2, 256, 128, 128) == lib.mlk_experts_w4_workspace_bytes(8192, 8, 2, 256, 128, 128)
-    for bad in ((0, 8, 2, 256, 128, 128), (4, 0, 2, 256, 128, 128), (4, 257, 2, 256, 128, 128), (4, 8, 33, 256, 128, 128), (4, 8, 2, 0, 128, 128),
-                (4, 8, 2, 256, 128, 0)):
+    assert lib.mlk_experts_w4_workspace_bytes(1 << 20, 8, 8, 2, 256, 128, 128) == lib.mlk_experts_w4_workspace_bytes(8192, 8, 8, 2, 256, 128, 128)
+    for bad in ((0, 8, 8, 2, 256, 128, 128), (4, 0, 8, 2, 256, 128, 128), (4, 257, 257, 2, 256, 128, 128), (4, 8, 8, 33, 256, 128, 128), (4, 8, 8, 2, 0, 128, 128),
+                (4, 8, 8, 2, 256, 128, 0), (4, 8, 0, 2, 256, 128, 128)):
         assert lib.mlk_experts_w4_workspace_bytes(*bad) == 0
 
 
