@@ -1126,7 +1126,8 @@ def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0,
 
     gating_output [T, E] fp16 / bf16 / fp32, E <= 256; experts_ids int32 [T, K] (`fused_routing_gate`); token_mask bool [T], False for padded
     tokens; cu_seqlens int32 [sequences + 1] on the device, non-decreasing, where each sequence begins and the last one ends (None: all tokens are
-    one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0.  A second derivative is refused."""
+    one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0.  A second derivative is refused.
+    Both passes may be recorded into a HIP graph, once run on its stream; as with any torch function no earlier loss of the same leaf may then be alive."""
     logits = gating_output
     key = ("balance", logits.shape, logits.dtype, logits.get_device(), experts_ids.shape, experts_ids.dtype, experts_ids.get_device(),
            None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.get_device()),
