@@ -13,7 +13,8 @@
 //   sum over the group of W x = s * (sum (16 + q) x - (16 + z) * sum x)
 // goes to the running sums with one or two fp32 operations per output, group and lane.  sum x comes from the matrix cores too (an operand of ones), in the
 // lanes and registers where the products end.  Widening to q - z instead would need a subtraction per pair of weights, which bf16 has no packed
-// instruction for; the 16 costs some two bits of the 24 that the fp32 sums hold.
+// instruction for; the 16 costs some two bits of the 24 that the fp32 sums hold, more where a group's activations do not average to zero (the offset of
+// one group is then larger than its sum).  The streaming loop takes the offset out of every group; the panels (mlk_w4_panel.cuh) let neighbours cancel.
 //
 // The products run with the tokens as rows and the weights as columns: a lane then holds one weight row (its column) and four tokens, so it needs
 // one scale per tile, not four.

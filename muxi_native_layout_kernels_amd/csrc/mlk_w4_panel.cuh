@@ -10,9 +10,14 @@
 // cores are busy for 63 % of the cycles, and the card runs at 1.85 GHz under this load (2.4 without it).  Nothing may be added to the loop.  So sum x, which the offset of
 // 16 + q calls for (mlk_w4.cuh), does not come into this loop: as initial values of the products' sums it took another half of the LDS reads
 // (27648 x 5120 at 2048 tokens: 549 us).  It is made by a launch ahead (w4_sums_kernel) and multiplied behind the weights, like 8 more k for every 32, 64 or
-// 128:  acc += sum over the groups of (-s (16 + z)) * sum x,  both factors as parts of 8 bits in bf16 whatever the activations' type:
-//   sum x = c1 + c2 + c3 (24 bits),   -s (16 + z) = b1 + b2 (16 bits at most: exact),   octets {c1 c2 c3 c1 c2 0 0 0} . {b1 b1 b1 b2 b2 0 0 0},
+// 128:  acc += sum over the groups of o * sum x,  o = -s (16 + z) or s (31 - z), both factors as parts of 8 bits in bf16 whatever the activations' type:
+//   sum x = c1 + c2 + c3 (24 bits),   o = b1 + b2 (16 bits at most: exact),   octets {c1 c2 c3 c1 c2 0 0 0} . {b1 b1 b1 b2 b2 0 0 0},
 // what is left out is below 2^-24 of the product.
+// Until then the running sums hold the offset, and where a token's activations do not average to zero they would grow with k, the result with its root only.  So
+// every second window (counted from the panel's first) multiplies its codes' complement, W + s (31 - z) in place of W - s (16 + z) with the scale's sign
+// turned: 31 - q = 16 + ~q, and the offsets of two neighbours cancel but for what their scales and activations differ.  Activations of mean 1, fp16, K = 14336, groups of
+// 64: the results were off by 1.27 roundings with all windows alike, and by 1.80 with K = 14208 whole in groups of 32; now by less than 1.05 at any mean.  It costs 1 % (2048 tokens
+// above: 532 -> 537 us; spread between the products, as the widening is, the 8 instructions of two windows cost 539).
 //
 // Tokens come into LDS in windows of 128 k by loads that write LDS directly, four windows deep; weights go straight to registers: no wave needs
 // another one's.  Order of a window t: tokens t + 3 and weights t + 2 are requested, the products of t run, the weights of t + 1 are widened, the first operands
@@ -25,6 +30,8 @@
 // The sixteen lanes whose 16-byte reads are served together (0..3, 12..15, 20..27 of an operand, and 4..11, 16..19, 28..31) then meet sixteen
 // different bank groups, and all but one bit of an operand's octet is an immediate offset: two address registers for all of them.
 #pragma once
+
+#include <type_traits>
 
 #include "mlk_panel_lds.cuh"
 #include "mlk_w4.cuh"
@@ -184,16 +191,24 @@ struct W4Panel {
 #pragma unroll
         for (int q = 0; q < RING; ++q) x[q] = operand(0, 0, q);
 
-        auto window = [&](int t, int buf, u32x4 (&wn)[8], u32x4 (&wt)[8]) {
+        // EVEN: t is even, so t + 1 takes the codes' complement
+        auto window = [&](int t, int buf, u32x4 (&wn)[8], u32x4 (&wt)[8], auto even) {
+            constexpr bool EVEN = decltype(even)::value;
             const int b1 = (buf + 1) & 3;
             const From f = from(t + 3);
             exchange();
+            if constexpr (EVEN) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) raw[r][j] = ~raw[r][j];
+            }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const int g = b % G, now = b & 1, then = now ^ 1;
                 const int pb = (b + NB - 1) % NB, ptb = pb / G;        // the block before, whose products are added now
-                const float scale = w4_scale<T, GS>(b ? sc : sp, pb % G);
+                const float scale = (b ? EVEN : !EVEN) ? w4_scale<T, GS>(b ? sc : sp, pb % G) : -w4_scale<T, GS>(b ? sc : sp, pb % G);
 #pragma unroll
                 for (int m = 0; m < NM; ++m) {
                     const int P = b * NM + m, ahead = P + RING;
@@ -234,11 +249,11 @@ struct W4Panel {
         };
         int buf = 0, t = 0;
         for (; t + 2 <= n; t += 2) {
-            buf = window(t, buf, w[0], w[1]);
-            buf = window(t + 1, buf, w[1], w[0]);
+            buf = window(t, buf, w[0], w[1], std::true_type());
+            buf = window(t + 1, buf, w[1], w[0], std::false_type());
         }
-        if (t < n) buf = window(t, buf, w[0], w[1]);
-        const float scale = w4_scale<T, GS>(sp, G - 1);
+        if (t < n) buf = window(t, buf, w[0], w[1], std::true_type());
+        const float scale = n & 1 ? w4_scale<T, GS>(sp, G - 1) : -w4_scale<T, GS>(sp, G - 1);
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[TB - 1][i] = fmaf(scale, d[1][i], acc[TB - 1][i]);
         // what the last window requested may not have landed
@@ -253,7 +268,8 @@ struct W4Panel {
             for (int q = 0; q < 8; ++q) {
                 const int e = c * 16 + 4 * (q >> 1) + 2 * h + (q & 1), u = min(e, n * G - 1) + t0 * G;       // group of this lane's octet
                 const size_t at = (size_t)w4_block(u / G, inv) * 16 * G + u % G;
-                const float b = -T::to_f32(rows.scales[at]) * (ZP ? 16.f + (float)rows.zeros[at] : 24.f);
+                const float z = ZP ? (float)rows.zeros[at] : 8.f;
+                const float b = T::to_f32(rows.scales[at]) * (e / G & 1 ? 31.f - z : -16.f - z);
                 const uint32_t b1 = e < n * G ? f32_to_bf16_bits(b) : 0u, b2 = e < n * G ? f32_to_bf16_bits(b - bf16_bits_to_f32(b1)) : 0u;
                 wc[q] = u32x4{b1 | b1 << 16, b1 | b2 << 16, b2, 0u};
             }

@@ -83,3 +83,45 @@ def test_product_against_64_bits(mlk, tokens, n, k, group, zeros, dtype):
     assert_within(got, 0.5 * want + bias.double(), size + bias.double().abs(), dtype, k, "product with alpha and bias")
     if tokens == 1:
         assert torch.equal(mlk.gemv_layoutA_w4(A, S, x.cuda(), Z, alpha=0.5, bias=bias.cuda()), got)
+
+
+def centred_weights(n, k, group, zeros, seed):
+    """fp16 weights as a quantiser leaves them: codes around their zero point, positive scales.  Row-major parts and the weights in 64 bits."""
+    g = torch.Generator().manual_seed(seed)
+    s = ((torch.rand((n, k // group), generator=g) + 0.5) * (k ** -0.5 / 2.6)).half()
+    z = torch.randint(5, 12, s.shape, generator=g, dtype=torch.uint8) if zeros else None
+    off = torch.full(s.shape, 8.0) if z is None else z.float()
+    q = (torch.randn((n, k // group, group), generator=g) * 2.6 + off.unsqueeze(-1)).round().clamp(0, 15)
+    w = ((q.double() - off.double().unsqueeze(-1)) * s.double().unsqueeze(-1)).flatten(-2)
+    q = q.flatten(-2).to(torch.uint8)
+    return (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous(), s, z, w
+
+
+def runs_panels(tokens, n, k, group):
+    """The panels' workspace: counters, sums of the activations, partial sums where k is split."""
+    from muxi_native_layout_kernels_amd import _lib
+    per = 128 // group if group < 128 else 1
+    need = _lib.load().mlk_gemm_w4_workspace_bytes(tokens, n, k, group) - 65536 - (tokens * (k // 128 * per + 1) * 16 + 255) // 256 * 256
+    return need >= 0 and need % (tokens * n * 4) == 0
+
+
+@pytest.mark.parametrize("mean", [0.0, 1.0, 20.0])
+@pytest.mark.parametrize("tokens,times,k,group,zeros", [(515, 4, 14336, 128, False), (400, 8, 14336, 32, True), (300, 8, 14336, 64, True), (400, 16, 14208, 128, False), (400, 16, 14208, 32, True)])
+def test_error_does_not_grow_with_the_mean_of_the_activations(mlk, tokens, times, k, group, zeros, mean):
+    """The 2-norm of the error is that of one rounding to fp16, give or take a twentieth, whatever the mean m of the activations and the number of tokens.
+
+    One rounding: 2^-11 / sqrt(3) times 0.72 (numbers spread over a binade), 2.0e-4 of the result; a twentieth more leaves sqrt(1.05^2 - 1) = 0.32 of that, 6.5e-5, to the
+    fp32 sums.  The result is 2.6 sqrt(k (1 + m^2)) s, 310 m s and more.  Rounding to nearest adds 2^-24 / sqrt(3) of what is held at every step:
+      within a window    k / 16 steps that hold half of 24 * 128 m s on average: sqrt(k / 48) * 1540 / 310 * 2^-24 = 5e-6 of the result
+      sums of groups     k / 32 steps at most.  Offsets that are taken out of every group leave nothing; such that cancel between neighbouring windows leave the difference
+                         of their scales, 24 * 128 * 0.41 m s, in k / 256 pairs at random: 9400 m s at the end.  sqrt(k / 96) * 9400 / 310 * 2^-24 = 2.2e-5 of the result
+    An offset that is held for all of k until the end, 24 k m s, comes to 1.2e-4 of the result, 1.2 roundings."""
+    codes, s, z, w = centred_weights(528, k, group, zeros, k + group)
+    x = (randn((tokens, k), torch.float32, 1.0, 3) + mean).half()
+    A, S, Z = mlk.pack_layout_a_w4(*[None if t is None else t.cuda().repeat(times, 1) for t in (codes, s, z)])
+    assert runs_panels(tokens, 528 * times, k, group), "the plan has no panels here: take another size"
+    want = x.double() @ w.t()
+    for rows in (slice(None), slice(0, 20)):                 # panels; few tokens
+        got = mlk.gemm_layoutA_w4(A, S, x[rows].cuda(), Z).cpu().double().unflatten(1, (times, 528)) - want[rows].unsqueeze(1)
+        one = (want[rows].half().double() - want[rows]).norm() * times ** 0.5
+        assert got.norm() <= 1.05 * one, "%g roundings" % (got.norm() / one).item()
