@@ -251,7 +251,8 @@ size_t mlk_gemm_noalloc_scratch_bytes(void);
  * `batch` independent matrices are processed back to back; src and dst on 4 bytes. */
 int mlk_pack_layout_a_w4(const void *src, void *dst, int64_t batch, int n, int k, void *stream);
 int mlk_unpack_layout_a_w4(const void *src, void *dst, int64_t batch, int n, int k, void *stream);
-/* Scales (elem_size 2) or zero points (1), row-major [N, K/G] -> [N/16, K/max(G,128), 16, max(1,128/G)]. */
+/* Scales (elem_size 2) or zero points (1), row-major [N, K/G] -> [N/16, K/max(G,128), 16, max(1,128/G)].  Zero points above 15 are the caller's to refuse:
+ * the products would take them for different numbers by their token count. */
 int mlk_pack_scales_w4(const void *src, void *dst, int64_t batch, int n, int k, int group, int elem_size, void *stream);
 int mlk_unpack_scales_w4(const void *src, void *dst, int64_t batch, int n, int k, int group, int elem_size, void *stream);
 

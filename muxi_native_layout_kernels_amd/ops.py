@@ -628,7 +628,8 @@ def pack_layout_a_w4(codes, scales, zeros=None):
 
     codes  uint8 [N, K/2] or [E, N, K/2], two codes 0..15 in a byte, element 2 i in the low half of byte i
     scales fp16 / bf16 [.., N, K/G], one for G consecutive weights of a row; G = 32, 64 or a multiple of 128
-    zeros  uint8 [.., N, K/G], 0..15, or None: 8 everywhere
+    zeros  uint8 [.., N, K/G], 0..15, or None: 8 everywhere.  Larger ones, which the kernels would not take alike, are refused: the call waits for the device
+           to look at them, so with zeros it cannot be recorded into a graph
     Returns (A [.., N/16, K/128, 64, 16] uint8, scale and zero [.., N/16, K/max(G,128), 16, max(1,128/G)])."""
     _check(codes.dtype == torch.uint8 and codes.dim() in (2, 3), "codes must be uint8 [N, K/2] or [E, N, K/2]")
     _check(scales.dtype in _KIND, "scales must be fp16 or bf16")
@@ -642,6 +643,7 @@ def pack_layout_a_w4(codes, scales, zeros=None):
     group = k // groups
     _check(group in (32, 64) or group % 128 == 0, "the group must be 32, 64 or a multiple of 128")
     _check(zeros is None or zeros.shape == scales.shape, "zeros must have the shape of scales")
+    _check(zeros is None or zeros.numel() == 0 or int(zeros.max()) <= 15, "zeros must be 0..15")
     _check_tensors(((codes, "codes"), (scales, "scales"), (zeros, "zeros")), codes.device)
     batch = codes.shape[0] if codes.dim() == 3 else 1
     per = max(1, 128 // group)

@@ -201,3 +201,12 @@ def test_c_interface_of_the_balance_loss_refuses():
         a = dict(topk_ids=FAKE, token_mask=None, n_tokens=4, topk=2, n_experts=8, accumulate=0, counts=FAKE, workspace=None, stream=None)
         a.update(kw)
         said(lib, lib.mlk_expert_counts(*a.values()), word)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_zero_points_that_take_more_than_four_bits_are_refused(device):
+    codes, s = torch.zeros(3, 32, 128, dtype=U8, device=device), torch.ones(3, 32, 2, dtype=BF, device=device)
+    for wrong in (16, 255):
+        z = torch.full((3, 32, 2), 15, dtype=U8, device=device)
+        z[2, 31, 1] = wrong
+        refused("0..15", mlk.pack_layout_a_w4, codes, s, z)
