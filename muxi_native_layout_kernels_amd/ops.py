@@ -13,6 +13,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib, arg_selector
 
@@ -1066,6 +1067,10 @@ def _balance_launch(logits, ids, mask, cu, score_fun, coef, plan):
     return loss, counts, share
 
 
+def _check_no_tangent(t):
+    _check(unpack_dual(t).tangent is None, "moe_balance_loss: there is no forward-mode derivative")
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, mask, cu, score_fun, coef, plan):
@@ -1100,6 +1105,7 @@ class _FirstDerivative(torch.autograd.Function):
 def _balance_backward(ctx, dloss):
     if dloss is None:
         return None, None, None, None, None, None, None
+    _check_no_tangent(dloss)
     logits, mask, cu, share = ctx.saved_tensors
     if logits.get_device() != torch.cuda.current_device():
         with torch.cuda.device(logits.device):
@@ -1128,9 +1134,11 @@ def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0,
 
     gating_output [T, E] fp16 / bf16 / fp32, E <= 256; experts_ids int32 [T, K] (`fused_routing_gate`); token_mask bool [T], False for padded
     tokens; cu_seqlens int32 [sequences + 1] on the device, non-decreasing, where each sequence begins and the last one ends (None: all tokens are
-    one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0.  A second derivative is refused.
+    one).  Masked rows and rows outside the sequences may hold anything; their gradient is 0.  A second derivative
+    and a derivative in forward mode are refused.
     Both passes may be recorded into a HIP graph, once run on its stream; as with any torch function no earlier loss of the same leaf may then be alive."""
     logits = gating_output
+    _check_no_tangent(logits)
     key = ("balance", logits.shape, logits.dtype, logits.get_device(), experts_ids.shape, experts_ids.dtype, experts_ids.get_device(),
            None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.get_device()),
            None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.dtype, cu_seqlens.get_device()))

@@ -198,3 +198,28 @@ def test_a_second_derivative_is_refused(mlk):
     with torch.no_grad():
         quiet, _ = mlk.moe_balance_loss(leaf, ids.cuda())
     assert not quiet.requires_grad and torch.equal(quiet, loss.detach())
+
+
+def test_forward_mode_is_refused(mlk):
+    """A tangent would be dropped: of the logits, of the gradient that comes in.  A plain tensor in a dual level is as good as outside."""
+    from torch.autograd import forward_ad
+    logits, ids = case(40, 16, 2, torch.float32, 7)
+    logits, ids = logits.cuda(), ids.cuda()
+    want = mlk.moe_balance_loss(logits, ids)[0]
+    leaf = logits.clone().requires_grad_(True)
+    with forward_ad.dual_level():
+        assert torch.equal(mlk.moe_balance_loss(logits, ids)[0], want)
+        for x in (logits, leaf):
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                mlk.moe_balance_loss(dual, ids)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                mlk.moe_balance_loss(dual, ids)
+        loss, _ = mlk.moe_balance_loss(leaf, ids)
+        up = forward_ad.make_dual(torch.ones((), device="cuda"), torch.ones((), device="cuda"))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(loss, leaf, grad_outputs=up)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: mlk.moe_balance_loss(x, ids)[0], (logits,), (torch.ones_like(logits),))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: mlk.moe_balance_loss(x, ids)[0])(logits)

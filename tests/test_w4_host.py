@@ -210,3 +210,11 @@ def test_zero_points_that_take_more_than_four_bits_are_refused(device):
         z = torch.full((3, 32, 2), 15, dtype=U8, device=device)
         z[2, 31, 1] = wrong
         refused("0..15", mlk.pack_layout_a_w4, codes, s, z)
+
+
+def test_balance_loss_refuses_forward_mode():
+    from torch.autograd import forward_ad
+    logits, ids = torch.zeros(5, 8), torch.zeros(5, 2, dtype=torch.int32)
+    with forward_ad.dual_level():
+        refused("forward-mode", mlk.moe_balance_loss, forward_ad.make_dual(logits, torch.ones(5, 8)), ids)
+        refused("CUDA", mlk.moe_balance_loss, logits, ids)
