@@ -134,9 +134,9 @@ __device__ __forceinline__ float bal_wave_sum(float v) {
     return v;
 }
 
-// Probabilities of one token (0 beyond the last expert); `sig`: the sigmoids.
+// Probabilities of one token (0 beyond the last expert); `rest`: 1 - sigmoid, 1 for softmax.  From e^-|x|, so that neither loses the bits of what is near 0.
 template <int LPT, int NV>
-__device__ __forceinline__ void bal_probs(const BalanceArgs &p, int l, const float (&x)[NV][4], float (&pr)[NV][4], float (&sig)[NV][4]) {
+__device__ __forceinline__ void bal_probs(const BalanceArgs &p, int l, const float (&x)[NV][4], float (&pr)[NV][4], float (&rest)[NV][4]) {
     float sum = 0.f, m = -INFINITY;
     if (p.score_fun == 0) {
 #pragma unroll
@@ -152,12 +152,14 @@ __device__ __forceinline__ void bal_probs(const BalanceArgs &p, int l, const flo
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool is = bal_expert<LPT>(v, l) + i < p.E;
-            sig[v][i] = 0.f;
+            rest[v][i] = 1.f;
             if (p.score_fun == 0) {
                 pr[v][i] = is ? expf(x[v][i] - m) : 0.f;
             } else {
-                sig[v][i] = is ? 1.f / (1.f + expf(-x[v][i])) : 0.f;
-                pr[v][i] = sig[v][i];
+                const float a = expf(-fabsf(x[v][i])), r = 1.f / (1.f + a);
+                const bool up = x[v][i] >= 0.f;
+                rest[v][i] = up ? a * r : r;
+                pr[v][i] = is ? (up ? r : a * r) : 0.f;
             }
             sum += pr[v][i];
         }
@@ -218,13 +220,13 @@ __global__ void __launch_bounds__(kBalThreads) balance_partial_kernel(BalanceArg
         float sum[NV][4] = {};
         int n = 0;
         for (int t = a + row; t < b; t += ROWS) {
-            float x[NV][4], pr[NV][4], sig[NV][4];
+            float x[NV][4], pr[NV][4], rest[NV][4];
             bal_unpack<L, NV, VEC>(next, x);
             const bool is = next_is;
             bal_load<L, LPT, NV, VEC>(p, min(t + ROWS, b - 1), l, next);
             next_is = bal_counts(p, min(t + ROWS, b - 1));
             if (!is) continue;                              // the lanes of a token agree
-            bal_probs<LPT, NV>(p, l, x, pr, sig);
+            bal_probs<LPT, NV>(p, l, x, pr, rest);
             ++n;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
@@ -385,8 +387,8 @@ __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(BalanceArgs p
             enter();
         }
         if (is && a <= t && t < b) {
-            float pr[NV][4], sig[NV][4];
-            bal_probs<LPT, NV>(p, l, x, pr, sig);
+            float pr[NV][4], rest[NV][4];
+            bal_probs<LPT, NV>(p, l, x, pr, rest);
             float dot = 0.f;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(BalanceArgs p
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[v][i] = pr[v][i] * (1.f - sig[v][i]) * (g[v][i] - dot) * up;
+                for (int i = 0; i < 4; ++i) d[v][i] = pr[v][i] * rest[v][i] * (g[v][i] - dot) * up;
         }
         typename L::V1 *out = reinterpret_cast<typename L::V1 *>(p.dlogits) + (size_t)t * p.E;
 #pragma unroll

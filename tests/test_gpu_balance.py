@@ -223,3 +223,24 @@ def test_forward_mode_is_refused(mlk):
         torch.func.jvp(lambda x: mlk.moe_balance_loss(x, ids)[0], (logits,), (torch.ones_like(logits),))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda x: mlk.moe_balance_loss(x, ids)[0])(logits)
+
+
+def relative(mlk, logits, ids, E):
+    """The largest error of the gradient's elements relative to their own size, where g - sum p g is not small against g (its own rounding counts there)."""
+    leaf = logits.cuda().requires_grad_(True)
+    loss, _ = mlk.moe_balance_loss(leaf, ids.cuda(), "sigmoid")
+    grad, = torch.autograd.grad(loss, leaf)
+    want, _, d, p, g = expected(logits, ids, True, 1.0, None, None)
+    assert abs(loss.item() - want) <= 2e-5 * want
+    clear = ((g - (p * g).sum(dim=-1, keepdim=True)).abs() > 0.1 * g.max()) & (d.abs() > 1e-30)
+    assert clear.sum() > 100
+    return ((grad.cpu().double() - d).abs() / d.abs())[clear].max().item()
+
+
+def test_sigmoid_saturated_upwards(mlk):
+    """1 - sigmoid of logits up to 15 keeps its bits: a gradient is a product of p, that and g - sum p g, each good to some ten roundings, of the last
+    of which a tenth of g may remain: 200 * 2^-24."""
+    T, E, K = 60, 16, 2
+    logits, ids = case(T, E, K, torch.float32, 11)
+    ids[:] = torch.tensor([3, 5], dtype=torch.int32)             # shares far apart
+    assert relative(mlk, logits + 0.2 * torch.arange(T).unsqueeze(1), ids, E) <= 200 * 2.0 ** -24
