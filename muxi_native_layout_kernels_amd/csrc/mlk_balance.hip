@@ -4,7 +4,7 @@
 //   c[s,e] = pairs of V_s routed to e,   P[s,e] = sum over V_s of p[t,e],   g[s,e] = coef / S' * E / (K n_s^2) * c[s,e],   loss = sum g P
 // with p = softmax(x) or sigmoid(x) / sum sigmoid(x); the counts are constants of the differentiation, so dloss/dp[t,e] = g[s(t),e] and
 //   softmax  dx = p (g - sum p g),      sigmoid  dx = p (1 - sigmoid) (g - sum p g).
-// A row whose probabilities sum to nothing (all logits -inf) has p = 0.
+// A row of logits that are all -inf has p = 0.
 //
 // Forward: a workgroup takes a chunk of consecutive tokens and walks the sequences that it meets; 4 to 16 lanes hold a token, 4 to 16 experts each, so that
 // a wave takes at least four tokens at a time and a sum over the experts is at most four exchanges within 16 lanes.  Its sums for (chunk c, sequence s)
@@ -134,19 +134,20 @@ __device__ __forceinline__ float bal_wave_sum(float v) {
     return v;
 }
 
-// Probabilities of one token (0 beyond the last expert); `rest`: 1 - sigmoid, 1 for softmax.  From e^-|x|, so that neither loses the bits of what is near 0.
+// Probabilities of one token (0 beyond the last expert); `rest`: 1 - sigmoid, 1 for softmax.  Sigmoids from e^-|x|, so that neither loses the bits of what is near 0.  Where all
+// logits are below 0 only what the sigmoids are to each other matters, and e^(x - max) / (1 + e^x) says it also where they would underflow.
 template <int LPT, int NV>
 __device__ __forceinline__ void bal_probs(const BalanceArgs &p, int l, const float (&x)[NV][4], float (&pr)[NV][4], float (&rest)[NV][4]) {
     float sum = 0.f, m = -INFINITY;
-    if (p.score_fun == 0) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (bal_expert<LPT>(v, l) + i < p.E) m = fmaxf(m, x[v][i]);
-        m = bal_max<LPT>(m);
-        if (m == -INFINITY) m = 0.f;
-    }
+        for (int i = 0; i < 4; ++i)
+            if (bal_expert<LPT>(v, l) + i < p.E) m = fmaxf(m, x[v][i]);
+    m = bal_max<LPT>(m);
+    if (m == -INFINITY) m = 0.f;
+    if (p.score_fun != 0) m = fminf(m, 0.f);
+    const float em = expf(m);                             // of sigmoids
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -156,10 +157,10 @@ __device__ __forceinline__ void bal_probs(const BalanceArgs &p, int l, const flo
             if (p.score_fun == 0) {
                 pr[v][i] = is ? expf(x[v][i] - m) : 0.f;
             } else {
-                const float a = expf(-fabsf(x[v][i])), r = 1.f / (1.f + a);
-                const bool up = x[v][i] >= 0.f;
-                rest[v][i] = up ? a * r : r;
-                pr[v][i] = is ? (up ? r : a * r) : 0.f;
+                const bool up = x[v][i] >= 0.f;           // then m = 0
+                const float e = expf(-fabsf(x[v][i]) - m), r = 1.f / fmaf(e, em, 1.f), er = e * r;
+                rest[v][i] = up ? er : r;
+                pr[v][i] = is ? (up ? r : er) : 0.f;
             }
             sum += pr[v][i];
         }

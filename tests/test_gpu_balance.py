@@ -244,3 +244,24 @@ def test_sigmoid_saturated_upwards(mlk):
     logits, ids = case(T, E, K, torch.float32, 11)
     ids[:] = torch.tensor([3, 5], dtype=torch.int32)             # shares far apart
     assert relative(mlk, logits + 0.2 * torch.arange(T).unsqueeze(1), ids, E) <= 200 * 2.0 ** -24
+
+
+def test_sigmoid_far_below_zero(mlk):
+    """Sigmoids over their sum are a distribution however small they are: rows around -20 to -500, where fp32 has no such sigmoids; tolerance as above, and the logits' own
+    rounding in x - max, which is exact."""
+    T, E, K = 60, 16, 2
+    logits, ids = case(T, E, K, torch.float32, 12)
+    ids[:] = torch.tensor([3, 5], dtype=torch.int32)
+    below = torch.cat((torch.linspace(-20, -110, 40), torch.linspace(-120, -500, 20))).unsqueeze(1)
+    logits = logits + below
+    assert relative(mlk, logits, ids, E) <= 200 * 2.0 ** -24
+    logits[5:10, 8:] = float("-inf")                     # some experts out of the question
+    logits[30:35, 8:] = float("-inf")
+    logits[50:55, 8:] = float("-inf")
+    assert relative(mlk, logits, ids, E) <= 200 * 2.0 ** -24
+    logits[35] = torch.tensor([-100.0] * 15 + [3.0])     # one expert takes all
+    check(mlk, logits, ids, True)
+    for dtype in (torch.float16, torch.bfloat16):
+        check(mlk, logits.to(dtype), ids, True, up=65536.0 if dtype == torch.float16 else 1.0)
+    check(mlk, torch.full((7, 8), -95.0), torch.zeros((7, 2), dtype=torch.int32), True)
+    check(mlk, torch.full((7, 256), -3.0e38), torch.zeros((7, 2), dtype=torch.int32))
