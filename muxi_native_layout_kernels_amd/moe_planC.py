@@ -111,8 +111,7 @@ def fused_moe(
                "n_groups must divide the number of experts")
     ops._check(1 <= topk_group <= num_expert_group, "topK_groups must be in 1..n_groups")
     ops._check(1 <= topk <= min(32, n_router_experts), "topK must be in 1..min(32, experts)")
-    if gating_bias is not None:
-        ops._check(gating_bias.dtype == gating_output.dtype, "Mismatched dtypes: load_balance_bias and gating_output.")
+    ops._check_gating_bias(gating_bias, gating_output)
     topk_ids, topk_weights = _routing_buffers(B, topk, hidden_states.dtype, hidden_states.device)
 
     if w1.dim() == 5:

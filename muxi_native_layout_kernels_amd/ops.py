@@ -755,6 +755,14 @@ def gemv_layoutA_w4(A, A_Scale, B, A_Zero=None, alpha=1, beta=0, bias=None):
 
 
 # ----------------------------------------------------------------------- MoE
+def _check_gating_bias(bias, gating_output):
+    """The router reads one element for every expert."""
+    if bias is not None:
+        _check(bias.dtype == gating_output.dtype, "Mismatched dtypes: load_balance_bias and gating_output.")
+        _check(bias.numel() >= gating_output.size(-1), "load_balance_bias must have an element for every expert")
+        _check(bias.device == gating_output.device and bias.is_contiguous(), "load_balance_bias must be contiguous and on gating_output's device")
+
+
 def fused_routing_gate(gating_output, score_fun, batch_size, hidden_size, n_groups, topK_groups, experts_ids,
                        selected_experts_weights, topK, load_balance_bias=None, renormalize=False):
     """Router: writes `experts_ids` (int32 [T, K]) and `selected_experts_weights` ([T, K]) in place and
@@ -762,9 +770,7 @@ def fused_routing_gate(gating_output, score_fun, batch_size, hidden_size, n_grou
     leaves the division to its Python caller (muxi_moe_planC.py:69-70)."""
     _check(gating_output.dtype == selected_experts_weights.dtype,
            "Mismatched dtypes: gating_output and selected_experts_weights.")
-    if load_balance_bias is not None:
-        _check(load_balance_bias.dtype == gating_output.dtype,
-               "Mismatched dtypes: load_balance_bias and gating_output.")
+    _check_gating_bias(load_balance_bias, gating_output)
     _check(gating_output.dtype in _KIND, "Invalid dtype for gating_output: must be kFloat16 or kBFloat16.")
     _check(experts_ids.dtype == torch.int32, "Invalid dtype for experts_ids: must be kInt32.")
     _check(experts_ids.device == selected_experts_weights.device,

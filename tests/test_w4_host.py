@@ -218,3 +218,17 @@ def test_balance_loss_refuses_forward_mode():
     with forward_ad.dual_level():
         refused("forward-mode", mlk.moe_balance_loss, forward_ad.make_dual(logits, torch.ones(5, 8)), ids)
         refused("CUDA", mlk.moe_balance_loss, logits, ids)
+
+
+def test_router_refuses_a_bias_that_it_would_read_past():
+    """Short, strided, of another type or elsewhere: said before the logits are looked at on the device."""
+    logits, ids, wts = torch.zeros(3, 8, dtype=BF), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2, dtype=BF)
+
+    def call(bias):
+        return mlk.fused_routing_gate(logits, 0, 3, 128, 1, 1, ids, wts, 2, bias, True)
+    refused("every expert", call, torch.zeros(7, dtype=BF))
+    refused("contiguous", call, torch.zeros(16, dtype=BF)[::2])
+    refused("contiguous", call, torch.zeros(8, dtype=BF, device="meta"))
+    refused("Mismatched dtypes", call, torch.zeros(8))
+    refused("CUDA", call, torch.zeros(8, dtype=BF))
+    refused("CUDA", call, torch.zeros(1, 8, dtype=BF))
