@@ -185,17 +185,24 @@ def fused_moe_w4(
     if score_func not in ("softmax", "sigmoid"):
         raise ValueError("Unsupported scoring function")
     ops._check(hidden_states.dim() == 2 and gating_output.dim() == 2 and hidden_states.shape[0] == gating_output.shape[0], "Number of tokens mismatch")
-    ops._check(hidden_states.is_cuda and hidden_states.device == gating_output.device, "hidden_states and gating_output must be on the same CUDA device")
     ops._check(hidden_states.dtype in ops._KIND and gating_output.dtype == hidden_states.dtype, "gating_output must have the activation dtype")
     ops._check(gating_output.shape[1] == (w1.shape[0] if experts_map is None else experts_map.numel()),
                "gating_output must have one column per expert of w1, or per entry of experts_map")
+    n_experts = gating_output.shape[1]
+    ops._check_gating_bias(gating_bias, gating_output)
+    ops._check(expert_load is None or (expert_load.dtype == torch.int32 and tuple(expert_load.shape) == (n_experts,)), "expert_load must be int32 [n_experts]")
+    ops._check(hidden_states.is_cuda and hidden_states.device == gating_output.device, "hidden_states and gating_output must be on the same CUDA device")
+    ops._check_tensors(((gating_output, "gating_output"), (expert_load, "expert_load")), hidden_states.device)
     with ops._OnDevice(hidden_states):
         topk_ids, topk_weights = _routing_buffers(hidden_states.shape[0], topk, hidden_states.dtype, hidden_states.device,
                                                   ops._stream_of(hidden_states))
+        # every check of the experts ahead of the router: a call that is refused launches nothing
+        plan = ops._experts_w4_plan(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
+        ops._check_experts_w4_aligned(w1, w2, w1_scale, w2_scale, w1_zero, w2_zero)
         if hidden_states.shape[0] > 0:
             ops.fused_routing_gate(gating_output, 0 if score_func == "softmax" else 1, hidden_states.shape[0], hidden_states.shape[1], num_expert_group,
                                    topk_group, topk_ids, topk_weights, topk, gating_bias, renormalize)
-        y = ops.fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
-        if expert_load is not None:                                    # last: a call that is refused counts nothing
-            ops.expert_counts(topk_ids, gating_output.shape[1], out=expert_load)
+        y = ops._experts_w4_launch(plan, hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
+        if expert_load is not None:
+            ops.expert_counts(topk_ids, n_experts, out=expert_load)
     return y

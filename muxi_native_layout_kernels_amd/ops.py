@@ -954,7 +954,18 @@ def fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2
     the router]: the expert's place in w1 / w2, -1 = on another card.  Ids outside the router's experts are dropped too; a token without an expert here
     gets zeros.  Returns y [T, H].  fp32 sums; the SiLU intermediate is rounded to the activation dtype, which the second product's matrix
     instructions take."""
-    x = hidden_states
+    plan = _experts_w4_plan(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
+    return _experts_w4_launch(plan, hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
+
+
+def _check_experts_w4_aligned(w1, w2, w1_scale, w2_scale, w1_zero, w2_zero):
+    """What the library would say of them, for a caller that launches something ahead of it."""
+    _check(((w1.data_ptr() | w2.data_ptr()) & 15) == 0, "w1 and w2 must lie on 16 bytes")
+    _check(((w1_scale.data_ptr() | w2_scale.data_ptr()) & 7) == 0, "scales must lie on 8 bytes")
+    _check(((_ptr(w1_zero) | _ptr(w2_zero)) & 3) == 0, "zero points must lie on 4 bytes")
+
+
+def _experts_w4_plan(x, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map):
     key = ("experts_w4", x.shape, w1.shape, w2.shape, topk_ids.shape, topk_weights.shape, w1_scale.shape, w2_scale.shape, x.dtype, w1.dtype, w2.dtype,
            topk_ids.dtype, topk_weights.dtype, w1_scale.dtype, w2_scale.dtype, x.device, w1.device, w2.device, topk_ids.device, topk_weights.device,
            w1_scale.device, w2_scale.device,
@@ -972,6 +983,7 @@ def fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2
         _check(group == group2, "w1 and w2 must have the same group size")
         _check((w1_zero is None) == (w2_zero is None), "zero points for both w1 and w2 or for none")
         _check(inter % 128 == 0 and hidden % 128 == 0, "hidden and intermediate sizes must be multiples of 128")
+        _check(max(hidden, inter) < 1 << 23, "hidden and intermediate sizes must be below 2^23")
         _check(1 <= E <= 256, "at most 256 experts")
         _check(x.dim() == 2 and x.size(1) == hidden, "hidden_states must be [T, H]")
         _check(x.dtype in _KIND, "hidden_states must be fp16 or bf16")
@@ -988,6 +1000,10 @@ def fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2
         E_router = E if experts_map is None else experts_map.numel()
         plan = _plans[key] = (x.size(0), E, E_router, K, hidden, inter, group, _KIND[x.dtype],
                               lib.mlk_experts_w4_workspace_bytes(x.size(0), E, E_router, K, hidden, inter, group), lib.mlk_fused_experts_w4)
+    return plan
+
+
+def _experts_w4_launch(plan, x, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map):
     T, E, E_router, K, hidden, inter, group, kind, ws_need, fn = plan
     with _OnDevice(x):
         if x.data_ptr() & 15:

@@ -449,3 +449,42 @@ def test_a_share_of_the_experts_whatever_comes(mlk, T, E, held, K, here):
     ids = ids.int().contiguous()
     y = mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2, experts_map=emap.cuda())
     check_experts(y, expected_experts(x, w1, w2, p1[1], p2[1], ids, wts, emap), BF, "experts here")
+
+
+def test_a_refused_layer_launches_nothing(mlk, monkeypatch):
+    """Whatever is wrong with the experts, the bias or the load is said ahead of the router."""
+    from muxi_layout_kernels.muxi_moe_planC import fused_moe_w4
+    p1, p2, _, _ = layer(4, 128, 128, 64, BF, True, 1)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    x, logits = randn((3, 128), BF, 1.0, 1).cuda(), randn((3, 4), BF, 1.0, 2).cuda()
+    load, bias = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=BF, device="cuda")
+    launched = []
+    real = mlk.ops.fused_routing_gate
+    monkeypatch.setattr(mlk.ops, "fused_routing_gate", lambda *a, **k: launched.append(1) or real(*a, **k))
+
+    def off(t, by):                                      # the same, so many bytes past 16
+        flat = torch.empty(t.numel() * t.element_size() + 16, dtype=torch.uint8, device="cuda")[by:by + t.numel() * t.element_size()].view(t.dtype)
+        return flat.view(t.shape).copy_(t)
+
+    def call(match, w1=a1, w2=a2, s1=s1, s2=s2, z1=z1, z2=z2, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            fused_moe_w4(x, w1, w2, logits, 2, True, s1, s2, z1, z2, **kw)
+        assert not launched, match
+    call("both w1 and w2", z2=None)
+    call("scales of w2", s2=s2[:, :, :, :8].contiguous())
+    call("activation dtype", s1=s1.half(), s2=s2.half())
+    call("CUDA", w2=a2.cpu())
+    call("contiguous", w1=a1.transpose(-1, -2).contiguous().transpose(-1, -2))
+    call("16 bytes", w1=off(a1, 8))
+    call("8 bytes", s2=off(s2, 4))
+    call("on 4", z1=off(z1, 2))
+    call("experts_map", experts_map=torch.zeros(4, dtype=torch.int64, device="cuda"))
+    call("n_experts", expert_load=load[:3])
+    call("n_experts", expert_load=load.long())
+    call("CUDA", expert_load=load.cpu())
+    call("contiguous", expert_load=torch.zeros(8, dtype=torch.int32, device="cuda")[::2])
+    call("every expert", gating_bias=bias[:3])
+    call("device", gating_bias=bias.cpu())
+    call("contiguous", gating_bias=torch.zeros(8, dtype=BF, device="cuda")[::2])
+    fused_moe_w4(x, a1, a2, logits, 2, True, s1, s2, z1, z2, gating_bias=bias, expert_load=load)
+    assert launched == [1] and load.sum() == 6

@@ -232,3 +232,17 @@ def test_router_refuses_a_bias_that_it_would_read_past():
     refused("Mismatched dtypes", call, torch.zeros(8))
     refused("CUDA", call, torch.zeros(8, dtype=BF))
     refused("CUDA", call, torch.zeros(1, 8, dtype=BF))
+
+
+def test_layer_refuses_its_own_arguments():
+    from muxi_native_layout_kernels_amd.moe_planC import fused_moe_w4
+    (w1, s1, z1), (w2, s2, z2) = packed(512, 128, 64, (4,)), packed(128, 256, 64, (4,))
+    x, logits = torch.zeros(3, 128, dtype=BF), torch.zeros(3, 4, dtype=BF)
+
+    def call(**kw):
+        return fused_moe_w4(x, w1, w2, logits, 2, True, s1, s2, z1, z2, **kw)
+    refused("n_experts", call, expert_load=torch.zeros(3, dtype=torch.int32))
+    refused("n_experts", call, expert_load=torch.zeros(4, dtype=torch.int64))
+    refused("n_experts", call, expert_load=torch.zeros(1, 4, dtype=torch.int32))
+    refused("every expert", call, gating_bias=torch.zeros(3, dtype=BF))
+    refused("CUDA", call, gating_bias=torch.zeros(4, dtype=BF), expert_load=torch.zeros(4, dtype=torch.int32))
