@@ -363,7 +363,8 @@ int mlk_moe_pass_plan(int n_tokens, int n_experts, int topk, int hidden, int int
                       int32_t *out);
 
 /* Expert compute over 4-bit weights from a routing decision: y[t] = T(sum over the token's pairs of weight * W2[e] . (SiLU(gate) * up)),
- * gate and up from W1[e] . x[t], fp32 sums, the SiLU intermediate rounded to the activations' kind.  w1 [E, 2I, H] and w2 [E, H, I], each
+ * gate and up from W1[e] . x[t], fp32 sums, the SiLU intermediate rounded to the activations' kind: a token with an infinity, or whose
+ * intermediate passes that kind's range (fp16: 65504), gives a row of NaN.  w1 [E, 2I, H] and w2 [E, H, I], each
  * expert packed by mlk_pack_layout_a_w4 / mlk_pack_scales_w4 (batch = E), of one group size G = 32, 64 or a multiple of 128 that divides H
  * and I; w1_zero and w2_zero both or neither.  topk_ids int32 [T*K], ids outside 0..n_router_experts-1 are dropped; experts_map int32
  * [n_router_experts] or NULL (n_router_experts == n_experts): -1 drops the pair.  topk_weights [T*K] of x_kind.  y is overwritten, a token

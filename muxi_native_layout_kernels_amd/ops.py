@@ -953,7 +953,7 @@ def fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2
     points from `pack_layout_a_w4`; topk_ids int32 [T, K], topk_weights [T, K] of the activation dtype; experts_map int32 [experts of
     the router]: the expert's place in w1 / w2, -1 = on another card.  Ids outside the router's experts are dropped too; a token without an expert here
     gets zeros.  Returns y [T, H].  fp32 sums; the SiLU intermediate is rounded to the activation dtype, which the second product's matrix
-    instructions take."""
+    instructions take, as in `fused_moe`.  A token with an infinity, or whose intermediate passes the range of that type (fp16: 65504), gives a row of NaN; other rows keep theirs."""
     plan = _experts_w4_plan(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
     return _experts_w4_launch(plan, hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
 

@@ -134,3 +134,21 @@ def test_layer_router_counts_and_experts_together(mlk):
         assert torch.equal(counts.cpu().long(), torch.bincount(ids.cpu().flatten().long(), minlength=E))
         assert torch.isfinite(loss)
     assert torch.equal(load.cpu().long(), total)
+
+
+@pytest.mark.parametrize("T", [1, 5, 40, 400])
+def test_an_intermediate_past_the_range_of_fp16_is_nan_in_its_row(mlk, T):
+    """A gate and an up of some hundred each: their product has no place in fp16.  One token, few, tasks of two blocks, panels."""
+    E, K, H, I, dtype = 6, 2, 256, 256, torch.float16
+    p1, p2, w1, _ = layer(E, H, I, 128, dtype, True, 1)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    x, (ids, wts) = randn((T, H), dtype, 1.0, T), routing(T, E, K, dtype, T)
+    call = lambda: mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2)
+    clean = call()
+    assert torch.isfinite(clean).all()
+    t = T // 2
+    x[t] *= 2000.0
+    g, u = (w1[ids[t, 0].long()] @ x[t].double()).split(I)
+    assert torch.isfinite(x).all() and (g * torch.sigmoid(g) * u).abs().max() > 2 * 65504
+    got = call()
+    assert got[t].isnan().all() and torch.equal(got[:t], clean[:t]) and torch.equal(got[t + 1:], clean[t + 1:])
