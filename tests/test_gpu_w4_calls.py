@@ -488,3 +488,21 @@ def test_a_refused_layer_launches_nothing(mlk, monkeypatch):
     call("contiguous", gating_bias=torch.zeros(8, dtype=BF, device="cuda")[::2])
     fused_moe_w4(x, a1, a2, logits, 2, True, s1, s2, z1, z2, gating_bias=bias, expert_load=load)
     assert launched == [1] and load.sum() == 6
+
+
+@pytest.mark.parametrize("group,zeros,dtype", [(128, False, BF), (32, True, HF), (64, True, BF)])
+@pytest.mark.parametrize("dropped", [False, True])
+def test_one_token_whose_intermediates_pass_128_kib(mlk, group, zeros, dtype, dropped):
+    """Eight picks of 8320: the down projection reads them from memory, not from LDS."""
+    E, K, H, I = 8, 8, 128, 8320
+    assert 2 * K * I > 128 * 1024
+    p1, p2, w1, w2 = layer(E, H, I, group, dtype, zeros, 3)
+    (a1, s1, z1), (a2, s2, z2) = mlk.pack_layout_a_w4(*on_gpu(*p1)), mlk.pack_layout_a_w4(*on_gpu(*p2))
+    x, (ids, wts) = randn((1, H), dtype, 1.0, 5), routing(1, E, K, dtype, 5)
+    if dropped:
+        ids[0, 3], ids[0, 7] = -1, ids[0, 6]             # nobody's, and one expert twice
+    got = mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2)
+    check_experts(got, expected_experts(x, w1, w2, p1[1], p2[1], ids, wts), dtype, "one token")
+    assert torch.equal(got, mlk.fused_experts_w4(x.cuda(), a1, a2, ids.cuda(), wts.cuda(), s1, s2, z1, z2))
+    gone = torch.full_like(ids, -1)
+    assert (mlk.fused_experts_w4(x.cuda(), a1, a2, gone.cuda(), wts.cuda(), s1, s2, z1, z2) == 0).all()
