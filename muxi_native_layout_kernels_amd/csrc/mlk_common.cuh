@@ -134,6 +134,9 @@ __device__ __forceinline__ void fp8x4_to_bf16x4_pow2(uint32_t w, float scale, ui
     hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, scale, true));
 }
 
+// Front of the workspace that all GeMMs of a stream share: arrival counters, zero between calls (mlk_gemm_counter_bytes()).
+constexpr size_t kCounterBytes = 64 * 1024;
+
 // One row of block scales (one fp32 per 128 k) kept in registers: lane l of register i holds
 // the scale of k block 64 i + l.  scale_at() fetches a wave-uniform entry with v_readlane, so
 // the streaming loops never wait on memory for a scale.  Covers K <= 32768.

@@ -7,8 +7,6 @@
 
 namespace mlk {
 
-constexpr size_t kCounterBytes = 64 * 1024;
-
 // Scratch of mlk_gemm_layout_a_noalloc(): arrival counters and fp32 partials of the cross-workgroup K splits,
 // for callers that can neither allocate nor pass a workspace.  One copy per GPU, held until the process ends.
 // The array has no initialiser, so it is zero-filled when the code object is loaded onto a device, and the K-split

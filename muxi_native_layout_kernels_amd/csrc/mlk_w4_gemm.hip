@@ -18,8 +18,6 @@ MLK_W4_EXTERN(BF16, 2)
 MLK_W4_EXTERN(BF16, 1)
 #undef MLK_W4_EXTERN
 
-constexpr size_t kW4CounterBytes = 64 * 1024;      // the front of the workspace that the GeMMs share
-
 struct W4Plan {
     int r, tt, wgs, waves;  // streaming kernels: row groups and blocks of 16 tokens of a workgroup
     int tb;                 // panels: blocks of 32 tokens; 0: streaming kernels
@@ -250,7 +248,7 @@ int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, con
     MLK_REQUIRE(((uintptr_t)scale & 7) == 0 && ((uintptr_t)zero & 3) == 0, "w4 gemm: scales must lie on 8 bytes, zero points on 4");
     const W4Plan pl = w4_plan(m, n, k, group);
     const size_t part = w4_partial_bytes(pl, m, n, k, group);
-    if (part && (!workspace || workspace_bytes < kW4CounterBytes + part)) return fail(MLK_ERR_WORKSPACE, "w4 gemm: workspace too small");
+    if (part && (!workspace || workspace_bytes < kCounterBytes + part)) return fail(MLK_ERR_WORKSPACE, "w4 gemm: workspace too small");
     const W4Matrix w = {(const uint8_t *)a, (const uint16_t *)scale, (const uint8_t *)zero};
     const int blocks = k / (group > 128 ? group : 128);
     const uint32_t inv = w4_inverse(group > 128 ? group / 128 : 1);
@@ -267,8 +265,8 @@ int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, con
         p.blocks = blocks;
         p.inv = inv;
         p.slices = pl.slices;
-        p.sums = (u32x4 *)((uint8_t *)workspace + kW4CounterBytes);
-        p.partial = (float *)((uint8_t *)workspace + kW4CounterBytes + w4_sums_bytes(m, k, group));
+        p.sums = (u32x4 *)((uint8_t *)workspace + kCounterBytes);
+        p.partial = (float *)((uint8_t *)workspace + kCounterBytes + w4_sums_bytes(m, k, group));
         return w4_panel(p, pl.tb, x_kind, group, (hipStream_t)stream);
     }
     W4GemmArgs p = {};
@@ -281,7 +279,7 @@ int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, con
     p.inv = inv;
     p.slices = pl.slices;
     p.counters = part ? (int *)workspace : nullptr;
-    p.partial = part ? (f32x4 *)((uint8_t *)workspace + kW4CounterBytes) : nullptr;
+    p.partial = part ? (f32x4 *)((uint8_t *)workspace + kCounterBytes) : nullptr;
     p.M = m;
     p.X = (const uint16_t *)b;
     p.C = (uint16_t *)c;
@@ -291,7 +289,7 @@ int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, con
 size_t mlk_gemm_w4_workspace_bytes(int m, int n, int k, int group) {
     if (m <= 0 || n <= 0 || k <= 0 || !w4_group_ok(k, group)) return 0;
     const size_t part = w4_partial_bytes(w4_plan(m, n, k, group), m, n, k, group);
-    return part ? kW4CounterBytes + part : 0;
+    return part ? kCounterBytes + part : 0;
 }
 
 }  // extern "C"

@@ -246,3 +246,10 @@ def test_layer_refuses_its_own_arguments():
     refused("n_experts", call, expert_load=torch.zeros(1, 4, dtype=torch.int32))
     refused("every expert", call, gating_bias=torch.zeros(3, dtype=BF))
     refused("CUDA", call, gating_bias=torch.zeros(4, dtype=BF), expert_load=torch.zeros(4, dtype=torch.int32))
+
+
+def test_counters_in_front_of_the_workspace_are_those_of_the_other_products():
+    """One buffer serves them all: behind the counters, 16 tokens through 4096 rows of 14336 keep the partial sums of each slice of k, a whole number of outputs in fp32."""
+    lib = _lib.load()
+    partial = lib.mlk_gemm_w4_workspace_bytes(16, 4096, 14336, 128) - lib.mlk_gemm_counter_bytes()
+    assert partial > 0 and partial % (16 * 4096 * 4) == 0
