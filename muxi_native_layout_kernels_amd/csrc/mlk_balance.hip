@@ -12,9 +12,9 @@
 // sequence in order, for 64 experts a workgroup; the last workgroup adds their shares of the loss.  No floating-point atomics: the results do not depend on
 // the order in which workgroups run.
 // Backward: the same walk, the logits are read again and their gradient written; a lane keeps the shares of its experts until the sequence changes.
-// 32749 tokens x 256 experts in fp32, 9 sequences (33.5 MB: 4.9 us forward, 9.7 backward): 19.4 + 5.8 us forward, 18.4 backward; with 64 lanes of four
-// experts a token and exchanges through LDS 22 and 33, without the next token's logits in flight 23 and 25.  Below about 16384 x 64 bf16 (4.4 + 7.5 and
-// 4.3 us) it is the launches and the dependent loads at a chunk's start.
+// 32749 tokens x 256 experts in fp32, 9 sequences (33.5 MB: 4.9 us forward, 9.7 backward), sigmoid: 20.4 + 6.0 us forward, 20.0 backward (in a graph 22.3 and 17.5 in all, softmax
+// 18.9 and 15.1); with 64 lanes of four experts a token and exchanges through LDS 22 and 33, without the next token's logits in flight 23 and 25, where this form took 19.4 and 18.4.
+// Below about 16384 x 64 bf16 (4.6 + 7.4 and 4.7 us) it is the launches and the dependent loads at a chunk's start.
 #include <algorithm>
 
 #include "mlk_common.cuh"

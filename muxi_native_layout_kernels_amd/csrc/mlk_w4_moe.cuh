@@ -1,8 +1,9 @@
 // Expert layers over 4-bit weights: grouped gate/up product with SiLU(gate) * up, grouped down product, weighted sum.
 //
 // Several tokens: the routed pairs are brought into expert order in blocks of 16 (moe_align_kernel); a task is a block, or up to two (panels: up to
-// eight) of one expert, which share one pass over its weights.  The intermediate is kept row-major [slot][I] in the activations' type (slot = place in the order), the
-// weighted products of the down projection in fp32 [pair][slice][H], and a last launch adds a token's pairs in the order of its picks.
+// eight) of one expert, which share one pass over its weights.  The intermediate is kept row-major [slot][I] in the activations' type (slot = place in the order): the matrix
+// instructions take 16 bits, and a second part for the bits below would double the products and the activations' bytes of the down projection, for errors of one rounding in place of 1.4.  The
+// weighted products of the down projection are kept in fp32 [pair][slice][H], and a last launch adds a token's pairs in the order of its picks.
 // One token: its picks are the tasks, no alignment; the down projection's waves deal the picks among themselves and write the output at once.
 #pragma once
 

@@ -6,7 +6,7 @@
 //   vector instr.   1700   one in 5.6 cycles beside matrix instructions, measured: 64 to widen a wave's weights of a window, which all its token blocks
 //                          share, and 64 to scale the sums of its four blocks
 //   LDS reads       1100   4.3 cycles each, measured: an operand of 32 tokens for every product
-// They overlap (widening, scaling and reads are spread between the products).  Measured at 27648 x 5120, 2048 tokens, groups of 128: 518 us, 1.12 PFLOP/s; the matrix
+// They overlap (widening, scaling and reads are spread between the products).  Measured at 27648 x 5120, 2048 tokens, groups of 128: 512 to 537 us by card, 1.08 to 1.13 PFLOP/s; the matrix
 // cores are busy for 63 % of the cycles, and the card runs at 1.85 GHz under this load (2.4 without it).  Nothing may be added to the loop.  So sum x, which the offset of
 // 16 + q calls for (mlk_w4.cuh), does not come into this loop: as initial values of the products' sums it took another half of the LDS reads
 // (27648 x 5120 at 2048 tokens: 549 us).  It is made by a launch ahead (w4_sums_kernel) and multiplied behind the weights, like 8 more k for every 32, 64 or

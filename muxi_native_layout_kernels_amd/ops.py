@@ -744,7 +744,7 @@ def _w4_launch(plan, A, A_Scale, B, A_Zero, alpha, bias, what):
 def gemm_layoutA_w4(A, A_Scale, B, A_Zero=None, alpha=1, beta=0, bias=None):
     """C[n, m] = alpha * B[n, k] . W^T (+ bias) with 4-bit weights W = s (q - z) from `pack_layout_a_w4`; any n >= 0, m % 16 == 0,
     k % 128 == 0.  fp32 sums, one rounding at the end, no weight rounded.  A row of B that holds an infinity, or bf16 numbers so large that 64
-    times the sum of their magnitudes passes the fp32 range, gives NaN."""
+    times the sum of their magnitudes passes the fp32 range, gives NaN.  No gradient: the result is detached."""
     return _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, "gemm_layoutA_w4")
 
 
@@ -953,7 +953,8 @@ def fused_experts_w4(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2
     points from `pack_layout_a_w4`; topk_ids int32 [T, K], topk_weights [T, K] of the activation dtype; experts_map int32 [experts of
     the router]: the expert's place in w1 / w2, -1 = on another card.  Ids outside the router's experts are dropped too; a token without an expert here
     gets zeros.  Returns y [T, H].  fp32 sums; the SiLU intermediate is rounded to the activation dtype, which the second product's matrix
-    instructions take, as in `fused_moe`.  A token with an infinity, or whose intermediate passes the range of that type (fp16: 65504), gives a row of NaN; other rows keep theirs."""
+    instructions take, as in `fused_moe`.  A token with an infinity, or whose intermediate passes the range of that type (fp16: 65504), gives a row of NaN; other rows keep theirs.
+    No gradient: the result is detached."""
     plan = _experts_w4_plan(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
     return _experts_w4_launch(plan, hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, w1_zero, w2_zero, experts_map)
 
