@@ -41,7 +41,7 @@ extern "C" {
 #define MLK_F16 0
 #define MLK_BF16 1
 #define MLK_FP8_E4M3 2 /* soft-FP8 weights: one e4m3 byte per element */
-#define MLK_F32 3      /* router logits of the balance loss only */
+#define MLK_F32 3      /* router logits of the balance loss and the routing, activations to quantise */
 
 /* output placement of the narrow GeMM */
 #define MLK_C_ROWMAJOR 0 /* C[M, N]                               */
@@ -264,6 +264,22 @@ int mlk_gemm_layout_a_w4(const void *a, const void *scale, const void *zero, con
                          int x_kind, float alpha, const void *bias, void *workspace, size_t workspace_bytes, void *stream);
 size_t mlk_gemm_w4_workspace_bytes(int m, int n, int k, int group);
 
+/* ------------------------------------------------------------- e4m3 products
+ * Weights as the soft-FP8 products take them: e4m3 bytes in layout A with one fp32 scale for 128 x 128 of them, a_scale [ceil(N/128), K/128].  Activations: e4m3 codes
+ * [M, K] with one fp32 scale for 128 of a row.  No counterpart in the reference, whose soft-FP8 products widen the weights and multiply in bf16. */
+
+/* x [n_tokens, K] of x_kind (MLK_F16, MLK_BF16 or MLK_F32) -> codes [n_tokens, K] e4m3 and the scale of block kb of row t at scales[t * scale_t + kb * scale_k]:
+ * the smallest power of two, 2^-100 at least, with max |x| of the block <= 448 * scale; codes are x / scale rounded to nearest even.  Infinities and NaN become the
+ * NaN code and do not count in the maximum.  K % 128 == 0, K < 2^25, at most 2^27 rows; x and codes on 16 bytes. */
+int mlk_quantize_fp8(const void *x, int x_kind, void *codes, float *scales, int64_t scale_t, int64_t scale_k, int64_t n_tokens, int k, void *stream);
+
+/* C[M, N] of c_kind (MLK_F16 or MLK_BF16) = T(alpha * B . W^T (+ bias[N])), any M >= 0, fp32 sums.  b_kind MLK_FP8_E4M3: codes with scales b_scale, row t's block kb at
+ * b_scale[t * b_scale_t + kb * b_scale_k]; else b_kind = c_kind, and the call quantises B as mlk_quantize_fp8 does, into the workspace.  N % 16 == 0, K % 128 == 0,
+ * K < 2^25.  a, b, c and workspace on 16 bytes.  workspace: mlk_gemm_fp8_workspace_bytes() bytes under the rules of mlk_gemm_layout_a; may be NULL where that is 0. */
+int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, int b_kind, const float *b_scale, int64_t b_scale_t, int64_t b_scale_k, void *c,
+                          int c_kind, int m, int n, int k, float alpha, const void *bias, void *workspace, size_t workspace_bytes, void *stream);
+size_t mlk_gemm_fp8_workspace_bytes(int m, int n, int k, int b_kind);
+
 /* ----------------------------------------------------------------------- MoE */
 
 /* Router: scores (score_fun 0 = softmax, 1 = sigmoid), optional correction
@@ -375,6 +391,31 @@ int mlk_fused_experts_w4(const void *w1, const void *w1_scale, const void *w1_ze
                          const int32_t *topk_ids, const void *topk_weights, const int32_t *experts_map, void *y, void *workspace,
                          size_t workspace_bytes, void *stream);
 size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter, int group);
+
+/* Expert compute in e4m3 from a routing decision: x is quantised as mlk_quantize_fp8 does, gate and up are W1[e] . x, SiLU(gate) * up is quantised likewise from fp32, and
+ * y[t] = T(sum over the token's pairs of weight * W2[e] . that), fp32 sums.  w1 [E, 2I, H] and w2 [E, H, I], each expert's e4m3 bytes in layout A, with fp32 scales
+ * w1_scale [E, 2I/128, H/128], w2_scale [E, H/128, I/128].  topk_ids int32 [T*K], ids outside 0..n_router_experts-1 are dropped; experts_map int32
+ * [n_router_experts] or NULL (n_router_experts == n_experts): -1 drops the pair.  topk_weights [T*K] of x_kind.  y is overwritten, a token without experts here
+ * gets zeros, a token with an infinity or NaN a row of NaN.  H % 128 == 0, I % 128 == 0, E <= 256, K <= 32.  w1, w2, x, y and workspace on 16 bytes.  workspace:
+ * at least mlk_experts_fp8_workspace_bytes(), no initialisation. */
+int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2, const float *w2_scale, const void *x, int n_tokens, int n_experts,
+                          int n_router_experts, int topk, int hidden, int inter, int x_kind, const int32_t *topk_ids, const void *topk_weights,
+                          const int32_t *experts_map, void *y, void *workspace, size_t workspace_bytes, void *stream);
+size_t mlk_experts_fp8_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter);
+
+/* ------------------------------------------------------------- routing that trains */
+
+/* Picks of each token, ids int32 [T, K], and their weights [T, K] of x_kind, from logits [T, E] of x_kind (MLK_F16, MLK_BF16 or MLK_F32).  An expert's rank is its logit, or with
+ * `bias` (fp32 [E]) its score + bias in 64 bits; scores are softmax (score_fun 0) or sigmoid (1).  With n_groups > 1 only the topk_groups best groups of consecutive experts stay: by their
+ * largest rank, with a bias by the sum of their two largest.  The K largest ranks are picked, in falling order; ties go to the lower expert, and to the lower group.  Weights are
+ * scaling * score, over the sum of the picks' scores if `renormalize`; fp32, one rounding.  An expert whose logit or bias is -inf or NaN is never picked: where too few are left,
+ * and where token_mask (NULL: none) is 0, ids are -1 and weights 0.  A logit of +inf counts as the largest finite number.  E <= 512, K <= min(32, E), n_groups
+ * divides E, and the kept groups hold K experts at least; T <= 2^30. */
+int mlk_moe_routing(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, int n_groups, int topk_groups, int topk, const float *bias,
+                    int renormalize, float scaling, const uint8_t *token_mask, int32_t *ids, void *weights, void *stream);
+/* dlogits [T, E] of x_kind from the ids that mlk_moe_routing left and the gradient of its weights, dweights [T, K] of x_kind; zeros where the weights do not depend on a logit. */
+int mlk_moe_routing_grad(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, int topk, int renormalize, float scaling, const int32_t *ids,
+                         const void *dweights, void *dlogits, void *stream);
 
 /* ------------------------------------------------------------- router balance */
 

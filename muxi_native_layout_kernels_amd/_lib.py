@@ -56,6 +56,14 @@ SIGNATURES = {
     "mlk_balance_counter_bytes": (c_size_t, []),
     "mlk_balance_loss_grad": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                       c_void_p, c_void_p]),
+    "mlk_quantize_fp8": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "mlk_gemm_layout_a_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_int,
+                                      c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mlk_gemm_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "mlk_fused_experts_fp8": (c_int, [c_void_p] * 5 + [c_int] * 7 + [c_void_p] * 5 + [c_size_t, c_void_p]),
+    "mlk_experts_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "mlk_moe_routing": (c_int, [c_void_p] + [c_int] * 7 + [c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mlk_moe_routing_grad": (c_int, [c_void_p] + [c_int] * 6 + [c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mlk_fused_routing_gate": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
                                        c_void_p, c_void_p, c_void_p]),
     "mlk_moe_align_tokens": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,

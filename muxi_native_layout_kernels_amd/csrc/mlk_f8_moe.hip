@@ -1,0 +1,274 @@
+// Expert layers in e4m3 with block scales: grouped gate/up product with SiLU(gate) * up, grouped down product, weighted sum.
+//
+// The routed pairs are brought into expert order in blocks of 16 (moe_align_kernel); a task is one or two blocks of one expert, which share a pass over its weights.  Activations are
+// quantised once.  A gate/up workgroup computes 128 consecutive intermediate values of its tokens, a block of the next product's activations, so it has their
+// maximum at hand and leaves codes and scale: [slot][I] and [I / 128][slot] (slot = place in the order).  The weighted products of the down projection are kept in fp32
+// [pair][H], and a last launch adds a token's pairs in the order of its picks.
+#include <algorithm>
+#include <initializer_list>
+
+#include "mlk_f8.cuh"
+#include "mlk_moe_args.cuh"
+
+namespace mlk {
+
+int launch_moe_align(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
+                     int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, hipStream_t s);
+
+constexpr int kF8MoePairs = 16384;      // routed pairs of a pass: bounds the scratch of long prompts
+
+struct F8MoeArgs {
+    const uint8_t *w1, *w2;      // of expert 0
+    const float *s1, *s2;
+    const uint8_t *X;            // [T][H] codes
+    const float *xs;             // [H / 128][T]
+    uint16_t *Y;                 // [T][H]
+    const int32_t *ids;          // [T * K]
+    const uint16_t *wts;         // [T * K]
+    const int32_t *map;          // [id_limit] or null
+    int id_limit, T, K, H, I, E, n_pairs, slots;
+    const int32_t *sorted;
+    const MoeTask *tasks;
+    const int32_t *n_tasks;
+    uint8_t *hbuf;               // [slot][I]
+    float *hs;                   // [I / 128][slot]
+    float *obuf;                 // [pair][H]
+};
+
+// Local expert of a pair, -1: dropped.
+__device__ __forceinline__ int f8_expert(const F8MoeArgs &p, int pair) {
+    int e = p.ids[pair];
+    if (e < 0 || e >= p.id_limit) return -1;
+    if (p.map) e = p.map[e];
+    return e >= 0 && e < p.E ? e : -1;
+}
+
+// Gate/up: wave w of eight streams the w-th row group of gate and the same one of up.
+template <int TT>
+__device__ __forceinline__ void f8_gate_up_blocks(const F8MoeArgs &p, const MoeTask &task, float *most) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t16 = lane & 15;
+    const int windows = p.H / kF8K, rg = blockIdx.x * 8 + wave;
+    const uint8_t *w = p.w1 + (size_t)task.expert * 2 * p.I * p.H;
+    const float *s = p.s1 + (size_t)task.expert * (p.I / 64) * windows;
+    F8Rows<2> rows;
+    f8_row(rows, 0, w, s, rg, windows);
+    f8_row(rows, 1, w, s, p.I / 16 + rg, windows);
+    F8Tokens<TT> tokens;
+    tokens.step = p.T;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        const int pair = p.sorted[(task.block0 + tt) * 16 + t16], row = pair < p.n_pairs ? pair / p.K : 0;
+        tokens.x[tt] = p.X + (size_t)row * p.H;
+        tokens.a[tt] = p.xs + row;
+    }
+    f32x4 acc[2][TT];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f8_stream<TT, 2, TT == 1 ? 4 : 2>(acc, rows, tokens, 0, windows, 1, lane);
+    f32x4 h[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            h[tt][i] = silu_mul(acc[0][tt][i], acc[1][tt][i]);
+            a = fmaxf(a, f8_magnitude(h[tt][i]));
+        }
+        a = fmaxf(a, __shfl_xor(a, 16));
+        a = fmaxf(a, __shfl_xor(a, 32));
+        if (lane < 16) most[(wave * TT + tt) * 16 + t16] = a;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        float a = 0.f;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) a = fmaxf(a, most[(v * TT + tt) * 16 + t16]);
+        const int e = f8_exponent(a), slot = (task.block0 + tt) * 16 + t16;
+        *reinterpret_cast<uint32_t *>(p.hbuf + (size_t)slot * p.I + rg * 16 + (lane >> 4) * 4) = f8_codes(h[tt][0], h[tt][1], h[tt][2], h[tt][3], f8_two_to(-e));
+        if (wave == 0 && lane < 16) p.hs[(size_t)blockIdx.x * p.slots + slot] = f8_two_to(e);
+    }
+}
+__global__ void __launch_bounds__(512) f8_moe_gate_up_kernel(F8MoeArgs p) {
+    __shared__ float most[8 * 2 * 16];
+    if ((int)blockIdx.y >= *p.n_tasks) return;
+    const MoeTask task = p.tasks[blockIdx.y];
+    if (task.nblocks == 1) f8_gate_up_blocks<1>(p, task, most);
+    else f8_gate_up_blocks<2>(p, task, most);
+}
+
+// Down: the waves share the windows of four row groups and add their sums in wave order.
+constexpr int kF8DownRows = 4;
+template <class T, int TT>
+__device__ __forceinline__ void f8_down_blocks(const F8MoeArgs &p, const MoeTask &task, f32x4 *red) {
+    constexpr int R = kF8DownRows, CELLS = R * TT;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, t16 = lane & 15;
+    const int windows = p.I / kF8K, rg0 = blockIdx.x * R;
+    F8Rows<R> rows;
+#pragma unroll
+    for (int r = 0; r < R; ++r) f8_row(rows, r, p.w2 + (size_t)task.expert * p.H * p.I, p.s2 + (size_t)task.expert * (p.H / 128) * windows, rg0 + r, windows);
+    F8Tokens<TT> tokens;
+    tokens.step = p.slots;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        const int slot = (task.block0 + tt) * 16 + t16;
+        tokens.x[tt] = p.hbuf + (size_t)slot * p.I;
+        tokens.a[tt] = p.hs + slot;
+    }
+    f32x4 acc[R][TT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f8_stream<TT, R, TT == 1 ? 2 : 1>(acc, rows, tokens, wave, windows, waves, lane);
+#pragma unroll
+    for (int c = 0; c < CELLS; ++c) red[(wave * CELLS + c) * 64 + lane] = acc[c / TT][c % TT];
+    __syncthreads();
+    for (int c = wave; c < CELLS; c += waves) {
+        const int r = c / TT, tt = c - r * TT;
+        f32x4 v = red[c * 64 + lane];
+        for (int w = 1; w < waves; ++w) v += red[(w * CELLS + c) * 64 + lane];
+        const int pair = p.sorted[(task.block0 + tt) * 16 + t16];
+        if (pair >= p.n_pairs) continue;
+        v *= T::to_f32(p.wts[pair]);
+        *reinterpret_cast<f32x4 *>(p.obuf + (size_t)pair * p.H + (rg0 + r) * 16 + (lane >> 4) * 4) = v;
+    }
+}
+template <class T>
+__global__ void __launch_bounds__(256) f8_moe_down_kernel(F8MoeArgs p) {
+    extern __shared__ f32x4 red[];
+    if ((int)blockIdx.y >= *p.n_tasks) return;
+    const MoeTask task = p.tasks[blockIdx.y];
+    if (task.nblocks == 1) f8_down_blocks<T, 1>(p, task, red);
+    else f8_down_blocks<T, 2>(p, task, red);
+}
+
+// y[t] = T(sum over the token's pairs on this card, in pick order)
+template <class T>
+__global__ void __launch_bounds__(256) f8_moe_combine_kernel(F8MoeArgs p) {
+    const int tok = blockIdx.x;
+    for (int n = (blockIdx.y * 256 + threadIdx.x) * 4; n < p.H; n += gridDim.y * 1024) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < p.K; ++k) {
+            const int pair = tok * p.K + k;
+            if (f8_expert(p, pair) >= 0) sum += *reinterpret_cast<const f32x4 *>(p.obuf + (size_t)pair * p.H + n);
+        }
+        *reinterpret_cast<u32x2 *>(p.Y + (size_t)tok * p.H + n) = u32x2{T::from_f32x2(sum[0], sum[1]), T::from_f32x2(sum[2], sum[3])};
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------------------- host
+static int f8_moe_pass_tokens(int n_tokens, int topk) { return n_tokens < kF8MoePairs / topk ? n_tokens : kF8MoePairs / topk; }
+
+struct F8MoeWorkspace {
+    MoeTask *tasks;
+    int32_t *n_tasks, *sorted, *cumsum, *padded, *experts_ids;
+    uint8_t *x, *hbuf;
+    float *xs, *hs, *obuf;
+};
+static int f8_moe_slots(int64_t pairs, int E) { return (int)((pairs + E * 15 + 15) / 16 * 16); }
+static size_t f8_moe_carve(uint8_t *base, int tokens, int E, int topk, int hidden, int inter, F8MoeWorkspace *ws) {
+    const int64_t pairs = (int64_t)tokens * topk, slots = f8_moe_slots(pairs, E), blocks = slots / 16;
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t *ptr = base ? base + off : nullptr;
+        off = (off + bytes + 255) / 256 * 256;
+        return ptr;
+    };
+    F8MoeWorkspace w;
+    w.tasks = (MoeTask *)take(sizeof(MoeTask) * (size_t)(blocks + 1));
+    w.n_tasks = (int32_t *)take(sizeof(int32_t));
+    w.sorted = (int32_t *)take(sizeof(int32_t) * (size_t)slots);
+    w.cumsum = (int32_t *)take(sizeof(int32_t) * (size_t)(E + 1));
+    w.padded = (int32_t *)take(sizeof(int32_t));
+    w.experts_ids = (int32_t *)take(sizeof(int32_t) * (size_t)blocks);
+    w.x = take((size_t)tokens * hidden);
+    w.xs = (float *)take((size_t)tokens * (hidden / kF8K) * 4);
+    w.hbuf = take((size_t)slots * inter);
+    w.hs = (float *)take((size_t)slots * (inter / kF8K) * 4);
+    w.obuf = (float *)take((size_t)pairs * hidden * 4);
+    if (ws) *ws = w;
+    return off;
+}
+
+template <class T>
+static int f8_launch_moe(const F8MoeArgs &a, int max_tasks, hipStream_t s) {
+    f8_moe_gate_up_kernel<<<dim3(a.I / 128, max_tasks), 512, 0, s>>>(a);
+    MLK_LAUNCH_CHECK();
+    f8_moe_down_kernel<T><<<dim3(a.H / 16 / kF8DownRows, max_tasks), 256, 4 * kF8DownRows * 2 * 1024, s>>>(a);
+    MLK_LAUNCH_CHECK();
+    f8_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
+}
+
+}  // namespace mlk
+
+using namespace mlk;
+
+extern "C" {
+
+size_t mlk_experts_fp8_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter) {
+    if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || n_router_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0) return 0;
+    return f8_moe_carve(nullptr, f8_moe_pass_tokens(n_tokens, topk), n_experts, topk, hidden, inter, nullptr);
+}
+
+int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2, const float *w2_scale, const void *x, int n_tokens, int n_experts,
+                          int n_router_experts, int topk, int hidden, int inter, int x_kind, const int32_t *topk_ids, const void *topk_weights,
+                          const int32_t *experts_map, void *y, void *workspace, size_t workspace_bytes, void *stream) {
+    MLK_REQUIRE(x_kind == MLK_F16 || x_kind == MLK_BF16, "experts fp8: activations must be fp16 or bf16");
+    MLK_REQUIRE(n_tokens >= 0, "experts fp8: negative token count");
+    MLK_REQUIRE(n_experts >= 1 && n_experts <= 256, "experts fp8: 1..256 experts");
+    MLK_REQUIRE(n_router_experts >= 1 && (experts_map || n_router_experts == n_experts), "experts fp8: fewer experts than the router's need an experts_map");
+    MLK_REQUIRE(topk >= 1 && topk <= 32, "experts fp8: topk must be in 1..32");
+    MLK_REQUIRE(hidden > 0 && inter > 0 && hidden % 128 == 0 && inter % 128 == 0, "experts fp8: hidden and intermediate sizes must be multiples of 128");
+    MLK_REQUIRE(hidden < (1 << 23) && inter < (1 << 23), "experts fp8: hidden and intermediate sizes must be below 2^23");
+    if (n_tokens == 0) return MLK_OK;
+    MLK_REQUIRE(w1 && w1_scale && w2 && w2_scale && x && topk_ids && topk_weights && y && workspace, "experts fp8: null pointer");
+    MLK_REQUIRE(aligned16(w1) && aligned16(w2) && aligned16(x) && aligned16(y) && aligned16(workspace),
+                "experts fp8: weights, activations, outputs and workspace must lie on 16 bytes");
+    if (workspace_bytes < mlk_experts_fp8_workspace_bytes(n_tokens, n_experts, n_router_experts, topk, hidden, inter)) return fail(MLK_ERR_WORKSPACE, "experts fp8: workspace too small");
+    hipStream_t s = (hipStream_t)stream;
+    F8MoeArgs a = {};
+    a.w1 = (const uint8_t *)w1;
+    a.w2 = (const uint8_t *)w2;
+    a.s1 = w1_scale;
+    a.s2 = w2_scale;
+    a.map = experts_map;
+    a.id_limit = n_router_experts;
+    a.K = topk;
+    a.H = hidden;
+    a.I = inter;
+    a.E = n_experts;
+    const int step = f8_moe_pass_tokens(n_tokens, topk);
+    for (int t0 = 0; t0 < n_tokens; t0 += step) {
+        a.T = std::min(step, n_tokens - t0);
+        a.n_pairs = a.T * topk;
+        a.slots = f8_moe_slots(a.n_pairs, n_experts);
+        a.Y = (uint16_t *)y + (size_t)t0 * hidden;
+        a.ids = topk_ids + (size_t)t0 * topk;
+        a.wts = (const uint16_t *)topk_weights + (size_t)t0 * topk;
+        F8MoeWorkspace ws;
+        f8_moe_carve((uint8_t *)workspace, a.T, n_experts, topk, hidden, inter, &ws);
+        a.X = ws.x;
+        a.xs = ws.xs;
+        a.sorted = ws.sorted;
+        a.tasks = ws.tasks;
+        a.n_tasks = ws.n_tasks;
+        a.hbuf = ws.hbuf;
+        a.hs = ws.hs;
+        a.obuf = ws.obuf;
+        int rc = launch_quantize_fp8((const uint16_t *)x + (size_t)t0 * hidden, x_kind, ws.x, ws.xs, 1, a.T, a.T, hidden, s);
+        if (rc != MLK_OK) return rc;
+        rc = launch_moe_align(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks, ws.n_tasks, 2, s);
+        if (rc != MLK_OK) return rc;
+        const int max_tasks = std::min(a.n_pairs, n_experts + a.n_pairs / 32);
+        rc = x_kind == MLK_F16 ? f8_launch_moe<F16>(a, max_tasks, s) : f8_launch_moe<BF16>(a, max_tasks, s);
+        if (rc != MLK_OK) return rc;
+    }
+    return MLK_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,385 @@
+// Routing to experts that trains: the picks of each token with their weights, and the gradient of the logits.
+//
+//   rank      the logits themselves, or with a bias the scores + bias in 64 bits (neighbours keep their order there); scores are softmax(x) or sigmoid(x)
+//   groups    score of a group: its largest rank, with a bias the sum of its two largest; the best `kept` groups stay, ties to the lower group
+//   picks     the K largest ranks, ties to the lower expert.  Experts with logits or biases of -inf or NaN are never picked: id -1, weight 0.  A logit of
+//             +inf counts as the largest finite number
+//   weights   w = c s / S (renormalised) or c s, s the score without bias and S its sum over the picks
+// Renormalised weights do not need the score's denominator: softmax gives exp(x - m) over their sum, sigmoids e^(x - min(m, 0)) / (1 + e^x), which neither loses the bits of
+// small ones nor underflows (m the largest picked logit).  With w' = s / S and g the gradient of w:
+//   dx_k = (c g_k - sum c g w') w'_k r_k  (renormalised),  c g_k s_k r_k  (sigmoid),  c g_k s_k - s_k sum c g s over the picks, - s_e sum c g s elsewhere  (softmax)
+// with r = 1 - sigmoid, 1 for softmax.
+//
+// 16 lanes take a token (64 where tokens are few), so that a wave takes four at a time and a maximum over the experts is four exchanges within 16 lanes.  After the
+// picks lane k holds pick k.
+#include "mlk_logits.cuh"
+
+namespace mlk {
+
+constexpr int kRouteExperts = 512;
+constexpr int kRoutePicks = 32;
+
+struct RouteArgs {
+    const void *logits;          // [T][E]
+    const float *bias;           // [E] or null
+    const uint8_t *mask;         // [T] or null
+    int T, E, K, G, kept, score_fun, renorm;
+    float scaling;
+    int32_t *ids;                // [T][K]
+    void *weights;               // [T][K]
+    const void *dweights;        // [T][K]
+    void *dlogits;               // [T][E]
+};
+
+template <int LPT, class V, class F>
+__device__ __forceinline__ V route_fold(V v, F f) {
+    if constexpr (sizeof(V) == 4) {
+        auto other = [](V x, auto step) {
+            return __builtin_bit_cast(V, bal_other<decltype(step)::value>(__builtin_bit_cast(float, x)));
+        };
+        v = f(v, other(v, std::integral_constant<int, 1>()));
+        v = f(v, other(v, std::integral_constant<int, 2>()));
+        v = f(v, other(v, std::integral_constant<int, 4>()));
+        v = f(v, other(v, std::integral_constant<int, 8>()));
+        if constexpr (LPT == 64) {
+            v = f(v, __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(float, v), 16)));
+            v = f(v, __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(float, v), 32)));
+        }
+    } else {
+        for (int m = 1; m < LPT; m <<= 1) v = f(v, __shfl_xor(v, m));
+    }
+    return v;
+}
+template <int LPT>
+__device__ __forceinline__ float route_sum(float v) { return route_fold<LPT>(v, [](float a, float b) { return a + b; }); }
+template <int LPT>
+__device__ __forceinline__ float route_max(float v) { return route_fold<LPT>(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <int LPT>
+__device__ __forceinline__ int route_min(int v) { return route_fold<LPT>(v, [](int a, int b) { return min(a, b); }); }
+
+// A logit as it counts: -inf for NaN, the largest finite number for +inf.
+__device__ __forceinline__ float route_logit(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
+
+// Experts of a lane: slot 4 v + i holds 4 (v LPT + lane) + i.
+template <int LPT>
+__device__ __forceinline__ int route_expert(int slot, int l) { return ((slot >> 2) * LPT + l) * 4 + (slot & 3); }
+template <class L, int LPT, int NE>
+__device__ __forceinline__ void route_load(const RouteArgs &p, int t, int l, bool vec, float (&x)[NE]) {
+    const typename L::V1 *row = reinterpret_cast<const typename L::V1 *>(p.logits) + (size_t)t * p.E;
+    if (vec) {
+        typename L::V4 raw[NE / 4];
+#pragma unroll
+        for (int v = 0; v < NE / 4; ++v) raw[v] = *reinterpret_cast<const typename L::V4 *>(row + min(route_expert<LPT>(4 * v, l), p.E - 4));
+#pragma unroll
+        for (int v = 0; v < NE / 4; ++v) {
+            float y[4];
+            L::unpack(raw[v], y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[4 * v + i] = route_expert<LPT>(4 * v, l) + i < p.E ? route_logit(y[i]) : -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < NE; ++s) {
+            const int e = route_expert<LPT>(s, l);
+            const float y = L::to_f32(row[min(e, p.E - 1)]);
+            x[s] = e < p.E ? route_logit(y) : -INFINITY;
+        }
+    }
+}
+
+// Score of the picks of a lane, 0 for none (x = -inf), and 1 - sigmoid.  m: the largest of the picks; renormalised: of sigmoids e^-min(m, 0) times, of softmax e^-m and
+// without the denominator.
+__device__ __forceinline__ float route_score(const RouteArgs &p, float x, float m, float &rest) {
+    rest = 1.f;
+    if (x == -INFINITY) return 0.f;
+    if (p.score_fun == 0) return expf(x - m);
+    const float low = p.renorm ? fminf(m, 0.f) : 0.f, e = expf(-fabsf(x)), r = 1.f / (1.f + e);
+    rest = x >= 0.f ? e * r : r;
+    return x >= 0.f ? r : expf(x - low) * r;
+}
+
+// V: what picks are ranked by, float or double.
+template <class L, int LPT, int NE, class V>
+__global__ void __launch_bounds__(64) route_kernel(RouteArgs p, bool vec) {
+    constexpr int TOK = 64 / LPT;
+    extern __shared__ char lds[];
+    const int l = threadIdx.x & (LPT - 1), mine = threadIdx.x / LPT, t = min((int)blockIdx.x * TOK + mine, p.T - 1);
+    const bool here = (int)blockIdx.x * TOK + mine < p.T;
+    const V lowest = -INFINITY;
+    float x[NE];
+    route_load<L, LPT, NE>(p, t, l, vec, x);
+    V rank[NE];
+    float top = -INFINITY, sum = 1.f;
+#pragma unroll
+    for (int s = 0; s < NE; ++s) {
+        top = fmaxf(top, x[s]);
+        rank[s] = x[s];
+    }
+    if constexpr (sizeof(V) == 8) {
+        top = route_max<LPT>(top);
+        double total = 0.;
+#pragma unroll
+        for (int s = 0; s < NE; ++s) {
+            if (p.score_fun == 0) rank[s] = x[s] == -INFINITY ? 0. : exp((double)x[s] - (double)top);
+            else rank[s] = 1. / (1. + exp(-(double)x[s]));
+            total += rank[s];
+        }
+        total = p.score_fun == 0 ? route_fold<LPT>(total, [](double a, double b) { return a + b; }) : 1.;
+        sum = (float)total;
+#pragma unroll
+        for (int s = 0; s < NE; ++s) {
+            const int e = route_expert<LPT>(s, l);
+            const float b = e < p.E ? p.bias[e] : -INFINITY;
+            rank[s] = x[s] == -INFINITY || b != b ? lowest : rank[s] / total + (double)b;
+        }
+    } else if (p.score_fun == 0 && !p.renorm) {
+        top = route_max<LPT>(top);
+        sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < NE; ++s) sum += x[s] == -INFINITY ? 0.f : expf(x[s] - top);
+        sum = route_sum<LPT>(sum);
+    }
+    if (p.G > 1) {
+        V *ranks = reinterpret_cast<V *>(lds) + (size_t)mine * (p.E + p.G);
+        V *best = ranks + p.E;
+#pragma unroll
+        for (int s = 0; s < NE; ++s) {
+            const int e = route_expert<LPT>(s, l);
+            if (e < p.E) ranks[e] = rank[s];
+        }
+        wave_lds_sync();
+        const int each = p.E / p.G;
+        for (int g = l; g < p.G; g += LPT) {
+            V a = lowest, b = lowest;
+            for (int i = 0; i < each; ++i) {
+                const V v = ranks[g * each + i];
+                b = v > a ? a : (v > b ? v : b);
+                a = v > a ? v : a;
+            }
+            best[g] = sizeof(V) == 8 && b != lowest ? a + b : a;
+        }
+        wave_lds_sync();
+        // a group stays if fewer than `kept` are better, or as good and lower
+#pragma unroll
+        for (int s = 0; s < NE; ++s) {
+            const int e = route_expert<LPT>(s, l), g = min(e / each, p.G - 1);
+            const V own = best[g];
+            int ahead = 0;
+            for (int q = 0; q < p.G; ++q) ahead += best[q] > own || (best[q] == own && q < g) ? 1 : 0;
+            if (ahead >= p.kept) rank[s] = lowest;
+        }
+    }
+    // K times the largest, then the lowest expert that has it
+    int id[2] = {-1, -1};
+    for (int k = 0; k < p.K; ++k) {
+        V high = rank[0];
+#pragma unroll
+        for (int s = 1; s < NE; ++s) high = rank[s] > high ? rank[s] : high;
+        high = route_fold<LPT>(high, [](V a, V b) { return a > b ? a : b; });
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int s = NE - 1; s >= 0; --s) at = rank[s] == high ? route_expert<LPT>(s, l) : at;
+        at = route_min<LPT>(at);
+#pragma unroll
+        for (int s = 0; s < NE; ++s) rank[s] = route_expert<LPT>(s, l) == at ? lowest : rank[s];
+        if ((k & (LPT - 1)) == l) id[k / LPT] = high == lowest ? -1 : at;
+    }
+    float xk[2], m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        xk[j] = id[j] >= 0 ? route_logit(L::to_f32(reinterpret_cast<const typename L::V1 *>(p.logits)[(size_t)t * p.E + id[j]])) : -INFINITY;
+        m = fmaxf(m, xk[j]);
+    }
+    m = p.renorm ? route_max<LPT>(m) : top;
+    float s[2], rest;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j] = route_score(p, xk[j], m, rest);
+    if (p.renorm) sum = route_sum<LPT>(s[0] + s[1]);
+    else if (p.score_fun != 0) sum = 1.f;
+    const bool valid = !p.mask || p.mask[t];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int k = j * LPT + l;
+        if (!here || k >= p.K) continue;
+        p.ids[(size_t)t * p.K + k] = valid ? id[j] : -1;
+        reinterpret_cast<typename L::V1 *>(p.weights)[(size_t)t * p.K + k] = L::from_f32(valid && id[j] >= 0 ? p.scaling * (s[j] / sum) : 0.f);
+    }
+}
+
+// The gradient of a token's row goes through LDS: zeros, or the share of the softmax's denominator, and the picks' on top.
+template <class L, int LPT, int NE>
+__global__ void __launch_bounds__(64) route_grad_kernel(RouteArgs p, bool vec) {
+    constexpr int TOK = 64 / LPT;
+    __shared__ float row[TOK][LPT * NE];
+    const int l = threadIdx.x & (LPT - 1), mine = threadIdx.x / LPT, t = min((int)blockIdx.x * TOK + mine, p.T - 1);
+    const bool here = (int)blockIdx.x * TOK + mine < p.T;
+    typedef typename L::V1 E1;
+    int id[2];
+    float g[2], xk[2], m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int k = j * LPT + l;
+        id[j] = k < p.K ? p.ids[(size_t)t * p.K + k] : -1;
+        g[j] = id[j] >= 0 ? p.scaling * L::to_f32(reinterpret_cast<const E1 *>(p.dweights)[(size_t)t * p.K + k]) : 0.f;
+        xk[j] = id[j] >= 0 ? route_logit(L::to_f32(reinterpret_cast<const E1 *>(p.logits)[(size_t)t * p.E + id[j]])) : -INFINITY;
+        m = fmaxf(m, xk[j]);
+    }
+    float d[NE];
+#pragma unroll
+    for (int s = 0; s < NE; ++s) d[s] = 0.f;
+    const bool all = p.score_fun == 0 && !p.renorm;       // every logit is in the denominator
+    float sum = 1.f;
+    if (all) {
+        float top = -INFINITY;
+        route_load<L, LPT, NE>(p, t, l, vec, d);
+#pragma unroll
+        for (int s = 0; s < NE; ++s) top = fmaxf(top, d[s]);
+        m = route_max<LPT>(top);
+        sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < NE; ++s) {
+            d[s] = d[s] == -INFINITY ? 0.f : expf(d[s] - m);
+            sum += d[s];
+        }
+        sum = route_sum<LPT>(sum);
+    } else {
+        m = route_max<LPT>(m);
+    }
+    float s[2], rest[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j] = route_score(p, xk[j], m, rest[j]);
+    if (p.renorm) sum = route_sum<LPT>(s[0] + s[1]);
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        s[j] *= inv;
+        dot = fmaf(g[j], s[j], dot);
+    }
+    dot = p.renorm || all ? route_sum<LPT>(dot) : 0.f;
+    if (all) {
+        const float c = -dot * inv;
+#pragma unroll
+        for (int q = 0; q < NE; ++q) d[q] *= c;
+    }
+#pragma unroll
+    for (int v = 0; v < NE / 4; ++v)
+        *reinterpret_cast<f32x4 *>(&row[mine][route_expert<LPT>(4 * v, l)]) = f32x4{d[4 * v], d[4 * v + 1], d[4 * v + 2], d[4 * v + 3]};
+    wave_lds_sync();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (id[j] >= 0) row[mine][id[j]] = (g[j] - dot) * s[j] * rest[j];
+    wave_lds_sync();
+    if (!here) return;
+    E1 *out = reinterpret_cast<E1 *>(p.dlogits) + (size_t)t * p.E;
+#pragma unroll
+    for (int v = 0; v < NE / 4; ++v) {
+        const int e = route_expert<LPT>(4 * v, l);
+        const f32x4 q = *reinterpret_cast<const f32x4 *>(&row[mine][e]);
+        const float y[4] = {q[0], q[1], q[2], q[3]};
+        if (vec) {
+            if (e < p.E) *reinterpret_cast<typename L::V4 *>(out + e) = L::pack(y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e + i < p.E) out[e + i] = L::from_f32(y[i]);
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------------------- host
+template <class L, int LPT, int NE>
+static void route_launch(const RouteArgs &a, bool vec, bool grad, hipStream_t s) {
+    const int wgs = (a.T + 64 / LPT - 1) / (64 / LPT);
+    const size_t lds = a.G > 1 ? (size_t)(64 / LPT) * (a.E + a.G) * (a.bias ? 8 : 4) : 0;
+    if (grad) route_grad_kernel<L, LPT, NE><<<wgs, 64, 0, s>>>(a, vec);
+    else if (a.bias) route_kernel<L, LPT, NE, double><<<wgs, 64, lds, s>>>(a, vec);
+    else route_kernel<L, LPT, NE, float><<<wgs, 64, lds, s>>>(a, vec);
+}
+template <class L>
+static void route_launch_size(const RouteArgs &a, bool vec, bool grad, hipStream_t s) {
+    if (a.T <= 1024) {
+        if (a.E <= 256) route_launch<L, 64, 4>(a, vec, grad, s);
+        else route_launch<L, 64, 8>(a, vec, grad, s);
+    } else if (a.E <= 64) {
+        route_launch<L, 16, 4>(a, vec, grad, s);
+    } else if (a.E <= 128) {
+        route_launch<L, 16, 8>(a, vec, grad, s);
+    } else if (a.E <= 256) {
+        route_launch<L, 16, 16>(a, vec, grad, s);
+    } else {
+        route_launch<L, 16, 32>(a, vec, grad, s);
+    }
+}
+static int route_launch_kind(const RouteArgs &a, int kind, bool vec, bool grad, hipStream_t s) {
+    if (kind == MLK_F32) route_launch_size<BalF32>(a, vec, grad, s);
+    else if (kind == MLK_F16) route_launch_size<Bal16<F16>>(a, vec, grad, s);
+    else route_launch_size<Bal16<BF16>>(a, vec, grad, s);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
+}
+static bool route_vec(const void *p, int kind, int E) { return E % 4 == 0 && ((uintptr_t)p & (kind == MLK_F32 ? 15 : 7)) == 0; }
+
+static int route_check(const void *logits, int kind, int score_fun, int T, int E, int K) {
+    MLK_REQUIRE(kind == MLK_F16 || kind == MLK_BF16 || kind == MLK_F32, "routing: logits must be fp16, bf16 or fp32");
+    MLK_REQUIRE(score_fun == 0 || score_fun == 1, "routing: score function must be 0 (softmax) or 1 (sigmoid)");
+    MLK_REQUIRE(T >= 0 && T <= (1 << 30), "routing: 0..2^30 tokens");
+    MLK_REQUIRE(E >= 1 && E <= kRouteExperts, "routing: 1..512 experts");
+    MLK_REQUIRE(K >= 1 && K <= kRoutePicks && K <= E, "routing: picks must be in 1..min(32, experts)");
+    MLK_REQUIRE(T == 0 || logits, "routing: null pointer");
+    return MLK_OK;
+}
+
+}  // namespace mlk
+
+using namespace mlk;
+
+extern "C" {
+
+int mlk_moe_routing(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, int n_groups, int topk_groups, int topk, const float *bias,
+                    int renormalize, float scaling, const uint8_t *token_mask, int32_t *ids, void *weights, void *stream) {
+    const int rc = route_check(logits, x_kind, score_fun, n_tokens, n_experts, topk);
+    if (rc != MLK_OK) return rc;
+    MLK_REQUIRE(n_groups >= 1 && n_experts % n_groups == 0, "routing: n_groups must divide the expert count");
+    MLK_REQUIRE(topk_groups >= 1 && topk_groups <= n_groups && topk <= n_experts / n_groups * topk_groups,
+                "routing: topk_groups must be in 1..n_groups, and the kept groups hold as many experts as are picked");
+    if (n_tokens == 0) return MLK_OK;
+    MLK_REQUIRE(ids && weights, "routing: null pointer");
+    RouteArgs a = {};
+    a.logits = logits;
+    a.bias = bias;
+    a.mask = token_mask;
+    a.T = n_tokens;
+    a.E = n_experts;
+    a.K = topk;
+    a.G = n_groups;
+    a.kept = topk_groups;
+    a.score_fun = score_fun;
+    a.renorm = renormalize != 0;
+    a.scaling = scaling;
+    a.ids = ids;
+    a.weights = weights;
+    return route_launch_kind(a, x_kind, route_vec(logits, x_kind, n_experts), false, (hipStream_t)stream);
+}
+
+int mlk_moe_routing_grad(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, int topk, int renormalize, float scaling, const int32_t *ids,
+                         const void *dweights, void *dlogits, void *stream) {
+    const int rc = route_check(logits, x_kind, score_fun, n_tokens, n_experts, topk);
+    if (rc != MLK_OK) return rc;
+    if (n_tokens == 0) return MLK_OK;
+    MLK_REQUIRE(ids && dweights && dlogits, "routing: null pointer");
+    RouteArgs a = {};
+    a.logits = logits;
+    a.T = n_tokens;
+    a.E = n_experts;
+    a.K = topk;
+    a.score_fun = score_fun;
+    a.renorm = renormalize != 0;
+    a.scaling = scaling;
+    a.ids = const_cast<int32_t *>(ids);
+    a.dweights = dweights;
+    a.dlogits = dlogits;
+    return route_launch_kind(a, x_kind, route_vec(logits, x_kind, n_experts) && route_vec(dlogits, x_kind, n_experts), true, (hipStream_t)stream);
+}
+
+}  // extern "C"

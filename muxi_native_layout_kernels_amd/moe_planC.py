@@ -206,3 +206,52 @@ def fused_moe_w4(
         if expert_load is not None:
             ops.expert_counts(topk_ids, n_experts, out=expert_load)
     return y
+
+
+def fused_moe_fp8(
+    hidden_states: torch.Tensor,  # [batch_size, hidden_size]
+    w1: torch.Tensor,             # [E, 2I/16, H/8, 16, 8] e4m3 bytes per-expert in layout-A (or [E, 2I, H])
+    w2: torch.Tensor,             # [E, H/16, I/8, 16, 8]
+    gating_output: torch.Tensor,  # [batch_size, num_experts]
+    topk: int,
+    renormalize: bool,
+    w1_scale: torch.Tensor,
+    w2_scale: torch.Tensor,
+    use_grouped_topk: bool = False,
+    num_expert_group: Optional[int] = None,
+    topk_group: Optional[int] = None,
+    gating_bias: Optional[torch.Tensor] = None,
+    score_func: str = "softmax",
+    scaling: float = 1.0,
+    token_mask: Optional[torch.Tensor] = None,
+    experts_map: Optional[torch.Tensor] = None,
+    expert_load: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """The MoE layer in e4m3: `moe_routing`, then `fused_experts_fp8`.  gating_output in the activation dtype or fp32, gating_bias fp32.  `expert_load` (int32 [num_experts], at most 256): the
+    picks of this call are added to it (`expert_counts`).  No gradient: the result is detached."""
+    if num_expert_group is None:
+        num_expert_group = 1
+    if topk_group is None:
+        topk_group = 1
+    if not use_grouped_topk and num_expert_group != 1:
+        raise ValueError("When use_grouped_topk is False, num_expert_group must be 1.")
+    ops._check(hidden_states.dim() == 2 and gating_output.dim() == 2 and hidden_states.shape[0] == gating_output.shape[0], "Number of tokens mismatch")
+    ops._check(hidden_states.dtype in ops._KIND and gating_output.dtype in (hidden_states.dtype, torch.float32), "gating_output must have the activation dtype or be fp32")
+    n_experts = gating_output.shape[1]
+    ops._check(n_experts == (w1.shape[0] if experts_map is None else experts_map.numel()),
+               "gating_output must have one column per expert of w1, or per entry of experts_map")
+    ops._check(hidden_states.is_cuda and hidden_states.device == gating_output.device, "hidden_states and gating_output must be on the same CUDA device")
+    ops._check(expert_load is None or (n_experts <= 256 and expert_load.dtype == torch.int32 and tuple(expert_load.shape) == (n_experts,)),
+               "expert_load must be int32 [n_experts], for at most 256 experts")
+    ops._check_tensors(((expert_load, "expert_load"),), hidden_states.device)
+    with torch.no_grad():
+        # every check of the experts ahead of the router: a call that is refused launches nothing
+        shape = (hidden_states.shape[0], topk)
+        ids, weights = hidden_states.new_empty(shape, dtype=torch.int32), hidden_states.new_empty(shape)
+        plan = ops._experts_fp8_plan(hidden_states, w1, w2, ids, weights, w1_scale, w2_scale, experts_map)
+        ops._check(((w1.data_ptr() | w2.data_ptr()) & 15) == 0, "w1 and w2 must lie on 16 bytes")
+        ids, weights = ops.moe_routing(gating_output, topk, score_func, renormalize, num_expert_group, topk_group, gating_bias, scaling, token_mask)
+        y = ops._experts_fp8_launch(plan, hidden_states, w1, w2, ids, weights.to(hidden_states.dtype), w1_scale, w2_scale, experts_map)
+        if expert_load is not None:
+            ops.expert_counts(ids, n_experts, out=expert_load)
+    return y

@@ -754,6 +754,101 @@ def gemv_layoutA_w4(A, A_Scale, B, A_Zero=None, alpha=1, beta=0, bias=None):
     return _w4_call(A, A_Scale, B, A_Zero, alpha, beta, bias, "gemv_layoutA_w4")
 
 
+# ------------------------------------------------------------- e4m3 products
+_ACTIVATION_KIND = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 3}
+_E4M3 = torch.float8_e4m3fn
+
+
+def quantize_fp8(x):
+    """Activations [.., K] fp16 / bf16 / fp32 -> (codes float8_e4m3fn [.., K], scales fp32 [.., K/128]): the left operand of `gemm_layoutA_fp8`, for
+    several products of the same activations.
+
+    The scale of 128 consecutive values is the smallest power of two, 2^-100 at least, with max |x| <= 448 scale; a code is x / scale rounded to nearest even.  Infinities
+    and NaN become the NaN code and do not count in the maximum.  K % 128 == 0, at most 2^27 rows.  The scales of one block lie side by side over the rows (a transposed view), as
+    the products read them.  No gradient: the results are detached."""
+    key = ("quantize_fp8", x.shape, x.dtype, x.get_device())
+    plan = _plans.get(key)
+    if plan is None or not x.is_contiguous():
+        _check(x.dtype in _ACTIVATION_KIND, "x must be fp16, bf16 or fp32")
+        _check(x.dim() >= 1 and x.size(-1) > 0 and x.size(-1) % 128 == 0, "the last size of x must be a multiple of 128")
+        _check_tensors(((x, "x"),), x.device)
+        rows, k = x.numel() // x.size(-1), x.size(-1)
+        plan = _plans[key] = (rows, k, _ACTIVATION_KIND[x.dtype], tuple(x.shape[:-1]) + (k // 128,), _lib.load().mlk_quantize_fp8)
+    rows, k, kind, scale_shape, fn = plan
+    with _OnDevice(x):
+        if x.data_ptr() & 15:
+            x = x.clone()
+        codes = torch.empty(x.shape, dtype=_E4M3, device=x.device)
+        scales = torch.empty((k // 128, rows), dtype=torch.float32, device=x.device)
+        rc = fn(x.data_ptr(), kind, codes.data_ptr(), scales.data_ptr(), 1, rows, rows, k, _stream_of(x))
+        if rc != 0:
+            _lib.check(rc, "quantize_fp8")
+    scales = scales.t()
+    return codes, scales if x.dim() == 2 else scales.view(scale_shape)
+
+
+def gemm_layoutA_fp8(A, A_Scale, B, B_Scale=None, alpha=1, beta=0, bias=None, out_dtype=None):
+    """C[n, m] = alpha * B[n, k] . A^T (+ bias), both operands in e4m3: the products run at the matrix cores' 8-bit rate, where `gemm_layoutA_soft_fp8` widens the
+    weights to bf16.
+
+    A [m/16, k/8, 16, 8] e4m3 bytes in layout-A and A_Scale fp32 [ceil(m/128), k/128], as the soft-FP8 products take them.  B fp16 / bf16: quantised in the call as by
+    `quantize_fp8`; or codes (float8_e4m3fn or uint8) with B_Scale fp32 [n, k/128], of any strides and any values.  Output of B's dtype, of codes bf16 unless `out_dtype` says
+    fp16.  Any n >= 0, m % 16 == 0, k % 128 == 0.  fp32 sums; the sum of 128 k is scaled by both scales in fp32.  A row of B with an infinity or NaN gives NaN.  No
+    gradient: the result is detached."""
+    key = ("gemm_fp8", A.shape, A.dtype, A.get_device(), A_Scale.shape, A_Scale.dtype, A_Scale.get_device(), B.shape, B.dtype, B.get_device(),
+           None if B_Scale is None else (B_Scale.shape, B_Scale.dtype, B_Scale.get_device()), None if bias is None else (bias.shape, bias.dtype, bias.get_device()),
+           out_dtype)
+    plan = _plans.get(key)
+    if plan is None or beta != 0 or not (A.is_contiguous() and A_Scale.is_contiguous() and B.is_contiguous() and (bias is None or bias.is_contiguous())):
+        _check_beta(beta)
+        m, k = _layout_a_dims(A)
+        _check(_is_fp8(A), "A must hold one e4m3 byte per element")
+        _check(k % 128 == 0, "k % 128 must be 0")
+        _check(A_Scale.dtype == torch.float32 and tuple(A_Scale.shape) == ((m + 127) // 128, k // 128), "A_Scale must be fp32 [ceil(m/128), k/128]")
+        _check(B.dim() == 2, "B must be a 2D tensor")
+        _check(B.size(1) == k, "A and B must have the same k")
+        if B_Scale is None:
+            _check(B.dtype in _KIND, "B must be fp16 or bf16, or e4m3 codes with a B_Scale")
+            _check(out_dtype is None or out_dtype == B.dtype, "out_dtype is that of B")
+            kind = c_kind = _KIND[B.dtype]
+        else:
+            _check(B.dtype in (_E4M3, torch.uint8), "B must hold e4m3 codes where there is a B_Scale")
+            _check(B_Scale.dtype == torch.float32 and tuple(B_Scale.shape) == (B.size(0), k // 128), "B_Scale must be fp32 [n, k/128]")
+            _check(B_Scale.is_cuda and B_Scale.device == B.device, "B_Scale must be on the same device as the others")
+            _check(out_dtype is None or out_dtype in _KIND, "out_dtype must be fp16 or bf16")
+            kind, c_kind = _FP8_KIND, _KIND[out_dtype or torch.bfloat16]
+        dtype = torch.float16 if c_kind == 0 else torch.bfloat16
+        _check(bias is None or (bias.dtype == dtype and bias.numel() == m), "bias must be [1, m] of the output dtype")
+        _check_tensors(((A, "A"), (A_Scale, "A_Scale"), (B, "B"), (bias, "bias")), B.device)
+        lib = _lib.load()
+        plan = _plans[key] = (B.size(0), m, k, kind, c_kind, dtype, lib.mlk_gemm_fp8_workspace_bytes(B.size(0), m, k, kind), lib.mlk_gemm_counter_bytes(),
+                              lib.mlk_gemm_layout_a_fp8)
+    if B.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(B.device):
+            return _gemm_fp8_launch(plan, A, A_Scale, B, B_Scale, alpha, bias)
+    return _gemm_fp8_launch(plan, A, A_Scale, B, B_Scale, alpha, bias)
+
+
+def _gemm_fp8_launch(plan, A, A_Scale, B, B_Scale, alpha, bias):
+    n, m, k, kind, c_kind, dtype, ws_need, counter_bytes, fn = plan
+    b_ptr = B.data_ptr()
+    if b_ptr & 15:
+        B = B.clone()
+        b_ptr = B.data_ptr()
+    C = B.new_empty((n, m), dtype=dtype)
+    stream = _stream_of(B)
+    scale = scale_t = scale_k = ws_ptr = ws_len = 0
+    if B_Scale is not None:
+        scale, (scale_t, scale_k) = B_Scale.data_ptr(), B_Scale.stride()
+    if ws_need:
+        ws = _gemm_pool.get(B.device, stream, ws_need, counter_bytes)
+        ws_ptr, ws_len = ws.data_ptr(), ws.numel()
+    rc = fn(A.data_ptr(), A_Scale.data_ptr(), b_ptr, kind, scale, scale_t, scale_k, C.data_ptr(), c_kind, n, m, k, float(alpha), _ptr(bias), ws_ptr, ws_len, stream)
+    if rc != 0:
+        _lib.check(rc, "gemm_layoutA_fp8")
+    return C
+
+
 # ----------------------------------------------------------------------- MoE
 def _check_gating_bias(bias, gating_output):
     """The router reads one element for every expert."""
@@ -1022,6 +1117,163 @@ def _experts_w4_launch(plan, x, w1, w2, topk_ids, topk_weights, w1_scale, w2_sca
     return y
 
 
+def fused_experts_fp8(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map=None):
+    """The two products of an expert layer in e4m3, from a routing decision (`moe_routing`, `fused_routing_gate`, or a caller's own).
+
+    hidden_states [T, H] fp16 / bf16, quantised in the call as by `quantize_fp8`; w1 [E, 2I/16, H/8, 16, 8] (gate rows, then up rows) and w2 [E, H/16, I/8, 16, 8] e4m3 bytes in
+    layout-A (or the flat [E, 2I, H] and [E, H, I] that `fused_moe` takes too), with fp32 scales [E, 2I/128, H/128] and [E, H/128, I/128]; topk_ids int32 [T, K],
+    topk_weights [T, K] of the activation dtype; experts_map int32 [experts of the router]: the expert's place in w1 / w2, -1 = on another card.  Ids outside the router's
+    experts are dropped too; a token without an expert here gets zeros.  Returns y [T, H].  SiLU(gate) * up is quantised from fp32 like the activations, all sums are fp32.  A
+    token with an infinity or NaN gives a row of NaN; other rows keep theirs.  No gradient: the result is detached."""
+    plan = _experts_fp8_plan(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map)
+    return _experts_fp8_launch(plan, hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map)
+
+
+def _experts_fp8_plan(x, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map):
+    key = ("experts_fp8", x.shape, w1.shape, w2.shape, topk_ids.shape, topk_weights.shape, w1_scale.shape, w2_scale.shape, x.dtype, w1.dtype, w2.dtype,
+           topk_ids.dtype, topk_weights.dtype, w1_scale.dtype, w2_scale.dtype, x.get_device(), w1.get_device(), w2.get_device(), topk_ids.get_device(),
+           topk_weights.get_device(), w1_scale.get_device(), w2_scale.get_device(),
+           None if experts_map is None else (experts_map.shape, experts_map.dtype, experts_map.get_device()))
+    plan = _plans.get(key)
+    if plan is None or not (x.is_contiguous() and w1.is_contiguous() and w2.is_contiguous() and topk_ids.is_contiguous() and topk_weights.is_contiguous() and
+                            w1_scale.is_contiguous() and w2_scale.is_contiguous() and (experts_map is None or experts_map.is_contiguous())):
+        _check(_is_fp8(w1) and _is_fp8(w2), "w1 and w2 must hold one e4m3 byte per element")
+        _check(w1.dim() == w2.dim() and w1.dim() in (3, 5), "expert weights must be [E, rows, cols] or in layout-A")
+        if w1.dim() == 5:
+            _check(tuple(w1.shape[-2:]) == (16, 8) and tuple(w2.shape[-2:]) == (16, 8), "w1 and w2 must be in layout-A")
+            m1, hidden, m2, inter = w1.size(1) * 16, w1.size(2) * 8, w2.size(1) * 16, w2.size(2) * 8
+        else:
+            m1, hidden, m2, inter = w1.size(1), w1.size(2), w2.size(1), w2.size(2)
+        E = w1.size(0)
+        _check(w2.size(0) == E and m1 == 2 * inter and m2 == hidden, "w1 must be [E, 2I, H] and w2 [E, H, I]")
+        _check(hidden > 0 and inter > 0 and inter % 128 == 0 and hidden % 128 == 0, "hidden and intermediate sizes must be multiples of 128")
+        _check(max(hidden, inter) < 1 << 23, "hidden and intermediate sizes must be below 2^23")
+        _check(1 <= E <= 256, "at most 256 experts")
+        _check(w1_scale.dtype == torch.float32 and w2_scale.dtype == torch.float32, "scales must be float32.")
+        _check(tuple(w1_scale.shape) == (E, m1 // 128, hidden // 128), "w1_scale must be [E, 2I/128, H/128]")
+        _check(tuple(w2_scale.shape) == (E, hidden // 128, inter // 128), "w2_scale must be [E, H/128, I/128]")
+        _check(x.dim() == 2 and x.size(1) == hidden, "hidden_states must be [T, H]")
+        _check(x.dtype in _KIND, "hidden_states must be fp16 or bf16")
+        _check(topk_ids.dim() == 2 and topk_ids.size(0) == x.size(0) and topk_ids.dtype == torch.int32, "topk_ids must be int32 [T, K]")
+        _check(topk_weights.shape == topk_ids.shape and topk_weights.dtype == x.dtype, "topk_weights must be [T, K] of the activation dtype")
+        K = topk_ids.size(1)
+        _check(1 <= K <= 32, "topK must be in 1..32")
+        _check(experts_map is None or (experts_map.dtype == torch.int32 and experts_map.dim() == 1 and experts_map.numel() > 0),
+               "experts_map must be int32 [experts of the router]")
+        _check_tensors(((x, "hidden_states"), (w1, "w1"), (w2, "w2"), (topk_ids, "topk_ids"), (topk_weights, "topk_weights"), (w1_scale, "w1_scale"),
+                        (w2_scale, "w2_scale"), (experts_map, "experts_map")), x.device)
+        lib = _lib.load()
+        E_router = E if experts_map is None else experts_map.numel()
+        plan = _plans[key] = (x.size(0), E, E_router, K, hidden, inter, _KIND[x.dtype], lib.mlk_experts_fp8_workspace_bytes(x.size(0), E, E_router, K, hidden, inter),
+                              lib.mlk_fused_experts_fp8)
+    return plan
+
+
+def _experts_fp8_launch(plan, x, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map):
+    T, E, E_router, K, hidden, inter, kind, ws_need, fn = plan
+    with _OnDevice(x):
+        if x.data_ptr() & 15:
+            x = x.clone()
+        y = x.new_empty((T, hidden))
+        if T == 0:
+            return y
+        stream = _stream_of(x)
+        ws = _moe_pool.get(x.device, stream, ws_need)
+        rc = fn(w1.data_ptr(), w1_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), x.data_ptr(), T, E, E_router, K, hidden, inter, kind,
+                topk_ids.data_ptr(), topk_weights.data_ptr(), _ptr(experts_map), y.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        if rc != 0:
+            _lib.check(rc, "fused_experts_fp8")
+    return y
+
+
+# --------------------------------------------------------- routing that trains
+class _Routing(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, mask, plan, options):
+        ids, weights = _routing_forward(logits, bias, mask, plan, options)
+        ctx.save_for_backward(logits, ids)
+        ctx.plan, ctx.options = plan, options
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        return ids, weights
+
+    @staticmethod
+    def backward(ctx, _, dweights):
+        if dweights is None:
+            return None, None, None, None, None
+        if torch.is_grad_enabled():                                             # create_graph
+            with torch.no_grad():
+                grad = _routing_backward(ctx, dweights)
+            return _FirstDerivative.apply(grad.requires_grad_(True), "moe_routing"), None, None, None, None
+        return _routing_backward(ctx, dweights), None, None, None, None
+
+
+def _routing_forward(logits, bias, mask, plan, options):
+    T, E, K, kind, fn, _ = plan
+    score_fun, renormalize, n_groups, topk_groups, scaling = options
+    with _OnDevice(logits):
+        ids = torch.empty((T, K), dtype=torch.int32, device=logits.device)
+        weights = logits.new_empty((T, K))
+        rc = fn(logits.data_ptr(), kind, score_fun, T, E, n_groups, topk_groups, K, _ptr(bias), renormalize, scaling, _ptr(mask), ids.data_ptr(),
+                weights.data_ptr(), _stream_of(logits))
+        if rc != 0:
+            _lib.check(rc, "moe_routing")
+    return ids, weights
+
+
+def _routing_backward(ctx, dweights):
+    _check_no_tangent(dweights, "moe_routing")
+    logits, ids = ctx.saved_tensors
+    T, E, K, kind, _, fn = ctx.plan
+    score_fun, renormalize, _, _, scaling = ctx.options
+    with _OnDevice(logits):
+        dweights = dweights.contiguous()
+        grad = torch.empty_like(logits)
+        rc = fn(logits.data_ptr(), kind, score_fun, T, E, K, renormalize, scaling, ids.data_ptr(), dweights.data_ptr(), grad.data_ptr(), _stream_of(logits))
+        if rc != 0:
+            _lib.check(rc, "moe_routing")
+    return grad
+
+
+def moe_routing(gating_output, topk, score_func="softmax", renormalize=True, num_expert_group=1, topk_group=1, gating_bias=None, scaling=1.0, token_mask=None):
+    """The experts of each token and their weights: (ids int32 [T, topk], weights [T, topk] of gating_output's dtype), differentiable in gating_output.  For the expert
+    layers, `expert_counts` and `moe_balance_loss`; `fused_routing_gate` is the reference's router, which rounds the scores ahead of the selection.
+
+    gating_output [T, E] fp16 / bf16 / fp32, E <= 512.  Experts are ranked by their logits, or with gating_bias (fp32 [E], a constant of the differentiation: the load's
+    correction) by score + bias in 64 bits; scores: softmax, or "sigmoid".  With num_expert_group groups of consecutive experts only the topk_group best stay: by
+    their largest rank, with a bias by the sum of their two largest.  ids: the topk <= 32 largest ranks in falling order; ties go to the lower expert and the lower group.
+    weights: scaling * score, over the sum of the picks' scores if `renormalize`.  An expert whose logit or bias is -inf or NaN is never picked; where too few are left, and
+    for padded tokens (token_mask bool [T] False), ids are -1, which the expert layers drop, and weights 0.  A logit of +inf counts as the largest finite number.
+    Masked rows may hold anything; their gradient is 0.  A second derivative and a derivative in forward mode are refused.  Both passes may be recorded into a HIP graph; as
+    with any torch function no earlier graph of the same leaf may then be alive."""
+    logits = gating_output
+    _check_no_tangent(logits, "moe_routing")
+    key = ("routing", logits.shape, logits.dtype, logits.get_device(), topk, num_expert_group, topk_group,
+           None if gating_bias is None else (gating_bias.shape, gating_bias.dtype, gating_bias.get_device()),
+           None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.get_device()))
+    plan = _plans.get(key)
+    if plan is None or not (logits.is_contiguous() and (gating_bias is None or gating_bias.is_contiguous()) and (token_mask is None or token_mask.is_contiguous())):
+        _check(logits.dim() == 2 and 1 <= logits.size(1) <= 512, "gating_output must be [T, E], at most 512 experts")
+        _check(logits.dtype in _LOGIT_KIND, "gating_output must be fp16, bf16 or fp32")
+        T, E = logits.shape
+        _check(isinstance(topk, int) and 1 <= topk <= min(32, E), "topk must be in 1..min(32, experts)")
+        _check(num_expert_group >= 1 and E % num_expert_group == 0, "num_expert_group must divide the number of experts")
+        _check(1 <= topk_group <= num_expert_group and topk <= E // num_expert_group * topk_group,
+               "topk_group must be in 1..num_expert_group, and the kept groups hold topk experts at least")
+        _check(gating_bias is None or (gating_bias.dtype == torch.float32 and tuple(gating_bias.shape) == (E,)), "gating_bias must be fp32 [E]")
+        _check(token_mask is None or (token_mask.dtype in (torch.bool, torch.uint8) and tuple(token_mask.shape) == (T,)), "token_mask must be bool [T]")
+        _check_tensors(((logits, "gating_output"), (gating_bias, "gating_bias"), (token_mask, "token_mask")), logits.device)
+        lib = _lib.load()
+        plan = _plans[key] = (T, E, topk, _LOGIT_KIND[logits.dtype], lib.mlk_moe_routing, lib.mlk_moe_routing_grad)
+    if score_func not in ("softmax", "sigmoid"):
+        raise ValueError("Unsupported scoring function")
+    _check(gating_bias is None or not (gating_bias.requires_grad and torch.is_grad_enabled()), "moe_routing: gating_bias has no gradient")
+    options = (0 if score_func == "softmax" else 1, int(bool(renormalize)), num_expert_group, topk_group, float(scaling))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Routing.apply(logits, gating_bias, token_mask, plan, options)
+    return _routing_forward(logits, gating_bias, token_mask, plan, options)
+
+
 # ------------------------------------------------------------- router balance
 def _check_routing(experts_ids, token_mask, device):
     _check(experts_ids.dtype == torch.int32 and experts_ids.dim() == 2 and experts_ids.size(1) >= 1, "experts_ids must be int32 [T, K]")
@@ -1090,8 +1342,8 @@ def _balance_launch(logits, ids, mask, cu, score_fun, coef, plan):
     return loss, counts, share
 
 
-def _check_no_tangent(t):
-    _check(unpack_dual(t).tangent is None, "moe_balance_loss: there is no forward-mode derivative")
+def _check_no_tangent(t, what):
+    _check(unpack_dual(t).tangent is None, "%s: there is no forward-mode derivative" % what)
 
 
 class _BalanceLoss(torch.autograd.Function):
@@ -1109,7 +1361,7 @@ class _BalanceLoss(torch.autograd.Function):
         if torch.is_grad_enabled() and dloss is not None:                       # create_graph
             with torch.no_grad():
                 grad = _balance_backward(ctx, dloss)[0]
-            return _FirstDerivative.apply(grad.requires_grad_(True)), None, None, None, None, None, None
+            return _FirstDerivative.apply(grad.requires_grad_(True), "moe_balance_loss"), None, None, None, None, None, None
         return _balance_backward(ctx, dloss)
 
 
@@ -1117,18 +1369,19 @@ class _FirstDerivative(torch.autograd.Function):
     """The gradient as it is; its own derivative is refused, not taken for zero."""
 
     @staticmethod
-    def forward(ctx, grad):
+    def forward(ctx, grad, what):
+        ctx.what = what
         return grad.view_as(grad)
 
     @staticmethod
     def backward(ctx, _):
-        raise RuntimeError("moe_balance_loss: the gradient cannot be differentiated again")
+        raise RuntimeError("%s: the gradient cannot be differentiated again" % ctx.what)
 
 
 def _balance_backward(ctx, dloss):
     if dloss is None:
         return None, None, None, None, None, None, None
-    _check_no_tangent(dloss)
+    _check_no_tangent(dloss, "moe_balance_loss")
     logits, mask, cu, share = ctx.saved_tensors
     if logits.get_device() != torch.cuda.current_device():
         with torch.cuda.device(logits.device):
@@ -1161,7 +1414,7 @@ def moe_balance_loss(gating_output, experts_ids, score_func="softmax", coef=1.0,
     and a derivative in forward mode are refused.
     Both passes may be recorded into a HIP graph, once run on its stream; as with any torch function no earlier loss of the same leaf may then be alive."""
     logits = gating_output
-    _check_no_tangent(logits)
+    _check_no_tangent(logits, "moe_balance_loss")
     key = ("balance", logits.shape, logits.dtype, logits.get_device(), experts_ids.shape, experts_ids.dtype, experts_ids.get_device(),
            None if token_mask is None else (token_mask.shape, token_mask.dtype, token_mask.get_device()),
            None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.dtype, cu_seqlens.get_device()))
@@ -1213,5 +1466,5 @@ __all__ = [
     "batched_routed_activation_indexed_to_expert_block_indexed", "fused_experts_compute",
     "pack_layout_a", "unpack_layout_a", "experts_compute_raw", "release_workspaces", "workspace_bytes_held",
     "fused_moe_raw", "pack_layout_a_w4", "unpack_layout_a_w4", "gemm_layoutA_w4", "gemv_layoutA_w4",
-    "fused_experts_w4", "expert_counts", "moe_balance_loss",
+    "fused_experts_w4", "expert_counts", "moe_balance_loss", "quantize_fp8", "gemm_layoutA_fp8", "fused_experts_fp8", "moe_routing",
 ]
