@@ -1,7 +1,7 @@
 // Quantising activations to e4m3, and the linear layers in e4m3: one token to prefill-sized batches.
 #include <algorithm>
 
-#include "mlk_f8.cuh"
+#include "mlk_f8_panel.cuh"
 
 namespace mlk {
 
@@ -101,8 +101,46 @@ static int f8_launch_stream(const F8GemmArgs &a, hipStream_t s) {
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }
+
+// Panels move and multiply like those of a 16-bit product of half the k: as many bytes, and the matrix cores take twice as many k in the time.
+extern template int f8_launch_panel<F16>(const F8PanelArgs &, int, int, hipStream_t);
+extern template int f8_launch_panel<BF16>(const F8PanelArgs &, int, int, hipStream_t);
+size_t panel8_arguments(Panel8Args &p, int m, int n, int k, int pr, int tb, int p3);
+void gemm_plan(int m, int n, int k, bool fp8, bool b_native, int32_t *out);
+
+struct F8Plan {
+    bool panels;
+    int pr, tb, p3;
+};
+static F8Plan f8_plan(int m, int n, int k) {
+    F8Plan pl = {};
+    // offsets within a panel are 32 bits
+    if (m <= 64 || k >= 1 << 23) return pl;
+    int32_t out[4];
+    gemm_plan(m, n, k / 2, false, false, out);
+    pl.panels = true;
+    pl.pr = out[1] / 2;
+    pl.tb = out[2];
+    pl.p3 = out[3];
+    return pl;
+}
 template <class T>
-static int f8_launch_gemm(const F8GemmArgs &a, hipStream_t s) {
+static int f8_launch_gemm(const F8GemmArgs &a, const F8Plan &pl, void *partial, size_t partial_bytes, hipStream_t s) {
+    if (pl.panels) {
+        F8PanelArgs g = {};
+        g.p.A = a.A;
+        g.p.B = reinterpret_cast<const uint16_t *>(a.X);
+        g.p.C = a.C;
+        g.p.bias = a.bias;
+        g.p.scale = a.a_scale;
+        g.p.partial = (f32x4 *)partial;
+        g.p.alpha = a.alpha;
+        if (panel8_arguments(g.p, a.M, a.N, a.K / 2, pl.pr, pl.tb, pl.p3) > partial_bytes) return fail(MLK_ERR_WORKSPACE, "gemm fp8: workspace too small");
+        g.x_scale = a.x_scale;
+        g.xs_t = (uint32_t)a.xs_t;
+        g.xs_k = (uint32_t)a.xs_k;
+        return f8_launch_panel<T>(g, pl.pr, pl.tb, s);
+    }
     if (a.M <= 16) return f8_launch_stream<T, 1, 2>(a, s);
     return f8_launch_stream<T, 2, 2>(a, s);
 }
@@ -110,8 +148,17 @@ static int f8_launch_gemm(const F8GemmArgs &a, hipStream_t s) {
 struct F8Scratch {
     uint8_t *codes;
     float *scales;
+    void *partial;
+    size_t partial_bytes;
 };
-static size_t f8_carve(uint8_t *base, int m, int k, F8Scratch *out) {
+static size_t f8_carve(uint8_t *base, int m, int n, int k, bool quantize, F8Scratch *out) {
+    const F8Plan pl = f8_plan(m, n, k);
+    Panel8Args p = {};
+    const size_t partial = pl.panels ? panel8_arguments(p, m, n, k / 2, pl.pr, pl.tb, pl.p3) : 0;
+    if (!quantize && partial == 0) {
+        if (out) *out = F8Scratch{};
+        return 0;
+    }
     size_t off = kCounterBytes;
     auto take = [&](size_t bytes) {
         uint8_t *ptr = base ? base + off : nullptr;
@@ -119,8 +166,10 @@ static size_t f8_carve(uint8_t *base, int m, int k, F8Scratch *out) {
         return ptr;
     };
     F8Scratch w;
-    w.codes = take((size_t)m * k);
-    w.scales = (float *)take((size_t)m * (k / kF8K) * 4);
+    w.codes = take(quantize ? (size_t)m * k : 0);
+    w.scales = (float *)take(quantize ? (size_t)m * (k / kF8K) * 4 : 0);
+    w.partial = take(partial);
+    w.partial_bytes = partial;
     if (out) *out = w;
     return off;
 }
@@ -143,7 +192,7 @@ int mlk_quantize_fp8(const void *x, int x_kind, void *codes, float *scales, int6
 
 size_t mlk_gemm_fp8_workspace_bytes(int m, int n, int k, int b_kind) {
     if (m <= 0 || n <= 0 || k <= 0 || k % 128 != 0) return 0;
-    return b_kind == MLK_FP8_E4M3 ? 0 : f8_carve(nullptr, m, k, nullptr);
+    return f8_carve(nullptr, m, n, k, b_kind != MLK_FP8_E4M3, nullptr);
 }
 
 int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, int b_kind, const float *b_scale, int64_t b_scale_t, int64_t b_scale_k, void *c,
@@ -170,18 +219,21 @@ int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, in
     p.M = m;
     p.N = n;
     p.K = k;
-    if (b_kind != MLK_FP8_E4M3) {
+    F8Scratch w;
+    if (f8_carve((uint8_t *)workspace, m, n, k, b_kind != MLK_FP8_E4M3, &w) > 0)
         MLK_REQUIRE(workspace && aligned16(workspace), "gemm fp8: workspace off 16 bytes");
-        F8Scratch w;
-        f8_carve((uint8_t *)workspace, m, k, &w);
+    F8Plan pl = f8_plan(m, n, k);
+    if (b_kind != MLK_FP8_E4M3) {
         const int rc = launch_quantize_fp8(b, b_kind, w.codes, w.scales, 1, m, m, k, s);
         if (rc != MLK_OK) return rc;
         p.X = w.codes;
         p.x_scale = w.scales;
         p.xs_t = 1;
         p.xs_k = m;
+    } else if (b_scale_t < 0 || b_scale_k < 0 || b_scale_t >= 1 << 21 || b_scale_k >= (1ll << 29) / (k / kF8K)) {
+        pl.panels = false;                                     // scales that far apart: the panels' offsets of them are 32 bits
     }
-    return c_kind == MLK_F16 ? f8_launch_gemm<F16>(p, s) : f8_launch_gemm<BF16>(p, s);
+    return c_kind == MLK_F16 ? f8_launch_gemm<F16>(p, pl, w.partial, w.partial_bytes, s) : f8_launch_gemm<BF16>(p, pl, w.partial, w.partial_bytes, s);
 }
 
 }  // extern "C"

@@ -391,6 +391,13 @@ void gemm_plan_off16(int m, int n, int k, bool fp8, bool b_native, bool c_native
     out[0] = 3, out[1] = small ? 2 : 4, out[2] = 1, out[3] = sk;
 }
 
+// Panels of other products that move and multiply like 16-bit ones of m x n x k: tiles, order and deal, and the bytes of their partial sums.
+size_t panel8_arguments(Panel8Args &p, int m, int n, int k, int pr, int tb, int p3) {
+    panel8_shape(p, m, n, k, pr, tb, panel8_slices(p3));
+    p.rows_first = p8_rows_first(p, m, n, k, false);
+    return panel8_partial_bytes(p, pr);
+}
+
 // whole_groups < 0: kernel id 8, p3 as it takes it; else kernel ids 3 and 5, p3 = K slices of the row tiles behind those groups
 int launch_panel8_gemm(const void *a, const void *b, void *c, int m, int n, int k, int a_kind, bool b_native, bool c_native,
                        float alpha, const void *bias, const float *scale, int pr, int tb, int p3, int whole_groups, void *partial,
