@@ -28,6 +28,10 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
     static constexpr int NB = 2 * WIN * 16 > 80 * 1024 ? 2 : 3;
     static constexpr size_t lds_bytes = (size_t)NB * WIN * 16;
     static constexpr int LOADS = 2 * PR + TB + 1;                           // of a wave and window
+    // They go out behind the barrier that frees their buffer: FIRST in the last step of a window, EACH in the steps that follow.  All at once in the last step they hold up every wave of the
+    // workgroup in the same place: 8192 x 8192 at 4096 tokens 278 us, two a step 254, three 258, four 259.
+    static constexpr int FIRST = 2, EACH = TT == 2 ? LOADS : 2;
+    static_assert(FIRST + (TT - 1) * EACH >= LOADS, "all loads of a window go out in one");
     static_assert(lds_bytes <= kP8MostLds, "the ring has to fit");
 
     __device__ static __forceinline__ int tile(int wave, int i) { return PR * wave + i; }
@@ -38,18 +42,19 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
         return (octet * 8 + (lane & 7)) * 16;
     }
 
-    __device__ static __forceinline__ void issue(const F8PanelSrc &src, int wave, int window, int buf) {
+    // Load l < LOADS of a wave and window: its weight tiles by slabs, its chunks of tokens, its scales.
+    __device__ static __forceinline__ void issue(const F8PanelSrc &src, int wave, int window, int buf, int l) {
         extern __shared__ u32x4 win[];
         u32x4 *at = win + buf * WIN;
-        __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void *)src.p.a, 0, 0xffffffffu, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < PR; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, at + tile(wave, i) * 128 + h * 64, 16, src.w_off, src.p.a_off[i] + window * 2048 + h * 1024, 0, 0);
-        Tok::issue(src.p, wave, at + A_WIN, window);
-        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)src.scales, 0, 0xffffffffu, 0x00020000);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at + A_WIN + B_WIN + wave * 16, 4, src.s_off, window * src.s_step, 0, 0);
+        if (l < 2 * PR) {
+            __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)src.p.a, 0, 0xffffffffu, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at + tile(wave, l >> 1) * 128 + (l & 1) * 64, 16, src.w_off, src.p.a_off[l >> 1] + window * 2048 + (l & 1) * 1024, 0, 0);
+        } else if (l < 2 * PR + TB) {
+            Tok::issue1(src.p, wave, at + A_WIN, window, l - 2 * PR);
+        } else {
+            __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)src.scales, 0, 0xffffffffu, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at + A_WIN + B_WIN + wave * 16, 4, src.s_off, window * src.s_step, 0, 0);
+        }
     }
 
     // Windows w0 .. w0 + n - 1.  On return nothing is in flight and LDS is free once the workgroup has met at a barrier.
@@ -61,7 +66,7 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
         extern __shared__ u32x4 win[];
         const int wr = wave & 3, wt = wave >> 2;
         const int last = w0 + n - 1;
-        auto fetch = [&](int w, int buf) { issue(src, wave, min(w0 + w, last), buf); };        // windows past the end: copies of the last one
+        auto fetch = [&](int w, int buf, int l) { issue(src, wave, min(w0 + w, last), buf, l); };        // windows past the end: copies of the last one
         const int q = lane >> 4, a_idx = wr * RT * 256 + ((q & 1) + (q & 2) * 2) * 16 + (lane & 15);       // in units of 8 bytes: octets 2 q, and 2 q + 1 at + 32
         const int b0 = A_WIN + Tok::operand16(src.p, 0, lane) + wt * TT * 128, b1 = A_WIN + Tok::operand16(src.p, 1, lane) + wt * TT * 128;
         const int s_idx = (A_WIN + B_WIN) * 4 + wt * TT * 16 + (lane & 15), ws_idx = (A_WIN + B_WIN + 64) * 4 + (wr * PR) / 4;
@@ -86,8 +91,11 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
 #pragma unroll
         for (int i = 0; i < RT; ++i) d[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < NB; ++w) fetch(w, w);
-        wait_vmcnt_le<(NB - 1) * LOADS>();                     // window 0
+        for (int w = 0; w < NB; ++w)
+#pragma unroll
+            for (int l = 0; l < LOADS; ++l)
+                if (w < NB - 1 || l < FIRST) fetch(w, w, l);
+        wait_vmcnt_le<(NB - 2) * LOADS + FIRST>();             // window 0
         bare_barrier();
         read_sw(0);
 #pragma unroll
@@ -96,7 +104,7 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
         int cur = 0;
 #pragma clang loop unroll(disable)
         for (int w = 0; w < n; ++w) {
-            const int nxt = cur == NB - 1 ? 0 : cur + 1;
+            const int nxt = cur == NB - 1 ? 0 : cur + 1, prv = cur == 0 ? NB - 1 : cur - 1;
 #pragma unroll
             for (int j = 0; j < TT; ++j) {
                 if (j == TT - 1) {
@@ -104,9 +112,12 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
                     wait_vmcnt_le<(NB - 2) * LOADS>();         // this wave's loads of window w + 1 have landed
                     wait_lds();                                // and it has all of window w, which is loaded over behind this barrier
                     bare_barrier();
-                    fetch(w + NB, cur);
+#pragma unroll
+                    for (int l = 0; l < FIRST; ++l) fetch(w + NB, cur, l);
                 } else {
                     read_b(cur, j + 1);
+#pragma unroll
+                    for (int l = FIRST + j * EACH; l < FIRST + (j + 1) * EACH && l < LOADS; ++l) fetch(w + NB - 1, prv, l);
                 }
                 const float last_scale = scale;
                 scale = s[j & 1] * sw;
@@ -127,6 +138,7 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
                 for (int i = 0; i < RT; ++i) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                     __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
                     if (j == TT - 1) __builtin_amdgcn_sched_group_barrier(0x100, 5, 0);
                     else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 }
