@@ -20,13 +20,13 @@ struct F8PanelSrc {
 
 template <int PR, int TB>
 struct F8PanelLoop : P8TokenPairs<TB, true> {
-    using Tok = P8TokenPairs<TB, true>;
+    using Tok = P8TokenPairs<TB, true>;          // its NB: chunks of tokens a wave fetches
     using Acc = P8Acc16<PR, TB>;
     static constexpr int RT = 2 * PR, TT = 2 * TB;                          // row tiles and token blocks of a wave
     static constexpr int A_WIN = 1024 * PR, B_WIN = Tok::B_PAIR, S_WIN = 128;       // granules of 16 bytes: weights, tokens, scales (256 of tokens, 256 of weights)
     static constexpr int WIN = A_WIN + B_WIN + S_WIN;
-    static constexpr int NB = 2 * WIN * 16 > 80 * 1024 ? 2 : 3;
-    static constexpr size_t lds_bytes = (size_t)NB * WIN * 16;
+    static constexpr int RING = 2 * WIN * 16 > 80 * 1024 ? 2 : 3;
+    static constexpr size_t lds_bytes = (size_t)RING * WIN * 16;
     static constexpr int LOADS = 2 * PR + TB + 1;                           // of a wave and window
     // They go out behind the barrier that frees their buffer: FIRST in the last step of a window, EACH in the steps that follow.  All at once in the last step they hold up every wave of the
     // workgroup in the same place: 8192 x 8192 at 4096 tokens 278 us, two a step 254, three 258, four 259.
@@ -61,7 +61,7 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
     //
     // A step multiplies the wave's row tiles with one block of 16 tokens.  While it does, the block of the next step is read, and the sums of the step before, whose products have
     // ended by then, are scaled and added.  The barrier of a window stands ahead of its last step, when all its operands are in registers: behind it the first operands of the next window are
-    // read into those that the last step leaves, and the loads of window w + NB go out into the buffer.
+    // read into those that the last step leaves, and the loads of window w + RING go out into the buffer.
     __device__ static __forceinline__ void run(Acc &out, const F8PanelSrc &src, int w0, int n, int wave, int lane) {
         extern __shared__ u32x4 win[];
         const int wr = wave & 3, wt = wave >> 2;
@@ -91,11 +91,11 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
 #pragma unroll
         for (int i = 0; i < RT; ++i) d[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < NB; ++w)
+        for (int w = 0; w < RING; ++w)
 #pragma unroll
             for (int l = 0; l < LOADS; ++l)
-                if (w < NB - 1 || l < FIRST) fetch(w, w, l);
-        wait_vmcnt_le<(NB - 2) * LOADS + FIRST>();             // window 0
+                if (w < RING - 1 || l < FIRST) fetch(w, w, l);
+        wait_vmcnt_le<(RING - 2) * LOADS + FIRST>();             // window 0
         bare_barrier();
         read_sw(0);
 #pragma unroll
@@ -104,20 +104,20 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
         int cur = 0;
 #pragma clang loop unroll(disable)
         for (int w = 0; w < n; ++w) {
-            const int nxt = cur == NB - 1 ? 0 : cur + 1, prv = cur == 0 ? NB - 1 : cur - 1;
+            const int nxt = cur == RING - 1 ? 0 : cur + 1, prv = cur == 0 ? RING - 1 : cur - 1;
 #pragma unroll
             for (int j = 0; j < TT; ++j) {
                 if (j == TT - 1) {
                     __builtin_amdgcn_sched_barrier(0);
-                    wait_vmcnt_le<(NB - 2) * LOADS>();         // this wave's loads of window w + 1 have landed
+                    wait_vmcnt_le<(RING - 2) * LOADS>();         // this wave's loads of window w + 1 have landed
                     wait_lds();                                // and it has all of window w, which is loaded over behind this barrier
                     bare_barrier();
 #pragma unroll
-                    for (int l = 0; l < FIRST; ++l) fetch(w + NB, cur, l);
+                    for (int l = 0; l < FIRST; ++l) fetch(w + RING, cur, l);
                 } else {
                     read_b(cur, j + 1);
 #pragma unroll
-                    for (int l = FIRST + j * EACH; l < FIRST + (j + 1) * EACH && l < LOADS; ++l) fetch(w + NB - 1, prv, l);
+                    for (int l = FIRST + j * EACH; l < FIRST + (j + 1) * EACH && l < LOADS; ++l) fetch(w + RING - 1, prv, l);
                 }
                 const float last_scale = scale;
                 scale = s[j & 1] * sw;

@@ -128,6 +128,22 @@ def test_exact_sums(mlk, tokens):
     assert torch.equal(got.cpu().double(), (q @ c.t()).double())
 
 
+@pytest.mark.parametrize("tokens,n,k", [
+    (65, 16, 256), (65, 16400, 256), (515, 8208, 256), (1300, 11024, 256), (200, 16400, 256), (4100, 4112, 256), (129, 16400, 256), (257, 16400, 256),
+    (390, 16400, 256), (2050, 8208, 256), (1030, 11024, 256), (2050, 16400, 2048), (70, 528, 2048), (150, 528, 4096), (300, 2064, 7168), (1030, 2064, 4096), (700, 8208, 7168), (70, 8208, 7168),
+    (150, 11024, 7168), (200, 16400, 7168), (257, 16400, 7168), (2050, 16400, 7168), (3000, 16400, 4096)])
+def test_exact_sums_in_panels_of_every_shape(mlk, tokens, n, k):
+    """Likewise with powers of two as scales, another one for every block, in panels of 128 and 256 rows x 64 to 256 tokens: whole, in slices of k, dealt, in several rounds."""
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    q = torch.randint(-2, 3, (tokens, k), generator=g, device="cuda")
+    c = torch.randint(-1, 2, (n, k), generator=g, device="cuda")
+    s = torch.randint(0, 2, ((n + 127) // 128, k // 128), generator=g, device="cuda").float().exp2()
+    a = torch.randint(0, 2, (tokens, k // 128), generator=g, device="cuda").float().exp2()
+    got = mlk.gemm_layoutA_fp8(mlk.pack_layout_a(c.to(F8)), s, q.to(F8), a)
+    want = (q * a.repeat_interleave(128, 1)) @ (c * s.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)).t()          # fp32, below 2^24
+    assert torch.equal(got, want.to(BF))
+
+
 @pytest.mark.parametrize("tokens", [2, 40, 300])
 def test_a_row_with_nan_or_infinity_keeps_to_itself(mlk, tokens):
     codes, s, _ = weights(528, 1024, 1)
