@@ -7,41 +7,16 @@
 #include <algorithm>
 #include <initializer_list>
 
-#include "mlk_f8.cuh"
-#include "mlk_moe_args.cuh"
+#include "mlk_f8_moe.cuh"
 
 namespace mlk {
 
-int launch_moe_align(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
-                     int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, hipStream_t s);
+int launch_moe_align_even(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
+                          int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, hipStream_t s);
+extern template int f8_launch_moe_panels<F16>(const F8MoeArgs &, int, hipStream_t);
+extern template int f8_launch_moe_panels<BF16>(const F8MoeArgs &, int, hipStream_t);
 
 constexpr int kF8MoePairs = 16384;      // routed pairs of a pass: bounds the scratch of long prompts
-
-struct F8MoeArgs {
-    const uint8_t *w1, *w2;      // of expert 0
-    const float *s1, *s2;
-    const uint8_t *X;            // [T][H] codes
-    const float *xs;             // [H / 128][T]
-    uint16_t *Y;                 // [T][H]
-    const int32_t *ids;          // [T * K]
-    const uint16_t *wts;         // [T * K]
-    const int32_t *map;          // [id_limit] or null
-    int id_limit, T, K, H, I, E, n_pairs, slots;
-    const int32_t *sorted;
-    const MoeTask *tasks;
-    const int32_t *n_tasks;
-    uint8_t *hbuf;               // [slot][I]
-    float *hs;                   // [I / 128][slot]
-    float *obuf;                 // [pair][H]
-};
-
-// Local expert of a pair, -1: dropped.
-__device__ __forceinline__ int f8_expert(const F8MoeArgs &p, int pair) {
-    int e = p.ids[pair];
-    if (e < 0 || e >= p.id_limit) return -1;
-    if (p.map) e = p.map[e];
-    return e >= 0 && e < p.E ? e : -1;
-}
 
 // Gate/up: wave w of eight streams the w-th row group of gate and the same one of up.
 template <int TT>
@@ -153,7 +128,10 @@ __global__ void __launch_bounds__(256) f8_moe_combine_kernel(F8MoeArgs p) {
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < p.K; ++k) {
             const int pair = tok * p.K + k;
-            if (f8_expert(p, pair) >= 0) sum += *reinterpret_cast<const f32x4 *>(p.obuf + (size_t)pair * p.H + n);
+            if (f8_expert(p, pair) < 0) continue;
+            f32x4 v = *reinterpret_cast<const f32x4 *>(p.obuf + (size_t)pair * p.slices * p.H + n);
+            for (int sl = 1; sl < p.slices; ++sl) v += *reinterpret_cast<const f32x4 *>(p.obuf + ((size_t)pair * p.slices + sl) * p.H + n);
+            sum += v;
         }
         *reinterpret_cast<u32x2 *>(p.Y + (size_t)tok * p.H + n) = u32x2{T::from_f32x2(sum[0], sum[1]), T::from_f32x2(sum[2], sum[3])};
     }
@@ -168,8 +146,26 @@ struct F8MoeWorkspace {
     uint8_t *x, *hbuf;
     float *xs, *hs, *obuf;
 };
+struct F8MoePlan {
+    bool panels;
+    int blocks;              // of 16 pairs, of a task at most
+    int max_tasks, slices;
+};
+static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidden, int inter) {
+    F8MoePlan pl = {};
+    const int pairs = tokens * topk;
+    // with E of the router's experts here that share of the pairs is expected here
+    const int here = (int)std::max<int64_t>(1, std::min<int64_t>(pairs, (int64_t)pairs * E / n_router));
+    const int reached = std::min(here, E), load = (here + reached - 1) / reached;
+    pl.slices = 1;
+    // offsets within an expert's weights and of a token are 32 bits
+    pl.panels = load > 32 && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
+    pl.blocks = pl.panels ? kF8PanelBlocks : 2;
+    pl.max_tasks = std::min(pairs, E + pairs / (16 * pl.blocks));
+    return pl;
+}
 static int f8_moe_slots(int64_t pairs, int E) { return (int)((pairs + E * 15 + 15) / 16 * 16); }
-static size_t f8_moe_carve(uint8_t *base, int tokens, int E, int topk, int hidden, int inter, F8MoeWorkspace *ws) {
+static size_t f8_moe_carve(uint8_t *base, const F8MoePlan &pl, int tokens, int E, int topk, int hidden, int inter, F8MoeWorkspace *ws) {
     const int64_t pairs = (int64_t)tokens * topk, slots = f8_moe_slots(pairs, E), blocks = slots / 16;
     size_t off = 0;
     auto take = [&](size_t bytes) {
@@ -188,17 +184,22 @@ static size_t f8_moe_carve(uint8_t *base, int tokens, int E, int topk, int hidde
     w.xs = (float *)take((size_t)tokens * (hidden / kF8K) * 4);
     w.hbuf = take((size_t)slots * inter);
     w.hs = (float *)take((size_t)slots * (inter / kF8K) * 4);
-    w.obuf = (float *)take((size_t)pairs * hidden * 4);
+    w.obuf = (float *)take((size_t)pairs * pl.slices * hidden * 4);
     if (ws) *ws = w;
     return off;
 }
 
 template <class T>
-static int f8_launch_moe(const F8MoeArgs &a, int max_tasks, hipStream_t s) {
-    f8_moe_gate_up_kernel<<<dim3(a.I / 128, max_tasks), 512, 0, s>>>(a);
-    MLK_LAUNCH_CHECK();
-    f8_moe_down_kernel<T><<<dim3(a.H / 16 / kF8DownRows, max_tasks), 256, 4 * kF8DownRows * 2 * 1024, s>>>(a);
-    MLK_LAUNCH_CHECK();
+static int f8_launch_moe(const F8MoeArgs &a, const F8MoePlan &pl, hipStream_t s) {
+    if (pl.panels) {
+        const int rc = f8_launch_moe_panels<T>(a, pl.max_tasks, s);
+        if (rc != MLK_OK) return rc;
+    } else {
+        f8_moe_gate_up_kernel<<<dim3(a.I / 128, pl.max_tasks), 512, 0, s>>>(a);
+        MLK_LAUNCH_CHECK();
+        f8_moe_down_kernel<T><<<dim3(a.H / 16 / kF8DownRows, pl.max_tasks), 256, 4 * kF8DownRows * 2 * 1024, s>>>(a);
+        MLK_LAUNCH_CHECK();
+    }
     f8_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
@@ -212,7 +213,12 @@ extern "C" {
 
 size_t mlk_experts_fp8_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter) {
     if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || n_router_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0) return 0;
-    return f8_moe_carve(nullptr, f8_moe_pass_tokens(n_tokens, topk), n_experts, topk, hidden, inter, nullptr);
+    // a long call goes in passes of one size and a shorter last one, whose plan may differ
+    const int step = f8_moe_pass_tokens(n_tokens, topk), rest = n_tokens % step;
+    size_t most = 0;
+    for (int t : {step, rest})
+        if (t > 0) most = std::max(most, f8_moe_carve(nullptr, f8_moe_plan(t, n_experts, n_router_experts, topk, hidden, inter), t, n_experts, topk, hidden, inter, nullptr));
+    return most;
 }
 
 int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2, const float *w2_scale, const void *x, int n_tokens, int n_experts,
@@ -250,8 +256,9 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
         a.Y = (uint16_t *)y + (size_t)t0 * hidden;
         a.ids = topk_ids + (size_t)t0 * topk;
         a.wts = (const uint16_t *)topk_weights + (size_t)t0 * topk;
+        const F8MoePlan pl = f8_moe_plan(a.T, n_experts, n_router_experts, topk, hidden, inter);
         F8MoeWorkspace ws;
-        f8_moe_carve((uint8_t *)workspace, a.T, n_experts, topk, hidden, inter, &ws);
+        f8_moe_carve((uint8_t *)workspace, pl, a.T, n_experts, topk, hidden, inter, &ws);
         a.X = ws.x;
         a.xs = ws.xs;
         a.sorted = ws.sorted;
@@ -262,10 +269,11 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
         a.obuf = ws.obuf;
         int rc = launch_quantize_fp8((const uint16_t *)x + (size_t)t0 * hidden, x_kind, ws.x, ws.xs, 1, a.T, a.T, hidden, s);
         if (rc != MLK_OK) return rc;
-        rc = launch_moe_align(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks, ws.n_tasks, 2, s);
+        a.slices = pl.slices;
+        rc = launch_moe_align_even(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks, ws.n_tasks,
+                                   pl.blocks, pl.panels ? 4 : 0, s);
         if (rc != MLK_OK) return rc;
-        const int max_tasks = std::min(a.n_pairs, n_experts + a.n_pairs / 32);
-        rc = x_kind == MLK_F16 ? f8_launch_moe<F16>(a, max_tasks, s) : f8_launch_moe<BF16>(a, max_tasks, s);
+        rc = x_kind == MLK_F16 ? f8_launch_moe<F16>(a, pl, s) : f8_launch_moe<BF16>(a, pl, s);
         if (rc != MLK_OK) return rc;
     }
     return MLK_OK;

@@ -18,7 +18,8 @@ struct F8PanelSrc {
     uint32_t s_step;            // bytes from one window to the next
 };
 
-template <int PR, int TB>
+// NS = 2: the first half of a wave's row tiles and the second have scales of their own, of which waves 4..7 fetch one each in lanes 0 and 1.
+template <int PR, int TB, int NS = 1>
 struct F8PanelLoop : P8TokenPairs<TB, true> {
     using Tok = P8TokenPairs<TB, true>;          // its NB: chunks of tokens a wave fetches
     using Acc = P8Acc16<PR, TB>;
@@ -69,10 +70,10 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
         auto fetch = [&](int w, int buf, int l) { issue(src, wave, min(w0 + w, last), buf, l); };        // windows past the end: copies of the last one
         const int q = lane >> 4, a_idx = wr * RT * 256 + ((q & 1) + (q & 2) * 2) * 16 + (lane & 15);       // in units of 8 bytes: octets 2 q, and 2 q + 1 at + 32
         const int b0 = A_WIN + Tok::operand16(src.p, 0, lane) + wt * TT * 128, b1 = A_WIN + Tok::operand16(src.p, 1, lane) + wt * TT * 128;
-        const int s_idx = (A_WIN + B_WIN) * 4 + wt * TT * 16 + (lane & 15), ws_idx = (A_WIN + B_WIN + 64) * 4 + (wr * PR) / 4;
+        const int s_idx = (A_WIN + B_WIN) * 4 + wt * TT * 16 + (lane & 15), ws_idx = (A_WIN + B_WIN + 64) * 4 + (NS == 2 ? 0 : (wr * PR) / 4);
         F8Operand a[RT], b[2];
         f32x4 d[2][RT];
-        float s[2], sw, scale = 0.f;
+        float s[2], sw[NS], scale[NS];
         auto read_a = [&](int buf, int i) {
             const u32x2 *at = reinterpret_cast<const u32x2 *>(win + buf * WIN) + a_idx + i * 256;
 #pragma unroll
@@ -86,8 +87,13 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
             b[j & 1].v[1] = win[buf * WIN + b1 + j * 128];
             s[j & 1] = reinterpret_cast<const float *>(win + buf * WIN)[s_idx + j * 16];
         };
-        auto read_sw = [&](int buf) { sw = reinterpret_cast<const float *>(win + buf * WIN)[ws_idx]; };
+        auto read_sw = [&](int buf) {
+#pragma unroll
+            for (int h = 0; h < NS; ++h) sw[h] = reinterpret_cast<const float *>(win + buf * WIN)[ws_idx + h];
+        };
         out.zero();
+#pragma unroll
+        for (int h = 0; h < NS; ++h) scale[h] = 0.f;
 #pragma unroll
         for (int i = 0; i < RT; ++i) d[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -119,8 +125,12 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
 #pragma unroll
                     for (int l = FIRST + j * EACH; l < FIRST + (j + 1) * EACH && l < LOADS; ++l) fetch(w + RING - 1, prv, l);
                 }
-                const float last_scale = scale;
-                scale = s[j & 1] * sw;
+                float last_scale[NS];
+#pragma unroll
+                for (int h = 0; h < NS; ++h) {
+                    last_scale[h] = scale[h];
+                    scale[h] = s[j & 1] * sw[h];
+                }
 #pragma unroll
                 for (int i = 0; i < RT; ++i) d[j & 1][i] = f8_mfma(a[i], b[j & 1], f32x4{0.f, 0.f, 0.f, 0.f});
                 if (j == TT - 1) {
@@ -133,7 +143,7 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) out.acc[i][before][v] = fmaf(last_scale, d[1 - (j & 1)][i][v], out.acc[i][before][v]);
+                    for (int v = 0; v < 4; ++v) out.acc[i][before][v] = fmaf(last_scale[i * NS / RT], d[1 - (j & 1)][i][v], out.acc[i][before][v]);
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -149,7 +159,7 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) out.acc[i][TT - 1][v] = fmaf(scale, d[1][i][v], out.acc[i][TT - 1][v]);
+            for (int v = 0; v < 4; ++v) out.acc[i][TT - 1][v] = fmaf(scale[i * NS / RT], d[1][i][v], out.acc[i][TT - 1][v]);
         __builtin_amdgcn_s_waitcnt(0);
         mfma_settle();
     }

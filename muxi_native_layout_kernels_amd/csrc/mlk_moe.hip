@@ -429,6 +429,15 @@ int launch_moe_align(const int32_t *topk_ids, int n_pairs, int E, const int32_t 
     return MLK_OK;
 }
 
+// The same with the tasks of an expert nearly equal in units of cb_unit blocks.
+int launch_moe_align_even(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
+                          int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, hipStream_t s) {
+    moe_align_kernel<<<1, 1024, 0, s>>>(topk_ids, n_pairs, E, experts_map, sorted, cumsum, padded, experts_ids, (n_pairs + E * 15 + 15) / 16, tasks,
+                                        n_tasks, cb_max, cb_unit, nullptr, id_limit);
+    MLK_LAUNCH_CHECK();
+    return MLK_OK;
+}
+
 // ------------------------------------------------------------ grouped GeMMs
 // The SiLU intermediate between the two GeMMs is private to this file.  It is kept as MFMA
 // activation fragments with the token index outermost inside a block:
