@@ -122,6 +122,12 @@ struct F8Tokens {
     const float *a[TT];
     size_t step;                 // floats from one window's scale to the next
 };
+// The same of one block of tokens that lies in LDS: windows first .. of this lane's token.
+struct F8Staged {
+    const u32x4 *x;              // eight pieces of 16 bytes a window
+    const float *a;
+    int first;
+};
 
 __device__ __forceinline__ void f8_load_weights(F8Operand &o, const uint8_t *tile, int lane) {
     const uint8_t *at = tile + (lane >> 4) * 256 + (lane & 15) * 8;
@@ -135,6 +141,20 @@ __device__ __forceinline__ void f8_load_tokens(F8Operand &o, const uint8_t *row,
     const uint8_t *at = row + (lane >> 4) * 16;
     o.v[0] = ld_global_u32x4(at);
     o.v[1] = ld_global_u32x4(at + 64);
+}
+
+// One window: acc += s a (w . x).
+template <int TT, int R>
+__device__ __forceinline__ void f8_window(f32x4 (&acc)[R][TT], const F8Operand (&w)[R], const float (&s)[R], const F8Operand (&x)[TT], const float (&a)[TT]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            const f32x4 d = f8_mfma(w[r], x[tt], f32x4{0.f, 0.f, 0.f, 0.f});
+            const float c = s[r] * a[tt];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[r][tt][v] = fmaf(c, d[v], acc[r][tt][v]);
+        }
 }
 
 // acc += the windows first, first + step, ... < end.  The loads of U windows are in flight.
@@ -162,15 +182,40 @@ __device__ __forceinline__ void f8_stream(f32x4 (&acc)[R][TT], const F8Rows<R> &
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (i + u < n) {
+                f8_window<TT, R>(acc, w[u], s[u], x[u], a[u]);
+                if (i + u + U < n) load(u, first + (i + u + U) * step);
+            }
+        }
+    }
+}
+
+// The same with the tokens in LDS: `ready` is called behind the first loads and ahead of the first read of a token.
+template <int R, int U, class Ready>
+__device__ __forceinline__ void f8_stream_staged(f32x4 (&acc)[R][1], const F8Rows<R> &rows, const F8Staged &tokens, int first, int end, int step, int lane, Ready ready) {
+    F8Operand w[U][R];
+    float s[U][R];
+    auto load = [&](int u, int t) {
 #pragma unroll
-                for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+            f8_load_weights(w[u][r], rows.w[r] + (size_t)t * kF8TileBytes, lane);
+            s[u][r] = rows.s[r][t];
+        }
+    };
+    const int n = end > first ? (end - first + step - 1) / step : 0;
 #pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) {
-                        const f32x4 d = f8_mfma(w[u][r], x[u][tt], f32x4{0.f, 0.f, 0.f, 0.f});
-                        const float c = s[u][r] * a[u][tt];
+    for (int u = 0; u < U; ++u)
+        if (u < n) load(u, first + u * step);
+    ready();
+    for (int i = 0; i < n; i += U) {
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[r][tt][v] = fmaf(c, d[v], acc[r][tt][v]);
-                    }
+        for (int u = 0; u < U; ++u) {
+            if (i + u < n) {
+                const int t = first + (i + u) * step - tokens.first;
+                F8Operand x[1];
+                x[0].v[0] = tokens.x[t * 8 + (lane >> 4)];
+                x[0].v[1] = tokens.x[t * 8 + 4 + (lane >> 4)];
+                const float a[1] = {tokens.a[t]};
+                f8_window<1, R>(acc, w[u], s[u], x, a);
                 if (i + u + U < n) load(u, first + (i + u + U) * step);
             }
         }

@@ -45,61 +45,175 @@ int launch_quantize_fp8(const void *x, int x_kind, uint8_t *codes, float *scales
 struct F8GemmArgs {
     const uint8_t *A;
     const float *a_scale;        // [ceil(N / 128)][K / 128]
-    const uint8_t *X;            // [M][K]
+    const uint8_t *X;            // [M][K] codes
     const float *x_scale;        // token t's window kb at t xs_t + kb xs_k
     int64_t xs_t, xs_k;
+    const void *raw;             // [M][K] activations that the kernel quantises by itself, or null
     uint16_t *C;
     const uint16_t *bias;
     float alpha;
     int M, N, K;
+    int slices;
+    int rg_each, rg_more;        // row groups of a workgroup; the first rg_more workgroups have one more
+    f32x4 *partial;              // [workgroup (x, z)][slice][cell][two planes of 64 x 8 bytes]
+    int *counters;               // [workgroup (x, z)], zero between calls
 };
 
-// A workgroup owns up to R consecutive row groups and TT blocks of 16 tokens (blockIdx.y); its waves deal the windows of 128 k among themselves (window t to wave
-// t mod waves, so that together they read each row group front to back) and add their sums through LDS in wave order.
-constexpr int kF8Waves = 8;
-template <class T, int TT, int R>
-__global__ void __launch_bounds__(kF8Waves * 64) f8_stream_kernel(F8GemmArgs p) {
-    extern __shared__ f32x4 red[];
+// Bytes of LDS that `m` staged tokens of `windows` windows take: 16 bytes between the rows, so that 16 tokens read different banks, and their scales.
+__host__ __device__ constexpr int f8_staged_pitch(int windows) { return windows * 8 + 1; }      // in pieces of 16 bytes
+__host__ __device__ constexpr size_t f8_staged_bytes(int m, int windows) { return ((size_t)m * f8_staged_pitch(windows) * 16 + (size_t)m * windows * 4 + 15) / 16 * 16; }
+
+// Windows t0 .. t0 + n - 1 of up to 16 tokens into LDS, from codes or (raw) from activations, which are quantised on the way: 16 lanes a block of 128.
+template <class T>
+__device__ __forceinline__ void f8_stage(const F8GemmArgs &p, u32x4 *lds, int t0, int n) {
+    float *scales = reinterpret_cast<float *>(lds + (size_t)p.M * f8_staged_pitch(n));
+    uint8_t *codes = reinterpret_cast<uint8_t *>(lds);
+    const int l = threadIdx.x & 15, lanes = blockDim.x >> 4;
+    for (int b = threadIdx.x >> 4; b < p.M * n; b += lanes) {
+        const int token = b / n, t = b - token * n;
+        const size_t at = (size_t)token * p.K + (size_t)(t0 + t) * kF8K + l * 8;
+        u32x2 q;
+        float scale;
+        if (p.raw) {
+            F8In<T> in;
+            float v[8];
+            in.raw = ld_global_u32x4(reinterpret_cast<const uint16_t *>(p.raw) + at);
+            in.values(v);
+            q = f8_block(v, scale);
+        } else {
+            q = *reinterpret_cast<const u32x2 *>(p.X + at);
+            scale = p.x_scale[token * p.xs_t + (t0 + t) * p.xs_k];
+        }
+        *reinterpret_cast<u32x2 *>(codes + (size_t)token * f8_staged_pitch(n) * 16 + t * kF8K + l * 8) = q;
+        if (l == 0) scales[token * n + t] = scale;
+    }
+}
+
+// Bound by the weights' bytes, with more tokens by what the workgroups read of the activations.  A workgroup owns up to R consecutive row groups, which are dealt out evenly over the
+// grid, and TT blocks of 16 tokens (blockIdx.z); its waves deal the windows of 128 k among themselves (window t to wave t mod waves, so that together they read each row
+// group front to back) and add their sums through LDS in wave order.  `slices` workgroups may share a set of row groups, each on its own range of k: the last one to arrive adds their
+// fp32 sums in the order of k.  STAGED: up to 16 tokens that fit lie in LDS.
+template <class T, int TT, int R, int U, bool STAGED>
+__global__ void __launch_bounds__(512) f8_stream_kernel(F8GemmArgs p) {
+    extern __shared__ u32x4 lds[];
+    __shared__ int s_last;
     constexpr int CELLS = R * TT;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int windows = p.K / kF8K, groups = p.N / 16, rg0 = blockIdx.x * R, m0 = blockIdx.y * (TT * 16);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int windows = p.K / kF8K, b = blockIdx.x, sl = blockIdx.y, m0 = blockIdx.z * (TT * 16);
+    const int rg0 = b * p.rg_each + min(b, p.rg_more), nr = p.rg_each + (b < p.rg_more ? 1 : 0);
+    const int t0 = (int)((long long)windows * sl / p.slices), t1 = (int)((long long)windows * (sl + 1) / p.slices);
     F8Rows<R> rows;
 #pragma unroll
-    for (int r = 0; r < R; ++r) f8_row(rows, r, p.A, p.a_scale, min(rg0 + r, groups - 1), windows);
-    F8Tokens<TT> tokens;
-    tokens.step = p.xs_k;
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-        const int64_t t = min(m0 + tt * 16 + (lane & 15), p.M - 1);
-        tokens.x[tt] = p.X + t * p.K;
-        tokens.a[tt] = p.x_scale + t * p.xs_t;
-    }
+    for (int r = 0; r < R; ++r) f8_row(rows, r, p.A, p.a_scale, rg0 + min(r, nr - 1), windows);
     f32x4 acc[R][TT];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f8_stream<TT, R, (CELLS <= 2 ? 4 : 2)>(acc, rows, tokens, wave, windows, kF8Waves, lane);
+    if constexpr (STAGED) {
+        const int n = t1 - t0, token = min(lane & 15, p.M - 1);
+        F8Staged tokens;
+        tokens.x = lds + (size_t)token * f8_staged_pitch(n);
+        tokens.a = reinterpret_cast<const float *>(lds + (size_t)p.M * f8_staged_pitch(n)) + token * n;
+        tokens.first = t0;
+        f8_stream_staged<R, U>(acc, rows, tokens, t0 + wave, t1, waves, lane, [&]() {
+            f8_stage<T>(p, lds, t0, n);
+            __syncthreads();
+        });
+    } else {
+        F8Tokens<TT> tokens;
+        tokens.step = p.xs_k;
 #pragma unroll
-    for (int c = 0; c < CELLS; ++c) red[(wave * CELLS + c) * 64 + lane] = acc[c / TT][c % TT];
-    __syncthreads();
-    for (int c = wave; c < CELLS; c += kF8Waves) {
+        for (int tt = 0; tt < TT; ++tt) {
+            const int64_t t = min(m0 + tt * 16 + (lane & 15), p.M - 1);
+            tokens.x[tt] = p.X + t * p.K;
+            tokens.a[tt] = p.x_scale + t * p.xs_t;
+        }
+        f8_stream<TT, R, U>(acc, rows, tokens, t0 + wave, t1, waves, lane);
+    }
+    auto store = [&](int c, f32x4 v) {
         const int r = c / TT, token = m0 + (c - r * TT) * 16 + (lane & 15), n = (rg0 + r) * 16 + (lane >> 4) * 4;
-        f32x4 v = red[c * 64 + lane];
-        for (int w = 1; w < kF8Waves; ++w) v += red[(w * CELLS + c) * 64 + lane];
-        if (rg0 + r >= groups || token >= p.M) continue;
+        if (r >= nr || token >= p.M) return;
         float o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = p.alpha * v[i] + (p.bias ? T::to_f32(p.bias[n + i]) : 0.f);
         *reinterpret_cast<u32x2 *>(p.C + (size_t)token * p.N + n) = u32x2{T::from_f32x2(o[0], o[1]), T::from_f32x2(o[2], o[3])};
+    };
+    const int set = blockIdx.z * gridDim.x + blockIdx.x;
+    auto part = [&](int s, int c) { return p.partial + (((size_t)set * p.slices + s) * CELLS + c) * 64; };
+    f32x4 *red = reinterpret_cast<f32x4 *>(lds);
+    if constexpr (STAGED) __syncthreads();                     // the other waves still read the tokens
+#pragma unroll
+    for (int c = 0; c < CELLS; ++c) red[(wave * CELLS + c) * 64 + lane] = acc[c / TT][c % TT];
+    __syncthreads();
+    for (int c = wave; c < CELLS; c += waves) {
+        f32x4 v = red[c * 64 + lane];
+        for (int w = 1; w < waves; ++w) v += red[(w * CELLS + c) * 64 + lane];
+        if (p.slices == 1) store(c, v);
+        else st_agent_planar(part(sl, c), 64, lane, v);
     }
+    if (p.slices == 1) return;
+    // every wave waits for its own stores before the barrier and the arrival is counted behind it: whoever sees all the others can read their sums
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int before = __hip_atomic_fetch_add(&p.counters[set], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = before == p.slices - 1;
+        if (s_last) __hip_atomic_store(&p.counters[set], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    for (int c = wave; c < CELLS; c += waves)
+        store(c, fold_agent_planar([&](int s) { return part(s, c); }, p.slices, 64, lane));
 }
 
-template <class T, int TT, int R>
-static int f8_launch_stream(const F8GemmArgs &a, hipStream_t s) {
-    f8_stream_kernel<T, TT, R><<<dim3((a.N / 16 + R - 1) / R, (a.M + TT * 16 - 1) / (TT * 16)), kF8Waves * 64, (size_t)kF8Waves * R * TT * 1024, s>>>(a);
+struct F8Plan {
+    bool panels;
+    int pr, tb, p3;              // of the panels
+    int r, tt, waves, slices;    // of the streaming kernel: row groups and blocks of tokens of a workgroup
+    bool staged;
+};
+
+template <class T, int TT, int R, int U, bool STAGED>
+static int f8_launch_stream_one(F8GemmArgs a, const F8Plan &pl, hipStream_t s) {
+    const int groups = a.N / 16, wgs = (groups + R - 1) / R, per_slice = (a.K / kF8K + pl.slices - 1) / pl.slices;
+    a.slices = pl.slices;
+    a.rg_each = groups / wgs;
+    a.rg_more = groups % wgs;
+    size_t lds = (size_t)pl.waves * R * TT * 1024;
+    if (STAGED) lds = std::max(lds, f8_staged_bytes(a.M, per_slice));
+    if (lds > 48 * 1024) {
+        static bool ready_on[64] = {};
+        const int rc = panel_lds_attribute(&f8_stream_kernel<T, TT, R, U, STAGED>, 150 * 1024, ready_on);
+        if (rc != MLK_OK) return rc;
+    }
+    f8_stream_kernel<T, TT, R, U, STAGED><<<dim3(wgs, pl.slices, (a.M + TT * 16 - 1) / (TT * 16)), pl.waves * 64, lds, s>>>(a);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
+}
+// Windows in flight: as many as fit the registers of eight waves a CU.
+__host__ __device__ constexpr int f8_ring(int tt, int r, bool staged) { return r == 1 && tt == 1 ? 8 : r * tt <= 2 ? 4 : (r + tt < 8 ? 2 : 1); }
+template <class T>
+static int f8_launch_stream(const F8GemmArgs &a, const F8Plan &pl, hipStream_t s) {
+#define MLK_F8_S(R) if (pl.staged && pl.r == R) return f8_launch_stream_one<T, 1, R, f8_ring(1, R, true), true>(a, pl, s)
+#define MLK_F8_R(TT, R) if (!pl.staged && pl.tt == TT && pl.r == R) return f8_launch_stream_one<T, TT, R, f8_ring(TT, R, false), false>(a, pl, s)
+    MLK_F8_S(1);
+    MLK_F8_S(2);
+    MLK_F8_S(4);
+    MLK_F8_R(1, 1);
+    MLK_F8_R(1, 2);
+    MLK_F8_R(1, 4);
+    MLK_F8_R(1, 8);
+    MLK_F8_R(2, 1);
+    MLK_F8_R(2, 2);
+    MLK_F8_R(2, 4);
+    MLK_F8_R(3, 2);
+    MLK_F8_R(3, 4);
+    MLK_F8_R(4, 2);
+    MLK_F8_R(4, 4);
+#undef MLK_F8_S
+#undef MLK_F8_R
+    return fail(MLK_ERR_INVALID, "gemm fp8: launch parameters");
 }
 
 // Panels move and multiply like those of a 16-bit product of half the k: as many bytes, and the matrix cores take twice as many k in the time.
@@ -108,24 +222,63 @@ extern template int f8_launch_panel<BF16>(const F8PanelArgs &, int, int, hipStre
 size_t panel8_arguments(Panel8Args &p, int m, int n, int k, int pr, int tb, int p3);
 void gemm_plan(int m, int n, int k, bool fp8, bool b_native, int32_t *out);
 
-struct F8Plan {
-    bool panels;
-    int pr, tb, p3;
-};
-static F8Plan f8_plan(int m, int n, int k) {
+constexpr size_t kF8StagedLds = 64 * 1024;      // of staged tokens
+
+static F8Plan f8_plan(int m, int n, int k, bool raw) {
     F8Plan pl = {};
-    // offsets within a panel are 32 bits
-    if (m <= 64 || k >= 1 << 23) return pl;
-    int32_t out[4];
-    gemm_plan(m, n, k / 2, false, false, out);
-    pl.panels = true;
-    pl.pr = out[1] / 2;
-    pl.tb = out[2];
-    pl.p3 = out[3];
+    const int groups = n / 16, windows = k / kF8K;
+    if (m > 64 && k < 1 << 23) {                           // offsets within a panel are 32 bits
+        int32_t out[4];
+        gemm_plan(m, n, k / 2, false, false, out);
+        pl.panels = true;
+        pl.pr = out[1] / 2;
+        pl.tb = out[2];
+        pl.p3 = out[3];
+        return pl;
+    }
+    pl.slices = 1;
+    pl.waves = 8;
+    pl.tt = std::min((m + 15) / 16, 4);
+    pl.staged = m <= 16 && f8_staged_bytes(m, windows) <= kF8StagedLds && (!raw || m * windows <= 256);
+    pl.r = pl.tt > 2 ? 2 : 2;
     return pl;
 }
+
+static size_t f8_partial_bytes(const F8Plan &pl, int m, int n) {
+    if (pl.panels || pl.slices == 1) return 0;
+    const size_t sets = (size_t)((n / 16 + pl.r - 1) / pl.r) * ((m + pl.tt * 16 - 1) / (pl.tt * 16));
+    return sets * pl.slices * pl.r * pl.tt * 1024;
+}
+struct F8Scratch {
+    uint8_t *codes;
+    float *scales;
+    void *partial;
+    size_t partial_bytes;
+};
+// quantize: activations that the call quantises with a launch of its own
+static size_t f8_carve(uint8_t *base, const F8Plan &pl, int m, int n, int k, bool quantize, F8Scratch *out) {
+    Panel8Args p = {};
+    const size_t partial = pl.panels ? panel8_arguments(p, m, n, k / 2, pl.pr, pl.tb, pl.p3) : f8_partial_bytes(pl, m, n);
+    F8Scratch w = {};
+    size_t off = 0;
+    if (quantize || partial > 0) {
+        off = kCounterBytes;
+        auto take = [&](size_t bytes) {
+            uint8_t *ptr = base ? base + off : nullptr;
+            off = (off + bytes + 255) / 256 * 256;
+            return ptr;
+        };
+        w.codes = take(quantize ? (size_t)m * k : 0);
+        w.scales = (float *)take(quantize ? (size_t)m * (k / kF8K) * 4 : 0);
+        w.partial = take(partial);
+        w.partial_bytes = partial;
+    }
+    if (out) *out = w;
+    return off;
+}
+
 template <class T>
-static int f8_launch_gemm(const F8GemmArgs &a, const F8Plan &pl, void *partial, size_t partial_bytes, hipStream_t s) {
+static int f8_launch_gemm(F8GemmArgs a, const F8Plan &pl, const F8Scratch &w, uint8_t *workspace, hipStream_t s) {
     if (pl.panels) {
         F8PanelArgs g = {};
         g.p.A = a.A;
@@ -133,45 +286,17 @@ static int f8_launch_gemm(const F8GemmArgs &a, const F8Plan &pl, void *partial, 
         g.p.C = a.C;
         g.p.bias = a.bias;
         g.p.scale = a.a_scale;
-        g.p.partial = (f32x4 *)partial;
+        g.p.partial = (f32x4 *)w.partial;
         g.p.alpha = a.alpha;
-        if (panel8_arguments(g.p, a.M, a.N, a.K / 2, pl.pr, pl.tb, pl.p3) > partial_bytes) return fail(MLK_ERR_WORKSPACE, "gemm fp8: workspace too small");
+        if (panel8_arguments(g.p, a.M, a.N, a.K / 2, pl.pr, pl.tb, pl.p3) > w.partial_bytes) return fail(MLK_ERR_WORKSPACE, "gemm fp8: workspace too small");
         g.x_scale = a.x_scale;
         g.xs_t = (uint32_t)a.xs_t;
         g.xs_k = (uint32_t)a.xs_k;
         return f8_launch_panel<T>(g, pl.pr, pl.tb, s);
     }
-    if (a.M <= 16) return f8_launch_stream<T, 1, 2>(a, s);
-    return f8_launch_stream<T, 2, 2>(a, s);
-}
-
-struct F8Scratch {
-    uint8_t *codes;
-    float *scales;
-    void *partial;
-    size_t partial_bytes;
-};
-static size_t f8_carve(uint8_t *base, int m, int n, int k, bool quantize, F8Scratch *out) {
-    const F8Plan pl = f8_plan(m, n, k);
-    Panel8Args p = {};
-    const size_t partial = pl.panels ? panel8_arguments(p, m, n, k / 2, pl.pr, pl.tb, pl.p3) : 0;
-    if (!quantize && partial == 0) {
-        if (out) *out = F8Scratch{};
-        return 0;
-    }
-    size_t off = kCounterBytes;
-    auto take = [&](size_t bytes) {
-        uint8_t *ptr = base ? base + off : nullptr;
-        off = (off + bytes + 255) / 256 * 256;
-        return ptr;
-    };
-    F8Scratch w;
-    w.codes = take(quantize ? (size_t)m * k : 0);
-    w.scales = (float *)take(quantize ? (size_t)m * (k / kF8K) * 4 : 0);
-    w.partial = take(partial);
-    w.partial_bytes = partial;
-    if (out) *out = w;
-    return off;
+    a.partial = (f32x4 *)w.partial;
+    a.counters = (int *)workspace;
+    return f8_launch_stream<T>(a, pl, s);
 }
 
 }  // namespace mlk
@@ -192,14 +317,16 @@ int mlk_quantize_fp8(const void *x, int x_kind, void *codes, float *scales, int6
 
 size_t mlk_gemm_fp8_workspace_bytes(int m, int n, int k, int b_kind) {
     if (m <= 0 || n <= 0 || k <= 0 || k % 128 != 0) return 0;
-    return f8_carve(nullptr, m, n, k, b_kind != MLK_FP8_E4M3, nullptr);
+    const bool raw = b_kind != MLK_FP8_E4M3;
+    const F8Plan pl = f8_plan(m, n, k, raw);
+    return f8_carve(nullptr, pl, m, n, k, raw && !pl.staged, nullptr);
 }
 
 int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, int b_kind, const float *b_scale, int64_t b_scale_t, int64_t b_scale_k, void *c,
                           int c_kind, int m, int n, int k, float alpha, const void *bias, void *workspace, size_t workspace_bytes, void *stream) {
     MLK_REQUIRE(c_kind == MLK_F16 || c_kind == MLK_BF16, "gemm fp8: outputs must be fp16 or bf16");
     MLK_REQUIRE(b_kind == MLK_FP8_E4M3 || b_kind == c_kind, "gemm fp8: activations must be e4m3 codes or of the output's kind");
-    MLK_REQUIRE(m >= 0, "gemm fp8: negative token count");
+    MLK_REQUIRE(m >= 0 && m <= (1 << 21), "gemm fp8: 0..2^21 tokens");
     MLK_REQUIRE(n > 0 && k > 0 && n % 16 == 0 && k % 128 == 0 && k < (1 << 25), "gemm fp8: N % 16 and K % 128 must be 0, K below 2^25");
     if (m == 0) return MLK_OK;
     MLK_REQUIRE(a && a_scale && b && c && (b_kind != MLK_FP8_E4M3 || b_scale), "gemm fp8: null pointer");
@@ -219,21 +346,28 @@ int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, in
     p.M = m;
     p.N = n;
     p.K = k;
+    const bool raw = b_kind != MLK_FP8_E4M3;
+    F8Plan pl = f8_plan(m, n, k, raw);
+    if (!raw && pl.panels && (b_scale_t < 0 || b_scale_k < 0 || b_scale_t >= 1 << 21 || b_scale_k >= (1ll << 29) / (k / kF8K))) {
+        pl = F8Plan{};                                         // scales that far apart: the panels' offsets of them are 32 bits
+        pl.r = pl.tt = 2;
+        pl.waves = 8;
+        pl.slices = 1;
+    }
     F8Scratch w;
-    if (f8_carve((uint8_t *)workspace, m, n, k, b_kind != MLK_FP8_E4M3, &w) > 0)
+    if (f8_carve((uint8_t *)workspace, pl, m, n, k, raw && !pl.staged, &w) > 0)
         MLK_REQUIRE(workspace && aligned16(workspace), "gemm fp8: workspace off 16 bytes");
-    F8Plan pl = f8_plan(m, n, k);
-    if (b_kind != MLK_FP8_E4M3) {
+    if (raw && pl.staged) {
+        p.raw = b;
+    } else if (raw) {
         const int rc = launch_quantize_fp8(b, b_kind, w.codes, w.scales, 1, m, m, k, s);
         if (rc != MLK_OK) return rc;
         p.X = w.codes;
         p.x_scale = w.scales;
         p.xs_t = 1;
         p.xs_k = m;
-    } else if (b_scale_t < 0 || b_scale_k < 0 || b_scale_t >= 1 << 21 || b_scale_k >= (1ll << 29) / (k / kF8K)) {
-        pl.panels = false;                                     // scales that far apart: the panels' offsets of them are 32 bits
     }
-    return c_kind == MLK_F16 ? f8_launch_gemm<F16>(p, pl, w.partial, w.partial_bytes, s) : f8_launch_gemm<BF16>(p, pl, w.partial, w.partial_bytes, s);
+    return c_kind == MLK_F16 ? f8_launch_gemm<F16>(p, pl, w, (uint8_t *)workspace, s) : f8_launch_gemm<BF16>(p, pl, w, (uint8_t *)workspace, s);
 }
 
 }  // extern "C"

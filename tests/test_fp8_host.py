@@ -111,8 +111,8 @@ def test_library_refuses_by_itself():
                        ((None, 1, p, p, 1, 1, 1, 128, None), b"null"), ((odd, 1, p, p, 1, 1, 1, 128, None), b"16 bytes"), ((p, 1, odd, p, 1, 1, 1, 128, None), b"16 bytes")):
         assert lib.mlk_quantize_fp8(*args) < 0 and word in lib.mlk_last_error()
     big = 1 << 40
-    good = [p, p, p, 1, None, 0, 0, p, 1, 4, 32, 256, 1.0, None, p, big, None]
-    for at, value, word in ((8, 2, b"fp16 or bf16"), (3, 0, b"output's kind"), (9, -1, b"negative"), (10, 24, b"N % 16"), (11, 192, b"K % 128"), (0, None, b"null"), (1, None, b"null"),
+    good = [p, p, p, 1, None, 0, 0, p, 1, 100, 32, 256, 1.0, None, p, big, None]
+    for at, value, word in ((8, 2, b"fp16 or bf16"), (3, 0, b"output's kind"), (9, -1, b"tokens"), (9, (1 << 21) + 1, b"tokens"), (10, 24, b"N % 16"), (11, 192, b"K % 128"), (0, None, b"null"), (1, None, b"null"),
                             (2, odd, b"16 bytes"), (7, odd, b"16 bytes"), (15, 64, b"too small"), (14, odd, b"workspace")):
         bad = list(good)
         bad[at] = value
@@ -137,7 +137,7 @@ def test_library_refuses_by_itself():
 
 def test_workspaces_grow_with_the_call():
     lib = _lib.load()
-    assert lib.mlk_gemm_fp8_workspace_bytes(4, 32, 256, 1) >= lib.mlk_gemm_counter_bytes() + 4 * 256 + 4 * 2 * 4
+    assert lib.mlk_gemm_fp8_workspace_bytes(100, 32, 256, 1) >= lib.mlk_gemm_counter_bytes() + 100 * 256 + 100 * 2 * 4
     assert lib.mlk_gemm_fp8_workspace_bytes(0, 32, 256, 1) == 0 and lib.mlk_gemm_fp8_workspace_bytes(4, 32, 200, 1) == 0
     last = 0
     for t in (1, 2, 17, 300, 1024, 5000, 100000):

@@ -184,7 +184,8 @@ def test_rows_behind_the_last_one_are_left(mlk, tokens, n, k):
                                    torch.cuda.current_stream().cuda_stream)
     assert rc == 0, lib.mlk_last_error()
     assert torch.equal(c[:tokens], mlk.gemm_layoutA_fp8(A, S, x)) and (c[tokens:] == 7.0).all() and (ws[need:] == 91).all()
-    assert (ws[:lib.mlk_gemm_counter_bytes()] == 0).all()
+    if need:
+        assert (ws[:lib.mlk_gemm_counter_bytes()] == 0).all()
 
 
 @pytest.mark.parametrize("tokens", [1, 40, 300])
