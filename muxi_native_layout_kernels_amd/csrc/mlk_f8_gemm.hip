@@ -195,6 +195,7 @@ static int f8_launch_stream_one(F8GemmArgs a, const F8Plan &pl, hipStream_t s) {
 __host__ __device__ constexpr int f8_ring(int tt, int r, bool staged) { return r == 1 && tt == 1 ? 8 : r * tt <= 2 ? 4 : (r + tt < 8 ? 2 : 1); }
 template <class T>
 static int f8_launch_stream(const F8GemmArgs &a, const F8Plan &pl, hipStream_t s) {
+    // what f8_plan() picks
 #define MLK_F8_S(R) if (pl.staged && pl.r == R) return f8_launch_stream_one<T, 1, R, f8_ring(1, R, true), true>(a, pl, s)
 #define MLK_F8_R(TT, R) if (!pl.staged && pl.tt == TT && pl.r == R) return f8_launch_stream_one<T, TT, R, f8_ring(TT, R, false), false>(a, pl, s)
     MLK_F8_S(1);
@@ -208,9 +209,7 @@ static int f8_launch_stream(const F8GemmArgs &a, const F8Plan &pl, hipStream_t s
     MLK_F8_R(2, 2);
     MLK_F8_R(2, 4);
     MLK_F8_R(3, 2);
-    MLK_F8_R(3, 4);
     MLK_F8_R(4, 2);
-    MLK_F8_R(4, 4);
 #undef MLK_F8_S
 #undef MLK_F8_R
     return fail(MLK_ERR_INVALID, "gemm fp8: launch parameters");
@@ -222,12 +221,26 @@ extern template int f8_launch_panel<BF16>(const F8PanelArgs &, int, int, hipStre
 size_t panel8_arguments(Panel8Args &p, int m, int n, int k, int pr, int tb, int p3);
 void gemm_plan(int m, int n, int k, bool fp8, bool b_native, int32_t *out);
 
-constexpr size_t kF8StagedLds = 64 * 1024;      // of staged tokens
+constexpr size_t kF8StagedLds = 140 * 1024;     // of staged tokens
 
+// Launches that are fastest, timed in graphs on weights from memory (us; g r, tt, waves, slices of the streaming kernel, s: tokens staged, p: panels of 128 rows x 64 tokens).  Activations that
+// are quantised in the call: staged they save a launch and cost every workgroup their quantising.
+//   few row groups       512 x 7168 codes g1,1,4,4 5.5, g1,1,4,1 7 and more; at 16 tokens 6.0; 1280 x 5120 g1,1,8,1 5.8, at 32 tokens g2,2,8,4 7.2, at 64 g2,4,8,4 8.8, p 10.9
+//   one a CU             4096 x 4096 g1,1,8,1 5.7, g2 7.2; at 64 tokens g2,2,8,1 10.1; 4096 x 14336 at 16 tokens g4,1,4,8 14.3, g1,1,8,1 16.3; at 32 g4,2,8,4 16.4, p in eight slices 18.1; at 64 p 19.7, g 21.7
+//   up to two            7168 x 2048 g2,1,4,1 5.5, 8192 x 3584 g2,1,8,1 7.5, w4 8.3; at 64 tokens g4,2,8,1 8.7; 5120 x 13824 at 8 g4,1,4,8 17.5, g2,1,8,1 19.4; at 24 p in six slices 20.0, g2,2,8,4 20.8
+//   up to four           13824 x 5120 at 4 tokens g4,1,8,1 15.2, g2 15.7; at 32 g4,2,8,1 18.0, p in two slices 19.8; at 64 p 21.0, g4,4,8,1 23.7
+//   more                 28672 x 8192 at 8 tokens g8,1,4,1 40.5, g2 41.8, g4 42.0; 37888 x 3584 at 8 g2,1,4,1 27.7, g8 32 and more; 28672 x 8192 at 17 p 43.2, g4,2,4,1 43.9, at 64 p 44.4, g 59.9
+//   staged, quantising   512 x 7168 one token s1,1,8,4 6.0, at 8 7.3 (g 8.6); 28672 x 8192 one token s2,1,4,1 38.4, g 43.4; at 4 both 43.4, at 8 s 49, g 43.8; 7168 x 2048 at 8 s2,1,8,1 7.6, g 8.5; at 16 9.6 and 8.8
+//   staged codes         one token of large weights only: 28672 x 8192 38.1, g 40.8; 4096 x 14336 13.1, g 14.1; 4096 x 4096 6.2, g 5.7
 static F8Plan f8_plan(int m, int n, int k, bool raw) {
     F8Plan pl = {};
-    const int groups = n / 16, windows = k / kF8K;
-    if (m > 64 && k < 1 << 23) {                           // offsets within a panel are 32 bits
+    const int groups = n / 16, windows = k / kF8K, cus = device_cus();
+    const bool panels_fit = k < 1 << 23;                   // offsets within a panel are 32 bits
+    // 96 windows and more: slices bring workgroups of a few row groups back
+    const bool deep = windows >= 96;
+    // up to 256 tokens through few rows: 512 x 7168 at 200 tokens g4,2,8,4 9.4, panels 12.2; at 300 12.5; 4096 x 4096 at 100 g4,2,8,1 12.6, panels 14.9; at 200 16.5
+    const bool narrow = m <= 64 || (m <= 128 && groups <= cus && !deep) || (m <= 256 && groups <= cus / 4);
+    if (!narrow && panels_fit) {
         int32_t out[4];
         gemm_plan(m, n, k / 2, false, false, out);
         pl.panels = true;
@@ -236,11 +249,46 @@ static F8Plan f8_plan(int m, int n, int k, bool raw) {
         pl.p3 = out[3];
         return pl;
     }
-    pl.slices = 1;
-    pl.waves = 8;
-    pl.tt = std::min((m + 15) / 16, 4);
-    pl.staged = m <= 16 && f8_staged_bytes(m, windows) <= kF8StagedLds && (!raw || m * windows <= 256);
-    pl.r = pl.tt > 2 ? 2 : 2;
+    if (panels_fit && ((m > 16 && (groups > 4 * cus || (deep && groups > cus))) || (m > 32 && m <= 64 && (groups > 2 * cus || (deep && groups > cus / 2))))) {
+        const int rows = (n + 127) / 128;
+        pl.panels = true;
+        pl.pr = pl.tb = 1;
+        pl.p3 = std::max(1, std::min(cus / rows, windows / 12));
+        return pl;
+    }
+    auto stream = [&](int r, int tt, int waves, int slices) {
+        pl.r = r;
+        pl.tt = tt;
+        pl.waves = waves;
+        pl.slices = std::max(1, std::min(slices, windows / waves));
+    };
+    const int blocks = std::min((m + 15) / 16, 4), thin = windows >= 32 ? 4 : 1;
+    if (raw ? m <= 16 : m == 1 && (int64_t)n * k >= 50000000) {
+        if (groups <= cus / 4) stream(1, 1, 8, thin);
+        else if (groups <= cus) stream(m * windows > 200 ? 2 : 1, 1, 8, m * windows > 200 ? 4 : 1);
+        else if (groups <= 2 * cus) stream(2, 1, deep ? 4 : 8, deep ? 4 : 1);
+        else if (groups <= 4 * cus && (m > 1 || groups <= 3 * cus)) stream(4, 1, 8, 1);
+        else stream(2, 1, 4, 1);
+        const int each = (windows + pl.slices - 1) / pl.slices;
+        pl.staged = f8_staged_bytes(m, each) <= kF8StagedLds && (m <= 4 || (m * each <= 160 && groups <= 2 * cus));
+        if (pl.staged) return pl;
+    }
+    if (m <= 16) {
+        if (groups <= cus / 4) stream(1, 1, 4, thin);
+        else if (groups <= 2 * cus && deep) stream(4, 1, 4, 8);
+        else if (groups <= cus) stream(1, 1, 8, 1);
+        else if (groups <= 2 * cus) stream(2, 1, windows >= 24 ? 8 : 4, 1);
+        else if (groups <= 4 * cus) stream(4, 1, 8, 1);
+        else stream(windows >= 48 ? 8 : 2, 1, 4, 1);
+    } else {
+        if (groups <= cus / 4 && m <= 64) stream(1, 2, 8, thin);
+        else if (m > 64) stream(m > 128 || groups > cus / 2 ? 4 : 2, 2, 8, groups <= cus / 4 ? thin : 1);
+        else if (groups <= cus / 2) stream(2, blocks, 8, 4);
+        else if (groups <= cus && deep) stream(4, 2, 8, 4);
+        else if (groups <= cus) stream(m <= 32 ? 1 : 2, 2, 8, 1);
+        else if (groups <= 2 * cus && m <= 48) stream(2, blocks, 8, 1);
+        else stream(4, 2, 8, 1);
+    }
     return pl;
 }
 

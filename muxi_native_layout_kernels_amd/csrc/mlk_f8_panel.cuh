@@ -26,7 +26,9 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
     static constexpr int RT = 2 * PR, TT = 2 * TB;                          // row tiles and token blocks of a wave
     static constexpr int A_WIN = 1024 * PR, B_WIN = Tok::B_PAIR, S_WIN = 128;       // granules of 16 bytes: weights, tokens, scales (256 of tokens, 256 of weights)
     static constexpr int WIN = A_WIN + B_WIN + S_WIN;
-    static constexpr int RING = 2 * WIN * 16 > 80 * 1024 ? 2 : 3;
+    // Three windows where they fit: 28672 x 8192 at 300 tokens in panels of 256 x 128 158 us with two, 117; 13824 x 5120 at 100 in 128 x 64 34.0, 23.5.  Four and five bring 3 % at most there, and
+    // two workgroups of 128 x 64 no longer share a CU (20480 x 5120 at 700 tokens 123 us, 136).
+    static constexpr int RING = 3 * WIN * 16 <= (int)kP8MostLds ? 3 : 2;
     static constexpr size_t lds_bytes = (size_t)RING * WIN * 16;
     static constexpr int LOADS = 2 * PR + TB + 1;                           // of a wave and window
     // They go out behind the barrier that frees their buffer: FIRST in the last step of a window, EACH in the steps that follow.  All at once in the last step they hold up every wave of the

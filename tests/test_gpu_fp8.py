@@ -144,6 +144,23 @@ def test_exact_sums_in_panels_of_every_shape(mlk, tokens, n, k):
     assert torch.equal(got, want.to(BF))
 
 
+@pytest.mark.parametrize("k", [512, 4608, 12416])
+@pytest.mark.parametrize("n", [160, 1616, 3216, 4816, 9616, 17616])
+def test_exact_sums_of_every_streaming_launch(mlk, n, k):
+    """Likewise through few tokens: rows for a quarter of the CUs' workgroups to more than four each, k whole and in slices, tokens in LDS and not, quantised in the call and ahead of it."""
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    c = torch.randint(-1, 2, (n, k), generator=g, device="cuda")
+    s = torch.randint(0, 2, ((n + 127) // 128, k // 128), generator=g, device="cuda").float().exp2()
+    w = (c * s.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)).t()
+    A = mlk.pack_layout_a(c.to(F8))
+    for tokens in (1, 2, 4, 7, 16, 17, 32, 33, 48, 64, 65, 100, 128, 129, 200, 256):
+        x = torch.randint(-2, 3, (tokens, k), generator=g, device="cuda").to(BF)
+        bias = torch.randint(-9, 10, (1, n), generator=g, device="cuda").to(BF)
+        want = (x.float() @ w + bias.float()).to(BF)
+        assert torch.equal(mlk.gemm_layoutA_fp8(A, s, x, bias=bias), want), tokens
+        assert torch.equal(mlk.gemm_layoutA_fp8(A, s, *mlk.quantize_fp8(x), bias=bias), want), tokens
+
+
 @pytest.mark.parametrize("tokens", [2, 40, 300])
 def test_a_row_with_nan_or_infinity_keeps_to_itself(mlk, tokens):
     codes, s, _ = weights(528, 1024, 1)
