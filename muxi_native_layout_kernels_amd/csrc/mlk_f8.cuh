@@ -88,6 +88,14 @@ struct F8In<float> {
     }
 };
 
+// Eight codes as bf16, exactly.
+__device__ __forceinline__ u32x4 f8_widen(u32x2 q) {
+    uint32_t a, b, c, d;
+    fp8x4_to_bf16x4_pow2(q[0], 1.f, a, b);
+    fp8x4_to_bf16x4_pow2(q[1], 1.f, c, d);
+    return u32x4{a, b, c, d};
+}
+
 // One block of 128 by 16 lanes of eight values: codes of this lane, scale of the block.
 __device__ __forceinline__ u32x2 f8_block(const float (&v)[8], float &scale) {
     float most = 0.f;
@@ -216,6 +224,109 @@ __device__ __forceinline__ void f8_stream_staged(f32x4 (&acc)[R][1], const F8Row
                 x[0].v[1] = tokens.x[t * 8 + 4 + (lane >> 4)];
                 const float a[1] = {tokens.a[t]};
                 f8_window<1, R>(acc, w[u], s[u], x, a);
+                if (i + u + U < n) load(u, first + (i + u + U) * step);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- products that feed codes
+// The matrix cores add eight products of e4m3 with 13 bits below the largest of them (measured: any shape of the instruction, cut off towards zero), 1.4e-5 of a sum over many in the
+// root mean square.  Against the rounding of a result that is nothing, but what becomes a code next moves to a neighbour wherever a border lies that near: quantised intermediates of 2048 from such sums
+// put the expert layer's result 1.7e-3 off, from sums in 32 bits 5e-5 (fp16 rounds by 2.1e-4, quantising itself costs 2.6e-2).  Where the weights' bytes set the pace the products of
+// gate and up therefore go through v_mfma_f32_16x16x32_bf16, whose products and sums are good to 1e-8: codes are exact in bf16, a window is four of them, and widening the weights hides behind
+// their loads.  Lane 16 q + r holds octet 4 j + q of row r: 512 bytes a load in a row.
+struct F8WideOperand {
+    u32x4 v[4];
+};
+struct F8RawTile {
+    u32x2 v[4];
+};
+__device__ __forceinline__ void f8_load_tile(F8RawTile &o, const uint8_t *tile, int lane) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.v[j] = ld_stream_u32x2(tile + j * 512 + lane * 8);
+}
+__device__ __forceinline__ f32x4 f8_wide_mfma(const F8RawTile &w, const F8WideOperand &x) {
+    f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d = BF16::mfma(f8_widen(w.v[j]), x.v[j], d);
+    return d;
+}
+
+// f8_stream with the tokens' codes as bf16, 256 bytes a window: tokens.x are rows of those.
+template <int TT, int R, int U>
+__device__ __forceinline__ void f8_wide_stream(f32x4 (&acc)[R][TT], const F8Rows<R> &rows, const F8Tokens<TT> &tokens, int first, int end, int step, int lane) {
+    F8RawTile w[U][R];
+    F8WideOperand x[U][TT];
+    float s[U][R], a[U][TT];
+    auto load = [&](int u, int t) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            f8_load_tile(w[u][r], rows.w[r] + (size_t)t * kF8TileBytes, lane);
+            s[u][r] = rows.s[r][t];
+        }
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u][tt].v[j] = ld_global_u32x4(tokens.x[tt] + (size_t)t * 256 + j * 64 + (lane >> 4) * 16);
+            a[u][tt] = tokens.a[tt][(size_t)t * tokens.step];
+        }
+    };
+    const int n = end > first ? (end - first + step - 1) / step : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (u < n) load(u, first + u * step);
+    for (int i = 0; i < n; i += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u < n) {
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) {
+                        const f32x4 d = f8_wide_mfma(w[u][r], x[u][tt]);
+                        const float c = s[u][r] * a[u][tt];
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) acc[r][tt][v] = fmaf(c, d[v], acc[r][tt][v]);
+                    }
+                if (i + u + U < n) load(u, first + (i + u + U) * step);
+            }
+        }
+    }
+}
+// The same of one token in LDS, whose windows begin at `x` (16 pieces of 16 bytes each) with scales at `a`: all sixteen columns are that token.
+template <int R, int U, class Ready>
+__device__ __forceinline__ void f8_wide_stream_staged(f32x4 (&acc)[R][1], const F8Rows<R> &rows, const u32x4 *x, const float *a, int first, int end, int step, int lane,
+                                                      Ready ready) {
+    F8RawTile w[U][R];
+    float s[U][R];
+    auto load = [&](int u, int t) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            f8_load_tile(w[u][r], rows.w[r] + (size_t)t * kF8TileBytes, lane);
+            s[u][r] = rows.s[r][t];
+        }
+    };
+    const int n = end > first ? (end - first + step - 1) / step : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (u < n) load(u, first + u * step);
+    ready();
+    for (int i = 0; i < n; i += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u < n) {
+                const int t = first + (i + u) * step;
+                F8WideOperand o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o.v[j] = x[t * 16 + j * 4 + (lane >> 4)];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const f32x4 d = f8_wide_mfma(w[u][r], o);
+                    const float c = s[u][r] * a[t];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[r][0][v] = fmaf(c, d[v], acc[r][0][v]);
+                }
                 if (i + u + U < n) load(u, first + (i + u + U) * step);
             }
         }

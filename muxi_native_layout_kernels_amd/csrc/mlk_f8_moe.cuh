@@ -9,7 +9,8 @@ namespace mlk {
 struct F8MoeArgs {
     const uint8_t *w1, *w2;      // of expert 0
     const float *s1, *s2;
-    const uint8_t *X;            // [T][H] codes
+    const uint8_t *X;            // [T][H] codes; as bf16 for f8_moe_gate_up_kernel
+    const void *raw;             // [T][H] activations (one token)
     const float *xs;             // [H / 128][T]
     uint16_t *Y;                 // [T][H]
     const int32_t *ids;          // [T * K]
@@ -21,6 +22,7 @@ struct F8MoeArgs {
     const int32_t *n_tasks;
     uint8_t *hbuf;               // [slot][I]
     float *hs;                   // [I / 128][slot]
+    float *hraw;                 // [pick][I] (one token)
     float *obuf;                 // [pair][slice][H]
     int slices;                  // of the down projection's k
 };

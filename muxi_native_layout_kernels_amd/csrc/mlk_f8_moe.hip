@@ -8,11 +8,13 @@
 #include <initializer_list>
 
 #include "mlk_f8_moe.cuh"
+#include "mlk_panel_lds.cuh"
 
 namespace mlk {
 
-int launch_moe_align_even(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
-                          int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, hipStream_t s);
+int launch_moe_align_quantize(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
+                              int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, int32_t *queues, const void *x, int x_kind,
+                              bool wide, void *codes, float *scales, int tokens, int k, hipStream_t s);
 extern template int f8_launch_moe_panels<F16>(const F8MoeArgs &, int, hipStream_t);
 extern template int f8_launch_moe_panels<BF16>(const F8MoeArgs &, int, hipStream_t);
 
@@ -33,7 +35,7 @@ __device__ __forceinline__ void f8_gate_up_blocks(const F8MoeArgs &p, const MoeT
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
         const int pair = p.sorted[(task.block0 + tt) * 16 + t16], row = pair < p.n_pairs ? pair / p.K : 0;
-        tokens.x[tt] = p.X + (size_t)row * p.H;
+        tokens.x[tt] = p.X + (size_t)row * p.H * 2;
         tokens.a[tt] = p.xs + row;
     }
     f32x4 acc[2][TT];
@@ -41,7 +43,7 @@ __device__ __forceinline__ void f8_gate_up_blocks(const F8MoeArgs &p, const MoeT
     for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f8_stream<TT, 2, TT == 1 ? 4 : 2>(acc, rows, tokens, 0, windows, 1, lane);
+    f8_wide_stream<TT, 2, TT == 1 ? 2 : 1>(acc, rows, tokens, 0, windows, 1, lane);
     f32x4 h[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
@@ -66,7 +68,7 @@ __device__ __forceinline__ void f8_gate_up_blocks(const F8MoeArgs &p, const MoeT
         if (wave == 0 && lane < 16) p.hs[(size_t)blockIdx.x * p.slots + slot] = f8_two_to(e);
     }
 }
-__global__ void __launch_bounds__(512) f8_moe_gate_up_kernel(F8MoeArgs p) {
+__global__ void __launch_bounds__(512, 4) f8_moe_gate_up_kernel(F8MoeArgs p) {
     __shared__ float most[8 * 2 * 16];
     if ((int)blockIdx.y >= *p.n_tasks) return;
     const MoeTask task = p.tasks[blockIdx.y];
@@ -127,13 +129,116 @@ __global__ void __launch_bounds__(256) f8_moe_combine_kernel(F8MoeArgs p) {
     for (int n = (blockIdx.y * 256 + threadIdx.x) * 4; n < p.H; n += gridDim.y * 1024) {
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < p.K; ++k) {
+            // loaded whether the pair is here or not: a branch would make every load wait for the one before
             const int pair = tok * p.K + k;
-            if (f8_expert(p, pair) < 0) continue;
             f32x4 v = *reinterpret_cast<const f32x4 *>(p.obuf + (size_t)pair * p.slices * p.H + n);
             for (int sl = 1; sl < p.slices; ++sl) v += *reinterpret_cast<const f32x4 *>(p.obuf + ((size_t)pair * p.slices + sl) * p.H + n);
-            sum += v;
+            const bool here = f8_expert(p, pair) >= 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += here ? v[i] : 0.f;
         }
         *reinterpret_cast<u32x2 *>(p.Y + (size_t)tok * p.H + n) = u32x2{T::from_f32x2(sum[0], sum[1]), T::from_f32x2(sum[2], sum[3])};
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------------- one token
+// Two launches.  gate/up: a workgroup takes a row group of gate and the one of up of a pick, its waves share the k and add their sums in wave order; every workgroup quantises the
+// token by itself, behind its first loads.  The intermediate is left in fp32, as a workgroup has 16 values of a block of 128.
+// down: a workgroup takes a row group through all picks, whose intermediates it quantises into LDS; wave w takes picks w % side, w % side + side, ... and of each the
+// windows of its place among the waves that share it; the weighted sums are added in wave order.
+constexpr int kF8OneWaves = 8;
+constexpr size_t kF8OneLds = 128 * 1024;         // of the token, of the intermediates
+
+template <class T>
+__global__ void __launch_bounds__(512) f8_moe1_gate_up_kernel(F8MoeArgs p) {
+    extern __shared__ u32x4 lds[];
+    const int e = f8_expert(p, blockIdx.y);
+    if (e < 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), windows = p.H / kF8K, rg = blockIdx.x;
+    F8Rows<2> rows;
+    const uint8_t *w = p.w1 + (size_t)e * 2 * p.I * p.H;
+    const float *s = p.s1 + (size_t)e * (p.I / 64) * windows;
+    f8_row(rows, 0, w, s, rg, windows);
+    f8_row(rows, 1, w, s, p.I / 16 + rg, windows);
+    float *scales = reinterpret_cast<float *>(lds + (size_t)windows * 16);
+    f32x4 acc[2][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}, {f32x4{0.f, 0.f, 0.f, 0.f}}};
+    f8_wide_stream_staged<2, 4>(acc, rows, lds, scales, wave, windows, kF8OneWaves, lane, [&]() {
+        const int l = threadIdx.x & 15;
+        for (int b = threadIdx.x >> 4; b < windows; b += kF8OneWaves * 4) {
+            F8In<T> in;
+            in.raw = ld_global_u32x4(reinterpret_cast<const uint16_t *>(p.raw) + (size_t)b * kF8K + l * 8);
+            float v[8], scale;
+            in.values(v);
+            lds[b * 16 + l] = f8_widen(f8_block(v, scale));
+            if (l == 0) scales[b] = scale;
+        }
+        __syncthreads();
+    });
+    __syncthreads();
+    // all columns are the same token: the lanes of column 0 hold four rows each
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds);
+    if ((lane & 15) == 0) {
+        part[(wave * 2) * 4 + (lane >> 4)] = acc[0][0];
+        part[(wave * 2 + 1) * 4 + (lane >> 4)] = acc[1][0];
+    }
+    __syncthreads();
+    const int i = threadIdx.x;
+    if (i < 16) {
+        const float *f = reinterpret_cast<const float *>(part);
+        float g = 0.f, u = 0.f;
+        for (int v = 0; v < kF8OneWaves; ++v) {
+            g += f[v * 32 + i];
+            u += f[v * 32 + 16 + i];
+        }
+        p.hraw[(size_t)blockIdx.y * p.I + rg * 16 + i] = silu_mul(g, u);
+    }
+}
+template <class T>
+__global__ void __launch_bounds__(512) f8_moe1_down_kernel(F8MoeArgs p) {
+    extern __shared__ u32x4 lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), windows = p.I / kF8K, rg = blockIdx.x;
+    float *scales = reinterpret_cast<float *>(lds + (size_t)p.K * windows * 8);
+    const int side = min(p.K, kF8OneWaves), mine = wave % side, place = wave / side, sharing = (kF8OneWaves - mine + side - 1) / side;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int k = mine; k < p.K; k += side) {
+        const int e = f8_expert(p, k);
+        F8Rows<1> rows;
+        f8_row(rows, 0, p.w2 + (size_t)max(e, 0) * p.H * p.I, p.s2 + (size_t)max(e, 0) * (p.H / 128) * windows, rg, windows);
+        F8Staged tokens;
+        tokens.x = lds + (size_t)k * windows * 8;
+        tokens.a = scales + k * windows;
+        tokens.first = 0;
+        f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
+        // a dropped pick has no windows
+        f8_stream_staged<1, 8>(acc, rows, tokens, place, e < 0 ? 0 : windows, sharing, lane, [&]() {
+            if (k != mine) return;
+            const int l = threadIdx.x & 15;
+            for (int b = threadIdx.x >> 4; b < p.K * windows; b += kF8OneWaves * 4) {
+                if (f8_expert(p, b / windows) < 0) continue;                  // its intermediate was not written
+                F8In<float> in;
+                in.lo = *reinterpret_cast<const f32x4 *>(p.hraw + (size_t)b * kF8K + l * 8);
+                in.hi = *reinterpret_cast<const f32x4 *>(p.hraw + (size_t)b * kF8K + l * 8 + 4);
+                float v[8], scale;
+                in.values(v);
+                reinterpret_cast<u32x2 *>(lds)[b * 16 + l] = f8_block(v, scale);
+                if (l == 0) scales[b] = scale;
+            }
+            __syncthreads();
+        });
+        const float wt = e < 0 ? 0.f : T::to_f32(p.wts[k]);
+        if (e >= 0)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) sum[v] = fmaf(wt, acc[0][0][v], sum[v]);
+    }
+    __syncthreads();
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds);
+    if ((lane & 15) == 0) part[wave * 4 + (lane >> 4)] = sum;
+    __syncthreads();
+    const int i = threadIdx.x;
+    if (i < 16) {
+        float v = 0.f;
+        for (int w = 0; w < kF8OneWaves; ++w) v += reinterpret_cast<const float *>(part)[w * 16 + i];
+        p.Y[rg * 16 + i] = (uint16_t)T::from_f32(v);
     }
 }
 
@@ -144,9 +249,12 @@ struct F8MoeWorkspace {
     MoeTask *tasks;
     int32_t *n_tasks, *sorted, *cumsum, *padded, *experts_ids;
     uint8_t *x, *hbuf;
-    float *xs, *hs, *obuf;
+    float *xs, *hs, *hraw, *obuf;
 };
+static size_t f8_one_lds(int picks, int k, bool wide) { return (size_t)picks * k * (wide ? 2 : 1) + (size_t)picks * (k / kF8K) * 4 + 64; }
+
 struct F8MoePlan {
+    bool one;                // one token
     bool panels;
     int blocks;              // of 16 pairs, of a task at most
     int max_tasks, slices;
@@ -154,10 +262,14 @@ struct F8MoePlan {
 static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidden, int inter) {
     F8MoePlan pl = {};
     const int pairs = tokens * topk;
+    pl.slices = 1;
+    if (tokens == 1 && f8_one_lds(1, hidden, true) <= kF8OneLds && f8_one_lds(topk, inter, false) <= kF8OneLds) {
+        pl.one = true;
+        return pl;
+    }
     // with E of the router's experts here that share of the pairs is expected here
     const int here = (int)std::max<int64_t>(1, std::min<int64_t>(pairs, (int64_t)pairs * E / n_router));
     const int reached = std::min(here, E), load = (here + reached - 1) / reached;
-    pl.slices = 1;
     // offsets within an expert's weights and of a token are 32 bits
     pl.panels = load > 32 && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
     pl.blocks = pl.panels ? kF8PanelBlocks : 2;
@@ -173,24 +285,41 @@ static size_t f8_moe_carve(uint8_t *base, const F8MoePlan &pl, int tokens, int E
         off = (off + bytes + 255) / 256 * 256;
         return ptr;
     };
-    F8MoeWorkspace w;
-    w.tasks = (MoeTask *)take(sizeof(MoeTask) * (size_t)(blocks + 1));
-    w.n_tasks = (int32_t *)take(sizeof(int32_t));
-    w.sorted = (int32_t *)take(sizeof(int32_t) * (size_t)slots);
-    w.cumsum = (int32_t *)take(sizeof(int32_t) * (size_t)(E + 1));
-    w.padded = (int32_t *)take(sizeof(int32_t));
-    w.experts_ids = (int32_t *)take(sizeof(int32_t) * (size_t)blocks);
-    w.x = take((size_t)tokens * hidden);
-    w.xs = (float *)take((size_t)tokens * (hidden / kF8K) * 4);
-    w.hbuf = take((size_t)slots * inter);
-    w.hs = (float *)take((size_t)slots * (inter / kF8K) * 4);
-    w.obuf = (float *)take((size_t)pairs * pl.slices * hidden * 4);
+    F8MoeWorkspace w = {};
+    if (pl.one) {
+        w.hraw = (float *)take((size_t)topk * inter * 4);
+    } else {
+        w.tasks = (MoeTask *)take(sizeof(MoeTask) * (size_t)(blocks + 1));
+        w.n_tasks = (int32_t *)take(sizeof(int32_t));
+        w.sorted = (int32_t *)take(sizeof(int32_t) * (size_t)slots);
+        w.cumsum = (int32_t *)take(sizeof(int32_t) * (size_t)(E + 1));
+        w.padded = (int32_t *)take(sizeof(int32_t));
+        w.experts_ids = (int32_t *)take(sizeof(int32_t) * (size_t)blocks);
+        w.x = take((size_t)tokens * hidden * (pl.panels ? 1 : 2));
+        w.xs = (float *)take((size_t)tokens * (hidden / kF8K) * 4);
+        w.hbuf = take((size_t)slots * inter);
+        w.hs = (float *)take((size_t)slots * (inter / kF8K) * 4);
+        w.obuf = (float *)take((size_t)pairs * pl.slices * hidden * 4);
+    }
     if (ws) *ws = w;
     return off;
 }
 
 template <class T>
 static int f8_launch_moe(const F8MoeArgs &a, const F8MoePlan &pl, hipStream_t s) {
+    if (pl.one) {
+        const size_t up = std::max(f8_one_lds(1, a.H, true), (size_t)kF8OneWaves * 128), down = std::max(f8_one_lds(a.K, a.I, false), (size_t)kF8OneWaves * 64);
+        static bool ready_up[64] = {}, ready_down[64] = {};
+        int rc = MLK_OK;
+        if (up > 48 * 1024) rc = panel_lds_attribute(&f8_moe1_gate_up_kernel<T>, 150 * 1024, ready_up);
+        if (rc == MLK_OK && down > 48 * 1024) rc = panel_lds_attribute(&f8_moe1_down_kernel<T>, 150 * 1024, ready_down);
+        if (rc != MLK_OK) return rc;
+        f8_moe1_gate_up_kernel<T><<<dim3(a.I / 16, a.K), kF8OneWaves * 64, up, s>>>(a);
+        MLK_LAUNCH_CHECK();
+        f8_moe1_down_kernel<T><<<a.H / 16, kF8OneWaves * 64, down, s>>>(a);
+        MLK_LAUNCH_CHECK();
+        return MLK_OK;
+    }
     if (pl.panels) {
         const int rc = f8_launch_moe_panels<T>(a, pl.max_tasks, s);
         if (rc != MLK_OK) return rc;
@@ -267,11 +396,13 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
         a.hbuf = ws.hbuf;
         a.hs = ws.hs;
         a.obuf = ws.obuf;
-        int rc = launch_quantize_fp8((const uint16_t *)x + (size_t)t0 * hidden, x_kind, ws.x, ws.xs, 1, a.T, a.T, hidden, s);
-        if (rc != MLK_OK) return rc;
+        a.hraw = ws.hraw;
+        a.raw = (const uint16_t *)x + (size_t)t0 * hidden;
         a.slices = pl.slices;
-        rc = launch_moe_align_even(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks, ws.n_tasks,
-                                   pl.blocks, pl.panels ? 4 : 0, s);
+        int rc = MLK_OK;
+        if (!pl.one)
+            rc = launch_moe_align_quantize(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks, ws.n_tasks,
+                                           pl.blocks, pl.panels ? 4 : 0, nullptr, a.raw, x_kind, !pl.panels, ws.x, ws.xs, a.T, hidden, s);
         if (rc != MLK_OK) return rc;
         rc = x_kind == MLK_F16 ? f8_launch_moe<F16>(a, pl, s) : f8_launch_moe<BF16>(a, pl, s);
         if (rc != MLK_OK) return rc;

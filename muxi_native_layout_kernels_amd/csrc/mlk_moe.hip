@@ -32,6 +32,7 @@
 #include <math.h>
 #include <string.h>
 
+#include "mlk_f8.cuh"
 #include "mlk_moe_args.cuh"
 
 namespace mlk {
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(64) router_kernel(const uint16_t *__restrict__
 // ------------------------------------------------------------------- align
 
 constexpr int kAlignBatch = 8;
-__global__ void __launch_bounds__(1024) moe_align_kernel(const int32_t *__restrict__ topk_ids, int n_pairs, int E,
+__device__ __forceinline__ void moe_align(const int32_t *__restrict__ topk_ids, int n_pairs, int E,
                                                          const int32_t *__restrict__ experts_map,
                                                          int32_t *__restrict__ sorted_ids,
                                                          int32_t *__restrict__ cumsum_out,
@@ -420,6 +421,13 @@ __global__ void __launch_bounds__(1024) moe_align_kernel(const int32_t *__restri
     });
 }
 
+__global__ void __launch_bounds__(1024) moe_align_kernel(const int32_t *__restrict__ topk_ids, int n_pairs, int E, const int32_t *__restrict__ experts_map,
+                                                         int32_t *__restrict__ sorted_ids, int32_t *__restrict__ cumsum_out, int32_t *__restrict__ padded_blocks,
+                                                         int32_t *__restrict__ experts_ids, int max_blocks, MoeTask *__restrict__ tasks, int32_t *__restrict__ n_tasks,
+                                                         int cb_max, int cb_unit, int32_t *__restrict__ queues, int id_limit) {
+    moe_align(topk_ids, n_pairs, E, experts_map, sorted_ids, cumsum_out, padded_blocks, experts_ids, max_blocks, tasks, n_tasks, cb_max, cb_unit, queues, id_limit);
+}
+
 // The alignment for the expert layers of other files: tasks of up to cb_max blocks; ids outside 0 .. id_limit - 1 are dropped.
 int launch_moe_align(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
                      int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, hipStream_t s) {
@@ -429,11 +437,54 @@ int launch_moe_align(const int32_t *topk_ids, int n_pairs, int E, const int32_t 
     return MLK_OK;
 }
 
-// The same with the tasks of an expert nearly equal in units of cb_unit blocks.
-int launch_moe_align_even(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
-                          int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, hipStream_t s) {
-    moe_align_kernel<<<1, 1024, 0, s>>>(topk_ids, n_pairs, E, experts_map, sorted, cumsum, padded, experts_ids, (n_pairs + E * 15 + 15) / 16, tasks,
-                                        n_tasks, cb_max, cb_unit, nullptr, id_limit);
+// The alignment, and beside it in the same launch the activations of the e4m3 expert layers: workgroup 0 aligns, the others quantise 64 blocks of 128 at a time, to codes or (WIDE) to the
+// codes' values in bf16.  Each alone takes 3 to 8 us, most of it waiting.
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(1024) moe_align_quantize_kernel(const int32_t *__restrict__ topk_ids, int n_pairs, int E, const int32_t *__restrict__ experts_map,
+                                                                  int32_t *__restrict__ sorted_ids, int32_t *__restrict__ cumsum_out,
+                                                                  int32_t *__restrict__ padded_blocks, int32_t *__restrict__ experts_ids, int max_blocks,
+                                                                  MoeTask *__restrict__ tasks, int32_t *__restrict__ n_tasks, int cb_max, int cb_unit,
+                                                                  int32_t *__restrict__ queues, int id_limit, const void *__restrict__ x, void *__restrict__ codes,
+                                                                  float *__restrict__ scales, int tokens, int windows) {
+    if (blockIdx.x == 0) {
+        moe_align(topk_ids, n_pairs, E, experts_map, sorted_ids, cumsum_out, padded_blocks, experts_ids, max_blocks, tasks, n_tasks, cb_max, cb_unit, queues, id_limit);
+        return;
+    }
+    const int l = threadIdx.x & 15, each = (gridDim.x - 1) * 64;
+    const int64_t blocks = (int64_t)tokens * windows;
+    for (int64_t b = (int64_t)(blockIdx.x - 1) * 64 + (threadIdx.x >> 4); b < blocks; b += each) {
+        const int64_t token = b / windows;
+        const int kb = (int)(b - token * windows);
+        F8In<T> in;
+        in.load(x, (size_t)b * kF8K + l * 8);
+        float v[8], scale;
+        in.values(v);
+        const u32x2 q = f8_block(v, scale);
+        if constexpr (WIDE) {
+            reinterpret_cast<u32x4 *>(codes)[b * 16 + l] = f8_widen(q);
+        } else {
+            reinterpret_cast<u32x2 *>(codes)[b * 16 + l] = q;
+        }
+        if (l == 0) scales[(size_t)kb * tokens + token] = scale;
+    }
+}
+// Tasks of up to cb_max blocks, with cb_unit those of an expert nearly equal in units of cb_unit blocks; x [tokens][k] to codes (wide: bf16) and scales [k / 128][tokens].
+int launch_moe_align_quantize(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
+                              int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, int32_t *queues, const void *x, int x_kind,
+                              bool wide, void *codes, float *scales, int tokens, int k, hipStream_t s) {
+    const int64_t wgs = ((int64_t)tokens * (k / kF8K) + 63) / 64;
+    const int grid = 1 + (int)(wgs < 1024 ? wgs : 1024);
+#define MLK_ALIGN(T, WIDE)                                                                                                                                              \
+    moe_align_quantize_kernel<T, WIDE><<<grid, 1024, 0, s>>>(topk_ids, n_pairs, E, experts_map, sorted, cumsum, padded, experts_ids, (n_pairs + E * 15 + 15) / 16, tasks, \
+                                                             n_tasks, cb_max, cb_unit, queues, id_limit, x, codes, scales, tokens, k / kF8K)
+    if (x_kind == MLK_F16) {
+        if (wide) MLK_ALIGN(F16, true);
+        else MLK_ALIGN(F16, false);
+    } else {
+        if (wide) MLK_ALIGN(BF16, true);
+        else MLK_ALIGN(BF16, false);
+    }
+#undef MLK_ALIGN
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }
