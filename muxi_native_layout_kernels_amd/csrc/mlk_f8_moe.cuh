@@ -23,6 +23,8 @@ struct F8MoeArgs {
     uint8_t *hbuf;               // [slot][I]
     float *hs;                   // [I / 128][slot]
     float *hraw;                 // [pick][I] (one token)
+    f32x4 *hpart;                // [task][I / 128][row group][block of pairs][64]
+    int32_t *counters;           // [task][I / 128]
     float *obuf;                 // [pair][slice][H]
     int slices;                  // of the down projection's k
 };

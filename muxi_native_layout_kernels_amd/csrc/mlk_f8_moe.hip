@@ -13,46 +13,49 @@
 namespace mlk {
 
 int launch_moe_align_quantize(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
-                              int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, int32_t *queues, const void *x, int x_kind,
+                              int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, int32_t *zero, int n_zero, const void *x, int x_kind,
                               bool wide, void *codes, float *scales, int tokens, int k, hipStream_t s);
 extern template int f8_launch_moe_panels<F16>(const F8MoeArgs &, int, hipStream_t);
 extern template int f8_launch_moe_panels<BF16>(const F8MoeArgs &, int, hipStream_t);
 
 constexpr int kF8MoePairs = 16384;      // routed pairs of a pass: bounds the scratch of long prompts
 
-// Gate/up: wave w of eight streams the w-th row group of gate and the same one of up.
-template <int TT>
-__device__ __forceinline__ void f8_gate_up_blocks(const F8MoeArgs &p, const MoeTask &task, float *most) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t16 = lane & 15;
-    const int windows = p.H / kF8K, rg = blockIdx.x * 8 + wave;
-    const uint8_t *w = p.w1 + (size_t)task.expert * 2 * p.I * p.H;
-    const float *s = p.s1 + (size_t)task.expert * (p.I / 64) * windows;
-    F8Rows<2> rows;
-    f8_row(rows, 0, w, s, rg, windows);
-    f8_row(rows, 1, w, s, p.I / 16 + rg, windows);
-    F8Tokens<TT> tokens;
-    tokens.step = p.T;
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-        const int pair = p.sorted[(task.block0 + tt) * 16 + t16], row = pair < p.n_pairs ? pair / p.K : 0;
-        tokens.x[tt] = p.X + (size_t)row * p.H * 2;
-        tokens.a[tt] = p.xs + row;
+// Gate/up: the four waves share the windows of two row groups of gate and the same two of up.  Bound by the weights' bytes: workgroups of a quarter of a block of 128 keep the card evenly
+// busy, and waves that share windows read far longer pieces than waves with row groups of their own.  The last workgroup of a block to arrive makes the codes, from fp32.
+// A workgroup a block, a row group of gate and of up a wave -> this: 64 experts of 2048 x 768 at 50 tokens 47.5 -> 35.9 us (192 MB of weights), 8 of 4096 x 14336 at 16 tokens
+// 180 -> 159 (940 MB, 5.9 TB/s), at 2 tokens 89 -> 45.
+constexpr int kF8UpWaves = 4, kF8UpGroups = 2, kF8UpParts = 8 / kF8UpGroups;
+__device__ __forceinline__ f32x4 *f8_part(const F8MoeArgs &p, int task, int kb, int r, int tt) {
+    return p.hpart + ((((size_t)task * (p.I / kF8K) + kb) * 8 + r) * 2 + tt) * 64;
+}
+// Whether this workgroup is the last of a block's.  Every wave waits for its own stores before the barrier and the arrival is counted behind it: the last one can read them all.
+__device__ __forceinline__ bool f8_last_part(const F8MoeArgs &p, int task, int kb, int *last) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int *at = &p.counters[task * (p.I / kF8K) + kb];
+        *last = __hip_atomic_fetch_add(at, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == kF8UpParts - 1;
     }
-    f32x4 acc[2][TT];
+    __syncthreads();
+    return *last;
+}
+// Codes and scales of a block of 128 from its values in fp32.
+template <int TT>
+__device__ __forceinline__ void f8_codes_of_block(const F8MoeArgs &p, int block0, int task, int kb, float *most) {
+    constexpr int W = kF8UpWaves, OWN = 8 / W;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t16 = lane & 15;
+    f32x4 h[OWN][TT];
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int j = 0; j < OWN; ++j)
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f8_wide_stream<TT, 2, TT == 1 ? 2 : 1>(acc, rows, tokens, 0, windows, 1, lane);
-    f32x4 h[TT];
+        for (int tt = 0; tt < TT; ++tt) h[j][tt] = ld_agent_planar(f8_part(p, task, kb, j * W + wave, tt), 64, lane);
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
         float a = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            h[tt][i] = silu_mul(acc[0][tt][i], acc[1][tt][i]);
-            a = fmaxf(a, f8_magnitude(h[tt][i]));
-        }
+        for (int j = 0; j < OWN; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a = fmaxf(a, f8_magnitude(h[j][tt][i]));
         a = fmaxf(a, __shfl_xor(a, 16));
         a = fmaxf(a, __shfl_xor(a, 32));
         if (lane < 16) most[(wave * TT + tt) * 16 + t16] = a;
@@ -62,26 +65,76 @@ __device__ __forceinline__ void f8_gate_up_blocks(const F8MoeArgs &p, const MoeT
     for (int tt = 0; tt < TT; ++tt) {
         float a = 0.f;
 #pragma unroll
-        for (int v = 0; v < 8; ++v) a = fmaxf(a, most[(v * TT + tt) * 16 + t16]);
-        const int e = f8_exponent(a), slot = (task.block0 + tt) * 16 + t16;
-        *reinterpret_cast<uint32_t *>(p.hbuf + (size_t)slot * p.I + rg * 16 + (lane >> 4) * 4) = f8_codes(h[tt][0], h[tt][1], h[tt][2], h[tt][3], f8_two_to(-e));
-        if (wave == 0 && lane < 16) p.hs[(size_t)blockIdx.x * p.slots + slot] = f8_two_to(e);
+        for (int v = 0; v < W; ++v) a = fmaxf(a, most[(v * TT + tt) * 16 + t16]);
+        const int e = f8_exponent(a), slot = (block0 + tt) * 16 + t16;
+        const float inverse = f8_two_to(-e);
+#pragma unroll
+        for (int j = 0; j < OWN; ++j)
+            *reinterpret_cast<uint32_t *>(p.hbuf + (size_t)slot * p.I + kb * kF8K + (j * W + wave) * 16 + (lane >> 4) * 4) =
+                f8_codes(h[j][tt][0], h[j][tt][1], h[j][tt][2], h[j][tt][3], inverse);
+        if (wave == 0 && lane < 16) p.hs[(size_t)kb * p.slots + slot] = f8_two_to(e);
     }
 }
-__global__ void __launch_bounds__(512, 4) f8_moe_gate_up_kernel(F8MoeArgs p) {
-    __shared__ float most[8 * 2 * 16];
+template <int TT>
+__device__ __forceinline__ void f8_gate_up_blocks(const F8MoeArgs &p, const MoeTask &task, f32x4 *red, float *most, int *last) {
+    constexpr int G = kF8UpGroups, W = kF8UpWaves, CELLS = G * TT;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t16 = lane & 15;
+    const int windows = p.H / kF8K, kb = blockIdx.x / kF8UpParts, rg0 = blockIdx.x * G;
+    const uint8_t *w = p.w1 + (size_t)task.expert * 2 * p.I * p.H;
+    const float *s = p.s1 + (size_t)task.expert * (p.I / 64) * windows;
+    F8Rows<2 * G> rows;
+#pragma unroll
+    for (int r = 0; r < G; ++r) {
+        f8_row(rows, r, w, s, rg0 + r, windows);
+        f8_row(rows, G + r, w, s, p.I / 16 + rg0 + r, windows);
+    }
+    F8Tokens<TT> tokens;
+    tokens.step = p.T;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        const int pair = p.sorted[(task.block0 + tt) * 16 + t16], row = pair < p.n_pairs ? pair / p.K : 0;
+        tokens.x[tt] = p.X + (size_t)row * p.H * 2;
+        tokens.a[tt] = p.xs + row;
+    }
+    f32x4 acc[2 * G][TT];
+#pragma unroll
+    for (int r = 0; r < 2 * G; ++r)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f8_wide_stream<TT, 2 * G, TT == 1 ? 2 : 1>(acc, rows, tokens, wave, windows, W, lane);
+#pragma unroll
+    for (int c = 0; c < 2 * CELLS; ++c) red[(wave * 2 * CELLS + c) * 64 + lane] = acc[c / TT][c % TT];
+    __syncthreads();
+    if (wave < CELLS) {
+        f32x4 g = red[wave * 64 + lane], u = red[(CELLS + wave) * 64 + lane], h;
+        for (int v = 1; v < W; ++v) {
+            g += red[(v * 2 * CELLS + wave) * 64 + lane];
+            u += red[(v * 2 * CELLS + CELLS + wave) * 64 + lane];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = silu_mul(g[i], u[i]);
+        st_agent_planar(f8_part(p, blockIdx.y, kb, (rg0 & 7) + wave / TT, wave % TT), 64, lane, h);
+    }
+    if (!f8_last_part(p, blockIdx.y, kb, last)) return;
+    f8_codes_of_block<TT>(p, task.block0, blockIdx.y, kb, most);
+}
+__global__ void __launch_bounds__(256) f8_moe_gate_up_kernel(F8MoeArgs p) {
+    __shared__ f32x4 red[kF8UpWaves * 2 * kF8UpGroups * 2 * 64];
+    __shared__ float most[kF8UpWaves * 2 * 16];
+    __shared__ int last;
     if ((int)blockIdx.y >= *p.n_tasks) return;
     const MoeTask task = p.tasks[blockIdx.y];
-    if (task.nblocks == 1) f8_gate_up_blocks<1>(p, task, most);
-    else f8_gate_up_blocks<2>(p, task, most);
+    if (task.nblocks == 1) f8_gate_up_blocks<1>(p, task, red, most, &last);
+    else f8_gate_up_blocks<2>(p, task, red, most, &last);
 }
 
-// Down: the waves share the windows of four row groups and add their sums in wave order.
-constexpr int kF8DownRows = 4;
+// Down: the four waves share the windows of four row groups and add their sums in wave order.  Waves with row groups of their own read 16 rows each at far places and
+// wait longer: 8 experts of 4096 x 14336 at 16 tokens 147 us with two row groups a wave, 72 us shared; 64 of 2048 x 768 at 50 tokens 31.7 and 18.2.
+constexpr int kF8DownRows = 4, kF8DownWaves = 4;
 template <class T, int TT>
 __device__ __forceinline__ void f8_down_blocks(const F8MoeArgs &p, const MoeTask &task, f32x4 *red) {
-    constexpr int R = kF8DownRows, CELLS = R * TT;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, t16 = lane & 15;
+    constexpr int R = kF8DownRows, W = kF8DownWaves, CELLS = R * TT;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t16 = lane & 15;
     const int windows = p.I / kF8K, rg0 = blockIdx.x * R;
     F8Rows<R> rows;
 #pragma unroll
@@ -99,14 +152,14 @@ __device__ __forceinline__ void f8_down_blocks(const F8MoeArgs &p, const MoeTask
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f8_stream<TT, R, TT == 1 ? 2 : 1>(acc, rows, tokens, wave, windows, waves, lane);
+    f8_stream<TT, R, TT == 1 ? 2 : 1>(acc, rows, tokens, wave, windows, W, lane);
 #pragma unroll
     for (int c = 0; c < CELLS; ++c) red[(wave * CELLS + c) * 64 + lane] = acc[c / TT][c % TT];
     __syncthreads();
-    for (int c = wave; c < CELLS; c += waves) {
+    for (int c = wave; c < CELLS; c += W) {
         const int r = c / TT, tt = c - r * TT;
         f32x4 v = red[c * 64 + lane];
-        for (int w = 1; w < waves; ++w) v += red[(w * CELLS + c) * 64 + lane];
+        for (int w = 1; w < W; ++w) v += red[(w * CELLS + c) * 64 + lane];
         const int pair = p.sorted[(task.block0 + tt) * 16 + t16];
         if (pair >= p.n_pairs) continue;
         v *= T::to_f32(p.wts[pair]);
@@ -115,7 +168,7 @@ __device__ __forceinline__ void f8_down_blocks(const F8MoeArgs &p, const MoeTask
 }
 template <class T>
 __global__ void __launch_bounds__(256) f8_moe_down_kernel(F8MoeArgs p) {
-    extern __shared__ f32x4 red[];
+    __shared__ f32x4 red[kF8DownWaves * kF8DownRows * 2 * 64];
     if ((int)blockIdx.y >= *p.n_tasks) return;
     const MoeTask task = p.tasks[blockIdx.y];
     if (task.nblocks == 1) f8_down_blocks<T, 1>(p, task, red);
@@ -125,46 +178,62 @@ __global__ void __launch_bounds__(256) f8_moe_down_kernel(F8MoeArgs p) {
 // y[t] = T(sum over the token's pairs on this card, in pick order)
 template <class T>
 __global__ void __launch_bounds__(256) f8_moe_combine_kernel(F8MoeArgs p) {
-    const int tok = blockIdx.x;
-    for (int n = (blockIdx.y * 256 + threadIdx.x) * 4; n < p.H; n += gridDim.y * 1024) {
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < p.K; ++k) {
-            // loaded whether the pair is here or not: a branch would make every load wait for the one before
-            const int pair = tok * p.K + k;
-            f32x4 v = *reinterpret_cast<const f32x4 *>(p.obuf + (size_t)pair * p.slices * p.H + n);
-            for (int sl = 1; sl < p.slices; ++sl) v += *reinterpret_cast<const f32x4 *>(p.obuf + ((size_t)pair * p.slices + sl) * p.H + n);
-            const bool here = f8_expert(p, pair) >= 0;
+    const int tok = blockIdx.x, lane = threadIdx.x & 63;
+    const size_t step = (size_t)p.slices * p.H;
+    f32x4 v[4];
+    auto load = [&](int k0, int n) {               // four picks' loads in flight, here or not
+        const float *pair = p.obuf + (size_t)tok * p.K * step + n;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += here ? v[i] : 0.f;
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4 *>(pair + min(k0 + j, p.K - 1) * step);
+        for (int sl = 1; sl < p.slices; ++sl)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += *reinterpret_cast<const f32x4 *>(pair + min(k0 + j, p.K - 1) * step + (size_t)sl * p.H);
+    };
+    const int first = (blockIdx.y * 256 + threadIdx.x) * 4;
+    if (first < p.H) load(0, first);
+    const uint64_t here = __ballot(lane < p.K && f8_expert(p, tok * p.K + min(lane, p.K - 1)) >= 0);
+    for (int n = first; n < p.H; n += gridDim.y * 1024) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < p.K; k0 += 4) {
+            if (k0 > 0 || n != first) load(k0, n);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (here >> (k0 + j) & 1) sum += v[j];
         }
         *reinterpret_cast<u32x2 *>(p.Y + (size_t)tok * p.H + n) = u32x2{T::from_f32x2(sum[0], sum[1]), T::from_f32x2(sum[2], sum[3])};
     }
 }
 
 // --------------------------------------------------------------------------------------------------------------- one token
-// Two launches.  gate/up: a workgroup takes a row group of gate and the one of up of a pick, its waves share the k and add their sums in wave order; every workgroup quantises the
-// token by itself, behind its first loads.  The intermediate is left in fp32, as a workgroup has 16 values of a block of 128.
+// Two launches.  gate/up: a workgroup takes two row groups of gate and of up of a pick, its waves share the windows; every workgroup quantises the token by itself, behind its first loads, and all
+// sixteen columns are the token.  The intermediate is left in fp32.
 // down: a workgroup takes a row group through all picks, whose intermediates it quantises into LDS; wave w takes picks w % side, w % side + side, ... and of each the
 // windows of its place among the waves that share it; the weighted sums are added in wave order.
-constexpr int kF8OneWaves = 8;
+constexpr int kF8OneWaves = 8;                   // down
 constexpr size_t kF8OneLds = 128 * 1024;         // of the token, of the intermediates
 
 template <class T>
-__global__ void __launch_bounds__(512) f8_moe1_gate_up_kernel(F8MoeArgs p) {
+__global__ void __launch_bounds__(256) f8_moe1_gate_up_kernel(F8MoeArgs p) {
     extern __shared__ u32x4 lds[];
+    constexpr int G = kF8UpGroups, W = kF8UpWaves;
     const int e = f8_expert(p, blockIdx.y);
     if (e < 0) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), windows = p.H / kF8K, rg = blockIdx.x;
-    F8Rows<2> rows;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), windows = p.H / kF8K, rg0 = blockIdx.x * G;
+    F8Rows<2 * G> rows;
     const uint8_t *w = p.w1 + (size_t)e * 2 * p.I * p.H;
     const float *s = p.s1 + (size_t)e * (p.I / 64) * windows;
-    f8_row(rows, 0, w, s, rg, windows);
-    f8_row(rows, 1, w, s, p.I / 16 + rg, windows);
+#pragma unroll
+    for (int r = 0; r < G; ++r) {
+        f8_row(rows, r, w, s, rg0 + r, windows);
+        f8_row(rows, G + r, w, s, p.I / 16 + rg0 + r, windows);
+    }
     float *scales = reinterpret_cast<float *>(lds + (size_t)windows * 16);
-    f32x4 acc[2][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}, {f32x4{0.f, 0.f, 0.f, 0.f}}};
-    f8_wide_stream_staged<2, 4>(acc, rows, lds, scales, wave, windows, kF8OneWaves, lane, [&]() {
+    f32x4 acc[2 * G][1];
+#pragma unroll
+    for (int r = 0; r < 2 * G; ++r) acc[r][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f8_wide_stream_staged<2 * G, 2>(acc, rows, lds, scales, wave, windows, W, lane, [&]() {
         const int l = threadIdx.x & 15;
-        for (int b = threadIdx.x >> 4; b < windows; b += kF8OneWaves * 4) {
+        for (int b = threadIdx.x >> 4; b < windows; b += W * 4) {
             F8In<T> in;
             in.raw = ld_global_u32x4(reinterpret_cast<const uint16_t *>(p.raw) + (size_t)b * kF8K + l * 8);
             float v[8], scale;
@@ -174,23 +243,20 @@ __global__ void __launch_bounds__(512) f8_moe1_gate_up_kernel(F8MoeArgs p) {
         }
         __syncthreads();
     });
+    __syncthreads();                             // the other waves still read the token
+    f32x4 *red = reinterpret_cast<f32x4 *>(lds);
+#pragma unroll
+    for (int r = 0; r < 2 * G; ++r) red[(wave * 2 * G + r) * 64 + lane] = acc[r][0];
     __syncthreads();
-    // all columns are the same token: the lanes of column 0 hold four rows each
-    f32x4 *part = reinterpret_cast<f32x4 *>(lds);
-    if ((lane & 15) == 0) {
-        part[(wave * 2) * 4 + (lane >> 4)] = acc[0][0];
-        part[(wave * 2 + 1) * 4 + (lane >> 4)] = acc[1][0];
-    }
-    __syncthreads();
-    const int i = threadIdx.x;
-    if (i < 16) {
-        const float *f = reinterpret_cast<const float *>(part);
-        float g = 0.f, u = 0.f;
-        for (int v = 0; v < kF8OneWaves; ++v) {
-            g += f[v * 32 + i];
-            u += f[v * 32 + 16 + i];
+    if (wave < G && (lane & 15) == 0) {
+        f32x4 g = red[wave * 64 + lane], u = red[(G + wave) * 64 + lane], h;
+        for (int v = 1; v < W; ++v) {
+            g += red[(v * 2 * G + wave) * 64 + lane];
+            u += red[(v * 2 * G + G + wave) * 64 + lane];
         }
-        p.hraw[(size_t)blockIdx.y * p.I + rg * 16 + i] = silu_mul(g, u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = silu_mul(g[i], u[i]);
+        *reinterpret_cast<f32x4 *>(p.hraw + (size_t)blockIdx.y * p.I + (rg0 + wave) * 16 + (lane >> 4) * 4) = h;
     }
 }
 template <class T>
@@ -213,15 +279,24 @@ __global__ void __launch_bounds__(512) f8_moe1_down_kernel(F8MoeArgs p) {
         f8_stream_staged<1, 8>(acc, rows, tokens, place, e < 0 ? 0 : windows, sharing, lane, [&]() {
             if (k != mine) return;
             const int l = threadIdx.x & 15;
-            for (int b = threadIdx.x >> 4; b < p.K * windows; b += kF8OneWaves * 4) {
-                if (f8_expert(p, b / windows) < 0) continue;                  // its intermediate was not written
-                F8In<float> in;
-                in.lo = *reinterpret_cast<const f32x4 *>(p.hraw + (size_t)b * kF8K + l * 8);
-                in.hi = *reinterpret_cast<const f32x4 *>(p.hraw + (size_t)b * kF8K + l * 8 + 4);
-                float v[8], scale;
-                in.values(v);
-                reinterpret_cast<u32x2 *>(lds)[b * 16 + l] = f8_block(v, scale);
-                if (l == 0) scales[b] = scale;
+            const int step = kF8OneWaves * 4, blocks = p.K * windows;
+            for (int b0 = threadIdx.x >> 4; b0 < blocks; b0 += 4 * step) {
+                F8In<float> in[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float *at = p.hraw + (size_t)min(b0 + j * step, blocks - 1) * kF8K + l * 8;
+                    in[j].lo = *reinterpret_cast<const f32x4 *>(at);
+                    in[j].hi = *reinterpret_cast<const f32x4 *>(at + 4);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int b = b0 + j * step;
+                    if (b >= blocks) break;
+                    float v[8], scale;
+                    in[j].values(v);
+                    reinterpret_cast<u32x2 *>(lds)[b * 16 + l] = f8_block(v, scale);       // of a dropped pick whatever lay there, which is not read
+                    if (l == 0) scales[b] = scale;
+                }
             }
             __syncthreads();
         });
@@ -250,8 +325,11 @@ struct F8MoeWorkspace {
     int32_t *n_tasks, *sorted, *cumsum, *padded, *experts_ids;
     uint8_t *x, *hbuf;
     float *xs, *hs, *hraw, *obuf;
+    f32x4 *hpart;
+    int32_t *counters;
 };
-static size_t f8_one_lds(int picks, int k, bool wide) { return (size_t)picks * k * (wide ? 2 : 1) + (size_t)picks * (k / kF8K) * 4 + 64; }
+static size_t f8_one_up_lds(int hidden) { return std::max((size_t)hidden * 2 + (size_t)(hidden / kF8K) * 4, (size_t)kF8UpWaves * 2 * kF8UpGroups * 1024); }
+static size_t f8_one_down_lds(int topk, int inter) { return std::max((size_t)topk * inter + (size_t)topk * (inter / kF8K) * 4, (size_t)kF8OneWaves * 64); }
 
 struct F8MoePlan {
     bool one;                // one token
@@ -263,15 +341,17 @@ static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidd
     F8MoePlan pl = {};
     const int pairs = tokens * topk;
     pl.slices = 1;
-    if (tokens == 1 && f8_one_lds(1, hidden, true) <= kF8OneLds && f8_one_lds(topk, inter, false) <= kF8OneLds) {
+    if (tokens == 1 && f8_one_up_lds(hidden) <= kF8OneLds && f8_one_down_lds(topk, inter) <= kF8OneLds) {
         pl.one = true;
         return pl;
     }
     // with E of the router's experts here that share of the pairs is expected here
     const int here = (int)std::max<int64_t>(1, std::min<int64_t>(pairs, (int64_t)pairs * E / n_router));
     const int reached = std::min(here, E), load = (here + reached - 1) / reached;
+    // Panels from 13 pairs an expert on, whose tasks then spend less time on the products than on waiting: 8 experts of 4096 x 14336 streamed -> panels at 12 pairs an expert 264 -> 283 us, at 16
+    // 317 -> 287, at 25 372 -> 295; 128 of 2048 x 768 at 9.4 pairs 141 -> 133, at 19 170 -> 146.
     // offsets within an expert's weights and of a token are 32 bits
-    pl.panels = load > 32 && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
+    pl.panels = load > 12 && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
     pl.blocks = pl.panels ? kF8PanelBlocks : 2;
     pl.max_tasks = std::min(pairs, E + pairs / (16 * pl.blocks));
     return pl;
@@ -288,18 +368,23 @@ static size_t f8_moe_carve(uint8_t *base, const F8MoePlan &pl, int tokens, int E
     F8MoeWorkspace w = {};
     if (pl.one) {
         w.hraw = (float *)take((size_t)topk * inter * 4);
-    } else {
-        w.tasks = (MoeTask *)take(sizeof(MoeTask) * (size_t)(blocks + 1));
-        w.n_tasks = (int32_t *)take(sizeof(int32_t));
-        w.sorted = (int32_t *)take(sizeof(int32_t) * (size_t)slots);
-        w.cumsum = (int32_t *)take(sizeof(int32_t) * (size_t)(E + 1));
-        w.padded = (int32_t *)take(sizeof(int32_t));
-        w.experts_ids = (int32_t *)take(sizeof(int32_t) * (size_t)blocks);
-        w.x = take((size_t)tokens * hidden * (pl.panels ? 1 : 2));
-        w.xs = (float *)take((size_t)tokens * (hidden / kF8K) * 4);
-        w.hbuf = take((size_t)slots * inter);
-        w.hs = (float *)take((size_t)slots * (inter / kF8K) * 4);
-        w.obuf = (float *)take((size_t)pairs * pl.slices * hidden * 4);
+        if (ws) *ws = w;
+        return off;
+    }
+    w.tasks = (MoeTask *)take(sizeof(MoeTask) * (size_t)(blocks + 1));
+    w.n_tasks = (int32_t *)take(sizeof(int32_t));
+    w.sorted = (int32_t *)take(sizeof(int32_t) * (size_t)slots);
+    w.cumsum = (int32_t *)take(sizeof(int32_t) * (size_t)(E + 1));
+    w.padded = (int32_t *)take(sizeof(int32_t));
+    w.experts_ids = (int32_t *)take(sizeof(int32_t) * (size_t)blocks);
+    w.x = take((size_t)tokens * hidden * (pl.panels ? 1 : 2));
+    w.xs = (float *)take((size_t)tokens * (hidden / kF8K) * 4);
+    w.hbuf = take((size_t)slots * inter);
+    w.hs = (float *)take((size_t)slots * (inter / kF8K) * 4);
+    w.obuf = (float *)take((size_t)pairs * pl.slices * hidden * 4);
+    if (!pl.panels) {
+        w.hpart = (f32x4 *)take((size_t)pl.max_tasks * (inter / kF8K) * 16 * 1024);
+        w.counters = (int32_t *)take((size_t)pl.max_tasks * (inter / kF8K) * 4);
     }
     if (ws) *ws = w;
     return off;
@@ -308,13 +393,13 @@ static size_t f8_moe_carve(uint8_t *base, const F8MoePlan &pl, int tokens, int E
 template <class T>
 static int f8_launch_moe(const F8MoeArgs &a, const F8MoePlan &pl, hipStream_t s) {
     if (pl.one) {
-        const size_t up = std::max(f8_one_lds(1, a.H, true), (size_t)kF8OneWaves * 128), down = std::max(f8_one_lds(a.K, a.I, false), (size_t)kF8OneWaves * 64);
+        const size_t up = f8_one_up_lds(a.H), down = f8_one_down_lds(a.K, a.I);
         static bool ready_up[64] = {}, ready_down[64] = {};
         int rc = MLK_OK;
         if (up > 48 * 1024) rc = panel_lds_attribute(&f8_moe1_gate_up_kernel<T>, 150 * 1024, ready_up);
         if (rc == MLK_OK && down > 48 * 1024) rc = panel_lds_attribute(&f8_moe1_down_kernel<T>, 150 * 1024, ready_down);
         if (rc != MLK_OK) return rc;
-        f8_moe1_gate_up_kernel<T><<<dim3(a.I / 16, a.K), kF8OneWaves * 64, up, s>>>(a);
+        f8_moe1_gate_up_kernel<T><<<dim3(a.I / 16 / kF8UpGroups, a.K), kF8UpWaves * 64, up, s>>>(a);
         MLK_LAUNCH_CHECK();
         f8_moe1_down_kernel<T><<<a.H / 16, kF8OneWaves * 64, down, s>>>(a);
         MLK_LAUNCH_CHECK();
@@ -324,9 +409,9 @@ static int f8_launch_moe(const F8MoeArgs &a, const F8MoePlan &pl, hipStream_t s)
         const int rc = f8_launch_moe_panels<T>(a, pl.max_tasks, s);
         if (rc != MLK_OK) return rc;
     } else {
-        f8_moe_gate_up_kernel<<<dim3(a.I / 128, pl.max_tasks), 512, 0, s>>>(a);
+        f8_moe_gate_up_kernel<<<dim3(a.I / 128 * kF8UpParts, pl.max_tasks), kF8UpWaves * 64, 0, s>>>(a);
         MLK_LAUNCH_CHECK();
-        f8_moe_down_kernel<T><<<dim3(a.H / 16 / kF8DownRows, pl.max_tasks), 256, 4 * kF8DownRows * 2 * 1024, s>>>(a);
+        f8_moe_down_kernel<T><<<dim3(a.H / 16 / kF8DownRows, pl.max_tasks), kF8DownWaves * 64, 0, s>>>(a);
         MLK_LAUNCH_CHECK();
     }
     f8_moe_combine_kernel<T><<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, s>>>(a);
@@ -381,11 +466,11 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
     for (int t0 = 0; t0 < n_tokens; t0 += step) {
         a.T = std::min(step, n_tokens - t0);
         a.n_pairs = a.T * topk;
-        a.slots = f8_moe_slots(a.n_pairs, n_experts);
         a.Y = (uint16_t *)y + (size_t)t0 * hidden;
         a.ids = topk_ids + (size_t)t0 * topk;
         a.wts = (const uint16_t *)topk_weights + (size_t)t0 * topk;
         const F8MoePlan pl = f8_moe_plan(a.T, n_experts, n_router_experts, topk, hidden, inter);
+        a.slots = f8_moe_slots(a.n_pairs, n_experts);
         F8MoeWorkspace ws;
         f8_moe_carve((uint8_t *)workspace, pl, a.T, n_experts, topk, hidden, inter, &ws);
         a.X = ws.x;
@@ -397,12 +482,15 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
         a.hs = ws.hs;
         a.obuf = ws.obuf;
         a.hraw = ws.hraw;
+        a.hpart = ws.hpart;
+        a.counters = ws.counters;
         a.raw = (const uint16_t *)x + (size_t)t0 * hidden;
         a.slices = pl.slices;
         int rc = MLK_OK;
         if (!pl.one)
             rc = launch_moe_align_quantize(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks, ws.n_tasks,
-                                           pl.blocks, pl.panels ? 4 : 0, nullptr, a.raw, x_kind, !pl.panels, ws.x, ws.xs, a.T, hidden, s);
+                                           pl.blocks, pl.panels ? 4 : 0, ws.counters, pl.panels ? 0 : pl.max_tasks * (inter / kF8K), a.raw, x_kind,
+                                           !pl.panels, ws.x, ws.xs, a.T, hidden, s);
         if (rc != MLK_OK) return rc;
         rc = x_kind == MLK_F16 ? f8_launch_moe<F16>(a, pl, s) : f8_launch_moe<BF16>(a, pl, s);
         if (rc != MLK_OK) return rc;

@@ -444,10 +444,11 @@ __global__ void __launch_bounds__(1024) moe_align_quantize_kernel(const int32_t 
                                                                   int32_t *__restrict__ sorted_ids, int32_t *__restrict__ cumsum_out,
                                                                   int32_t *__restrict__ padded_blocks, int32_t *__restrict__ experts_ids, int max_blocks,
                                                                   MoeTask *__restrict__ tasks, int32_t *__restrict__ n_tasks, int cb_max, int cb_unit,
-                                                                  int32_t *__restrict__ queues, int id_limit, const void *__restrict__ x, void *__restrict__ codes,
+                                                                  int32_t *__restrict__ zero, int n_zero, int id_limit, const void *__restrict__ x, void *__restrict__ codes,
                                                                   float *__restrict__ scales, int tokens, int windows) {
     if (blockIdx.x == 0) {
-        moe_align(topk_ids, n_pairs, E, experts_map, sorted_ids, cumsum_out, padded_blocks, experts_ids, max_blocks, tasks, n_tasks, cb_max, cb_unit, queues, id_limit);
+        moe_align(topk_ids, n_pairs, E, experts_map, sorted_ids, cumsum_out, padded_blocks, experts_ids, max_blocks, tasks, n_tasks, cb_max, cb_unit, nullptr, id_limit);
+        for (int i = threadIdx.x; i < n_zero; i += 1024) zero[i] = 0;
         return;
     }
     const int l = threadIdx.x & 15, each = (gridDim.x - 1) * 64;
@@ -468,15 +469,15 @@ __global__ void __launch_bounds__(1024) moe_align_quantize_kernel(const int32_t 
         if (l == 0) scales[(size_t)kb * tokens + token] = scale;
     }
 }
-// Tasks of up to cb_max blocks, with cb_unit those of an expert nearly equal in units of cb_unit blocks; x [tokens][k] to codes (wide: bf16) and scales [k / 128][tokens].
+// zero[0 .. n_zero) is cleared.  Tasks of up to cb_max blocks, with cb_unit those of an expert nearly equal in units of cb_unit blocks; x [tokens][k] to codes (wide: bf16) and scales [k / 128][tokens].
 int launch_moe_align_quantize(const int32_t *topk_ids, int n_pairs, int E, const int32_t *experts_map, int id_limit, int32_t *sorted, int32_t *cumsum,
-                              int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, int32_t *queues, const void *x, int x_kind,
+                              int32_t *padded, int32_t *experts_ids, MoeTask *tasks, int32_t *n_tasks, int cb_max, int cb_unit, int32_t *zero, int n_zero, const void *x, int x_kind,
                               bool wide, void *codes, float *scales, int tokens, int k, hipStream_t s) {
     const int64_t wgs = ((int64_t)tokens * (k / kF8K) + 63) / 64;
     const int grid = 1 + (int)(wgs < 1024 ? wgs : 1024);
 #define MLK_ALIGN(T, WIDE)                                                                                                                                              \
     moe_align_quantize_kernel<T, WIDE><<<grid, 1024, 0, s>>>(topk_ids, n_pairs, E, experts_map, sorted, cumsum, padded, experts_ids, (n_pairs + E * 15 + 15) / 16, tasks, \
-                                                             n_tasks, cb_max, cb_unit, queues, id_limit, x, codes, scales, tokens, k / kF8K)
+                                                             n_tasks, cb_max, cb_unit, zero, n_zero, id_limit, x, codes, scales, tokens, k / kF8K)
     if (x_kind == MLK_F16) {
         if (wide) MLK_ALIGN(F16, true);
         else MLK_ALIGN(F16, false);
