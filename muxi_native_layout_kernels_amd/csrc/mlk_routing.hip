@@ -10,8 +10,12 @@
 //   dx_k = (c g_k - sum c g w') w'_k r_k  (renormalised),  c g_k s_k r_k  (sigmoid),  c g_k s_k - s_k sum c g s over the picks, - s_e sum c g s elsewhere  (softmax)
 // with r = 1 - sigmoid, 1 for softmax.
 //
-// 16 lanes take a token (64 where tokens are few), so that a wave takes four at a time and a maximum over the experts is four exchanges within 16 lanes.  After the
-// picks lane k holds pick k.
+// 16 lanes take a token (64 where tokens are few and experts many), so that a wave takes four at a time and a maximum over the experts is four exchanges within 16 lanes.
+// After the picks lane k holds pick k.
+//
+// What bounds it: a chain of dependent steps (the load, of biased ranks the exponentials and divisions in 64 bits, then K times a maximum over registers and lanes), not the bytes.
+// 256 experts in 8 groups, 8 picks, bias, fp32: 16 tokens 7.1 us, 8191 tokens 17.2 us (9 MB; 27.3 with 64-bit exchanges through LDS, all ranks of a group read by its lane and
+// the picks' logits read again from memory); 64 experts, 6 picks, bf16, 16384 tokens 5.7 us.  Gradient of the same: 3.6, 4.6 and 4.4 us, of which a launch is 3.
 #include "mlk_logits.cuh"
 
 namespace mlk {
@@ -31,23 +35,33 @@ struct RouteArgs {
     void *dlogits;               // [T][E]
 };
 
+// A value of another lane of the same 16 (bal_other), of 32 or 64 bits; of lane `from` of the wave.
+template <int STEP, class V>
+__device__ __forceinline__ V route_other(V v) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, bal_other<STEP>(__builtin_bit_cast(float, v)));
+    } else {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __float_as_uint(bal_other<STEP>(__uint_as_float((uint32_t)b))), hi = __float_as_uint(bal_other<STEP>(__uint_as_float((uint32_t)(b >> 32))));
+        return __builtin_bit_cast(V, (uint64_t)hi << 32 | lo);
+    }
+}
+template <class V>
+__device__ __forceinline__ V route_from(V v, int from) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), from));
+    } else {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(V, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, from));
+    }
+}
 template <int LPT, class V, class F>
 __device__ __forceinline__ V route_fold(V v, F f) {
-    if constexpr (sizeof(V) == 4) {
-        auto other = [](V x, auto step) {
-            return __builtin_bit_cast(V, bal_other<decltype(step)::value>(__builtin_bit_cast(float, x)));
-        };
-        v = f(v, other(v, std::integral_constant<int, 1>()));
-        v = f(v, other(v, std::integral_constant<int, 2>()));
-        v = f(v, other(v, std::integral_constant<int, 4>()));
-        v = f(v, other(v, std::integral_constant<int, 8>()));
-        if constexpr (LPT == 64) {
-            v = f(v, __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(float, v), 16)));
-            v = f(v, __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(float, v), 32)));
-        }
-    } else {
-        for (int m = 1; m < LPT; m <<= 1) v = f(v, __shfl_xor(v, m));
-    }
+    v = f(v, route_other<1>(v));
+    v = f(v, route_other<2>(v));
+    v = f(v, route_other<4>(v));
+    v = f(v, route_other<8>(v));
+    if constexpr (LPT == 64) v = f(f(route_from(v, 0), route_from(v, 16)), f(route_from(v, 32), route_from(v, 48)));
     return v;
 }
 template <int LPT>
@@ -98,16 +112,37 @@ __device__ __forceinline__ float route_score(const RouteArgs &p, float x, float 
     return x >= 0.f ? r : expf(x - low) * r;
 }
 
+// The two largest of a group's ranks, as they come.
+template <class V>
+struct RouteBest {
+    V a, b;
+    __device__ __forceinline__ void add(V v) {
+        b = v > a ? a : (v > b ? v : b);
+        a = v > a ? v : a;
+    }
+};
+
+// Places of the ranks and of the groups of a token in LDS; an even number, so that the next token's lie on whole words.
+__host__ __device__ __forceinline__ int route_lds(int E, int G) { return G > 1 ? (E + G + 1) & ~1 : 0; }
+
 // V: what picks are ranked by, float or double.
+// LDS of a token, in V: two largest of each four consecutive experts that share a group (QUADS) or all ranks, a score and then a flag a group; then, of doubles, the logits.
 template <class L, int LPT, int NE, class V>
 __global__ void __launch_bounds__(64) route_kernel(RouteArgs p, bool vec) {
     constexpr int TOK = 64 / LPT;
+    constexpr bool BIASED = sizeof(V) == 8;
     extern __shared__ char lds[];
     const int l = threadIdx.x & (LPT - 1), mine = threadIdx.x / LPT, t = min((int)blockIdx.x * TOK + mine, p.T - 1);
     const bool here = (int)blockIdx.x * TOK + mine < p.T;
     const V lowest = -INFINITY;
-    float x[NE];
+    V *ranks = reinterpret_cast<V *>(lds) + (size_t)mine * route_lds(p.E, p.G), *best = ranks + p.E;
+    float *logits = reinterpret_cast<float *>(reinterpret_cast<V *>(lds) + (size_t)TOK * route_lds(p.E, p.G)) + (size_t)mine * p.E;
+    float x[NE], bias[NE];
+    if constexpr (BIASED)
+#pragma unroll
+        for (int s = 0; s < NE; ++s) bias[s] = p.bias[min(route_expert<LPT>(s, l), p.E - 1)];
     route_load<L, LPT, NE>(p, t, l, vec, x);
+    const bool valid = !p.mask || p.mask[t];
     V rank[NE];
     float top = -INFINITY, sum = 1.f;
 #pragma unroll
@@ -115,22 +150,29 @@ __global__ void __launch_bounds__(64) route_kernel(RouteArgs p, bool vec) {
         top = fmaxf(top, x[s]);
         rank[s] = x[s];
     }
-    if constexpr (sizeof(V) == 8) {
-        top = route_max<LPT>(top);
-        double total = 0.;
+    if constexpr (BIASED) {
+        double total = 1.;
+        if (p.score_fun == 0) {
+            top = route_max<LPT>(top);
+            total = 0.;
 #pragma unroll
-        for (int s = 0; s < NE; ++s) {
-            if (p.score_fun == 0) rank[s] = x[s] == -INFINITY ? 0. : exp((double)x[s] - (double)top);
-            else rank[s] = 1. / (1. + exp(-(double)x[s]));
-            total += rank[s];
+            for (int s = 0; s < NE; ++s) {
+                rank[s] = x[s] == -INFINITY ? 0. : exp((double)x[s] - (double)top);
+                total += rank[s];
+            }
+            total = route_fold<LPT>(total, [](double a, double b) { return a + b; });
+            sum = (float)total;
+#pragma unroll
+            for (int s = 0; s < NE; ++s) rank[s] /= total;
+        } else {
+#pragma unroll
+            for (int s = 0; s < NE; ++s) rank[s] = 1. / (1. + exp(-(double)x[s]));
         }
-        total = p.score_fun == 0 ? route_fold<LPT>(total, [](double a, double b) { return a + b; }) : 1.;
-        sum = (float)total;
 #pragma unroll
         for (int s = 0; s < NE; ++s) {
             const int e = route_expert<LPT>(s, l);
-            const float b = e < p.E ? p.bias[e] : -INFINITY;
-            rank[s] = x[s] == -INFINITY || b != b ? lowest : rank[s] / total + (double)b;
+            if (e < p.E) logits[e] = x[s];
+            rank[s] = e >= p.E || x[s] == -INFINITY || bias[s] != bias[s] ? lowest : rank[s] + (double)bias[s];
         }
     } else if (p.score_fun == 0 && !p.renorm) {
         top = route_max<LPT>(top);
@@ -140,37 +182,59 @@ __global__ void __launch_bounds__(64) route_kernel(RouteArgs p, bool vec) {
         sum = route_sum<LPT>(sum);
     }
     if (p.G > 1) {
-        V *ranks = reinterpret_cast<V *>(lds) + (size_t)mine * (p.E + p.G);
-        V *best = ranks + p.E;
-#pragma unroll
-        for (int s = 0; s < NE; ++s) {
-            const int e = route_expert<LPT>(s, l);
-            if (e < p.E) ranks[e] = rank[s];
-        }
-        wave_lds_sync();
         const int each = p.E / p.G;
-        for (int g = l; g < p.G; g += LPT) {
-            V a = lowest, b = lowest;
-            for (int i = 0; i < each; ++i) {
-                const V v = ranks[g * each + i];
-                b = v > a ? a : (v > b ? v : b);
-                a = v > a ? v : a;
+        const bool quads = (each & 3) == 0;
+        if (quads) {
+#pragma unroll
+            for (int v = 0; v < NE / 4; ++v) {
+                RouteBest<V> q = {rank[4 * v], lowest};
+                for (int i = 1; i < 4; ++i) q.add(rank[4 * v + i]);
+                const int e = route_expert<LPT>(4 * v, l);
+                if (e < p.E) {
+                    ranks[e >> 1] = q.a;
+                    ranks[(e >> 1) + 1] = q.b;
+                }
             }
-            best[g] = sizeof(V) == 8 && b != lowest ? a + b : a;
+        } else {
+#pragma unroll
+            for (int s = 0; s < NE; ++s) {
+                const int e = route_expert<LPT>(s, l);
+                if (e < p.E) ranks[e] = rank[s];
+            }
         }
         wave_lds_sync();
-        // a group stays if fewer than `kept` are better, or as good and lower
-#pragma unroll
-        for (int s = 0; s < NE; ++s) {
-            const int e = route_expert<LPT>(s, l), g = min(e / each, p.G - 1);
+        const int n = quads ? each >> 1 : each;
+        for (int g = l; g < p.G; g += LPT) {
+            RouteBest<V> q = {lowest, lowest};
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) q.add(ranks[g * n + i]);
+            best[g] = BIASED && q.b != lowest ? q.a + q.b : q.a;
+        }
+        wave_lds_sync();
+        // a group stays if fewer than `kept` are better, or as good and lower; the flags take the place of the ranks
+        for (int g = l; g < p.G; g += LPT) {
             const V own = best[g];
             int ahead = 0;
+#pragma unroll 8
             for (int q = 0; q < p.G; ++q) ahead += best[q] > own || (best[q] == own && q < g) ? 1 : 0;
-            if (ahead >= p.kept) rank[s] = lowest;
+            ranks[g] = ahead < p.kept ? (V)0 : lowest;
+        }
+        wave_lds_sync();
+        if (quads) {
+#pragma unroll
+            for (int v = 0; v < NE / 4; ++v) {
+                const V keep = ranks[min(route_expert<LPT>(4 * v, l) / each, p.G - 1)];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rank[4 * v + i] = keep == lowest ? lowest : rank[4 * v + i];
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < NE; ++s) rank[s] = ranks[min(route_expert<LPT>(s, l) / each, p.G - 1)] == lowest ? lowest : rank[s];
         }
     }
     // K times the largest, then the lowest expert that has it
     int id[2] = {-1, -1};
+    float xk[2] = {-INFINITY, -INFINITY};
     for (int k = 0; k < p.K; ++k) {
         V high = rank[0];
 #pragma unroll
@@ -182,21 +246,23 @@ __global__ void __launch_bounds__(64) route_kernel(RouteArgs p, bool vec) {
         at = route_min<LPT>(at);
 #pragma unroll
         for (int s = 0; s < NE; ++s) rank[s] = route_expert<LPT>(s, l) == at ? lowest : rank[s];
-        if ((k & (LPT - 1)) == l) id[k / LPT] = high == lowest ? -1 : at;
+        if ((k & (LPT - 1)) == l && high != lowest) {
+            id[k / LPT] = at;
+            if constexpr (!BIASED) xk[k / LPT] = high;
+        }
     }
-    float xk[2], m = -INFINITY;
+    if constexpr (BIASED) {
+        wave_lds_sync();
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        xk[j] = id[j] >= 0 ? route_logit(L::to_f32(reinterpret_cast<const typename L::V1 *>(p.logits)[(size_t)t * p.E + id[j]])) : -INFINITY;
-        m = fmaxf(m, xk[j]);
+        for (int j = 0; j < 2; ++j)
+            if (id[j] >= 0) xk[j] = logits[id[j]];
     }
-    m = p.renorm ? route_max<LPT>(m) : top;
+    const float m = p.renorm ? route_max<LPT>(fmaxf(xk[0], xk[1])) : top;
     float s[2], rest;
 #pragma unroll
     for (int j = 0; j < 2; ++j) s[j] = route_score(p, xk[j], m, rest);
     if (p.renorm) sum = route_sum<LPT>(s[0] + s[1]);
     else if (p.score_fun != 0) sum = 1.f;
-    const bool valid = !p.mask || p.mask[t];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int k = j * LPT + l;
@@ -291,14 +357,16 @@ __global__ void __launch_bounds__(64) route_grad_kernel(RouteArgs p, bool vec) {
 template <class L, int LPT, int NE>
 static void route_launch(const RouteArgs &a, bool vec, bool grad, hipStream_t s) {
     const int wgs = (a.T + 64 / LPT - 1) / (64 / LPT);
-    const size_t lds = a.G > 1 ? (size_t)(64 / LPT) * (a.E + a.G) * (a.bias ? 8 : 4) : 0;
+    const size_t lds = (size_t)(64 / LPT) * (route_lds(a.E, a.G) * (a.bias ? 8 : 4) + (a.bias ? a.E * 4 : 0));
     if (grad) route_grad_kernel<L, LPT, NE><<<wgs, 64, 0, s>>>(a, vec);
     else if (a.bias) route_kernel<L, LPT, NE, double><<<wgs, 64, lds, s>>>(a, vec);
     else route_kernel<L, LPT, NE, float><<<wgs, 64, lds, s>>>(a, vec);
 }
 template <class L>
 static void route_launch_size(const RouteArgs &a, bool vec, bool grad, hipStream_t s) {
-    if (a.T <= 1024) {
+    // 16 -> 64 lanes a token: 256 experts with bias at 16 tokens 11.1 -> 7.1 us, 2048 12.2 -> 10.4, 4096 12.9 -> 12.8, 8191 17.2 -> 21.1; 512 at 4096 19.2 -> 16.6, 8191
+    // 26.6 -> 28.2; 160 experts without bias at 1024 6.8 -> 5.4; 64 experts at 16 tokens 3.4 -> 4.8
+    if (a.T <= 4096 && a.E > 64) {
         if (a.E <= 256) route_launch<L, 64, 4>(a, vec, grad, s);
         else route_launch<L, 64, 8>(a, vec, grad, s);
     } else if (a.E <= 64) {

@@ -251,7 +251,8 @@ def fused_moe_fp8(
         plan = ops._experts_fp8_plan(hidden_states, w1, w2, ids, weights, w1_scale, w2_scale, experts_map)
         ops._check(((w1.data_ptr() | w2.data_ptr()) & 15) == 0, "w1 and w2 must lie on 16 bytes")
         ids, weights = ops.moe_routing(gating_output, topk, score_func, renormalize, num_expert_group, topk_group, gating_bias, scaling, token_mask)
-        y = ops._experts_fp8_launch(plan, hidden_states, w1, w2, ids, weights.to(hidden_states.dtype), w1_scale, w2_scale, experts_map)
+        with ops._OnDevice(hidden_states):
+            y = ops._experts_fp8_launch(plan, hidden_states, w1, w2, ids, weights.to(hidden_states.dtype), w1_scale, w2_scale, experts_map)
         if expert_load is not None:
             ops.expert_counts(ids, n_experts, out=expert_load)
     return y

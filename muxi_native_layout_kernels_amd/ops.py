@@ -13,6 +13,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib, arg_selector
@@ -26,6 +27,8 @@ def _stream():
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# The current device where a tensor on one shows that torch has set the devices up: torch.cuda.current_device looks for that at every call.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream_of(t):
@@ -605,7 +608,7 @@ class _OnDevice:
     """The library launches on the current device: makes the tensor's device current for the call where it is another one."""
 
     def __init__(self, t):
-        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+        self.guard = torch.cuda.device(t.device) if t.get_device() != _current_device() else None
 
     def __enter__(self):
         if self.guard is not None:
@@ -774,16 +777,23 @@ def quantize_fp8(x):
         _check_tensors(((x, "x"),), x.device)
         rows, k = x.numel() // x.size(-1), x.size(-1)
         plan = _plans[key] = (rows, k, _ACTIVATION_KIND[x.dtype], tuple(x.shape[:-1]) + (k // 128,), _lib.load().mlk_quantize_fp8)
+    if x.get_device() != _current_device():
+        with torch.cuda.device(x.device):
+            return _quantize_launch(plan, x)
+    return _quantize_launch(plan, x)
+
+
+def _quantize_launch(plan, x):
     rows, k, kind, scale_shape, fn = plan
-    with _OnDevice(x):
-        if x.data_ptr() & 15:
-            x = x.clone()
-        codes = torch.empty(x.shape, dtype=_E4M3, device=x.device)
-        scales = torch.empty((k // 128, rows), dtype=torch.float32, device=x.device)
-        rc = fn(x.data_ptr(), kind, codes.data_ptr(), scales.data_ptr(), 1, rows, rows, k, _stream_of(x))
-        if rc != 0:
-            _lib.check(rc, "quantize_fp8")
-    scales = scales.t()
+    x_ptr = x.data_ptr()
+    if x_ptr & 15:
+        x = x.clone()
+        x_ptr = x.data_ptr()
+    codes = torch.empty_like(x, dtype=_E4M3)
+    scales = torch.empty_strided((rows, k // 128), (1, rows), dtype=torch.float32, device=x.device)
+    rc = fn(x_ptr, kind, codes.data_ptr(), scales.data_ptr(), 1, rows, rows, k, _stream_of(x))
+    if rc != 0:
+        _lib.check(rc, "quantize_fp8")
     return codes, scales if x.dim() == 2 else scales.view(scale_shape)
 
 
@@ -823,7 +833,7 @@ def gemm_layoutA_fp8(A, A_Scale, B, B_Scale=None, alpha=1, beta=0, bias=None, ou
         lib = _lib.load()
         plan = _plans[key] = (B.size(0), m, k, kind, c_kind, dtype, lib.mlk_gemm_fp8_workspace_bytes(B.size(0), m, k, kind), lib.mlk_gemm_counter_bytes(),
                               lib.mlk_gemm_layout_a_fp8)
-    if B.get_device() != torch.cuda.current_device():
+    if B.get_device() != _current_device():
         with torch.cuda.device(B.device):
             return _gemm_fp8_launch(plan, A, A_Scale, B, B_Scale, alpha, bias)
     return _gemm_fp8_launch(plan, A, A_Scale, B, B_Scale, alpha, bias)
@@ -1126,7 +1136,8 @@ def fused_experts_fp8(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w
     experts are dropped too; a token without an expert here gets zeros.  Returns y [T, H].  SiLU(gate) * up is quantised from fp32 like the activations, all sums are fp32.  A
     token with an infinity or NaN gives a row of NaN; other rows keep theirs.  No gradient: the result is detached."""
     plan = _experts_fp8_plan(hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map)
-    return _experts_fp8_launch(plan, hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map)
+    with _OnDevice(hidden_states):
+        return _experts_fp8_launch(plan, hidden_states, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map)
 
 
 def _experts_fp8_plan(x, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map):
@@ -1171,18 +1182,17 @@ def _experts_fp8_plan(x, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, exp
 
 def _experts_fp8_launch(plan, x, w1, w2, topk_ids, topk_weights, w1_scale, w2_scale, experts_map):
     T, E, E_router, K, hidden, inter, kind, ws_need, fn = plan
-    with _OnDevice(x):
-        if x.data_ptr() & 15:
-            x = x.clone()
-        y = x.new_empty((T, hidden))
-        if T == 0:
-            return y
-        stream = _stream_of(x)
-        ws = _moe_pool.get(x.device, stream, ws_need)
-        rc = fn(w1.data_ptr(), w1_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), x.data_ptr(), T, E, E_router, K, hidden, inter, kind,
-                topk_ids.data_ptr(), topk_weights.data_ptr(), _ptr(experts_map), y.data_ptr(), ws.data_ptr(), ws.numel(), stream)
-        if rc != 0:
-            _lib.check(rc, "fused_experts_fp8")
+    if x.data_ptr() & 15:
+        x = x.clone()
+    y = x.new_empty((T, hidden))
+    if T == 0:
+        return y
+    stream = _stream_of(x)
+    ws = _moe_pool.get(x.device, stream, ws_need)
+    rc = fn(w1.data_ptr(), w1_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), x.data_ptr(), T, E, E_router, K, hidden, inter, kind, topk_ids.data_ptr(),
+            topk_weights.data_ptr(), _ptr(experts_map), y.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    if rc != 0:
+        _lib.check(rc, "fused_experts_fp8")
     return y
 
 
@@ -1209,29 +1219,41 @@ class _Routing(torch.autograd.Function):
 
 
 def _routing_forward(logits, bias, mask, plan, options):
+    if logits.get_device() != _current_device():
+        with torch.cuda.device(logits.device):
+            return _routing_launch(logits, bias, mask, plan, options)
+    return _routing_launch(logits, bias, mask, plan, options)
+
+
+def _routing_launch(logits, bias, mask, plan, options):
     T, E, K, kind, fn, _ = plan
     score_fun, renormalize, n_groups, topk_groups, scaling = options
-    with _OnDevice(logits):
-        ids = torch.empty((T, K), dtype=torch.int32, device=logits.device)
-        weights = logits.new_empty((T, K))
-        rc = fn(logits.data_ptr(), kind, score_fun, T, E, n_groups, topk_groups, K, _ptr(bias), renormalize, scaling, _ptr(mask), ids.data_ptr(),
-                weights.data_ptr(), _stream_of(logits))
-        if rc != 0:
-            _lib.check(rc, "moe_routing")
+    weights = logits.new_empty((T, K))
+    ids = torch.empty_like(weights, dtype=torch.int32)
+    rc = fn(logits.data_ptr(), kind, score_fun, T, E, n_groups, topk_groups, K, _ptr(bias), renormalize, scaling, _ptr(mask), ids.data_ptr(), weights.data_ptr(),
+            _stream_of(logits))
+    if rc != 0:
+        _lib.check(rc, "moe_routing")
     return ids, weights
 
 
 def _routing_backward(ctx, dweights):
     _check_no_tangent(dweights, "moe_routing")
     logits, ids = ctx.saved_tensors
-    T, E, K, kind, _, fn = ctx.plan
-    score_fun, renormalize, _, _, scaling = ctx.options
-    with _OnDevice(logits):
-        dweights = dweights.contiguous()
-        grad = torch.empty_like(logits)
-        rc = fn(logits.data_ptr(), kind, score_fun, T, E, K, renormalize, scaling, ids.data_ptr(), dweights.data_ptr(), grad.data_ptr(), _stream_of(logits))
-        if rc != 0:
-            _lib.check(rc, "moe_routing")
+    if logits.get_device() != _current_device():
+        with torch.cuda.device(logits.device):
+            return _routing_grad_launch(logits, ids, dweights, ctx.plan, ctx.options)
+    return _routing_grad_launch(logits, ids, dweights, ctx.plan, ctx.options)
+
+
+def _routing_grad_launch(logits, ids, dweights, plan, options):
+    T, E, K, kind, _, fn = plan
+    score_fun, renormalize, _, _, scaling = options
+    dweights = dweights.contiguous()
+    grad = torch.empty_like(logits)
+    rc = fn(logits.data_ptr(), kind, score_fun, T, E, K, renormalize, scaling, ids.data_ptr(), dweights.data_ptr(), grad.data_ptr(), _stream_of(logits))
+    if rc != 0:
+        _lib.check(rc, "moe_routing")
     return grad
 
 
@@ -1343,7 +1365,9 @@ def _balance_launch(logits, ids, mask, cu, score_fun, coef, plan):
 
 
 def _check_no_tangent(t, what):
-    _check(unpack_dual(t).tangent is None, "%s: there is no forward-mode derivative" % what)
+    # outside of a dual level (negative) no tensor has a tangent
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _check(unpack_dual(t).tangent is None, "%s: there is no forward-mode derivative" % what)
 
 
 class _BalanceLoss(torch.autograd.Function):
