@@ -24,7 +24,7 @@ struct F8MoeArgs {
     float *hs;                   // [I / 128][slot]
     float *hraw;                 // [pick][I] (one token)
     f32x4 *hpart;                // [task][I / 128][row group][block of pairs][64]
-    int32_t *counters;           // [task][I / 128]
+    int32_t *counters;           // [task][I / 128]; of the panels the queues
     float *obuf;                 // [pair][slice][H]
     int slices;                  // of the down projection's k
 };

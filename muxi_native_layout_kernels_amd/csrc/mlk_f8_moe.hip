@@ -5,6 +5,7 @@
 // maximum at hand and leaves codes and scale: [slot][I] and [I / 128][slot] (slot = place in the order).  The weighted products of the down projection are kept in fp32
 // [pair][H], and a last launch adds a token's pairs in the order of its picks.
 #include <algorithm>
+#include <cmath>
 #include <initializer_list>
 
 #include "mlk_f8_moe.cuh"
@@ -337,6 +338,15 @@ struct F8MoePlan {
     int blocks;              // of 16 pairs, of a task at most
     int max_tasks, slices;
 };
+// Slices of the down panels' k: two where k is long and they spare a quarter of the rounds over the card, for the sums of a second slice to be written and read.  One -> two at 8 experts of
+// 4096 x 14336 and 64 tokens 109 -> 88 us, 300 198 -> 132, 512 182 -> 167 (through the queues), 2000 379 -> 346 and 9 more to add them; at 1000, where the rounds are the same, 192 -> 210; four 94, 146, 149,
+// 342, 193 and up to 35 more.  Of 2048 x 768 two cost 30 %.
+static int f8_moe_slices(int load, int reached, int hidden, int inter) {
+    if (inter < 64 * kF8K) return 1;
+    const int width = 16 * kF8PanelBlocks, high = load + (int)std::sqrt((double)load);
+    const int items = (hidden + 255) / 256 * reached * ((high + width - 1) / width), cus = device_cus();
+    return (2 * items + cus - 1) / cus * 2 <= (items + cus - 1) / cus * 3 ? 2 : 1;
+}
 static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidden, int inter) {
     F8MoePlan pl = {};
     const int pairs = tokens * topk;
@@ -352,11 +362,14 @@ static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidd
     // 317 -> 287, at 25 372 -> 295; 128 of 2048 x 768 at 9.4 pairs 141 -> 133, at 19 170 -> 146.
     // offsets within an expert's weights and of a token are 32 bits
     pl.panels = load > 12 && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
+    if (pl.panels) pl.slices = f8_moe_slices(load, reached, hidden, inter);
     pl.blocks = pl.panels ? kF8PanelBlocks : 2;
     pl.max_tasks = std::min(pairs, E + pairs / (16 * pl.blocks));
     return pl;
 }
 static int f8_moe_slots(int64_t pairs, int E) { return (int)((pairs + E * 15 + 15) / 16 * 16); }
+// Counters that the alignment clears: the arrivals of the blocks of 128, or the queues of the panels.
+static int f8_moe_counters(const F8MoePlan &pl, int inter) { return pl.panels ? kWideQueues * kWideQueueStep : pl.max_tasks * (inter / kF8K); }
 static size_t f8_moe_carve(uint8_t *base, const F8MoePlan &pl, int tokens, int E, int topk, int hidden, int inter, F8MoeWorkspace *ws) {
     const int64_t pairs = (int64_t)tokens * topk, slots = f8_moe_slots(pairs, E), blocks = slots / 16;
     size_t off = 0;
@@ -382,10 +395,8 @@ static size_t f8_moe_carve(uint8_t *base, const F8MoePlan &pl, int tokens, int E
     w.hbuf = take((size_t)slots * inter);
     w.hs = (float *)take((size_t)slots * (inter / kF8K) * 4);
     w.obuf = (float *)take((size_t)pairs * pl.slices * hidden * 4);
-    if (!pl.panels) {
-        w.hpart = (f32x4 *)take((size_t)pl.max_tasks * (inter / kF8K) * 16 * 1024);
-        w.counters = (int32_t *)take((size_t)pl.max_tasks * (inter / kF8K) * 4);
-    }
+    w.counters = (int32_t *)take((size_t)f8_moe_counters(pl, inter) * 4);
+    if (!pl.panels) w.hpart = (f32x4 *)take((size_t)pl.max_tasks * (inter / kF8K) * 16 * 1024);
     if (ws) *ws = w;
     return off;
 }
@@ -489,7 +500,7 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
         int rc = MLK_OK;
         if (!pl.one)
             rc = launch_moe_align_quantize(a.ids, a.n_pairs, n_experts, experts_map, a.id_limit, ws.sorted, ws.cumsum, ws.padded, ws.experts_ids, ws.tasks, ws.n_tasks,
-                                           pl.blocks, pl.panels ? 4 : 0, ws.counters, pl.panels ? 0 : pl.max_tasks * (inter / kF8K), a.raw, x_kind,
+                                           pl.blocks, pl.panels ? 4 : 0, ws.counters, f8_moe_counters(pl, inter), a.raw, x_kind,
                                            !pl.panels, ws.x, ws.xs, a.T, hidden, s);
         if (rc != MLK_OK) return rc;
         rc = x_kind == MLK_F16 ? f8_launch_moe<F16>(a, pl, s) : f8_launch_moe<BF16>(a, pl, s);

@@ -15,8 +15,19 @@ namespace mlk {
 
 constexpr int kF8OutPitch = 128 + 16;                          // gate/up turn-around buffer: bytes per token
 
-template <int TB>
-__device__ __forceinline__ void f8_moe_gate_up_panel(const F8MoeArgs &p, const MoeTask &tk, int rt, int wave, int lane) {
+// The arguments and the place in the workgroup, taken afresh for every item of a kernel that loops over them (as wide_args does).
+__device__ __forceinline__ const F8MoeArgs &f8_moe_args(int &lane, int &wave) {
+    auto at = __builtin_amdgcn_kernarg_segment_ptr();
+    int tid = threadIdx.x;
+    asm volatile("" : "+s"(at), "+v"(tid));
+    lane = tid & 63;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    return *(const F8MoeArgs *)at;
+}
+
+// Both panels return a ticket of the next item (QUEUE, wave 0).
+template <bool QUEUE, int TB>
+__device__ __forceinline__ int f8_moe_gate_up_panel(const F8MoeArgs &p, const MoeTask &tk, int rt, int wave, int lane) {
     extern __shared__ u32x4 win[];
     using Loop = F8PanelLoop<2, TB, 2>;
     const int wr = wave & 3, wt = wave >> 2, groups_i = p.I >> 4, windows = p.H >> 7, slots = tk.nblocks * 16;
@@ -46,6 +57,7 @@ __device__ __forceinline__ void f8_moe_gate_up_panel(const F8MoeArgs &p, const M
     }
     typename Loop::Acc acc;
     Loop::run(acc, src, 0, windows, wave, lane);
+    const int ticket = QUEUE && wave == 0 ? wide_ticket(p.counters, blockIdx.x & 7, lane) : 0;
     __syncthreads();
     float *most = reinterpret_cast<float *>(win);              // [4][64 TB]
     uint8_t *out = reinterpret_cast<uint8_t *>(win) + 4 * 256 * 4;
@@ -86,10 +98,11 @@ __device__ __forceinline__ void f8_moe_gate_up_panel(const F8MoeArgs &p, const M
         const int slot = it * 64 + (tid >> 3);
         if (slot < slots) *reinterpret_cast<u32x4 *>(dst + (size_t)slot * p.I) = *reinterpret_cast<const u32x4 *>(out + slot * kF8OutPitch + q * 16);
     }
+    return ticket;
 }
 
-template <class T, int TB>
-__device__ __forceinline__ void f8_moe_down_panel(const F8MoeArgs &p, const MoeTask &tk, int rt, int sk, int wave, int lane) {
+template <class T, bool QUEUE, int TB>
+__device__ __forceinline__ int f8_moe_down_panel(const F8MoeArgs &p, const MoeTask &tk, int rt, int sk, int wave, int lane) {
     extern __shared__ u32x4 win[];
     using Loop = F8PanelLoop<2, TB>;
     const int wr = wave & 3, wt = wave >> 2, groups = p.H >> 4, rgp = rt * 16, windows = p.I >> 7, slots = tk.nblocks * 16;
@@ -115,11 +128,12 @@ __device__ __forceinline__ void f8_moe_down_panel(const F8MoeArgs &p, const MoeT
     const int w0 = (int)((long long)sk * windows / p.slices), w1 = (int)((long long)(sk + 1) * windows / p.slices);
     typename Loop::Acc acc;
     Loop::run(acc, src, w0, w1 - w0, wave, lane);
+    const int ticket = QUEUE && wave == 0 ? wide_ticket(p.counters + 8 * kWideQueueStep, blockIdx.x & 7, lane) : 0;
     __syncthreads();
     // every wave turns its 32 rows x 32 TB tokens around in its own part of LDS, one row pair after the other, and stores 128 bytes of a pair with eight lanes
     uint8_t *out = reinterpret_cast<uint8_t *>(win) + (size_t)wave * 128 * kWideDownPitch;
     const int t8 = lane >> 3, q = lane & 7, n0 = (rgp + wr * 4) * 16;
-    if (n0 >= p.H) return;
+    if (n0 >= p.H) return ticket;
     const int32_t *sorted = p.sorted + tk.block0 * 16;
 #pragma unroll
     for (int pr = 0; pr < 2; ++pr) {
@@ -138,6 +152,7 @@ __device__ __forceinline__ void f8_moe_down_panel(const F8MoeArgs &p, const MoeT
         }
         wave_lds_sync();
     }
+    return ticket;
 }
 
 // Task of an item: items of an expert are (rest, task) with tasks fastest, `rest` of `per_task`.
@@ -148,32 +163,69 @@ __device__ __forceinline__ MoeTask f8_moe_item(const F8MoeArgs &p, int item, int
     return p.tasks[t0.first + local % t0.count];
 }
 
-__global__ void __launch_bounds__(512) f8_moe_gate_up_panel_kernel(F8MoeArgs p) {
-    const int row_tiles = p.I >> 7, n = row_tiles * p.n_tasks[0], item = wide_item(blockIdx.x, n);
-    if (item >= n) return;
+template <bool QUEUE>
+__device__ __forceinline__ int f8_moe_gate_up_item(const F8MoeArgs &p, int item, int wave, int lane) {
     int rt;
-    const MoeTask tk = f8_moe_item(p, item, row_tiles, rt);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const MoeTask tk = f8_moe_item(p, item, p.I >> 7, rt);
     switch ((tk.nblocks + 3) >> 2) {
-        case 1: return f8_moe_gate_up_panel<1>(p, tk, rt, wave, lane);
-        case 2: return f8_moe_gate_up_panel<2>(p, tk, rt, wave, lane);
-        case 3: return f8_moe_gate_up_panel<3>(p, tk, rt, wave, lane);
-        default: return f8_moe_gate_up_panel<4>(p, tk, rt, wave, lane);
+        case 1: return f8_moe_gate_up_panel<QUEUE, 1>(p, tk, rt, wave, lane);
+        case 2: return f8_moe_gate_up_panel<QUEUE, 2>(p, tk, rt, wave, lane);
+        case 3: return f8_moe_gate_up_panel<QUEUE, 3>(p, tk, rt, wave, lane);
+        default: return f8_moe_gate_up_panel<QUEUE, 4>(p, tk, rt, wave, lane);
     }
+}
+template <class T, bool QUEUE>
+__device__ __forceinline__ int f8_moe_down_item(const F8MoeArgs &p, int item, int wave, int lane) {
+    int rest;
+    const int row_tiles = (p.H + 255) >> 8;
+    const MoeTask tk = f8_moe_item(p, item, row_tiles * p.slices, rest);
+    const int sk = rest / row_tiles, rt = rest - sk * row_tiles;             // slices slowest: workgroups that run together share a window of k
+    switch ((tk.nblocks + 3) >> 2) {
+        case 1: return f8_moe_down_panel<T, QUEUE, 1>(p, tk, rt, sk, wave, lane);
+        case 2: return f8_moe_down_panel<T, QUEUE, 2>(p, tk, rt, sk, wave, lane);
+        case 3: return f8_moe_down_panel<T, QUEUE, 3>(p, tk, rt, sk, wave, lane);
+        default: return f8_moe_down_panel<T, QUEUE, 4>(p, tk, rt, sk, wave, lane);
+    }
+}
+__device__ __forceinline__ int f8_moe_up_items(const F8MoeArgs &p) { return (p.I >> 7) * p.n_tasks[0]; }
+__device__ __forceinline__ int f8_moe_down_items(const F8MoeArgs &p) { return ((p.H + 255) >> 8) * p.slices * p.n_tasks[0]; }
+
+__global__ void __launch_bounds__(512) f8_moe_gate_up_panel_kernel(F8MoeArgs p) {
+    const int n = f8_moe_up_items(p), item = wide_item(blockIdx.x, n);
+    if (item >= n) return;
+    f8_moe_gate_up_item<false>(p, item, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63);
 }
 template <class T>
 __global__ void __launch_bounds__(512) f8_moe_down_panel_kernel(F8MoeArgs p) {
-    const int row_tiles = (p.H + 255) >> 8, n = row_tiles * p.slices * p.n_tasks[0], item = wide_item(blockIdx.x, n);
+    const int n = f8_moe_down_items(p), item = wide_item(blockIdx.x, n);
     if (item >= n) return;
-    int rest;
-    const MoeTask tk = f8_moe_item(p, item, row_tiles * p.slices, rest);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sk = rest / row_tiles, rt = rest - sk * row_tiles;             // slices slowest: workgroups that run together share a window of k
-    switch ((tk.nblocks + 3) >> 2) {
-        case 1: return f8_moe_down_panel<T, 1>(p, tk, rt, sk, wave, lane);
-        case 2: return f8_moe_down_panel<T, 2>(p, tk, rt, sk, wave, lane);
-        case 3: return f8_moe_down_panel<T, 3>(p, tk, rt, sk, wave, lane);
-        default: return f8_moe_down_panel<T, 4>(p, tk, rt, sk, wave, lane);
+    f8_moe_down_item<T, false>(p, item, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63);
+}
+__global__ void __launch_bounds__(512) f8_moe_gate_up_queue_kernel(F8MoeArgs) {
+    __shared__ int s_item;
+    int ticket = blockIdx.x >> 3;
+    for (;;) {
+        int lane, wave;
+        const F8MoeArgs &p = f8_moe_args(lane, wave);
+        if (wave == 0) s_item = wide_next(p.counters, f8_moe_up_items(p), blockIdx.x & 7, ticket, lane);
+        __syncthreads();                                       // also: LDS is free again
+        const int item = __builtin_amdgcn_readfirstlane(s_item);
+        if (item < 0) return;
+        ticket = f8_moe_gate_up_item<true>(p, item, wave, lane);
+    }
+}
+template <class T>
+__global__ void __launch_bounds__(512) f8_moe_down_queue_kernel(F8MoeArgs) {
+    __shared__ int s_item;
+    int ticket = blockIdx.x >> 3;
+    for (;;) {
+        int lane, wave;
+        const F8MoeArgs &p = f8_moe_args(lane, wave);
+        if (wave == 0) s_item = wide_next(p.counters + 8 * kWideQueueStep, f8_moe_down_items(p), blockIdx.x & 7, ticket, lane);
+        __syncthreads();                                       // also: LDS is free again
+        const int item = __builtin_amdgcn_readfirstlane(s_item);
+        if (item < 0) return;
+        ticket = f8_moe_down_item<T, true>(p, item, wave, lane);
     }
 }
 
@@ -182,16 +234,28 @@ template <int NS>
 constexpr size_t f8_moe_ring() {
     return f8_most(f8_most(F8PanelLoop<2, 1, NS>::lds_bytes, F8PanelLoop<2, 2, NS>::lds_bytes), f8_most(F8PanelLoop<2, 3, NS>::lds_bytes, F8PanelLoop<2, 4, NS>::lds_bytes));
 }
+// Do at most n items of `windows` each go through the queues (wide_queue_pays)?  They cost 1 to 3 us a kernel and win where tasks differ in width: gate/up of 8 experts of 4096 x 14336 at 300
+// tokens 260 -> 198 us, at 512 244 -> 230, at 1000 349 -> 338, at 2000 530 -> 498 (down in two slices 346 -> 321, at 512 192 -> 167), at 128 184 -> 177, at 64 175 -> 178; of 64 experts of 2048 x 1408 at
+// 500 85.6 -> 87.7, at 2000 129 -> 127.
+static inline bool f8_queue_pays(const F8MoeArgs &a, int n, int windows) {
+    const double mean = (double)a.n_pairs / a.E, spread = 3 * sqrt(mean);
+    if (ceil(fmax(mean - spread, 1) / 64) == ceil((mean + spread) / 64)) return false;
+    return n > device_cus() && (double)n / device_cus() * windows >= 80;
+}
 template <class T>
 int f8_launch_moe_panels(const F8MoeArgs &a, int max_tasks, hipStream_t s) {
     constexpr size_t lds_up = f8_most(f8_moe_ring<2>(), 4096 + 256 * kF8OutPitch), lds_down = f8_most(f8_moe_ring<1>(), kWideDownOut);
-    static bool ready_up[64] = {}, ready_down[64] = {};
-    int rc = panel_lds_attribute(&f8_moe_gate_up_panel_kernel, lds_up, ready_up);
-    if (rc == MLK_OK) rc = panel_lds_attribute(&f8_moe_down_panel_kernel<T>, lds_down, ready_down);
+    static bool ready_up[2][64] = {}, ready_down[2][64] = {};
+    const int items_up = (a.I >> 7) * max_tasks, items_down = ((a.H + 255) >> 8) * a.slices * max_tasks;
+    const bool queue_up = f8_queue_pays(a, items_up, a.H >> 7), queue_down = f8_queue_pays(a, items_down, (a.I >> 7) / a.slices);
+    const auto up = queue_up ? &f8_moe_gate_up_queue_kernel : &f8_moe_gate_up_panel_kernel;
+    const auto down = queue_down ? &f8_moe_down_queue_kernel<T> : &f8_moe_down_panel_kernel<T>;
+    int rc = panel_lds_attribute(up, lds_up, ready_up[queue_up]);
+    if (rc == MLK_OK) rc = panel_lds_attribute(down, lds_down, ready_down[queue_down]);
     if (rc != MLK_OK) return rc;
-    f8_moe_gate_up_panel_kernel<<<((a.I >> 7) * max_tasks + 7) / 8 * 8, 512, lds_up, s>>>(a);
+    up<<<queue_up ? device_cus() : (items_up + 7) / 8 * 8, 512, lds_up, s>>>(a);
     MLK_LAUNCH_CHECK();
-    f8_moe_down_panel_kernel<T><<<(((a.H + 255) >> 8) * a.slices * max_tasks + 7) / 8 * 8, 512, lds_down, s>>>(a);
+    down<<<queue_down ? device_cus() : (items_down + 7) / 8 * 8, 512, lds_down, s>>>(a);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }
