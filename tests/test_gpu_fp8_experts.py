@@ -152,3 +152,105 @@ def test_router_products_and_load_together(mlk):
     assert torch.equal(y, z)
     assert torch.equal(load.cpu(), torch.bincount(ids[:33].cpu().flatten().long(), minlength=E).int())
     assert torch.equal(load, mlk.expert_counts(ids, E))
+
+
+def exact_layer(T, E, K, H, I, dtype, held, seed):
+    """Arguments of a layer whose every step is exact, and its result: a gate of 32, 64 or 128 for a token, whose SiLU is the gate itself in fp32; up sums of at most 16 products of -1, 0
+    and 1, so that an intermediate is a small integer times a power of two, which a code holds; -1, 0 and 1 again in the down projection, whose sums are whole numbers below 2^24; scales
+    and weights are powers of two."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def ints(low, high, shape):
+        return torch.randint(low, high, shape, generator=g, device="cuda")
+
+    code = torch.tensor([0xb8, 0, 0x38], dtype=torch.uint8, device="cuda")                    # -1, 0, 1
+    w1 = torch.zeros((held, 2 * I, H), dtype=torch.uint8, device="cuda")
+    w1[:, :I, 0] = 0x38
+    w1[:, I:].scatter_(2, ints(1, H, (held, I, 16)), code[ints(0, 2, (held, I, 16)) * 2])
+    w2 = code[ints(0, 3, (held, H, I))]
+    s1 = torch.ones((held, 2 * I // 128, H // 128), device="cuda")
+    s1[:, I // 128:] = 2.0 ** ints(0, 2, (held, I // 128, 1))
+    s2 = 2.0 ** ints(0, 2, (held, H // 128, I // 128)).float()
+    x = ints(-1, 2, (T, H)).float()
+    x[:, 0] = 2.0 ** ints(5, 8, (T,))
+    # some experts are picked far more often than others: tasks of every width
+    order = torch.rand((T, E), generator=g, device="cuda") + torch.rand(E, generator=g, device="cuda") * 0.6
+    ids = order.topk(K, dim=-1)[1].int()
+    wts = 2.0 ** ints(-2, 2, (T, K)).float()
+    place = None
+    if held < E:
+        place = torch.full((E,), -1, dtype=torch.int32, device="cuda")
+        place[torch.randperm(E, generator=g, device="cuda")[:held]] = torch.arange(held, dtype=torch.int32, device="cuda")
+    y = torch.zeros((T, H), dtype=torch.float64, device="cuda")
+    local = ids if place is None else place[ids.long()]
+    table = torch.zeros(256, device="cuda")
+    table[0xb8], table[0x38] = -1.0, 1.0
+    for e in range(held):
+        token, pick = (local == e).nonzero(as_tuple=True)
+        up = (x[token] @ table[w1[e, I:].int()].t()) * s1[e, I // 128:, 0].repeat_interleave(128)
+        h = up * x[token, :1]
+        down = table[w2[e].int()] * s2[e].repeat_interleave(128, 0).repeat_interleave(128, 1)
+        y.index_add_(0, token, (h.double() @ down.double().t()) * wts[token, pick].double().unsqueeze(1))
+    assert y.abs().max() < 2 ** 24
+    y = y.to(dtype)
+    assert y.isfinite().all()
+    return (x.to(dtype), w1, w2, ids, wts.to(dtype), s1, s2, place), y
+
+
+@pytest.mark.parametrize("T,E,K,H,I,held", [
+    (1, 8, 2, 4096, 14336, 8), (1, 40, 12, 512, 384, 40), (1, 16, 9, 1024, 256, 5), (2, 8, 2, 4096, 1024, 8), (16, 8, 2, 1152, 2048, 8), (50, 64, 8, 2048, 768, 32),
+    (30, 2, 1, 896, 640, 2), (100, 5, 2, 640, 1024, 5), (300, 8, 2, 1024, 8192, 8), (513, 8, 2, 4096, 14336, 8), (700, 3, 1, 640, 1024, 3), (900, 8, 2, 4096, 14336, 3),
+    (2048, 8, 2, 4096, 8192, 8), (2500, 16, 8, 256, 384, 16), (1300, 300, 4, 256, 128, 77)])
+def test_exact_layers(mlk, T, E, K, H, I, held):
+    """Each plan at sizes where it is taken: one token, streamed, panels of every width, the queues, two slices of the down projection, several passes."""
+    (x, w1, w2, ids, wts, s1, s2, place), want = exact_layer(T, E, K, H, I, BF, held, T + E)
+    a1, a2 = mlk.pack_layout_a(w1), mlk.pack_layout_a(w2)
+    del w1, w2
+    got = mlk.fused_experts_fp8(x, a1, a2, ids, wts, s1, s2, experts_map=place)
+    assert torch.equal(got, want)
+    for n in (1, T // 2, T - 1):                                                              # other plans of the same layer
+        if n > 0:
+            assert torch.equal(mlk.fused_experts_fp8(x[:n], a1, a2, ids[:n], wts[:n], s1, s2, experts_map=place), want[:n])
+
+
+@pytest.mark.parametrize("T", [1, 30, 200])
+def test_two_graphs_of_a_stream_and_eager_calls(mlk, T):
+    """They share the stream's workspace, which a layer leaves with whatever it last held."""
+    layers = [on_gpu(mlk, *layer(4, 256, 128, s)[:2]) for s in (1, 5)]
+    ids, wts = (t.cuda() for t in routing(T, 4, 2, BF, T))
+    x = randn((T, 256), BF, 1.0, 2).cuda()
+
+    def run(i):
+        a1, a2, s1, s2 = layers[i]
+        return mlk.fused_experts_fp8(x, a1, a2, ids, wts, s1, s2)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        run(0)
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=side):
+            outs.append(run(i))
+    for i in range(3):
+        x.copy_(randn((T, 256), BF, 1.0 + i, 10 + i))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+            eager = run(1)
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], run(0)) and torch.equal(outs[1], run(1)) and torch.equal(eager, outs[1])
+
+
+def test_a_long_batch_leaves_nothing_behind_for_a_short_one(mlk):
+    """One workspace, every plan in turn: counters and queues are cleared by the call that uses them."""
+    l1, l2, _, _ = layer(8, 256, 256, 9)
+    a1, a2, s1, s2 = on_gpu(mlk, l1, l2)
+    x = randn((2300, 256), BF, 1.0, 3).cuda()
+    ids, wts = (t.cuda() for t in routing(2300, 8, 8, BF, 4))
+    alone = {}
+    for n in (2300, 1, 40, 7, 300, 2, 2300, 7, 1, 40):
+        y = mlk.fused_experts_fp8(x[:n], a1, a2, ids[:n], wts[:n], s1, s2)
+        assert torch.equal(y, alone.setdefault(n, y))
