@@ -261,3 +261,26 @@ def test_offsets_past_32_bits(mlk):
         tol = alone(x[:tokens].abs()).float() * 2.0 ** -14 + 2.0 ** -7 * last.float().abs()
         assert ((got[:, -32:].float() - last.float()).abs() <= tol).all()
         del got
+
+
+@pytest.mark.parametrize("tokens", [300, 1 << 21])
+def test_scales_far_apart(mlk, tokens):
+    """A step from block to block that 32 bits do not hold (here of a single block, so that nothing lies there) leaves the panels, whose offsets of scales are 32 bits."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    A = torch.randint(0, 120, (2, 16, 16, 8), generator=g, device="cuda", dtype=torch.uint8)
+    S, a = torch.rand((1, 1), generator=g, device="cuda") + 0.5, torch.rand((tokens, 1), generator=g, device="cuda")
+    q = torch.randint(0, 120, (tokens, 128), generator=g, device="cuda", dtype=torch.uint8)
+    far = a.as_strided((tokens, 1), (1, 1 << 30))
+    assert torch.equal(mlk.gemm_layoutA_fp8(A, S, q, far), mlk.gemm_layoutA_fp8(A, S, q, a))
+
+
+def test_calls_from_a_backward_pass_and_under_grad(mlk):
+    """The products are detached: they neither record nor stop a graph around them."""
+    codes, s, _ = weights(144, 256, 1)
+    A, S = mlk.pack_layout_a(codes.cuda()), s.cuda()
+    x = randn((3, 256), BF, 1.0, 1).cuda().requires_grad_(True)
+    y = mlk.gemm_layoutA_fp8(A, S, x)
+    q, a = mlk.quantize_fp8(x)
+    assert not y.requires_grad and not a.requires_grad and not q.requires_grad
+    (x.float().sum() + y.float().sum()).backward()
+    assert (x.grad == 1).all()
