@@ -5,6 +5,10 @@
 // down     256 outputs; `slices` workgroups share the k of a panel, the weighted sums of each go to obuf [pair][slice][H] in fp32.
 //
 // Order of the work: (expert, row tile, task of the expert) with tasks fastest, one line cut into eight equal runs, one per XCD: the tasks of an expert share a row tile's weights in one L2.
+//
+// 8 experts of 4096 x 14336, two picks, 1000 tokens: gate/up 317 us (470 GFLOP), down 210 (235 GFLOP).  The loop runs as fast as in the linear layers' panels (1.87 us a window of 256 x 256); what is
+// missing to their rate are columns that pad a task to 64, an item's first loads and its epilogue, beside which the CU has nothing else (32 windows an item in gate/up), and of the down projection
+// the 16 x 11 panels for 256 CUs.
 #pragma once
 
 #include "mlk_f8_moe.cuh"

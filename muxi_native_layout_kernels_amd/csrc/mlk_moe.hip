@@ -438,7 +438,7 @@ int launch_moe_align(const int32_t *topk_ids, int n_pairs, int E, const int32_t 
 }
 
 // The alignment, and beside it in the same launch the activations of the e4m3 expert layers: workgroup 0 aligns, the others quantise 64 blocks of 128 at a time, to codes or (WIDE) to the
-// codes' values in bf16.  Each alone takes 3 to 8 us, most of it waiting.
+// codes' values in bf16.  Each alone takes 3 to 8 us, most of it waiting; together 5.2 at 50 tokens of 2048 with 8 picks, 9.2 at 1000 of 4096 with 2.
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(1024) moe_align_quantize_kernel(const int32_t *__restrict__ topk_ids, int n_pairs, int E, const int32_t *__restrict__ experts_map,
                                                                   int32_t *__restrict__ sorted_ids, int32_t *__restrict__ cumsum_out,
