@@ -180,25 +180,29 @@ template <class T>
 __global__ void __launch_bounds__(256) f8_moe_combine_kernel(F8MoeArgs p) {
     const int tok = blockIdx.x, lane = threadIdx.x & 63;
     const size_t step = (size_t)p.slices * p.H;
-    f32x4 v[4];
-    auto load = [&](int k0, int n) {               // four picks' loads in flight, here or not
-        const float *pair = p.obuf + (size_t)tok * p.K * step + n;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4 *>(pair + min(k0 + j, p.K - 1) * step);
-        for (int sl = 1; sl < p.slices; ++sl)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] += *reinterpret_cast<const f32x4 *>(pair + min(k0 + j, p.K - 1) * step + (size_t)sl * p.H);
-    };
-    const int first = (blockIdx.y * 256 + threadIdx.x) * 4;
-    if (first < p.H) load(0, first);
     const uint64_t here = __ballot(lane < p.K && f8_expert(p, tok * p.K + min(lane, p.K - 1)) >= 0);
-    for (int n = first; n < p.H; n += gridDim.y * 1024) {
+    for (int n = (blockIdx.y * 256 + threadIdx.x) * 4; n < p.H; n += gridDim.y * 1024) {
+        const float *pair = p.obuf + (size_t)tok * p.K * step + n;
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int k0 = 0; k0 < p.K; k0 += 4) {
-            if (k0 > 0 || n != first) load(k0, n);
+        for (uint64_t left = here; left != 0;) {
+            // the loads of four picks in flight, of the last one again where fewer are left: behind a branch each would wait for the one before
+            int k[4];
+            bool on[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                on[j] = left != 0;
+                k[j] = on[j] ? __builtin_ctzll(left) : k[j == 0 ? 0 : j - 1];
+                left &= left - 1;
+            }
+            f32x4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4 *>(pair + k[j] * step);
+            for (int sl = 1; sl < p.slices; ++sl)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += *reinterpret_cast<const f32x4 *>(pair + k[j] * step + (size_t)sl * p.H);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (here >> (k0 + j) & 1) sum += v[j];
+                if (on[j]) sum += v[j];
         }
         *reinterpret_cast<u32x2 *>(p.Y + (size_t)tok * p.H + n) = u32x2{T::from_f32x2(sum[0], sum[1]), T::from_f32x2(sum[2], sum[3])};
     }

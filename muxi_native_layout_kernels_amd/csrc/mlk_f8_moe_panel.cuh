@@ -242,7 +242,7 @@ constexpr size_t f8_moe_ring() {
 // tokens 260 -> 198 us, at 512 244 -> 230, at 1000 349 -> 338, at 2000 530 -> 498 (down in two slices 346 -> 321, at 512 192 -> 167), at 128 184 -> 177, at 64 175 -> 178; of 64 experts of 2048 x 1408 at
 // 500 85.6 -> 87.7, at 2000 129 -> 127.
 static inline bool f8_queue_pays(const F8MoeArgs &a, int n, int windows) {
-    const double mean = (double)a.n_pairs / a.E, spread = 3 * sqrt(mean);
+    const double mean = (double)a.n_pairs / a.id_limit, spread = 3 * sqrt(mean);
     if (ceil(fmax(mean - spread, 1) / 64) == ceil((mean + spread) / 64)) return false;
     return n > device_cus() && (double)n / device_cus() * windows >= 80;
 }

@@ -198,11 +198,11 @@ def exact_layer(T, E, K, H, I, dtype, held, seed):
 
 
 @pytest.mark.parametrize("T,E,K,H,I,held", [
-    (1, 8, 2, 4096, 14336, 8), (1, 40, 12, 512, 384, 40), (1, 16, 9, 1024, 256, 5), (2, 8, 2, 4096, 1024, 8), (16, 8, 2, 1152, 2048, 8), (50, 64, 8, 2048, 768, 32),
+    (1, 8, 2, 4096, 14336, 8), (1, 16, 12, 256, 14336, 16), (1, 2, 1, 65664, 128, 2), (1, 40, 12, 512, 384, 40), (1, 16, 9, 1024, 256, 5), (2, 8, 2, 4096, 1024, 8), (16, 8, 2, 1152, 2048, 8), (50, 64, 8, 2048, 768, 32),
     (30, 2, 1, 896, 640, 2), (100, 5, 2, 640, 1024, 5), (300, 8, 2, 1024, 8192, 8), (513, 8, 2, 4096, 14336, 8), (700, 3, 1, 640, 1024, 3), (900, 8, 2, 4096, 14336, 3),
     (2048, 8, 2, 4096, 8192, 8), (2500, 16, 8, 256, 384, 16), (1300, 300, 4, 256, 128, 77)])
 def test_exact_layers(mlk, T, E, K, H, I, held):
-    """Each plan at sizes where it is taken: one token, streamed, panels of every width, the queues, two slices of the down projection, several passes."""
+    """Each plan at sizes where it is taken: one token (also where it or its intermediates do not fit LDS), streamed, panels of every width, the queues, two slices of the down projection, several passes."""
     (x, w1, w2, ids, wts, s1, s2, place), want = exact_layer(T, E, K, H, I, BF, held, T + E)
     a1, a2 = mlk.pack_layout_a(w1), mlk.pack_layout_a(w2)
     del w1, w2
