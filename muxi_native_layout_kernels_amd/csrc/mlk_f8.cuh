@@ -230,6 +230,70 @@ __device__ __forceinline__ void f8_stream_staged(f32x4 (&acc)[R][1], const F8Row
     }
 }
 
+// The same with tokens of 16 bits that the wave quantises on the way: a window of a token lies in four lanes, 32 values in each, so its maximum is two exchanges.  Each window of the
+// tokens is quantised once a workgroup, by the wave that multiplies it.
+struct F8Raw {
+    u32x4 v[4];                  // values 16 q .. + 7, + 8 .. + 15, 64 + 16 q .. and + 8 of the window
+};
+template <int TT>
+struct F8RawTokens {
+    const uint16_t *x[TT];
+};
+template <class T>
+__device__ __forceinline__ void f8_quantize_operand(const F8Raw &in, F8Operand &o, float &scale) {
+    float v[32], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        v[2 * i] = T::to_f32(in.v[i >> 2][i & 3] & 0xffffu);
+        v[2 * i + 1] = T::to_f32(in.v[i >> 2][i & 3] >> 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) most = fmaxf(most, f8_magnitude(v[i]));
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const int e = f8_exponent(most);
+    scale = f8_two_to(e);
+    const float inverse = f8_two_to(-e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.v[i >> 2][i & 3] = f8_codes(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inverse);
+}
+template <class T, int TT, int R, int U>
+__device__ __forceinline__ void f8_stream_raw(f32x4 (&acc)[R][TT], const F8Rows<R> &rows, const F8RawTokens<TT> &tokens, int first, int end, int step, int lane) {
+    F8Operand w[U][R];
+    F8Raw x[U][TT];
+    float s[U][R];
+    auto load = [&](int u, int t) {
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            const uint16_t *at = tokens.x[tt] + (size_t)t * kF8K + (lane >> 4) * 16;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u][tt].v[j] = ld_global_u32x4(at + (j >> 1) * 64 + (j & 1) * 8);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            f8_load_weights(w[u][r], rows.w[r] + (size_t)t * kF8TileBytes, lane);
+            s[u][r] = rows.s[r][t];
+        }
+    };
+    const int n = end > first ? (end - first + step - 1) / step : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (u < n) load(u, first + u * step);
+    for (int i = 0; i < n; i += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u < n) {
+                F8Operand o[TT];
+                float a[TT];
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) f8_quantize_operand<T>(x[u][tt], o[tt], a[tt]);
+                f8_window<TT, R>(acc, w[u], s[u], o, a);
+                if (i + u + U < n) load(u, first + (i + u + U) * step);
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------------- products that feed codes
 // The matrix cores add eight products of e4m3 with 13 bits below the largest of them (measured: any shape of the instruction, cut off towards zero), 1.4e-5 of a sum over many in the
 // root mean square.  Against the rounding of a result that is nothing, but what becomes a code next moves to a neighbour wherever a border lies that near: quantised intermediates of 2048 from such sums

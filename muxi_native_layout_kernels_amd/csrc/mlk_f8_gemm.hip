@@ -89,12 +89,15 @@ __device__ __forceinline__ void f8_stage(const F8GemmArgs &p, u32x4 *lds, int t0
     }
 }
 
+// Where a workgroup has its tokens from: codes, up to 16 tokens in LDS (codes, or activations that the workgroup quantises), activations that each wave quantises for its own windows.
+enum F8Feed { kF8Codes, kF8InLds, kF8Quantise };
+
 // Bound by the weights' bytes, with more tokens by what the workgroups read of the activations.  A workgroup owns up to R consecutive row groups, which are dealt out evenly over the
 // grid, and TT blocks of 16 tokens (blockIdx.z); its waves deal the windows of 128 k among themselves (window t to wave t mod waves, so that together they read each row
 // group front to back) and add their sums through LDS in wave order.  `slices` workgroups may share a set of row groups, each on its own range of k: the last one to arrive adds their
-// fp32 sums in the order of k.  STAGED: up to 16 tokens that fit lie in LDS.  28672 x 8192 at 16 tokens 38.3 us (6.1 TB/s; a large read reaches 6.9), 512 x 7168 at one token 5.9 (launch,
-// first loads and the fold of four slices).
-template <class T, int TT, int R, int U, bool STAGED>
+// fp32 sums in the order of k.  28672 x 8192 at 16 tokens 40.6 us (5.8 TB/s; a large read reaches 6.9; 38.3 from codes), 512 x 7168 at one token 5.9 (launch, first loads and the fold of four
+// slices).
+template <class T, int TT, int R, int U, int FEED>
 __global__ void __launch_bounds__(512) f8_stream_kernel(F8GemmArgs p) {
     extern __shared__ u32x4 lds[];
     __shared__ int s_last;
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(512) f8_stream_kernel(F8GemmArgs p) {
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if constexpr (STAGED) {
+    if constexpr (FEED == kF8InLds) {
         const int n = t1 - t0, token = min(lane & 15, p.M - 1);
         F8Staged tokens;
         tokens.x = lds + (size_t)token * f8_staged_pitch(n);
@@ -121,6 +124,11 @@ __global__ void __launch_bounds__(512) f8_stream_kernel(F8GemmArgs p) {
             f8_stage<T>(p, lds, t0, n);
             __syncthreads();
         });
+    } else if constexpr (FEED == kF8Quantise) {
+        F8RawTokens<TT> tokens;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) tokens.x[tt] = reinterpret_cast<const uint16_t *>(p.raw) + (size_t)min(m0 + tt * 16 + (lane & 15), p.M - 1) * p.K;
+        f8_stream_raw<T, TT, R, U>(acc, rows, tokens, t0 + wave, t1, waves, lane);
     } else {
         F8Tokens<TT> tokens;
         tokens.step = p.xs_k;
@@ -143,7 +151,7 @@ __global__ void __launch_bounds__(512) f8_stream_kernel(F8GemmArgs p) {
     const int set = blockIdx.z * gridDim.x + blockIdx.x;
     auto part = [&](int s, int c) { return p.partial + (((size_t)set * p.slices + s) * CELLS + c) * 64; };
     f32x4 *red = reinterpret_cast<f32x4 *>(lds);
-    if constexpr (STAGED) __syncthreads();                     // the other waves still read the tokens
+    if constexpr (FEED == kF8InLds) __syncthreads();                     // the other waves still read the tokens
 #pragma unroll
     for (int c = 0; c < CELLS; ++c) red[(wave * CELLS + c) * 64 + lane] = acc[c / TT][c % TT];
     __syncthreads();
@@ -172,36 +180,45 @@ struct F8Plan {
     bool panels;
     int pr, tb, p3;              // of the panels
     int r, tt, waves, slices;    // of the streaming kernel: row groups and blocks of tokens of a workgroup
-    bool staged;
+    F8Feed feed;
 };
 
-template <class T, int TT, int R, int U, bool STAGED>
+template <class T, int TT, int R, int U, int FEED>
 static int f8_launch_stream_one(F8GemmArgs a, const F8Plan &pl, hipStream_t s) {
     const int groups = a.N / 16, wgs = (groups + R - 1) / R, per_slice = (a.K / kF8K + pl.slices - 1) / pl.slices;
     a.slices = pl.slices;
     a.rg_each = groups / wgs;
     a.rg_more = groups % wgs;
     size_t lds = (size_t)pl.waves * R * TT * 1024;
-    if (STAGED) lds = std::max(lds, f8_staged_bytes(a.M, per_slice));
+    if (FEED == kF8InLds) lds = std::max(lds, f8_staged_bytes(a.M, per_slice));
     if (lds > 48 * 1024) {
         static bool ready_on[64] = {};
-        const int rc = panel_lds_attribute(&f8_stream_kernel<T, TT, R, U, STAGED>, 150 * 1024, ready_on);
+        const int rc = panel_lds_attribute(&f8_stream_kernel<T, TT, R, U, FEED>, 150 * 1024, ready_on);
         if (rc != MLK_OK) return rc;
     }
-    f8_stream_kernel<T, TT, R, U, STAGED><<<dim3(wgs, pl.slices, (a.M + TT * 16 - 1) / (TT * 16)), pl.waves * 64, lds, s>>>(a);
+    f8_stream_kernel<T, TT, R, U, FEED><<<dim3(wgs, pl.slices, (a.M + TT * 16 - 1) / (TT * 16)), pl.waves * 64, lds, s>>>(a);
     MLK_LAUNCH_CHECK();
     return MLK_OK;
 }
 // Windows in flight: as many as fit the registers of eight waves a CU.
-__host__ __device__ constexpr int f8_ring(int tt, int r, bool staged) { return r == 1 && tt == 1 ? 8 : r * tt <= 2 ? 4 : (r + tt < 8 ? 2 : 1); }
+__host__ __device__ constexpr int f8_ring(int tt, int r) { return r == 1 && tt == 1 ? 8 : r * tt <= 2 ? 4 : (r + tt < 8 ? 2 : 1); }
+__host__ __device__ constexpr int f8_raw_ring(int tt, int r) { return r * tt == 1 ? 2 : 1; }       // more registers than workgroups pay for: 4096 x 14336 at 4 tokens, two rows, two windows 15.5 us, one 14.6
 template <class T>
 static int f8_launch_stream(const F8GemmArgs &a, const F8Plan &pl, hipStream_t s) {
     // what f8_plan() picks
-#define MLK_F8_S(R) if (pl.staged && pl.r == R) return f8_launch_stream_one<T, 1, R, f8_ring(1, R, true), true>(a, pl, s)
-#define MLK_F8_R(TT, R) if (!pl.staged && pl.tt == TT && pl.r == R) return f8_launch_stream_one<T, TT, R, f8_ring(TT, R, false), false>(a, pl, s)
+#define MLK_F8_S(R) if (pl.feed == kF8InLds && pl.r == R) return f8_launch_stream_one<T, 1, R, f8_ring(1, R), kF8InLds>(a, pl, s)
+#define MLK_F8_Q(TT, R) if (pl.feed == kF8Quantise && pl.tt == TT && pl.r == R) return f8_launch_stream_one<T, TT, R, f8_raw_ring(TT, R), kF8Quantise>(a, pl, s)
+#define MLK_F8_R(TT, R) if (pl.feed == kF8Codes && pl.tt == TT && pl.r == R) return f8_launch_stream_one<T, TT, R, f8_ring(TT, R), kF8Codes>(a, pl, s)
     MLK_F8_S(1);
     MLK_F8_S(2);
     MLK_F8_S(4);
+    MLK_F8_Q(1, 1);
+    MLK_F8_Q(1, 2);
+    MLK_F8_Q(1, 4);
+    MLK_F8_Q(1, 8);
+    MLK_F8_Q(2, 1);
+    MLK_F8_Q(2, 2);
+    MLK_F8_Q(2, 4);
     MLK_F8_R(1, 1);
     MLK_F8_R(1, 2);
     MLK_F8_R(1, 4);
@@ -212,6 +229,7 @@ static int f8_launch_stream(const F8GemmArgs &a, const F8Plan &pl, hipStream_t s
     MLK_F8_R(3, 2);
     MLK_F8_R(4, 2);
 #undef MLK_F8_S
+#undef MLK_F8_Q
 #undef MLK_F8_R
     return fail(MLK_ERR_INVALID, "gemm fp8: launch parameters");
 }
@@ -224,14 +242,19 @@ void gemm_plan(int m, int n, int k, bool fp8, bool b_native, int32_t *out);
 
 constexpr size_t kF8StagedLds = 140 * 1024;     // of staged tokens
 
-// Launches that are fastest, timed in graphs on weights from memory (us; g r, tt, waves, slices of the streaming kernel, s: tokens staged, p: panels of 128 rows x 64 tokens).  Activations that
-// are quantised in the call: staged they save a launch and cost every workgroup their quantising.
+// Launches that are fastest, timed in graphs on weights from memory (us; g r, tt, waves, slices of the streaming kernel, s: tokens staged in LDS, q: quantised by
+// the waves that multiply them, p: panels of 128 rows x 64 tokens).  Quantised by the workgroups, activations save a launch.
 //   few row groups       512 x 7168 codes g1,1,4,4 5.5, g1,1,4,1 7 and more; at 16 tokens 6.0; 1280 x 5120 g1,1,8,1 5.8, at 32 tokens g2,2,8,4 7.2, at 64 g2,4,8,4 8.8, p 10.9
 //   one a CU             4096 x 4096 g1,1,8,1 5.7, g2 7.2; at 64 tokens g2,2,8,1 10.1; 4096 x 14336 at 16 tokens g4,1,4,8 14.3, g1,1,8,1 16.3; at 32 g4,2,8,4 16.4, p in eight slices 18.1; at 64 p 19.7, g 21.7
 //   up to two            7168 x 2048 g2,1,4,1 5.5, 8192 x 3584 g2,1,8,1 7.5, w4 8.3; at 64 tokens g4,2,8,1 8.7; 5120 x 13824 at 8 g4,1,4,8 17.5, g2,1,8,1 19.4; at 24 p in six slices 20.0, g2,2,8,4 20.8
 //   up to four           13824 x 5120 at 4 tokens g4,1,8,1 15.2, g2 15.7; at 32 g4,2,8,1 18.0, p in two slices 19.8; at 64 p 21.0, g4,4,8,1 23.7
 //   more                 28672 x 8192 at 8 tokens g8,1,4,1 40.5, g2 41.8, g4 42.0; 37888 x 3584 at 8 g2,1,4,1 27.7, g8 32 and more; 28672 x 8192 at 17 p 43.2, g4,2,4,1 43.9, at 64 p 44.4, g 59.9
-//   staged, quantising   512 x 7168 one token s1,1,8,4 6.0, at 8 7.3 (g 8.6); 28672 x 8192 one token s2,1,4,1 38.4, g 43.4; at 4 both 43.4, at 8 s 49, g 43.8; 7168 x 2048 at 8 s2,1,8,1 7.6, g 8.5; at 16 9.6 and 8.8
+//   quantising, s or q   512 x 7168 one token s1,1,8,4 6.0, q1,1,4,8 6.7; at 8 tokens 7.3 and 6.8; 4096 x 4096 at 2 s1,1,8,1 7.2, q2,1,8,4 7.7; at 4 8.0 and 7.7; 4608 x 7168 at 2 s2,1,8,1 11.1, q 11.9; 8192 x 8192 at
+//                        2 15.6 and 14.3; 37888 x 3584 at 2 s2,1,4,1 24.9, q4,1,8,1 26.9; 28672 x 8192 at 2 39.4, q8,1,4,1 41.1; at 4 43.3 and 41.0; 16000 x 1024 at 2 s4,1,8,1 5.8, q 6.3
+//   quantising, q or a launch ahead of g or p    512 x 7168 at 16 tokens q1,1,4,8 7.1, g 9.1; at 32 q1,2,4,8 8.2, g 10.0; 4096 x 4096 at 16 q2,1,8,4 8.2, g 10.7; at 32 q4,2,8,4 10.0, g 11.7; 4096 x 14336 at 8 q4,1,8,4 14.5,
+//                        g 17.9; at 32 19.3 and 21.3; 3584 x 18944 at 32 25.0 and 23.6; 2048 x 2048 at 7 q1,1,8,1 5.3, in two slices of two rows 6.1, s and g 5.5; 7168 x 2048 at 16 q2,1,8,1 6.5, g 9.0; at 24 8.1 and
+//                        10.2; 8192 x 8192 at 32 23.9 and 21.8; 5120 x 13824 at 16 q4,1,8,4 21.9, q2,1,8,1 23.5, g 21.2; at 32 35 and 23.5; 13824 x 5120 at 8 q4,1,8,1 15.7, g 19.2; at 24 20.5 and 22.1, at 32 24.3 and 22.8;
+//                        22016 x 4096 at 7 q2,1,4,1 20.2, q4,1,8,1 22.0, g 21.1; 28672 x 8192 at 16 q8,1,4,1 40.7, g 44.0; at 24 q4,2,4,1 54.8, p 49.6
 //   staged codes         one token of large weights only: 28672 x 8192 38.1, g 40.8; 4096 x 14336 13.1, g 14.1; 4096 x 4096 6.2, g 5.7
 static F8Plan f8_plan(int m, int n, int k, bool raw) {
     F8Plan pl = {};
@@ -250,29 +273,49 @@ static F8Plan f8_plan(int m, int n, int k, bool raw) {
         pl.p3 = out[3];
         return pl;
     }
-    if (panels_fit && ((m > 16 && (groups > 4 * cus || (deep && groups > cus))) || (m > 32 && m <= 64 && (groups > 2 * cus || (deep && groups > cus / 2))))) {
-        const int rows = (n + 127) / 128;
-        pl.panels = true;
-        pl.pr = pl.tb = 1;
-        pl.p3 = std::max(1, std::min(cus / rows, windows / 12));
-        return pl;
-    }
     auto stream = [&](int r, int tt, int waves, int slices) {
         pl.r = r;
         pl.tt = tt;
         pl.waves = waves;
         pl.slices = std::max(1, std::min(slices, windows / waves));
     };
-    const int blocks = std::min((m + 15) / 16, 4), thin = windows >= 32 ? 4 : 1;
-    if (raw ? m <= 16 : m == 1 && (int64_t)n * k >= 50000000) {
+    const int blocks = std::min((m + 15) / 16, 4), thin = windows >= 32 ? 4 : 1, many = windows >= 16 ? 8 : 4;
+    // in LDS
+    const bool lds = raw ? m <= 4 && (groups <= cus / 4 || (m <= 2 && groups <= cus && !deep) || (m <= 2 && groups <= cus * 3 / 2) || (m == 1 && groups <= 2 * cus) ||
+                                      (m <= 2 && (groups > 4 * cus || (groups > 2 * cus && windows < 16))))
+                         : m == 1 && (int64_t)n * k >= 50000000;
+    if (lds) {
         if (groups <= cus / 4) stream(1, 1, 8, thin);
         else if (groups <= cus) stream(m * windows > 200 ? 2 : 1, 1, 8, m * windows > 200 ? 4 : 1);
         else if (groups <= 2 * cus) stream(2, 1, deep ? 4 : 8, deep ? 4 : 1);
-        else if (groups <= 4 * cus && (m > 1 || groups <= 3 * cus)) stream(4, 1, 8, 1);
+        else if (groups <= 3 * cus) stream(4, 1, 8, 1);
         else stream(2, 1, 4, 1);
-        const int each = (windows + pl.slices - 1) / pl.slices;
-        pl.staged = f8_staged_bytes(m, each) <= kF8StagedLds && (m <= 4 || (m * each <= 160 && groups <= 2 * cus));
-        if (pl.staged) return pl;
+        if (f8_staged_bytes(m, (windows + pl.slices - 1) / pl.slices) <= kF8StagedLds) {
+            pl.feed = kF8InLds;
+            return pl;
+        }
+    }
+    // quantised by the waves
+    const bool two = m > 16 && m <= 32 && (groups <= cus ? m * windows <= 4096 : groups <= 2 * cus ? windows <= 32 : groups <= 4 * cus && m * windows <= 1000);
+    if (raw && (m <= 16 || two)) {
+        const int tt = two ? 2 : 1;
+        pl.feed = kF8Quantise;
+        if (groups <= cus / 4) stream(1, tt, 4, windows >= 16 ? 8 : 1);
+        else if (groups <= cus && windows < 32) stream(1, tt, many, 1);
+        else if (groups <= cus) stream(two || deep ? 4 : 2, tt, 8, 4);
+        else if (groups <= 2 * cus && deep) stream(4, tt, 8, 4);
+        else if (groups <= 2 * cus) stream(2, tt, many, 1);
+        else if (groups <= 4 * cus) stream(4, tt, many, 1);
+        else if (windows < 48) stream(groups < 6 * cus ? 2 : 4, tt, groups < 6 * cus ? 4 : many, 1);
+        else stream(8, tt, 4, 1);
+        return pl;
+    }
+    if (panels_fit && ((m > 16 && (groups > 4 * cus || (deep && groups > cus))) || (m > 32 && m <= 64 && (groups > 2 * cus || (deep && groups > cus / 2))))) {
+        const int rows = (n + 127) / 128;
+        pl.panels = true;
+        pl.pr = pl.tb = 1;
+        pl.p3 = std::max(1, std::min(cus / rows, windows / 12));
+        return pl;
     }
     if (m <= 16) {
         if (groups <= cus / 4) stream(1, 1, 4, thin);
@@ -368,7 +411,7 @@ size_t mlk_gemm_fp8_workspace_bytes(int m, int n, int k, int b_kind) {
     if (m <= 0 || n <= 0 || k <= 0 || k % 128 != 0) return 0;
     const bool raw = b_kind != MLK_FP8_E4M3;
     const F8Plan pl = f8_plan(m, n, k, raw);
-    return f8_carve(nullptr, pl, m, n, k, raw && !pl.staged, nullptr);
+    return f8_carve(nullptr, pl, m, n, k, raw && pl.feed == kF8Codes, nullptr);
 }
 
 int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, int b_kind, const float *b_scale, int64_t b_scale_t, int64_t b_scale_k, void *c,
@@ -405,9 +448,9 @@ int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, in
         pl.slices = 1;
     }
     F8Scratch w;
-    if (f8_carve((uint8_t *)workspace, pl, m, n, k, raw && !pl.staged, &w) > 0)
+    if (f8_carve((uint8_t *)workspace, pl, m, n, k, raw && pl.feed == kF8Codes, &w) > 0)
         MLK_REQUIRE(workspace && aligned16(workspace), "gemm fp8: workspace off 16 bytes");
-    if (raw && pl.staged) {
+    if (raw && pl.feed != kF8Codes) {
         p.raw = b;
     } else if (raw) {
         const int rc = launch_quantize_fp8(b, b_kind, w.codes, w.scales, 1, m, m, k, s);
