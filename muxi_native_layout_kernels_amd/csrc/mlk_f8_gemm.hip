@@ -249,6 +249,7 @@ constexpr size_t kF8StagedLds = 140 * 1024;     // of staged tokens
 //   up to two            7168 x 2048 g2,1,4,1 5.5, 8192 x 3584 g2,1,8,1 7.5, w4 8.3; at 64 tokens g4,2,8,1 8.7; 5120 x 13824 at 8 g4,1,4,8 17.5, g2,1,8,1 19.4; at 24 p in six slices 20.0, g2,2,8,4 20.8
 //   up to four           13824 x 5120 at 4 tokens g4,1,8,1 15.2, g2 15.7; at 32 g4,2,8,1 18.0, p in two slices 19.8; at 64 p 21.0, g4,4,8,1 23.7
 //   more                 28672 x 8192 at 8 tokens g8,1,4,1 40.5, g2 41.8, g4 42.0; 37888 x 3584 at 8 g2,1,4,1 27.7, g8 32 and more; 28672 x 8192 at 17 p 43.2, g4,2,4,1 43.9, at 64 p 44.4, g 59.9
+//   64, long k           8192 x 8192 p in four slices 24.8, g4,4,8,1 27.6, both with quantising; 4608 x 7168 in seven 19.8 and 23.4
 //   quantising, s or q   512 x 7168 one token s1,1,8,4 6.0, q1,1,4,8 6.7; at 8 tokens 7.3 and 6.8; 4096 x 4096 at 2 s1,1,8,1 7.2, q2,1,8,4 7.7; at 4 8.0 and 7.7; 4608 x 7168 at 2 s2,1,8,1 11.1, q 11.9; 8192 x 8192 at
 //                        2 15.6 and 14.3; 37888 x 3584 at 2 s2,1,4,1 24.9, q4,1,8,1 26.9; 28672 x 8192 at 2 39.4, q8,1,4,1 41.1; at 4 43.3 and 41.0; 16000 x 1024 at 2 s4,1,8,1 5.8, q 6.3
 //   quantising, q or a launch ahead of g or p    512 x 7168 at 16 tokens q1,1,4,8 7.1, g 9.1; at 32 q1,2,4,8 8.2, g 10.0; 4096 x 4096 at 16 q2,1,8,4 8.2, g 10.7; at 32 q4,2,8,4 10.0, g 11.7; 4096 x 14336 at 8 q4,1,8,4 14.5,
@@ -264,14 +265,18 @@ static F8Plan f8_plan(int m, int n, int k, bool raw) {
     const bool deep = windows >= 96;
     // up to 256 tokens through few rows: 512 x 7168 at 200 tokens g4,2,8,4 9.4, panels 12.2; at 300 12.5; 4096 x 4096 at 100 g4,2,8,1 12.6, panels 14.9; at 200 16.5
     const bool narrow = m <= 64 || (m <= 128 && groups <= cus && !deep) || (m <= 256 && groups <= cus / 4);
+    const int rows = (n + 127) / 128;
+    auto panels = [&](int pr, int tb, int p3) {
+        pl.panels = true;
+        pl.pr = pr;
+        pl.tb = tb;
+        pl.p3 = std::max(1, p3);
+        return pl;
+    };
     if (!narrow && panels_fit) {
         int32_t out[4];
         gemm_plan(m, n, k / 2, false, false, out);
-        pl.panels = true;
-        pl.pr = out[1] / 2;
-        pl.tb = out[2];
-        pl.p3 = out[3];
-        return pl;
+        return panels(out[1] / 2, out[2], out[3]);
     }
     auto stream = [&](int r, int tt, int waves, int slices) {
         pl.r = r;
@@ -310,13 +315,8 @@ static F8Plan f8_plan(int m, int n, int k, bool raw) {
         else stream(8, tt, 4, 1);
         return pl;
     }
-    if (panels_fit && ((m > 16 && (groups > 4 * cus || (deep && groups > cus))) || (m > 32 && m <= 64 && (groups > 2 * cus || (deep && groups > cus / 2))))) {
-        const int rows = (n + 127) / 128;
-        pl.panels = true;
-        pl.pr = pl.tb = 1;
-        pl.p3 = std::max(1, std::min(cus / rows, windows / 12));
-        return pl;
-    }
+    if (panels_fit && ((m > 16 && (groups > 4 * cus || (deep && groups > cus))) || (m > 32 && m <= 64 && (groups > 2 * cus || (windows >= 48 && groups > cus) || (deep && groups > cus / 2)))))
+        return panels(1, 1, std::min(cus / rows, windows / 12));
     if (m <= 16) {
         if (groups <= cus / 4) stream(1, 1, 4, thin);
         else if (groups <= 2 * cus && deep) stream(4, 1, 4, 8);
