@@ -310,6 +310,10 @@ __device__ __forceinline__ void f8_load_tile(F8RawTile &o, const uint8_t *tile, 
 #pragma unroll
     for (int j = 0; j < 4; ++j) o.v[j] = ld_stream_u32x2(tile + j * 512 + lane * 8);
 }
+__device__ __forceinline__ void f8_widen(const F8Operand &in, F8WideOperand &o) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.v[j] = f8_widen(u32x2{in.v[j >> 1][(j & 1) * 2], in.v[j >> 1][(j & 1) * 2 + 1]});
+}
 __device__ __forceinline__ f32x4 f8_wide_mfma(const F8RawTile &w, const F8WideOperand &x) {
     f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

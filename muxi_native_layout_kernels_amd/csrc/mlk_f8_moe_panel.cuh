@@ -30,10 +30,10 @@ __device__ __forceinline__ const F8MoeArgs &f8_moe_args(int &lane, int &wave) {
 }
 
 // Both panels return a ticket of the next item (QUEUE, wave 0).
-template <bool QUEUE, int TB>
+template <bool QUEUE, bool EXACT, int TB>
 __device__ __forceinline__ int f8_moe_gate_up_panel(const F8MoeArgs &p, const MoeTask &tk, int rt, int wave, int lane) {
     extern __shared__ u32x4 win[];
-    using Loop = F8PanelLoop<2, TB, 2>;
+    using Loop = F8PanelLoop<2, TB, 2, EXACT>;
     const int wr = wave & 3, wt = wave >> 2, groups_i = p.I >> 4, windows = p.H >> 7, slots = tk.nblocks * 16;
     const uint32_t tile_row = (uint32_t)p.H * 16u;             // bytes of a row group
     const int32_t *sorted = p.sorted + tk.block0 * 16;
@@ -167,15 +167,29 @@ __device__ __forceinline__ MoeTask f8_moe_item(const F8MoeArgs &p, int item, int
     return p.tasks[t0.first + local % t0.count];
 }
 
-template <bool QUEUE>
+// EXACT: panels of up to 128 pairs, the registers of larger ones go to the widened weights; a task of more takes its row tile twice.
+template <bool QUEUE, bool EXACT>
 __device__ __forceinline__ int f8_moe_gate_up_item(const F8MoeArgs &p, int item, int wave, int lane) {
     int rt;
     const MoeTask tk = f8_moe_item(p, item, p.I >> 7, rt);
-    switch ((tk.nblocks + 3) >> 2) {
-        case 1: return f8_moe_gate_up_panel<QUEUE, 1>(p, tk, rt, wave, lane);
-        case 2: return f8_moe_gate_up_panel<QUEUE, 2>(p, tk, rt, wave, lane);
-        case 3: return f8_moe_gate_up_panel<QUEUE, 3>(p, tk, rt, wave, lane);
-        default: return f8_moe_gate_up_panel<QUEUE, 4>(p, tk, rt, wave, lane);
+    if constexpr (EXACT) {
+        MoeTask half = tk;
+        half.nblocks = min(tk.nblocks, 8);
+        if (tk.nblocks > 8) {
+            f8_moe_gate_up_panel<false, true, 2>(p, half, rt, wave, lane);
+            __syncthreads();
+            half.block0 += 8;
+            half.nblocks = tk.nblocks - 8;
+        }
+        if (half.nblocks <= 4) return f8_moe_gate_up_panel<QUEUE, true, 1>(p, half, rt, wave, lane);
+        return f8_moe_gate_up_panel<QUEUE, true, 2>(p, half, rt, wave, lane);
+    } else {
+        switch ((tk.nblocks + 3) >> 2) {
+            case 1: return f8_moe_gate_up_panel<QUEUE, false, 1>(p, tk, rt, wave, lane);
+            case 2: return f8_moe_gate_up_panel<QUEUE, false, 2>(p, tk, rt, wave, lane);
+            case 3: return f8_moe_gate_up_panel<QUEUE, false, 3>(p, tk, rt, wave, lane);
+            default: return f8_moe_gate_up_panel<QUEUE, false, 4>(p, tk, rt, wave, lane);
+        }
     }
 }
 template <class T, bool QUEUE>
@@ -194,10 +208,11 @@ __device__ __forceinline__ int f8_moe_down_item(const F8MoeArgs &p, int item, in
 __device__ __forceinline__ int f8_moe_up_items(const F8MoeArgs &p) { return (p.I >> 7) * p.n_tasks[0]; }
 __device__ __forceinline__ int f8_moe_down_items(const F8MoeArgs &p) { return ((p.H + 255) >> 8) * p.slices * p.n_tasks[0]; }
 
+template <bool EXACT>
 __global__ void __launch_bounds__(512) f8_moe_gate_up_panel_kernel(F8MoeArgs p) {
     const int n = f8_moe_up_items(p), item = wide_item(blockIdx.x, n);
     if (item >= n) return;
-    f8_moe_gate_up_item<false>(p, item, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63);
+    f8_moe_gate_up_item<false, EXACT>(p, item, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63);
 }
 template <class T>
 __global__ void __launch_bounds__(512) f8_moe_down_panel_kernel(F8MoeArgs p) {
@@ -205,6 +220,7 @@ __global__ void __launch_bounds__(512) f8_moe_down_panel_kernel(F8MoeArgs p) {
     if (item >= n) return;
     f8_moe_down_item<T, false>(p, item, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63);
 }
+template <bool EXACT>
 __global__ void __launch_bounds__(512) f8_moe_gate_up_queue_kernel(F8MoeArgs) {
     __shared__ int s_item;
     int ticket = blockIdx.x >> 3;
@@ -215,7 +231,7 @@ __global__ void __launch_bounds__(512) f8_moe_gate_up_queue_kernel(F8MoeArgs) {
         __syncthreads();                                       // also: LDS is free again
         const int item = __builtin_amdgcn_readfirstlane(s_item);
         if (item < 0) return;
-        ticket = f8_moe_gate_up_item<true>(p, item, wave, lane);
+        ticket = f8_moe_gate_up_item<true, EXACT>(p, item, wave, lane);
     }
 }
 template <class T>
@@ -252,7 +268,8 @@ int f8_launch_moe_panels(const F8MoeArgs &a, int max_tasks, hipStream_t s) {
     static bool ready_up[2][64] = {}, ready_down[2][64] = {};
     const int items_up = (a.I >> 7) * max_tasks, items_down = ((a.H + 255) >> 8) * a.slices * max_tasks;
     const bool queue_up = f8_queue_pays(a, items_up, a.H >> 7), queue_down = f8_queue_pays(a, items_down, (a.I >> 7) / a.slices);
-    const auto up = queue_up ? &f8_moe_gate_up_queue_kernel : &f8_moe_gate_up_panel_kernel;
+    constexpr bool EXACT = std::is_same<T, F16>::value;
+    const auto up = queue_up ? &f8_moe_gate_up_queue_kernel<EXACT> : &f8_moe_gate_up_panel_kernel<EXACT>;
     const auto down = queue_down ? &f8_moe_down_queue_kernel<T> : &f8_moe_down_panel_kernel<T>;
     int rc = panel_lds_attribute(up, lds_up, ready_up[queue_up]);
     if (rc == MLK_OK) rc = panel_lds_attribute(down, lds_down, ready_down[queue_down]);

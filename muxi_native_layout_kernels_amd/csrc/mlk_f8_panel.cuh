@@ -23,7 +23,8 @@ struct F8PanelSrc {
 };
 
 // NS = 2: the first half of a wave's row tiles and the second have scales of their own, of which waves 4..7 fetch one each in lanes 0 and 1.
-template <int PR, int TB, int NS = 1>
+// EXACT: products of 16 bits of the same codes (products that feed codes, mlk_f8.cuh).  A window's weights are widened once, each block of tokens ahead of its products.
+template <int PR, int TB, int NS = 1, bool EXACT = false>
 struct F8PanelLoop : P8TokenPairs<TB, true> {
     using Tok = P8TokenPairs<TB, true>;          // its NB: chunks of tokens a wave fetches
     using Acc = P8Acc16<PR, TB>;
@@ -78,6 +79,7 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
         const int b0 = A_WIN + Tok::operand16(src.p, 0, lane) + wt * TT * 128, b1 = A_WIN + Tok::operand16(src.p, 1, lane) + wt * TT * 128;
         const int s_idx = (A_WIN + B_WIN) * 4 + wt * TT * 16 + (lane & 15), ws_idx = (A_WIN + B_WIN + 64) * 4 + (NS == 2 ? 0 : (wr * PR) / 4);
         F8Operand a[RT], b[2];
+        F8WideOperand wide[EXACT ? RT : 1];
         f32x4 d[2][RT];
         float s[2], sw[NS], scale[NS];
         auto read_a = [&](int buf, int i) {
@@ -138,7 +140,22 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
                     scale[h] = s[j & 1] * sw[h];
                 }
 #pragma unroll
-                for (int i = 0; i < RT; ++i) d[j & 1][i] = f8_mfma(a[i], b[j & 1], f32x4{0.f, 0.f, 0.f, 0.f});
+                for (int i = 0; i < RT; ++i) {
+                    if constexpr (EXACT) {
+                        if (j == 0) f8_widen(a[i], wide[i]);
+                        d[j & 1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    } else {
+                        d[j & 1][i] = f8_mfma(a[i], b[j & 1], f32x4{0.f, 0.f, 0.f, 0.f});
+                    }
+                }
+                if constexpr (EXACT) {
+                    F8WideOperand x;
+                    f8_widen(b[j & 1], x);
+#pragma unroll
+                    for (int o = 0; o < 4; ++o)
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) d[j & 1][i] = BF16::mfma(wide[i].v[o], x.v[o], d[j & 1][i]);
+                }
                 if (j == TT - 1) {
                     read_sw(nxt);
 #pragma unroll
@@ -151,7 +168,7 @@ struct F8PanelLoop : P8TokenPairs<TB, true> {
 #pragma unroll
                     for (int v = 0; v < 4; ++v) out.acc[i][before][v] = fmaf(last_scale[i * NS / RT], d[1 - (j & 1)][i][v], out.acc[i][before][v]);
 #pragma unroll
-                for (int i = 0; i < RT; ++i) {
+                for (int i = 0; i < (EXACT ? 0 : RT); ++i) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                     __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
                     __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
