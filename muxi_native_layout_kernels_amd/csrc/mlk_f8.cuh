@@ -299,7 +299,7 @@ __device__ __forceinline__ void f8_stream_raw(f32x4 (&acc)[R][TT], const F8Rows<
 // root mean square.  Against the rounding of a result that is nothing, but what becomes a code next moves to a neighbour wherever a border lies that near: quantised intermediates of 2048 from such sums
 // put the expert layer's result 1.7e-3 off, from sums in 32 bits 5e-5 (bf16 rounds by 1.7e-3, fp16 by 2.1e-4, quantising itself costs 2.6e-2).  So gate and up go through
 // v_mfma_f32_16x16x32_bf16, whose products and sums are good to 1e-8, where the weights' bytes set the pace, and in fp16 layers everywhere: codes are exact in bf16, a window is four of them.
-// Widening the weights hides behind their loads; in the panels it takes longer than the products.  Lane 16 q + r holds octet 4 j + q of row r: 512 bytes a load in a row.
+// Widening the weights hides behind their loads; the panels pay twice the matrix cores' time and 10 % for widening.  Lane 16 q + r holds octet 4 j + q of row r: 512 bytes a load in a row.
 struct F8WideOperand {
     u32x4 v[4];
 };
