@@ -67,12 +67,13 @@ def test_the_same_expert_twice_and_all_on_one(mlk, T):
     compare(mlk, T, 3, 2, 128, 128, BF, ids)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("T", [2, 20, 150])
-def test_a_token_with_nan_or_infinity_keeps_to_itself(mlk, T):
+def test_a_token_with_nan_or_infinity_keeps_to_itself(mlk, T, dtype):
     l1, l2, _, _ = layer(4, 256, 128, 1)
     a1, a2, s1, s2 = on_gpu(mlk, l1, l2)
-    ids, wts = (t.cuda() for t in routing(T, 4, 2, BF, T))
-    x = randn((T, 256), BF, 1.0, 2).cuda()
+    ids, wts = (t.cuda() for t in routing(T, 4, 2, dtype, T))
+    x = randn((T, 256), dtype, 1.0, 2).cuda()
     clean = mlk.fused_experts_fp8(x, a1, a2, ids, wts, s1, s2)
     x[0, 3], x[T - 1, 200] = float("nan"), float("-inf")
     got = mlk.fused_experts_fp8(x, a1, a2, ids, wts, s1, s2)
