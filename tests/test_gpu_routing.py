@@ -112,7 +112,8 @@ def check(mlk, logits, K, sigmoid=False, renorm=True, G=1, kept=1, bias=None, sc
 
 
 SIZES = [(1, 1, 1), (1, 8, 2), (3, 2, 2), (7, 64, 6), (33, 17, 17), (64, 65, 5), (100, 256, 8), (31, 257, 9), (16, 512, 32), (1025, 8, 2), (1030, 60, 4), (1027, 129, 8), (1031, 256, 20),
-         (1026, 300, 3), (1029, 512, 10)]
+         (1026, 300, 3), (1029, 512, 10),
+         (4100, 130, 5), (4097, 257, 3)]
 
 
 @pytest.mark.parametrize("renorm", [True, False])
@@ -126,7 +127,8 @@ def test_picks_weights_and_gradient(mlk, T, E, K, dtype, sigmoid, renorm):
 @pytest.mark.parametrize("sigmoid", [True, False])
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("T,E,K,G,kept", [(1, 256, 8, 8, 4), (50, 256, 8, 8, 4), (9, 24, 4, 3, 2), (33, 160, 6, 8, 3), (12, 16, 3, 16, 5), (20, 512, 32, 64, 8), (1100, 256, 8, 8, 4),
-                                          (1030, 160, 6, 20, 3), (1027, 512, 8, 32, 16)])
+                                          (1030, 160, 6, 20, 3), (1027, 512, 8, 32, 16), (4100, 256, 8, 8, 4), (4101, 512, 8, 32, 16),
+                                          (4098, 120, 7, 40, 9), (4103, 66, 4, 11, 5)])
 def test_bias_groups_and_masks(mlk, T, E, K, G, kept, dtype, sigmoid):
     g = torch.Generator().manual_seed(E)
     bias = torch.randn(E, generator=g) * 0.2
