@@ -296,10 +296,11 @@ __device__ __forceinline__ void f8_stream_raw(f32x4 (&acc)[R][TT], const F8Rows<
 
 // ---------------------------------------------------------------------------------------------------------------- products that feed codes
 // The matrix cores add eight products of e4m3 with 13 bits below the largest of them (measured: any shape of the instruction, cut off towards zero), 1.4e-5 of a sum over many in the
-// root mean square.  Against the rounding of a result that is nothing, but what becomes a code next moves to a neighbour wherever a border lies that near: quantised intermediates of 2048 from such sums
-// put the expert layer's result 1.7e-3 off, from sums in 32 bits 5e-5 (bf16 rounds by 1.7e-3, fp16 by 2.1e-4, quantising itself costs 2.6e-2).  So gate and up go through
-// v_mfma_f32_16x16x32_bf16, whose products and sums are good to 1e-8, where the weights' bytes set the pace, and in fp16 layers everywhere: codes are exact in bf16, a window is four of them.
-// Widening the weights hides behind their loads; the panels pay twice the matrix cores' time and 10 % for widening.  Lane 16 q + r holds octet 4 j + q of row r: 512 bytes a load in a row.
+// root mean square, and up to 9e-5 where a few columns of the activations are 30 to 1000 times larger than the rest.  Against the rounding of a result that is little (fp16 of such columns 2.07e-4 ->
+// 2.26e-4, bf16 not to be seen), but what becomes a code next moves to a neighbour wherever a border lies that near, and with the largest of a block its scale: expert layers of 2048 x 512 with gate
+// and up from such sums are 1.8e-3 to 3.6e-3 off the definition, single tokens up to 1.9e-2, where bf16 rounds by 1.66e-3 (fp16 by 2.1e-4, quantising itself costs 2.6e-2).  So gate and up go through
+// v_mfma_f32_16x16x32_bf16: codes are exact in bf16 and so are their products, a window is four instructions, whose sums round to fp32 as those of the windows do.  Then only the results' own rounding is seen.
+// Where the weights' bytes set the pace widening the weights hides behind their loads; the panels pay for it (mlk_f8_moe_panel.cuh).  Lane 16 q + r holds octet 4 j + q of row r: 512 bytes a load in a row.
 struct F8WideOperand {
     u32x4 v[4];
 };

@@ -351,7 +351,7 @@ static int f8_moe_slices(int load, int reached, int hidden, int inter) {
     const int items = (hidden + 255) / 256 * reached * ((high + width - 1) / width), cus = device_cus();
     return (2 * items + cus - 1) / cus * 2 <= (items + cus - 1) / cus * 3 ? 2 : 1;
 }
-static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidden, int inter, bool exact) {
+static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidden, int inter) {
     F8MoePlan pl = {};
     const int pairs = tokens * topk;
     pl.slices = 1;
@@ -362,10 +362,10 @@ static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidd
     // with E of the router's experts here that share of the pairs is expected here
     const int here = (int)std::max<int64_t>(1, std::min<int64_t>(pairs, (int64_t)pairs * E / n_router));
     const int reached = std::min(here, E), load = (here + reached - 1) / reached;
-    // Panels from 13 pairs an expert on (fp16, whose panels take longer, from 19), whose tasks then spend less time on the products than on waiting: 8 experts of 4096 x 14336 streamed -> panels at 12 pairs an expert 264 -> 283 us, at 16
-    // 317 -> 287, at 25 372 -> 295; 128 of 2048 x 768 at 9.4 pairs 141 -> 133, at 19 170 -> 146.
+    // Panels from 19 pairs an expert on: below, tasks of the streaming kernels pass over the weights about as often and start sooner.  The whole layer on the last count of pairs that is streamed and the first
+    // of the panels: 8 experts of 4096 x 14336 286 and 277 us, 128 of 2048 x 768 160 and 154.
     // offsets within an expert's weights and of a token are 32 bits
-    pl.panels = load > (exact ? 18 : 12) && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
+    pl.panels = load > 18 && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
     if (pl.panels) pl.slices = f8_moe_slices(load, reached, hidden, inter);
     pl.blocks = pl.panels ? kF8PanelBlocks : 2;
     pl.max_tasks = std::min(pairs, E + pairs / (16 * pl.blocks));
@@ -442,12 +442,11 @@ extern "C" {
 
 size_t mlk_experts_fp8_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter) {
     if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || n_router_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0) return 0;
-    // a long call goes in passes of one size and a shorter last one, whose plan may differ, as may that of fp16
+    // a long call goes in passes of one size and a shorter last one, whose plan may differ
     const int step = f8_moe_pass_tokens(n_tokens, topk), rest = n_tokens % step;
     size_t most = 0;
     for (int t : {step, rest})
-        for (bool exact : {false, true})
-            if (t > 0) most = std::max(most, f8_moe_carve(nullptr, f8_moe_plan(t, n_experts, n_router_experts, topk, hidden, inter, exact), t, n_experts, topk, hidden, inter, nullptr));
+        if (t > 0) most = std::max(most, f8_moe_carve(nullptr, f8_moe_plan(t, n_experts, n_router_experts, topk, hidden, inter), t, n_experts, topk, hidden, inter, nullptr));
     return most;
 }
 
@@ -485,7 +484,7 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
         a.Y = (uint16_t *)y + (size_t)t0 * hidden;
         a.ids = topk_ids + (size_t)t0 * topk;
         a.wts = (const uint16_t *)topk_weights + (size_t)t0 * topk;
-        const F8MoePlan pl = f8_moe_plan(a.T, n_experts, n_router_experts, topk, hidden, inter, x_kind == MLK_F16);
+        const F8MoePlan pl = f8_moe_plan(a.T, n_experts, n_router_experts, topk, hidden, inter);
         a.slots = f8_moe_slots(a.n_pairs, n_experts);
         F8MoeWorkspace ws;
         f8_moe_carve((uint8_t *)workspace, pl, a.T, n_experts, topk, hidden, inter, &ws);

@@ -6,9 +6,13 @@
 //
 // Order of the work: (expert, row tile, task of the expert) with tasks fastest, one line cut into eight equal runs, one per XCD: the tasks of an expert share a row tile's weights in one L2.
 //
-// 8 experts of 4096 x 14336, two picks, 1000 tokens: gate/up 317 us (470 GFLOP), down 210 (235 GFLOP).  The loop runs as fast as in the linear layers' panels (1.87 us a window of 256 x 256); what is
-// missing to their rate are columns that pad a task to 64, an item's first loads and its epilogue, beside which the CU has nothing else (32 windows an item in gate/up), and of the down projection
-// the 16 x 11 panels for 256 CUs.
+// gate/up multiplies codes as 16-bit numbers (products that feed codes, mlk_f8.cuh), in panels of up to 128 pairs: the registers of larger ones go to the widened weights, and a task of more takes
+// its row tile twice.
+//
+// 8 experts of 4096 x 14336, two picks, 1000 tokens: gate/up 509 us (470 GFLOP, 0.92 PFLOP/s), down 210 (235 GFLOP).  The down loop runs as fast as in the linear layers' panels (1.87 us a window of 256 x 256); what is
+// missing to their rate are columns that pad a task to 64, an item's first loads and its epilogue, beside which the CU has nothing else, and the 16 x 11 panels for 256 CUs.  gate/up takes 1.6 times what
+// 8-bit products in panels of 256 pairs take (317 us; 64 experts of 2048 x 1408 at 2000 tokens 210 and 127): each half of a task reads its weights from LDS and widens them again, in both token halves of the
+// workgroup.  16-bit panels of 256 tokens reach 1.2 PFLOP/s on products of this kind (mlk_moe_wide.cuh).
 #pragma once
 
 #include "mlk_f8_moe.cuh"
@@ -30,10 +34,10 @@ __device__ __forceinline__ const F8MoeArgs &f8_moe_args(int &lane, int &wave) {
 }
 
 // Both panels return a ticket of the next item (QUEUE, wave 0).
-template <bool QUEUE, bool EXACT, int TB>
+template <bool QUEUE, int TB>
 __device__ __forceinline__ int f8_moe_gate_up_panel(const F8MoeArgs &p, const MoeTask &tk, int rt, int wave, int lane) {
     extern __shared__ u32x4 win[];
-    using Loop = F8PanelLoop<2, TB, 2, EXACT>;
+    using Loop = F8PanelLoop<2, TB, 2, true>;
     const int wr = wave & 3, wt = wave >> 2, groups_i = p.I >> 4, windows = p.H >> 7, slots = tk.nblocks * 16;
     const uint32_t tile_row = (uint32_t)p.H * 16u;             // bytes of a row group
     const int32_t *sorted = p.sorted + tk.block0 * 16;
@@ -167,31 +171,20 @@ __device__ __forceinline__ MoeTask f8_moe_item(const F8MoeArgs &p, int item, int
     return p.tasks[t0.first + local % t0.count];
 }
 
-// EXACT (fp16): panels of up to 128 pairs, the registers of larger ones go to the widened weights; a task of more takes its row tile twice.  The 16-bit products bound it (without
-// widening a layer of 1000 tokens took 744 of 831 us): 8 experts of 4096 x 14336, codes -> exact at 64 tokens 183 -> 231 us, 300 198 -> 258, 1000 347 -> 610.
-template <bool QUEUE, bool EXACT>
+template <bool QUEUE>
 __device__ __forceinline__ int f8_moe_gate_up_item(const F8MoeArgs &p, int item, int wave, int lane) {
     int rt;
     const MoeTask tk = f8_moe_item(p, item, p.I >> 7, rt);
-    if constexpr (EXACT) {
-        MoeTask half = tk;
-        half.nblocks = min(tk.nblocks, 8);
-        if (tk.nblocks > 8) {
-            f8_moe_gate_up_panel<false, true, 2>(p, half, rt, wave, lane);
-            __syncthreads();
-            half.block0 += 8;
-            half.nblocks = tk.nblocks - 8;
-        }
-        if (half.nblocks <= 4) return f8_moe_gate_up_panel<QUEUE, true, 1>(p, half, rt, wave, lane);
-        return f8_moe_gate_up_panel<QUEUE, true, 2>(p, half, rt, wave, lane);
-    } else {
-        switch ((tk.nblocks + 3) >> 2) {
-            case 1: return f8_moe_gate_up_panel<QUEUE, false, 1>(p, tk, rt, wave, lane);
-            case 2: return f8_moe_gate_up_panel<QUEUE, false, 2>(p, tk, rt, wave, lane);
-            case 3: return f8_moe_gate_up_panel<QUEUE, false, 3>(p, tk, rt, wave, lane);
-            default: return f8_moe_gate_up_panel<QUEUE, false, 4>(p, tk, rt, wave, lane);
-        }
+    MoeTask half = tk;
+    half.nblocks = min(tk.nblocks, 8);
+    if (tk.nblocks > 8) {
+        f8_moe_gate_up_panel<false, 2>(p, half, rt, wave, lane);
+        __syncthreads();
+        half.block0 += 8;
+        half.nblocks = tk.nblocks - 8;
     }
+    if (half.nblocks <= 4) return f8_moe_gate_up_panel<QUEUE, 1>(p, half, rt, wave, lane);
+    return f8_moe_gate_up_panel<QUEUE, 2>(p, half, rt, wave, lane);
 }
 template <class T, bool QUEUE>
 __device__ __forceinline__ int f8_moe_down_item(const F8MoeArgs &p, int item, int wave, int lane) {
@@ -209,11 +202,10 @@ __device__ __forceinline__ int f8_moe_down_item(const F8MoeArgs &p, int item, in
 __device__ __forceinline__ int f8_moe_up_items(const F8MoeArgs &p) { return (p.I >> 7) * p.n_tasks[0]; }
 __device__ __forceinline__ int f8_moe_down_items(const F8MoeArgs &p) { return ((p.H + 255) >> 8) * p.slices * p.n_tasks[0]; }
 
-template <bool EXACT>
 __global__ void __launch_bounds__(512) f8_moe_gate_up_panel_kernel(F8MoeArgs p) {
     const int n = f8_moe_up_items(p), item = wide_item(blockIdx.x, n);
     if (item >= n) return;
-    f8_moe_gate_up_item<false, EXACT>(p, item, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63);
+    f8_moe_gate_up_item<false>(p, item, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63);
 }
 template <class T>
 __global__ void __launch_bounds__(512) f8_moe_down_panel_kernel(F8MoeArgs p) {
@@ -221,7 +213,6 @@ __global__ void __launch_bounds__(512) f8_moe_down_panel_kernel(F8MoeArgs p) {
     if (item >= n) return;
     f8_moe_down_item<T, false>(p, item, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63);
 }
-template <bool EXACT>
 __global__ void __launch_bounds__(512) f8_moe_gate_up_queue_kernel(F8MoeArgs) {
     __shared__ int s_item;
     int ticket = blockIdx.x >> 3;
@@ -232,7 +223,7 @@ __global__ void __launch_bounds__(512) f8_moe_gate_up_queue_kernel(F8MoeArgs) {
         __syncthreads();                                       // also: LDS is free again
         const int item = __builtin_amdgcn_readfirstlane(s_item);
         if (item < 0) return;
-        ticket = f8_moe_gate_up_item<true, EXACT>(p, item, wave, lane);
+        ticket = f8_moe_gate_up_item<true>(p, item, wave, lane);
     }
 }
 template <class T>
@@ -251,13 +242,13 @@ __global__ void __launch_bounds__(512) f8_moe_down_queue_kernel(F8MoeArgs) {
 }
 
 constexpr size_t f8_most(size_t a, size_t b) { return a > b ? a : b; }
-template <int NS>
-constexpr size_t f8_moe_ring() {
-    return f8_most(f8_most(F8PanelLoop<2, 1, NS>::lds_bytes, F8PanelLoop<2, 2, NS>::lds_bytes), f8_most(F8PanelLoop<2, 3, NS>::lds_bytes, F8PanelLoop<2, 4, NS>::lds_bytes));
+constexpr size_t f8_moe_up_ring() { return f8_most(F8PanelLoop<2, 1, 2, true>::lds_bytes, F8PanelLoop<2, 2, 2, true>::lds_bytes); }
+constexpr size_t f8_moe_down_ring() {
+    return f8_most(f8_most(F8PanelLoop<2, 1>::lds_bytes, F8PanelLoop<2, 2>::lds_bytes), f8_most(F8PanelLoop<2, 3>::lds_bytes, F8PanelLoop<2, 4>::lds_bytes));
 }
-// Do at most n items of `windows` each go through the queues (wide_queue_pays)?  They cost 1 to 3 us a kernel and win where tasks differ in width: gate/up of 8 experts of 4096 x 14336 at 300
-// tokens 260 -> 198 us, at 512 244 -> 230, at 1000 349 -> 338, at 2000 530 -> 498 (down in two slices 346 -> 321, at 512 192 -> 167), at 128 184 -> 177, at 64 175 -> 178; of 64 experts of 2048 x 1408 at
-// 500 85.6 -> 87.7, at 2000 129 -> 127.
+// Do at most n items of `windows` each go through the queues (wide_queue_pays)?  They cost 1 to 4 us a kernel and win where tasks differ in width: gate/up of 8 experts of 4096 x 14336 at 300
+// tokens 263 -> 262 us, at 512 402 -> 331, at 1000 581 -> 505, at 2000 916 -> 906 (down in two slices 342 -> 331, at 512 115 -> 117, at 1000 in one 208 -> 212), at 128 206 -> 203, at 100 214 -> 225; of 64 experts
+// of 2048 x 1408 at 500 86 -> 85, at 2000 215 -> 214.
 static inline bool f8_queue_pays(const F8MoeArgs &a, int n, int windows) {
     const double mean = (double)a.n_pairs / a.id_limit, spread = 3 * sqrt(mean);
     if (ceil(fmax(mean - spread, 1) / 64) == ceil((mean + spread) / 64)) return false;
@@ -265,12 +256,11 @@ static inline bool f8_queue_pays(const F8MoeArgs &a, int n, int windows) {
 }
 template <class T>
 int f8_launch_moe_panels(const F8MoeArgs &a, int max_tasks, hipStream_t s) {
-    constexpr size_t lds_up = f8_most(f8_moe_ring<2>(), 4096 + 256 * kF8OutPitch), lds_down = f8_most(f8_moe_ring<1>(), kWideDownOut);
+    constexpr size_t lds_up = f8_most(f8_moe_up_ring(), 4096 + 256 * kF8OutPitch), lds_down = f8_most(f8_moe_down_ring(), kWideDownOut);
     static bool ready_up[2][64] = {}, ready_down[2][64] = {};
     const int items_up = (a.I >> 7) * max_tasks, items_down = ((a.H + 255) >> 8) * a.slices * max_tasks;
     const bool queue_up = f8_queue_pays(a, items_up, a.H >> 7), queue_down = f8_queue_pays(a, items_down, (a.I >> 7) / a.slices);
-    constexpr bool EXACT = std::is_same<T, F16>::value;
-    const auto up = queue_up ? &f8_moe_gate_up_queue_kernel<EXACT> : &f8_moe_gate_up_panel_kernel<EXACT>;
+    const auto up = queue_up ? &f8_moe_gate_up_queue_kernel : &f8_moe_gate_up_panel_kernel;
     const auto down = queue_down ? &f8_moe_down_queue_kernel<T> : &f8_moe_down_panel_kernel<T>;
     int rc = panel_lds_attribute(up, lds_up, ready_up[queue_up]);
     if (rc == MLK_OK) rc = panel_lds_attribute(down, lds_down, ready_down[queue_down]);

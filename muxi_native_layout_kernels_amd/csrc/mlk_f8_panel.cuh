@@ -23,7 +23,7 @@ struct F8PanelSrc {
 };
 
 // NS = 2: the first half of a wave's row tiles and the second have scales of their own, of which waves 4..7 fetch one each in lanes 0 and 1.
-// EXACT: products of 16 bits of the same codes (products that feed codes, mlk_f8.cuh).  A window's weights are widened once, each block of tokens ahead of its products.
+// EXACT: products of 16 bits of the same codes (products that feed codes, mlk_f8.cuh).  A wave widens a window's weights once, each block of tokens ahead of its products.
 template <int PR, int TB, int NS = 1, bool EXACT = false>
 struct F8PanelLoop : P8TokenPairs<TB, true> {
     using Tok = P8TokenPairs<TB, true>;          // its NB: chunks of tokens a wave fetches
