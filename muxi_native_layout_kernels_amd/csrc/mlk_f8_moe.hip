@@ -323,7 +323,12 @@ __global__ void __launch_bounds__(512) f8_moe1_down_kernel(F8MoeArgs p) {
 }
 
 // -------------------------------------------------------------------------------------------------------------------- host
-static int f8_moe_pass_tokens(int n_tokens, int topk) { return n_tokens < kF8MoePairs / topk ? n_tokens : kF8MoePairs / topk; }
+// Tokens of a pass.  The down panels' offsets of the intermediate's scales [I / 128][slot] are 32 bits: a pass of n pairs has at most n + 15 E + 15 slots (f8_moe_slots), and slots * I / 32 bytes stay
+// within 2^32.  With I below 2^23 that leaves 12500 pairs at least.
+static int f8_moe_pass_tokens(int n_tokens, int topk, int E, int inter) {
+    const int64_t pairs = std::min<int64_t>(kF8MoePairs, (1ll << 37) / inter - 15 * E - 15);
+    return (int)std::min<int64_t>(n_tokens, pairs / topk);
+}
 
 struct F8MoeWorkspace {
     MoeTask *tasks;
@@ -441,9 +446,9 @@ using namespace mlk;
 extern "C" {
 
 size_t mlk_experts_fp8_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter) {
-    if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || n_router_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0) return 0;
+    if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || n_router_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0 || hidden >= (1 << 23) || inter >= (1 << 23)) return 0;
     // a long call goes in passes of one size and a shorter last one, whose plan may differ
-    const int step = f8_moe_pass_tokens(n_tokens, topk), rest = n_tokens % step;
+    const int step = f8_moe_pass_tokens(n_tokens, topk, n_experts, inter), rest = n_tokens % step;
     size_t most = 0;
     for (int t : {step, rest})
         if (t > 0) most = std::max(most, f8_moe_carve(nullptr, f8_moe_plan(t, n_experts, n_router_experts, topk, hidden, inter), t, n_experts, topk, hidden, inter, nullptr));
@@ -477,7 +482,7 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
     a.H = hidden;
     a.I = inter;
     a.E = n_experts;
-    const int step = f8_moe_pass_tokens(n_tokens, topk);
+    const int step = f8_moe_pass_tokens(n_tokens, topk, n_experts, inter);
     for (int t0 = 0; t0 < n_tokens; t0 += step) {
         a.T = std::min(step, n_tokens - t0);
         a.n_pairs = a.T * topk;

@@ -1,0 +1,11 @@
+"""CPU: sizes at the ends of what the e4m3 products, their expert layers and the routing promise."""
+from muxi_native_layout_kernels_amd import _lib
+
+
+def test_scales_of_an_intermediate_stay_within_32_bits():
+    """The down panels address the scales [I/128, slots] of a pass with 32 bits: codes of slots * I bytes and scales of a 32nd of that, at most 2^37 and 2^32.  Beside them one token's row, sums and tables are small."""
+    lib = _lib.load()
+    hidden, inter = 128, (1 << 23) - 128
+    for tokens, experts, picks in ((16384, 1, 1), (16384, 16, 1), (8192, 16, 2), (100000, 8, 4)):
+        need = lib.mlk_experts_fp8_workspace_bytes(tokens, experts, experts, picks, hidden, inter)
+        assert (1 << 36) < need <= (1 << 37) + (1 << 32) + (1 << 26), (tokens, experts, picks)
