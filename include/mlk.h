@@ -397,7 +397,7 @@ size_t mlk_experts_w4_workspace_bytes(int n_tokens, int n_experts, int n_router_
  * w1_scale [E, 2I/128, H/128], w2_scale [E, H/128, I/128].  topk_ids int32 [T*K], ids outside 0..n_router_experts-1 are dropped; experts_map int32
  * [n_router_experts] or NULL (n_router_experts == n_experts): -1 drops the pair.  topk_weights [T*K] of x_kind.  y is overwritten, a token without experts here
  * gets zeros, a token with an infinity or NaN a row of NaN.  H % 128 == 0, I % 128 == 0, E <= 256, K <= 32.  w1, w2, x, y and workspace on 16 bytes.  workspace:
- * at least mlk_experts_fp8_workspace_bytes(), no initialisation. */
+ * at least mlk_experts_fp8_workspace_bytes(), no initialisation; what that gives for a count of tokens is enough for every smaller one. */
 int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2, const float *w2_scale, const void *x, int n_tokens, int n_experts,
                           int n_router_experts, int topk, int hidden, int inter, int x_kind, const int32_t *topk_ids, const void *topk_weights,
                           const int32_t *experts_map, void *y, void *workspace, size_t workspace_bytes, void *stream);

@@ -347,15 +347,29 @@ struct F8MoePlan {
     int blocks;              // of 16 pairs, of a task at most
     int max_tasks, slices;
 };
+// Experts that get pairs, and how many each: with E of the router's experts here that share of the pairs is expected here.
+struct F8MoeLoad {
+    int reached, load;
+};
+static F8MoeLoad f8_moe_load(int tokens, int E, int n_router, int topk) {
+    const int pairs = tokens * topk, here = (int)std::max<int64_t>(1, std::min<int64_t>(pairs, (int64_t)pairs * E / n_router));
+    const int reached = std::min(here, E);
+    return {reached, (here + reached - 1) / reached};
+}
+// Panels' tasks of an expert with a little more than `load` pairs.
+static int f8_moe_tasks(int load) {
+    const int width = 16 * kF8PanelBlocks, high = load + (int)std::sqrt((double)load);
+    return (high + width - 1) / width;
+}
 // Slices of the down panels' k: two where k is long and they spare a quarter of the rounds over the card, for the sums of a second slice to be written and read.  One -> two at 8 experts of
 // 4096 x 14336 and 64 tokens 109 -> 88 us, 300 198 -> 132, 512 182 -> 167 (through the queues), 2000 379 -> 346 and 9 more to add them; at 1000, where the rounds are the same, 192 -> 210; four 94, 146, 149,
 // 342, 193 and up to 35 more.  Of 2048 x 768 two cost 30 %.
 static int f8_moe_slices(int load, int reached, int hidden, int inter) {
     if (inter < 64 * kF8K) return 1;
-    const int width = 16 * kF8PanelBlocks, high = load + (int)std::sqrt((double)load);
-    const int items = (hidden + 255) / 256 * reached * ((high + width - 1) / width), cus = device_cus();
+    const int items = (hidden + 255) / 256 * reached * f8_moe_tasks(load), cus = device_cus();
     return (2 * items + cus - 1) / cus * 2 <= (items + cus - 1) / cus * 3 ? 2 : 1;
 }
+constexpr int kF8MoeStreamed = 18;      // pairs an expert of the streaming kernels
 static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidden, int inter) {
     F8MoePlan pl = {};
     const int pairs = tokens * topk;
@@ -364,14 +378,12 @@ static F8MoePlan f8_moe_plan(int tokens, int E, int n_router, int topk, int hidd
         pl.one = true;
         return pl;
     }
-    // with E of the router's experts here that share of the pairs is expected here
-    const int here = (int)std::max<int64_t>(1, std::min<int64_t>(pairs, (int64_t)pairs * E / n_router));
-    const int reached = std::min(here, E), load = (here + reached - 1) / reached;
     // Panels from 19 pairs an expert on: below, tasks of the streaming kernels pass over the weights about as often and start sooner.  The whole layer on the last count of pairs that is streamed and the first
     // of the panels: 8 experts of 4096 x 14336 286 and 277 us, 128 of 2048 x 768 160 and 154.
     // offsets within an expert's weights and of a token are 32 bits
-    pl.panels = load > 18 && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
-    if (pl.panels) pl.slices = f8_moe_slices(load, reached, hidden, inter);
+    const F8MoeLoad l = f8_moe_load(tokens, E, n_router, topk);
+    pl.panels = l.load > kF8MoeStreamed && (int64_t)hidden * inter < (1ll << 31) && (int64_t)tokens * hidden < (1ll << 31);
+    if (pl.panels) pl.slices = f8_moe_slices(l.load, l.reached, hidden, inter);
     pl.blocks = pl.panels ? kF8PanelBlocks : 2;
     pl.max_tasks = std::min(pairs, E + pairs / (16 * pl.blocks));
     return pl;
@@ -408,6 +420,16 @@ static size_t f8_moe_carve(uint8_t *base, const F8MoePlan &pl, int tokens, int E
     if (!pl.panels) w.hpart = (f32x4 *)take((size_t)pl.max_tasks * (inter / kF8K) * 16 * 1024);
     if (ws) *ws = w;
     return off;
+}
+
+static size_t f8_moe_pass_bytes(int tokens, int E, int n_router, int topk, int hidden, int inter) {
+    return f8_moe_carve(nullptr, f8_moe_plan(tokens, E, n_router, topk, hidden, inter), tokens, E, topk, hidden, inter, nullptr);
+}
+// What the passes of a call take: some of one size, and a shorter last one, whose plan may differ.
+static size_t f8_moe_call_bytes(int n_tokens, int E, int n_router, int topk, int hidden, int inter) {
+    const int step = f8_moe_pass_tokens(n_tokens, topk, E, inter), rest = n_tokens % step;
+    const size_t whole = f8_moe_pass_bytes(step, E, n_router, topk, hidden, inter);
+    return rest ? std::max(whole, f8_moe_pass_bytes(rest, E, n_router, topk, hidden, inter)) : whole;
 }
 
 template <class T>
@@ -447,11 +469,23 @@ extern "C" {
 
 size_t mlk_experts_fp8_workspace_bytes(int n_tokens, int n_experts, int n_router_experts, int topk, int hidden, int inter) {
     if (n_tokens <= 0 || n_experts <= 0 || n_experts > 256 || n_router_experts <= 0 || topk <= 0 || topk > 32 || hidden <= 0 || inter <= 0 || hidden >= (1 << 23) || inter >= (1 << 23)) return 0;
-    // a long call goes in passes of one size and a shorter last one, whose plan may differ
-    const int step = f8_moe_pass_tokens(n_tokens, topk, n_experts, inter), rest = n_tokens % step;
-    size_t most = 0;
-    for (int t : {step, rest})
-        if (t > 0) most = std::max(most, f8_moe_carve(nullptr, f8_moe_plan(t, n_experts, n_router_experts, topk, hidden, inter), t, n_experts, topk, hidden, inter, nullptr));
+    // Enough for every shorter call too, some of whose plans take more (the partial sums of streamed tasks, two slices of the down projection).  Plans follow from the stage of a count of tokens, which
+    // never falls; within a stage longer passes take more, so that its last one counts.
+    const int longest = f8_moe_pass_tokens(n_tokens, topk, n_experts, inter);
+    auto stage = [&](int t) {
+        const int load = f8_moe_load(t, n_experts, n_router_experts, topk).load;
+        return (int64_t)t * hidden >= (1ll << 31) ? 1 << 20 : load <= kF8MoeStreamed ? 0 : f8_moe_tasks(load);
+    };
+    size_t most = f8_moe_pass_bytes(1, n_experts, n_router_experts, topk, hidden, inter);
+    for (int t = 1; t <= longest; ++t) {
+        int high = longest;                                    // the last one of t's stage is in t .. high
+        while (t < high) {
+            const int mid = t + (high - t + 1) / 2;
+            if (stage(mid) == stage(t)) t = mid;
+            else high = mid - 1;
+        }
+        most = std::max(most, f8_moe_pass_bytes(t, n_experts, n_router_experts, topk, hidden, inter));
+    }
     return most;
 }
 
@@ -469,7 +503,7 @@ int mlk_fused_experts_fp8(const void *w1, const float *w1_scale, const void *w2,
     MLK_REQUIRE(w1 && w1_scale && w2 && w2_scale && x && topk_ids && topk_weights && y && workspace, "experts fp8: null pointer");
     MLK_REQUIRE(aligned16(w1) && aligned16(w2) && aligned16(x) && aligned16(y) && aligned16(workspace),
                 "experts fp8: weights, activations, outputs and workspace must lie on 16 bytes");
-    if (workspace_bytes < mlk_experts_fp8_workspace_bytes(n_tokens, n_experts, n_router_experts, topk, hidden, inter)) return fail(MLK_ERR_WORKSPACE, "experts fp8: workspace too small");
+    if (workspace_bytes < f8_moe_call_bytes(n_tokens, n_experts, n_router_experts, topk, hidden, inter)) return fail(MLK_ERR_WORKSPACE, "experts fp8: workspace too small");
     hipStream_t s = (hipStream_t)stream;
     F8MoeArgs a = {};
     a.w1 = (const uint8_t *)w1;

@@ -9,3 +9,14 @@ def test_scales_of_an_intermediate_stay_within_32_bits():
     for tokens, experts, picks in ((16384, 1, 1), (16384, 16, 1), (8192, 16, 2), (100000, 8, 4)):
         need = lib.mlk_experts_fp8_workspace_bytes(tokens, experts, experts, picks, hidden, inter)
         assert (1 << 36) < need <= (1 << 37) + (1 << 32) + (1 << 26), (tokens, experts, picks)
+
+
+def test_scratch_of_an_expert_layer_serves_every_shorter_call():
+    lib = _lib.load()
+    for experts, router, picks, hidden, inter in ((8, 8, 2, 4096, 14336), (16, 16, 4, 512, 256), (64, 128, 8, 2048, 768), (1, 1, 1, 256, 128), (3, 300, 32, 256, 8192), (2, 2, 1, 128, (1 << 23) - 128),
+                                                  (32, 256, 8, 7168, 2048), (4, 4, 2, 1 << 20, 128)):
+        last = 0
+        for tokens in list(range(1, 2101)) + [2600, 4096, 5000, 8192, 8193, 16384, 16385, 20000, 100000]:
+            need = lib.mlk_experts_fp8_workspace_bytes(tokens, experts, router, picks, hidden, inter)
+            assert need >= last > -1, (experts, router, picks, hidden, inter, tokens)
+            last = need
