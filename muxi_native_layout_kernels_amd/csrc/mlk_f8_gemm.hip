@@ -326,7 +326,8 @@ static F8Plan f8_plan(int m, int n, int k, bool raw) {
         else stream(windows >= 48 ? 8 : 2, 1, 4, 1);
     } else {
         if (groups <= cus / 4 && m <= 64) stream(1, 2, 8, thin);
-        else if (m > 64) stream(m > 128 || groups > cus / 2 ? 4 : 2, 2, 8, groups <= cus / 4 ? thin : 1);
+        // more than 256 tokens come here only with k that the panels do not take: whole, as arrivals of any number of tokens do not fit the counters
+        else if (m > 64) stream(m > 128 || groups > cus / 2 ? 4 : 2, 2, 8, groups <= cus / 4 && m <= 256 ? thin : 1);
         else if (groups <= cus / 2) stream(2, blocks, 8, 4);
         else if (groups <= cus && deep) stream(4, 2, 8, 4);
         else if (groups <= cus) stream(m <= 32 ? 1 : 2, 2, 8, 1);

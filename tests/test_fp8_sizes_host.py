@@ -20,3 +20,11 @@ def test_scratch_of_an_expert_layer_serves_every_shorter_call():
             need = lib.mlk_experts_fp8_workspace_bytes(tokens, experts, router, picks, hidden, inter)
             assert need >= last > -1, (experts, router, picks, hidden, inter, tokens)
             last = need
+
+
+def test_arrivals_fit_the_counters():
+    """k past the panels' offsets, so that thousands of tokens stream: 16 sets of rows x tokens / 32 workgroups count their arrivals in 16384 counters, if k is in slices; from 32769 tokens on they do not fit."""
+    lib = _lib.load()
+    few = lib.mlk_gemm_fp8_workspace_bytes(256, 1024, 1 << 23, 2)
+    for tokens in (257, 32768, 32769, 40000):
+        assert lib.mlk_gemm_fp8_workspace_bytes(tokens, 1024, 1 << 23, 2) <= few, tokens
