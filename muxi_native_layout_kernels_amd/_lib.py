@@ -60,6 +60,7 @@ SIGNATURES = {
     "mlk_gemm_layout_a_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_int,
                                       c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mlk_gemm_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "mlk_gemm_fp8_needs_workspace": (c_int, [c_int, c_int, c_int, c_int]),
     "mlk_fused_experts_fp8": (c_int, [c_void_p] * 5 + [c_int] * 7 + [c_void_p] * 5 + [c_size_t, c_void_p]),
     "mlk_experts_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "mlk_moe_routing": (c_int, [c_void_p] + [c_int] * 7 + [c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),

@@ -257,14 +257,19 @@ constexpr size_t kF8StagedLds = 140 * 1024;     // of staged tokens
 //                        10.2; 8192 x 8192 at 32 23.9 and 21.8; 5120 x 13824 at 16 q4,1,8,4 21.9, q2,1,8,1 23.5, g 21.2; at 32 35 and 23.5; 13824 x 5120 at 8 q4,1,8,1 15.7, g 19.2; at 24 20.5 and 22.1, at 32 24.3 and 22.8;
 //                        22016 x 4096 at 7 q2,1,4,1 20.2, q4,1,8,1 22.0, g 21.1; 28672 x 8192 at 16 q8,1,4,1 40.7, g 44.0; at 24 q4,2,4,1 54.8, p 49.6
 //   staged codes         one token of large weights only: 28672 x 8192 38.1, g 40.8; 4096 x 14336 13.1, g 14.1; 4096 x 4096 6.2, g 5.7
+static bool f8_panels_fit(int k) { return k < 1 << 23; }            // offsets within a panel are 32 bits
+static bool f8_deep(int k) { return k / kF8K >= 96; }                // slices bring workgroups of a few row groups back
+// Whether the panels' own plan is taken: from some number of tokens on, 257 at the latest.
+static bool f8_wide(int m, int n, int k) {
+    const int groups = n / 16, cus = device_cus();
+    // up to 256 tokens through few rows: 512 x 7168 at 200 tokens g4,2,8,4 9.4, panels 12.2; at 300 12.5; 4096 x 4096 at 100 g4,2,8,1 12.6, panels 14.9; at 200 16.5
+    const bool narrow = m <= 64 || (m <= 128 && groups <= cus && !f8_deep(k)) || (m <= 256 && groups <= cus / 4);
+    return !narrow && f8_panels_fit(k);
+}
 static F8Plan f8_plan(int m, int n, int k, bool raw) {
     F8Plan pl = {};
     const int groups = n / 16, windows = k / kF8K, cus = device_cus();
-    const bool panels_fit = k < 1 << 23;                   // offsets within a panel are 32 bits
-    // 96 windows and more: slices bring workgroups of a few row groups back
-    const bool deep = windows >= 96;
-    // up to 256 tokens through few rows: 512 x 7168 at 200 tokens g4,2,8,4 9.4, panels 12.2; at 300 12.5; 4096 x 4096 at 100 g4,2,8,1 12.6, panels 14.9; at 200 16.5
-    const bool narrow = m <= 64 || (m <= 128 && groups <= cus && !deep) || (m <= 256 && groups <= cus / 4);
+    const bool panels_fit = f8_panels_fit(k), deep = f8_deep(k);
     const int rows = (n + 127) / 128;
     auto panels = [&](int pr, int tb, int p3) {
         pl.panels = true;
@@ -273,7 +278,7 @@ static F8Plan f8_plan(int m, int n, int k, bool raw) {
         pl.p3 = std::max(1, p3);
         return pl;
     };
-    if (!narrow && panels_fit) {
+    if (f8_wide(m, n, k)) {
         int32_t out[4];
         gemm_plan(m, n, k / 2, false, false, out);
         return panels(out[1] / 2, out[2], out[3]);
@@ -337,8 +342,10 @@ static F8Plan f8_plan(int m, int n, int k, bool raw) {
     return pl;
 }
 
-static size_t f8_partial_bytes(const F8Plan &pl, int m, int n) {
-    if (pl.panels || pl.slices == 1) return 0;
+static size_t f8_partial_bytes(const F8Plan &pl, int m, int n, int k) {
+    Panel8Args p = {};
+    if (pl.panels) return panel8_arguments(p, m, n, k / 2, pl.pr, pl.tb, pl.p3);
+    if (pl.slices == 1) return 0;
     const size_t sets = (size_t)((n / 16 + pl.r - 1) / pl.r) * ((m + pl.tt * 16 - 1) / (pl.tt * 16));
     return sets * pl.slices * pl.r * pl.tt * 1024;
 }
@@ -349,9 +356,7 @@ struct F8Scratch {
     size_t partial_bytes;
 };
 // quantize: activations that the call quantises with a launch of its own
-static size_t f8_carve(uint8_t *base, const F8Plan &pl, int m, int n, int k, bool quantize, F8Scratch *out) {
-    Panel8Args p = {};
-    const size_t partial = pl.panels ? panel8_arguments(p, m, n, k / 2, pl.pr, pl.tb, pl.p3) : f8_partial_bytes(pl, m, n);
+static size_t f8_carve(uint8_t *base, size_t partial, int m, int k, bool quantize, F8Scratch *out) {
     F8Scratch w = {};
     size_t off = 0;
     if (quantize || partial > 0) {
@@ -368,6 +373,23 @@ static size_t f8_carve(uint8_t *base, const F8Plan &pl, int m, int n, int k, boo
     }
     if (out) *out = w;
     return off;
+}
+static bool f8_quantises(const F8Plan &pl, bool raw) { return raw && pl.feed == kF8Codes; }
+static size_t f8_call_bytes(const F8Plan &pl, int m, int n, int k, bool raw) { return f8_carve(nullptr, f8_partial_bytes(pl, m, n, k), m, k, f8_quantises(pl, raw), nullptr); }
+// The most that a call of 1 .. m tokens takes.  The panels' plan follows from the tokens' number of blocks of 64, and within one the last count takes most.  Above 16384 tokens the
+// bound of all plans: a slot of at most 256 x 256 sums a CU where panels are cut in slices, two where they are dealt.
+static size_t f8_most_bytes(int m, int n, int k, bool raw) {
+    size_t most = 0, partial = 0;
+    int t = 1;
+    for (; t <= m && t <= 257 && !f8_wide(t, n, k); ++t) most = std::max(most, f8_call_bytes(f8_plan(t, n, k, raw), t, n, k, raw));
+    if (t > m) return most;
+    if (!f8_wide(t, n, k)) return std::max(most, f8_call_bytes(f8_plan(m, n, k, raw), m, n, k, raw));            // the panels do not take this k
+    for (int end = (t + 63) / 64 * 64; t <= m && t <= 16384; t = end + 1, end += 64) {
+        const int last = std::min(end, m);
+        partial = std::max(partial, f8_partial_bytes(f8_plan(last, n, k, raw), last, n, k));
+    }
+    if (m > 16384) partial = std::max(partial, (size_t)device_cus() * 2 * 256 * 256 * 4);
+    return std::max(most, f8_carve(nullptr, partial, m, k, raw, nullptr));
 }
 
 template <class T>
@@ -411,8 +433,13 @@ int mlk_quantize_fp8(const void *x, int x_kind, void *codes, float *scales, int6
 size_t mlk_gemm_fp8_workspace_bytes(int m, int n, int k, int b_kind) {
     if (m <= 0 || n <= 0 || k <= 0 || k % 128 != 0) return 0;
     const bool raw = b_kind != MLK_FP8_E4M3;
-    const F8Plan pl = f8_plan(m, n, k, raw);
-    return f8_carve(nullptr, pl, m, n, k, raw && pl.feed == kF8Codes, nullptr);
+    return f8_most_bytes(m, n, k, raw);
+}
+
+int mlk_gemm_fp8_needs_workspace(int m, int n, int k, int b_kind) {
+    if (m <= 0 || n <= 0 || k <= 0 || k % 128 != 0) return 0;
+    const bool raw = b_kind != MLK_FP8_E4M3;
+    return f8_call_bytes(f8_plan(m, n, k, raw), m, n, k, raw) > 0;
 }
 
 int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, int b_kind, const float *b_scale, int64_t b_scale_t, int64_t b_scale_k, void *c,
@@ -424,7 +451,6 @@ int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, in
     if (m == 0) return MLK_OK;
     MLK_REQUIRE(a && a_scale && b && c && (b_kind != MLK_FP8_E4M3 || b_scale), "gemm fp8: null pointer");
     MLK_REQUIRE(aligned16(a) && aligned16(b) && aligned16(c), "gemm fp8: weights, activations and outputs must lie on 16 bytes");
-    if (workspace_bytes < mlk_gemm_fp8_workspace_bytes(m, n, k, b_kind)) return fail(MLK_ERR_WORKSPACE, "gemm fp8: workspace too small");
     hipStream_t s = (hipStream_t)stream;
     F8GemmArgs p = {};
     p.A = (const uint8_t *)a;
@@ -449,8 +475,9 @@ int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, in
         pl.slices = 1;
     }
     F8Scratch w;
-    if (f8_carve((uint8_t *)workspace, pl, m, n, k, raw && pl.feed == kF8Codes, &w) > 0)
-        MLK_REQUIRE(workspace && aligned16(workspace), "gemm fp8: workspace off 16 bytes");
+    const size_t need = f8_carve((uint8_t *)workspace, f8_partial_bytes(pl, m, n, k), m, k, f8_quantises(pl, raw), &w);
+    if (workspace_bytes < need) return fail(MLK_ERR_WORKSPACE, "gemm fp8: workspace too small");
+    MLK_REQUIRE(need == 0 || (workspace && aligned16(workspace)), "gemm fp8: workspace off 16 bytes");
     if (raw && pl.feed != kF8Codes) {
         p.raw = b;
     } else if (raw) {

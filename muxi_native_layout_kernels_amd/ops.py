@@ -831,8 +831,9 @@ def gemm_layoutA_fp8(A, A_Scale, B, B_Scale=None, alpha=1, beta=0, bias=None, ou
         _check(bias is None or (bias.dtype == dtype and bias.numel() == m), "bias must be [1, m] of the output dtype")
         _check_tensors(((A, "A"), (A_Scale, "A_Scale"), (B, "B"), (bias, "bias")), B.device)
         lib = _lib.load()
-        plan = _plans[key] = (B.size(0), m, k, kind, c_kind, dtype, lib.mlk_gemm_fp8_workspace_bytes(B.size(0), m, k, kind), lib.mlk_gemm_counter_bytes(),
-                              lib.mlk_gemm_layout_a_fp8)
+        # what every shorter call needs too, so that the pool does not grow for one that a graph captures later
+        need = lib.mlk_gemm_fp8_workspace_bytes(B.size(0), m, k, kind) if lib.mlk_gemm_fp8_needs_workspace(B.size(0), m, k, kind) else 0
+        plan = _plans[key] = (B.size(0), m, k, kind, c_kind, dtype, need, lib.mlk_gemm_counter_bytes(), lib.mlk_gemm_layout_a_fp8)
     if B.get_device() != _current_device():
         with torch.cuda.device(B.device):
             return _gemm_fp8_launch(plan, A, A_Scale, B, B_Scale, alpha, bias)

@@ -28,3 +28,16 @@ def test_arrivals_fit_the_counters():
     few = lib.mlk_gemm_fp8_workspace_bytes(256, 1024, 1 << 23, 2)
     for tokens in (257, 32768, 32769, 40000):
         assert lib.mlk_gemm_fp8_workspace_bytes(tokens, 1024, 1 << 23, 2) <= few, tokens
+
+
+def test_scratch_of_a_product_serves_every_shorter_call():
+    lib = _lib.load()
+    for n, k in ((8192, 8192), (4096, 14336), (512, 7168), (28672, 8192), (13824, 5120), (16, 128), (1040, 12416), (37888, 3584), (272, 640), (1024, 1 << 23), (4096, (1 << 23) - 128)):
+        for kind in (0, 1, 2):
+            last = 0
+            for tokens in list(range(1, 700)) + list(range(700, 4500, 37)) + [8191, 8192, 16384, 16385, 30000, 1 << 20, 1 << 21]:
+                need = lib.mlk_gemm_fp8_workspace_bytes(tokens, n, k, kind)
+                assert need >= last, (n, k, kind, tokens)
+                assert need > 0 or not lib.mlk_gemm_fp8_needs_workspace(tokens, n, k, kind)
+                last = need
+    assert lib.mlk_gemm_fp8_needs_workspace(100, 32, 256, 1) and not lib.mlk_gemm_fp8_needs_workspace(8, 4096, 4096, 2)

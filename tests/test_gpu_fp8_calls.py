@@ -63,3 +63,35 @@ def test_a_shorter_layer_captured_after_the_longest(mlk):
     x = randn((most, H), BF, 1.0, 4).cuda()
     ids, wts = (t.cuda() for t in routing(most, E, K, BF, 5))
     captured_after_the_longest(mlk, lambda n: mlk.fused_experts_fp8(x[:n], a1, a2, ids[:n], wts[:n], s1, s2), most, (72, 1, 40, 80))
+
+
+@pytest.mark.parametrize("n,k", [(8192, 8192), (528, 4096), (2064, 7168)])
+def test_scratch_of_the_longest_product_serves_shorter_ones(mlk, n, k):
+    from muxi_native_layout_kernels_amd import _lib
+    lib = _lib.load()
+    A, S = products(mlk, n, k)
+    most = 700
+    x = randn((most, k), BF, 1.0, 4).cuda()
+    need = lib.mlk_gemm_fp8_workspace_bytes(most, n, k, 1)
+    ws = torch.zeros(need + 4096, dtype=torch.uint8, device="cuda")
+    ws[need:] = 91
+    for T in (most, 1, 3, 20, 33, 64, 65, 128, 129, 200, 256, 300):
+        c = torch.full((T + 8, n), 7.0, dtype=BF, device="cuda")
+        rc = lib.mlk_gemm_layout_a_fp8(A.data_ptr(), S.data_ptr(), x.data_ptr(), 1, None, 0, 0, c.data_ptr(), 1, T, n, k, 1.0, None, ws.data_ptr(), need,
+                                       torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, (T, lib.mlk_last_error())
+        assert torch.equal(c[:T], mlk.gemm_layoutA_fp8(A, S, x[:T])), T
+        assert (c[T:] == 7.0).all() and (ws[need:] == 91).all() and (ws[:lib.mlk_gemm_counter_bytes()] == 0).all()
+
+
+def products(mlk, n, k):
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    codes = (torch.randn((n, k), generator=g, device="cuda") * 40).clamp_(-448, 448).to(torch.float8_e4m3fn)
+    return mlk.pack_layout_a(codes), torch.rand(((n + 127) // 128, k // 128), generator=g, device="cuda") * 1e-3 + 1e-4
+
+
+def test_a_shorter_product_captured_after_the_longest(mlk):
+    n, k, most = 8192, 8192, 129
+    A, S = products(mlk, n, k)
+    x = randn((most, k), BF, 1.0, 4).cuda()
+    captured_after_the_longest(mlk, lambda t: mlk.gemm_layoutA_fp8(A, S, x[:t]), most, (128, 1, 64, 16))
