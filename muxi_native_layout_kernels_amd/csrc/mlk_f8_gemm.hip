@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(256) f8_quantize_kernel(const void *__restrict
     }
 }
 
+constexpr int kF8MostK = 65535 * 512;   // of the quantising kernel's grid, whose workgroups take 512 k
 int launch_quantize_fp8(const void *x, int x_kind, uint8_t *codes, float *scales, int64_t scale_t, int64_t scale_k, int64_t T, int K, hipStream_t s) {
     constexpr int NB = 4;
     const int blocks = K / kF8K;
@@ -423,7 +424,7 @@ extern "C" {
 int mlk_quantize_fp8(const void *x, int x_kind, void *codes, float *scales, int64_t scale_t, int64_t scale_k, int64_t n_tokens, int k, void *stream) {
     MLK_REQUIRE(x_kind == MLK_F16 || x_kind == MLK_BF16 || x_kind == MLK_F32, "quantize_fp8: activations must be fp16, bf16 or fp32");
     MLK_REQUIRE(n_tokens >= 0 && n_tokens <= (1ll << 27), "quantize_fp8: 0..2^27 rows");
-    MLK_REQUIRE(k >= 0 && k % 128 == 0 && k / 512 < 65535, "quantize_fp8: K % 128 must be 0, K below 2^25");
+    MLK_REQUIRE(k >= 0 && k % 128 == 0 && k <= kF8MostK, "quantize_fp8: K % 128 must be 0, K at most 33553920");
     if (n_tokens == 0 || k == 0) return MLK_OK;
     MLK_REQUIRE(x && codes && scales, "quantize_fp8: null pointer");
     MLK_REQUIRE(aligned16(x) && aligned16(codes), "quantize_fp8: activations and codes must lie on 16 bytes");
@@ -447,7 +448,7 @@ int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, in
     MLK_REQUIRE(c_kind == MLK_F16 || c_kind == MLK_BF16, "gemm fp8: outputs must be fp16 or bf16");
     MLK_REQUIRE(b_kind == MLK_FP8_E4M3 || b_kind == c_kind, "gemm fp8: activations must be e4m3 codes or of the output's kind");
     MLK_REQUIRE(m >= 0 && m <= (1 << 21), "gemm fp8: 0..2^21 tokens");
-    MLK_REQUIRE(n > 0 && k > 0 && n % 16 == 0 && k % 128 == 0 && k < (1 << 25), "gemm fp8: N % 16 and K % 128 must be 0, K below 2^25");
+    MLK_REQUIRE(n > 0 && k > 0 && n % 16 == 0 && k % 128 == 0 && k <= kF8MostK, "gemm fp8: N % 16 and K % 128 must be 0, K at most 33553920");
     if (m == 0) return MLK_OK;
     MLK_REQUIRE(a && a_scale && b && c && (b_kind != MLK_FP8_E4M3 || b_scale), "gemm fp8: null pointer");
     MLK_REQUIRE(aligned16(a) && aligned16(b) && aligned16(c), "gemm fp8: weights, activations and outputs must lie on 16 bytes");

@@ -41,3 +41,15 @@ def test_scratch_of_a_product_serves_every_shorter_call():
                 assert need > 0 or not lib.mlk_gemm_fp8_needs_workspace(tokens, n, k, kind)
                 last = need
     assert lib.mlk_gemm_fp8_needs_workspace(100, 32, 256, 1) and not lib.mlk_gemm_fp8_needs_workspace(8, 4096, 4096, 2)
+
+
+def test_one_limit_of_k():
+    """Quantising and the product that quantises its activations refuse the same k, with pointers that are never read."""
+    lib = _lib.load()
+    p, big = 4096, 1 << 60
+    for k in (65535 * 512 + 128, (1 << 25) - 128, 1 << 25):
+        assert lib.mlk_quantize_fp8(p, 1, p, p, 1, 1, 1, k, None) < 0 and b"33553920" in lib.mlk_last_error()
+        for kind in (1, 2):
+            assert lib.mlk_gemm_layout_a_fp8(p, p, p, kind, p, 1, 1, p, 1, 100, 32, k, 1.0, None, p, big, None) < 0 and b"33553920" in lib.mlk_last_error(), (k, kind)
+    # the last one that is taken is refused for its workspace, which is checked behind it
+    assert lib.mlk_gemm_layout_a_fp8(p, p, p, 1, None, 0, 0, p, 1, 100, 32, 65535 * 512, 1.0, None, p, 64, None) < 0 and b"too small" in lib.mlk_last_error()
