@@ -16,6 +16,8 @@
 // What bounds it: a chain of dependent steps (the load, of biased ranks the exponentials and divisions in 64 bits, then K times a maximum over registers and lanes), not the bytes.
 // 256 experts in 8 groups, 8 picks, bias, fp32: 16 tokens 7.1 us, 8191 tokens 17.2 us (9 MB; 27.3 with 64-bit exchanges through LDS, all ranks of a group read by its lane and
 // the picks' logits read again from memory); 64 experts, 6 picks, bf16, 16384 tokens 5.7 us.  Gradient of the same: 3.6, 4.6 and 4.4 us, of which a launch is 3.
+#include <algorithm>
+
 #include "mlk_logits.cuh"
 
 namespace mlk {
@@ -379,11 +381,28 @@ static void route_launch_size(const RouteArgs &a, bool vec, bool grad, hipStream
         route_launch<L, 16, 32>(a, vec, grad, s);
     }
 }
-static int route_launch_kind(const RouteArgs &a, int kind, bool vec, bool grad, hipStream_t s) {
+static void route_launch_kind(const RouteArgs &a, int kind, bool vec, bool grad, hipStream_t s) {
     if (kind == MLK_F32) route_launch_size<BalF32>(a, vec, grad, s);
     else if (kind == MLK_F16) route_launch_size<Bal16<F16>>(a, vec, grad, s);
     else route_launch_size<Bal16<BF16>>(a, vec, grad, s);
-    MLK_LAUNCH_CHECK();
+}
+// A launch has fewer than 2^32 threads: at 16 a token up to 2^27 tokens each, 128 tokens of whatever type on 16 bytes (route_vec holds for all parts).
+constexpr int kRouteTokens = 1 << 27;
+static int route_launch_all(const RouteArgs &all, int kind, bool vec, bool grad, hipStream_t s) {
+    const size_t size = kind == MLK_F32 ? 4 : 2;
+    auto at = [&](const void *p, size_t bytes) { return p ? (void *)((uintptr_t)p + bytes) : nullptr; };
+    for (int t0 = 0; t0 < all.T; t0 += std::min(kRouteTokens, all.T - t0)) {
+        RouteArgs a = all;
+        a.T = std::min(kRouteTokens, all.T - t0);
+        a.logits = at(all.logits, (size_t)t0 * a.E * size);
+        a.mask = all.mask ? all.mask + t0 : nullptr;
+        a.ids = all.ids + (size_t)t0 * a.K;
+        a.weights = at(all.weights, (size_t)t0 * a.K * size);
+        a.dweights = at(all.dweights, (size_t)t0 * a.K * size);
+        a.dlogits = at(all.dlogits, (size_t)t0 * a.E * size);
+        route_launch_kind(a, kind, vec, grad, s);
+        MLK_LAUNCH_CHECK();
+    }
     return MLK_OK;
 }
 static bool route_vec(const void *p, int kind, int E) { return E % 4 == 0 && ((uintptr_t)p & (kind == MLK_F32 ? 15 : 7)) == 0; }
@@ -427,7 +446,7 @@ int mlk_moe_routing(const void *logits, int x_kind, int score_fun, int n_tokens,
     a.scaling = scaling;
     a.ids = ids;
     a.weights = weights;
-    return route_launch_kind(a, x_kind, route_vec(logits, x_kind, n_experts), false, (hipStream_t)stream);
+    return route_launch_all(a, x_kind, route_vec(logits, x_kind, n_experts), false, (hipStream_t)stream);
 }
 
 int mlk_moe_routing_grad(const void *logits, int x_kind, int score_fun, int n_tokens, int n_experts, int topk, int renormalize, float scaling, const int32_t *ids,
@@ -447,7 +466,7 @@ int mlk_moe_routing_grad(const void *logits, int x_kind, int score_fun, int n_to
     a.ids = const_cast<int32_t *>(ids);
     a.dweights = dweights;
     a.dlogits = dlogits;
-    return route_launch_kind(a, x_kind, route_vec(logits, x_kind, n_experts) && route_vec(dlogits, x_kind, n_experts), true, (hipStream_t)stream);
+    return route_launch_all(a, x_kind, route_vec(logits, x_kind, n_experts) && route_vec(dlogits, x_kind, n_experts), true, (hipStream_t)stream);
 }
 
 }  // extern "C"
