@@ -274,7 +274,7 @@ size_t mlk_gemm_w4_workspace_bytes(int m, int n, int k, int group);
 int mlk_quantize_fp8(const void *x, int x_kind, void *codes, float *scales, int64_t scale_t, int64_t scale_k, int64_t n_tokens, int k, void *stream);
 
 /* C[M, N] of c_kind (MLK_F16 or MLK_BF16) = T(alpha * B . W^T (+ bias[N])), M of 0..2^21, fp32 sums.  b_kind MLK_FP8_E4M3: codes with scales b_scale, row t's block kb at
- * b_scale[t * b_scale_t + kb * b_scale_k]; else b_kind = c_kind, and the call quantises B as mlk_quantize_fp8 does, into the workspace.  N % 16 == 0, K % 128 == 0,
+ * b_scale[t * b_scale_t + kb * b_scale_k]; else b_kind = c_kind, and the call quantises B as mlk_quantize_fp8 does, into the workspace.  N % 16 == 0, N <= 2^27, K % 128 == 0,
  * K <= 33553920.  a, b, c and workspace on 16 bytes.  workspace: mlk_gemm_fp8_workspace_bytes() bytes under the rules of mlk_gemm_layout_a; what that gives for m is enough for every smaller m.  May be NULL for
  * calls that mlk_gemm_fp8_needs_workspace() says 0 of. */
 int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, int b_kind, const float *b_scale, int64_t b_scale_t, int64_t b_scale_k, void *c,

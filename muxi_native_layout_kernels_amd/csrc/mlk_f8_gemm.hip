@@ -449,6 +449,8 @@ int mlk_gemm_layout_a_fp8(const void *a, const float *a_scale, const void *b, in
     MLK_REQUIRE(b_kind == MLK_FP8_E4M3 || b_kind == c_kind, "gemm fp8: activations must be e4m3 codes or of the output's kind");
     MLK_REQUIRE(m >= 0 && m <= (1 << 21), "gemm fp8: 0..2^21 tokens");
     MLK_REQUIRE(n > 0 && k > 0 && n % 16 == 0 && k % 128 == 0 && k <= kF8MostK, "gemm fp8: N % 16 and K % 128 must be 0, K at most 33553920");
+    // a launch has fewer than 2^32 threads, and the streaming kernels use up to 16 a row
+    MLK_REQUIRE(n <= (1 << 27), "gemm fp8: at most 2^27 rows of weights");
     if (m == 0) return MLK_OK;
     MLK_REQUIRE(a && a_scale && b && c && (b_kind != MLK_FP8_E4M3 || b_scale), "gemm fp8: null pointer");
     MLK_REQUIRE(aligned16(a) && aligned16(b) && aligned16(c), "gemm fp8: weights, activations and outputs must lie on 16 bytes");

@@ -291,7 +291,9 @@ static int f8_launch_panel_shape(const F8PanelArgs &g, hipStream_t s) {
     static bool ready_on[64] = {};
     const int rc = panel_lds_attribute(&f8_panel_kernel<T, PR, TB>, lds, ready_on);
     if (rc != MLK_OK) return rc;
-    f8_panel_kernel<T, PR, TB><<<p.band > 0 ? (p.whole + p.deal) * 8 : (p.whole + p.deal + 7) / 8 * 8, 512, lds, s>>>(g);
+    const int64_t wgs = p.band > 0 ? ((int64_t)p.whole + p.deal) * 8 : (p.whole + p.deal + 7) / 8 * 8;
+    MLK_REQUIRE(wgs < 1 << 23, "gemm fp8: more panels than a launch takes");         // of 2^32 threads
+    f8_panel_kernel<T, PR, TB><<<(int)wgs, 512, lds, s>>>(g);
     MLK_LAUNCH_CHECK();
     if (p.deal > 0) {
         gemm_panel8_fold_kernel<T><<<dim3(4 * PR * TB, p.panels - p.whole, p.band > 0 ? 8 : 1), 256, 0, s>>>(p, PR, TB);

@@ -803,7 +803,7 @@ def gemm_layoutA_fp8(A, A_Scale, B, B_Scale=None, alpha=1, beta=0, bias=None, ou
 
     A [m/16, k/8, 16, 8] e4m3 bytes in layout-A and A_Scale fp32 [ceil(m/128), k/128], as the soft-FP8 products take them.  B fp16 / bf16: quantised in the call as by
     `quantize_fp8`; or codes (float8_e4m3fn or uint8) with B_Scale fp32 [n, k/128], of any strides and any values.  Output of B's dtype, of codes bf16 unless `out_dtype` says
-    fp16.  Any n up to 2^21, m % 16 == 0, k % 128 == 0, k <= 33553920.  fp32 sums; the sum of 128 k is scaled by both scales in fp32.  A row of B with an infinity or NaN gives NaN.  No
+    fp16.  Any n up to 2^21, m % 16 == 0, m <= 2^27, k % 128 == 0, k <= 33553920.  fp32 sums; the sum of 128 k is scaled by both scales in fp32.  A row of B with an infinity or NaN gives NaN.  No
     gradient: the result is detached."""
     key = ("gemm_fp8", A.shape, A.dtype, A.get_device(), A_Scale.shape, A_Scale.dtype, A_Scale.get_device(), B.shape, B.dtype, B.get_device(),
            None if B_Scale is None else (B_Scale.shape, B_Scale.dtype, B_Scale.get_device()), None if bias is None else (bias.shape, bias.dtype, bias.get_device()),

@@ -53,3 +53,11 @@ def test_one_limit_of_k():
             assert lib.mlk_gemm_layout_a_fp8(p, p, p, kind, p, 1, 1, p, 1, 100, 32, k, 1.0, None, p, big, None) < 0 and b"33553920" in lib.mlk_last_error(), (k, kind)
     # the last one that is taken is refused for its workspace, which is checked behind it
     assert lib.mlk_gemm_layout_a_fp8(p, p, p, 1, None, 0, 0, p, 1, 100, 32, 65535 * 512, 1.0, None, p, 64, None) < 0 and b"too small" in lib.mlk_last_error()
+
+
+def test_rows_of_weights_that_a_launch_has_threads_for():
+    lib = _lib.load()
+    p, big = 4096, 1 << 60
+    for n in ((1 << 27) + 16, 1 << 29, (1 << 31) - 16):
+        for kind in (1, 2):
+            assert lib.mlk_gemm_layout_a_fp8(p, p, p, kind, p, 1, 1, p, 1, 1, n, 128, 1.0, None, p, big, None) < 0 and b"2^27 rows" in lib.mlk_last_error(), (n, kind)
