@@ -227,7 +227,8 @@ def fused_moe_fp8(
     experts_map: Optional[torch.Tensor] = None,
     expert_load: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """The MoE layer in e4m3: `moe_routing`, then `fused_experts_fp8`.  gating_output in the activation dtype or fp32, gating_bias fp32.  `expert_load` (int32 [num_experts], at most 256): the
+    """The MoE layer in e4m3: `moe_routing`, then `fused_experts_fp8`.  gating_output in the activation dtype or fp32, gating_bias fp32.  The weights of fp32 logits are
+    rounded to the activation dtype, in which `fused_experts_fp8` takes them.  `expert_load` (int32 [num_experts], at most 256): the
     picks of this call are added to it (`expert_counts`).  No gradient: the result is detached."""
     if num_expert_group is None:
         num_expert_group = 1
@@ -252,6 +253,7 @@ def fused_moe_fp8(
         ops._check(((w1.data_ptr() | w2.data_ptr()) & 15) == 0, "w1 and w2 must lie on 16 bytes")
         ids, weights = ops.moe_routing(gating_output, topk, score_func, renormalize, num_expert_group, topk_group, gating_bias, scaling, token_mask)
         with ops._OnDevice(hidden_states):
+            # weights of fp32 logits to 16 bits, the experts' interface: half a step of each, no more than the result's own rounding
             y = ops._experts_fp8_launch(plan, hidden_states, w1, w2, ids, weights.to(hidden_states.dtype), w1_scale, w2_scale, experts_map)
         if expert_load is not None:
             ops.expert_counts(ids, n_experts, out=expert_load)
