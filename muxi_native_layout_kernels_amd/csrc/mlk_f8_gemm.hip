@@ -60,11 +60,11 @@ struct F8GemmArgs {
     int *counters;               // [workgroup (x, z)], zero between calls
 };
 
-// Bytes of LDS that `m` staged tokens of `windows` windows take: 16 bytes between the rows, so that 16 tokens read different banks, and their scales.
+// Bytes of LDS that `m` staged tokens of `windows` windows take: 16 bytes between the rows, so that tokens read different banks, and their scales.
 __host__ __device__ constexpr int f8_staged_pitch(int windows) { return windows * 8 + 1; }      // in pieces of 16 bytes
 __host__ __device__ constexpr size_t f8_staged_bytes(int m, int windows) { return ((size_t)m * f8_staged_pitch(windows) * 16 + (size_t)m * windows * 4 + 15) / 16 * 16; }
 
-// Windows t0 .. t0 + n - 1 of up to 16 tokens into LDS, from codes or (raw) from activations, which are quantised on the way: 16 lanes a block of 128.
+// Windows t0 .. t0 + n - 1 of all tokens, up to four (of codes one, f8_plan), into LDS, from codes or (raw) from activations, which are quantised on the way: 16 lanes a block of 128.
 template <class T>
 __device__ __forceinline__ void f8_stage(const F8GemmArgs &p, u32x4 *lds, int t0, int n) {
     float *scales = reinterpret_cast<float *>(lds + (size_t)p.M * f8_staged_pitch(n));
@@ -90,7 +90,7 @@ __device__ __forceinline__ void f8_stage(const F8GemmArgs &p, u32x4 *lds, int t0
     }
 }
 
-// Where a workgroup has its tokens from: codes, up to 16 tokens in LDS (codes, or activations that the workgroup quantises), activations that each wave quantises for its own windows.
+// Where a workgroup has its tokens from: codes, up to four tokens in LDS (codes of one, or activations that the workgroup quantises), activations that each wave quantises for its own windows.
 enum F8Feed { kF8Codes, kF8InLds, kF8Quantise };
 
 // Bound by the weights' bytes, with more tokens by what the workgroups read of the activations.  A workgroup owns up to R consecutive row groups, which are dealt out evenly over the

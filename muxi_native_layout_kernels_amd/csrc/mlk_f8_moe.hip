@@ -3,9 +3,9 @@
 // The routed pairs are brought into expert order in blocks of 16, and in the same launch the activations are quantised; a task is one or two blocks of one expert, which share a pass over its
 // weights.  The intermediate is quantised from fp32 to [slot][I] and [I / 128][slot] (slot = place in the order).  The weighted products of the down projection are kept in fp32
 // [pair][H], and a last launch adds a token's pairs in the order of its picks.  One token needs neither order nor last launch; many pairs an expert go through panels (mlk_f8_moe_panel.cuh).
+// Gate and up are sums of exact products in all of them (products that feed codes, mlk_f8.cuh).
 #include <algorithm>
 #include <cmath>
-#include <initializer_list>
 
 #include "mlk_f8_moe.cuh"
 #include "mlk_panel_lds.cuh"

@@ -9,7 +9,7 @@
 // gate/up multiplies codes as 16-bit numbers (products that feed codes, mlk_f8.cuh), in panels of up to 128 pairs: the registers of larger ones go to the widened weights, and a task of more takes
 // its row tile twice.
 //
-// 8 experts of 4096 x 14336, two picks, 1000 tokens: gate/up 509 us (470 GFLOP, 0.92 PFLOP/s), down 210 (235 GFLOP).  The down loop runs as fast as in the linear layers' panels (1.87 us a window of 256 x 256); what is
+// 8 experts of 4096 x 14336, two picks, 1000 tokens: gate/up 509 us (470 GFLOP, 0.92 PFLOP/s), down 210 (235 GFLOP).  The down loop runs as fast as in the linear layers' panels (1.7 to 1.9 us a window of 256 x 256); what is
 // missing to their rate are columns that pad a task to 64, an item's first loads and its epilogue, beside which the CU has nothing else, and the 16 x 11 panels for 256 CUs.  gate/up takes 1.6 times what
 // 8-bit products in panels of 256 pairs take (317 us; 64 experts of 2048 x 1408 at 2000 tokens 210 and 127): each half of a task reads its weights from LDS and widens them again, in both token halves of the
 // workgroup.  16-bit panels of 256 tokens reach 1.2 PFLOP/s on products of this kind (mlk_moe_wide.cuh).

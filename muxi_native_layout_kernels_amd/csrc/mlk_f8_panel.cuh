@@ -3,8 +3,9 @@
 // A window of 128 k is, byte for byte, two k32 slabs of the 16-bit panels (mlk_panel8.cuh): a weight tile of 16 rows is two runs of 1 KiB, a token's piece one line of 128
 // bytes.  So tokens come in the same chunks of eight with the same swizzle (P8TokenPairs), and what comes out goes through the same stores and the same fold.
 //
-// What bounds it: the matrix cores and the reads from LDS about alike.  A window of 256 x 256 keeps a SIMD's matrix core busy for 2048 cycles and LDS for 2000 (192 KB read, 64 written), and takes 3700 at
-// about 2 GHz: 8192 x 8192 at 4000 tokens 222 to 256 us by card (2.1 to 2.4 PFLOP/s), the matrix cores busy 67 % of the cycles.  A panel of 128 x 64 takes 700 cycles of LDS for 256 of products:
+// What bounds it: the matrix cores and the reads from LDS about alike.  A window of 256 x 256 keeps a SIMD's matrix core busy for 2048 cycles and LDS for 2000 (192 KB read, 64 written), and takes 3000 with its share
+// of first loads and stores (8192 x 8192 at 4000 tokens: a CU is busy for 383 thousand cycles in two rounds of 64 windows, at 1.7 GHz, the clock that power holds): 222 to 256 us by card (2.1 to 2.4 PFLOP/s), the matrix
+// cores busy 67 % of the cycles.  A panel of 128 x 64 takes 700 cycles of LDS for 256 of products:
 // 13824 x 5120 at 100 tokens 22 us, the matrix cores busy 24 %.
 #pragma once
 
